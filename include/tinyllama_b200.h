@@ -51,7 +51,9 @@ typedef enum tlb_dtype {
     TLB_FLOAT16 = 1,
     TLB_BFLOAT16 = 2,
     TLB_INT32 = 3,
-    TLB_INT64 = 4
+    TLB_INT64 = 4,
+    TLB_FLOAT8_E4M3 = 5, /* 8-bit cache types, with scales (see below) */
+    TLB_INT8 = 6
 } tlb_dtype;
 
 /* Bits of the per-device status word (tlb_get_device_status). */
@@ -390,6 +392,117 @@ TLB_API int tlb_step_metadata(const int32_t* prompt_lens, const int32_t* prompt_
                         int64_t num_decode, int64_t decode_max_blocks,
                         int64_t block_size, int64_t num_tokens, int64_t alignment,
                         int64_t* positions_out, int64_t* slots_out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit KV caches (no reference counterpart: the reference's caches have the
+ * model dtype, src/core/cache_engine.py:55-108).
+ *
+ *   key_cache, value_cache   : [num_blocks, num_kv_heads, block_size, head_size]
+ *                              TLB_FLOAT8_E4M3 or TLB_INT8
+ *   key_scales, value_scales : [num_blocks, num_kv_heads, block_size] bytes, one
+ *                              per row: byte b stands for the scale 2^(b - 127)
+ *                              (1 .. 254; 0 reads as a scale of 0, 255 is not
+ *                              a scale)
+ *
+ * A row x is stored as round_to_nearest_even(x_i / 2^E), 2^E the smallest power
+ * of two with max|x| <= 448 * 2^E (e4m3) or 127 * 2^E (int8), E in [-126, 127].
+ * The maximum is over the finite values; infinities saturate, NaN stays NaN
+ * in e4m3 and is stored as 0 in int8.
+ *
+ * tlb_reshape_and_cache_quantized writes rows at their slots, as
+ * tlb_reshape_and_cache does (negative slots skipped, slots outside the cache
+ * skipped and flagged). The slots of one call must differ: of a row that two
+ * tokens write, data and scale may come from different ones.
+ *   key, value : [num_tokens, num_kv_heads, head_size] of dtype (fp16, bf16,
+ *                fp32); key_stride / value_stride elements between tokens
+ *
+ * tlb_dequantize_blocks reads blocks back: out[n] = the values of block
+ * block_ids[n], [num_ids, num_kv_heads, block_size, head_size] of dtype, zeros
+ * for ids < 0 or outside the cache (the latter flagged,
+ * TLB_STATUS_BAD_BLOCK_ID).
+ * ---------------------------------------------------------------------- */
+TLB_API int tlb_reshape_and_cache_quantized(const void* key, const void* value, void* key_cache,
+                        void* value_cache, void* key_scales, void* value_scales,
+                        const void* slots, int slot_dtype, int64_t num_tokens,
+                        int64_t num_kv_heads, int64_t head_size, int64_t num_blocks,
+                        int64_t block_size, int64_t key_stride, int64_t value_stride,
+                        int dtype, int cache_dtype, void* stream);
+
+TLB_API int tlb_dequantize_blocks(void* key_out, void* value_out, const void* key_cache,
+                        const void* value_cache, const void* key_scales,
+                        const void* value_scales, const void* block_ids, int id_dtype,
+                        int64_t num_ids, int64_t num_kv_heads, int64_t head_size,
+                        int64_t num_blocks, int64_t block_size, int dtype,
+                        int cache_dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * RMS norm of each query and key head, the NeoX rotation, and the KV-cache
+ * write, in one pass (no reference counterpart; the rotation and the write are
+ * those of tlb_rotary_embedding_neox and its _with_cache form).
+ *
+ * For each head row x of query and key: y_i = x_i * rsqrt(mean(x^2) + eps) *
+ * w_i, then the pairs (i, i + rot_dim/2) are rotated, in fp32 with one rounding
+ * to dtype. Neither query nor key is modified.
+ *   query_weight, key_weight : [head_size] of dtype
+ *   query_out : [num_tokens, num_heads * head_size] dense
+ *   key_cache == NULL: the key goes to key_out [num_tokens, num_kv_heads *
+ *     head_size] dense; value and the cache arguments are not used.
+ *   key_cache != NULL: key and value go to their rows of the caches (slots, or
+ *     positions and block_tables when slots is NULL, as tlb_rotary_embedding_
+ *     neox_with_cache), key_out is not used. cache_dtype is dtype, or an 8-bit
+ *     type with scales: then the rows stored are those that
+ *     tlb_reshape_and_cache_quantized stores for the rounded key.
+ * Positions outside the table leave the normed row unrotated and set
+ * TLB_STATUS_BAD_POSITION. flags: TLB_ROPE_OVERLAP_PREVIOUS as above (the
+ * norm weights too must not be written by the kernel before).
+ * ---------------------------------------------------------------------- */
+TLB_API int tlb_qk_norm_rotary_embedding_neox(
+    void* query_out, void* key_out, const void* positions, int pos_dtype,
+    const void* query, const void* key, const void* value, const void* query_weight,
+    const void* key_weight, float eps, void* key_cache, void* value_cache,
+    void* key_scales, void* value_scales, const void* slots, int slot_dtype,
+    const int32_t* block_tables, int64_t max_blocks_per_seq, int64_t num_tokens,
+    int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
+    const void* cos_sin_cache, int64_t cache_rows, int64_t rot_dim, int64_t num_blocks,
+    int64_t block_size, int64_t query_stride, int64_t key_stride, int64_t value_stride,
+    int dtype, int cache_dtype, unsigned flags, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged decode attention over 8-bit caches, and with capped, distance-biased
+ * or windowed scores over caches of the query dtype (no reference counterpart;
+ * without these it is tlb_paged_attention).
+ *
+ * Token j of a sequence of L tokens scores, for query head h,
+ *   x = scale * (q . k_j);  x = softcap * tanh(x / softcap) if softcap > 0;
+ *   x += alibi_slopes[h] * (j - (L - 1)) if alibi_slopes is not NULL;
+ * and is seen if j >= L - window (window > 0) and its block id is not
+ * negative. Out is the softmax-weighted sum of the values, zeros when no
+ * token is seen. Sequences longer than the block table hold
+ * max_blocks_per_seq * block_size tokens (TLB_STATUS_SEQ_TOO_LONG).
+ *
+ *   query        : [num_seqs, num_heads, head_dim], rows query_stride apart
+ *   out          : dense
+ *   alibi_slopes : [num_heads] float or NULL
+ *   cache_dtype  : dtype, or TLB_FLOAT8_E4M3 / TLB_INT8 with scales
+ * `workspace`: device scratch of the size that the _workspace_size call gives
+ * for these shapes on this device (16-byte aligned; may be uninitialised, holds
+ * nothing between calls; NULL when the size is 0). Calls that overlap in time
+ * need separate buffers. flags: TLB_ATTN_OVERLAP_PROLOGUE as above.
+ * ---------------------------------------------------------------------- */
+TLB_API int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t num_kv_heads,
+                        int64_t head_dim, int64_t block_size, int dtype,
+                        int cache_dtype, size_t* bytes_out);
+
+TLB_API int tlb_paged_attention_scored(void* out, const void* query, const void* key_cache,
+                        const void* value_cache, const void* key_scales,
+                        const void* value_scales, const int32_t* block_tables,
+                        const int32_t* seq_lens, const float* alibi_slopes,
+                        int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                        int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                        int64_t max_blocks_per_seq, int64_t query_stride, int64_t window,
+                        float scale, float softcap, int dtype, int cache_dtype,
+                        void* workspace, size_t workspace_bytes, unsigned flags,
+                        void* stream);
 
 #ifdef __cplusplus
 }

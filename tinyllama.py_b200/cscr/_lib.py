@@ -25,6 +25,8 @@ DTYPE_CODE = {
     torch.bfloat16: 2,
     torch.int32: 3,
     torch.int64: 4,
+    torch.float8_e4m3fn: 5,
+    torch.int8: 6,
 }
 
 _vp = ctypes.c_void_p
@@ -65,6 +67,19 @@ _PROTOS = {
     "tlb_decode_metadata": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp],
     "tlb_step_metadata": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
                           _vp],
+    "tlb_reshape_and_cache_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64,
+                                        _i64, _i64, _i64, _i64, _i32, _i32, _vp],
+    "tlb_dequantize_blocks": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64,
+                              _i64, _i32, _i32, _vp],
+    "tlb_qk_norm_rotary_embedding_neox": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _vp,
+                                          _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64,
+                                          _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                          _i32, _i32, ctypes.c_uint, _vp],
+    "tlb_paged_attention_scored_workspace_size": [_i64, _i64, _i64, _i64, _i32, _i32,
+                                                  ctypes.POINTER(_sz)],
+    "tlb_paged_attention_scored": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                   _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _i32, _i32, _vp,
+                                   _sz, ctypes.c_uint, _vp],
 }
 _RESTYPES = {"tlb_last_error": ctypes.c_char_p, "tlb_version": ctypes.c_char_p}
 

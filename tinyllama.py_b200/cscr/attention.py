@@ -5,6 +5,12 @@ keeps the signature, keyword names, checks and error messages of
 cscr/attention.cpp:7-48 (bound at :50-56) and returns a new
 ``[num_seqs, num_heads, head_dim]`` tensor, computed asynchronously on the
 current CUDA stream by the sm_100a kernels of libtinyllama_b200.so.
+
+Not in the reference: ``paged_attention_with_rope`` (the decode step in one
+launch), ``paged_prefill_attention`` (prompt chunks),
+``paged_attention_quantized`` (decode over 8-bit caches) and
+``paged_attention_biased`` (decode with capped, distance-biased or windowed
+scores).
 """
 
 from __future__ import annotations
@@ -283,3 +289,146 @@ def paged_prefill_attention(query: torch.Tensor, key_cache: torch.Tensor,
             float(scale), DTYPE_CODE[query.dtype], _lib.stream_of(dev))
         _lib.check(rc)
     return out
+
+
+_CACHE8_TYPES = (torch.float8_e4m3fn, torch.int8)
+_scored_ws_sizes: dict[tuple, int] = {}
+
+
+def _scored_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
+                            dtype: torch.dtype, cache_dtype: torch.dtype,
+                            device_index: int) -> int:
+    key = (num_heads, num_kv_heads, head_dim, block_size, dtype, cache_dtype, device_index)
+    n = _scored_ws_sizes.get(key)
+    if n is None:
+        size = ctypes.c_size_t(0)
+        _lib.check(_lib.load().tlb_paged_attention_scored_workspace_size(
+            num_heads, num_kv_heads, head_dim, block_size, DTYPE_CODE[dtype],
+            DTYPE_CODE[cache_dtype], ctypes.byref(size)))
+        n = _scored_ws_sizes[key] = size.value
+    return n
+
+
+def _paged_attention_scored(query, key_cache, value_cache, key_scales, value_scales, block_tables,
+                            seq_lens, scale, softcap, alibi_slopes, window, overlap_prologue):
+    """Checks shared by the two entry points below, and the launch."""
+    dev = query.device
+    shape, cshape = query.shape, key_cache.shape
+    torch_check(query.is_cuda, "query must be a CUDA tensor")
+    torch_check(key_cache.device == dev and value_cache.device == dev
+                and block_tables.device == dev and seq_lens.device == dev,
+                "all tensors must be on the same CUDA device")
+    torch_check(len(shape) == 3, "query must be [num_seqs, num_heads, head_dim]")
+    torch_check(len(cshape) == 4,
+                "key_cache must be [num_blocks, num_kv_heads, block_size, head_dim]")
+    torch_check(value_cache.shape == cshape, "value_cache must have the same shape as key_cache")
+    num_seqs, num_heads, head_dim = shape
+    num_blocks, num_kv_heads, block_size, cache_head_dim = cshape
+    torch_check(num_seqs > 0, "query must contain at least one sequence")
+    torch_check(head_dim == cache_head_dim, "query head_dim must match the cache head_dim")
+    torch_check(head_dim <= 1024, "head_dim must not exceed 1024")
+    torch_check(num_kv_heads > 0 and num_heads % num_kv_heads == 0,
+                "num_heads must be divisible by num_kv_heads")
+    q_stride = query.stride()
+    torch_check(q_stride[2] == 1 and q_stride[1] == head_dim,
+                "query must hold each sequence's heads contiguously")
+    torch_check(key_cache.is_contiguous() and value_cache.is_contiguous(),
+                "key_cache and value_cache must be contiguous")
+    torch_check(block_tables.dim() == 2 and block_tables.dtype == torch.int32
+                and block_tables.is_contiguous() and block_tables.size(0) == num_seqs,
+                "block_tables must be a contiguous [num_seqs, max_blocks_per_seq] int32 tensor")
+    torch_check(seq_lens.dim() == 1 and seq_lens.dtype == torch.int32 and seq_lens.is_contiguous()
+                and seq_lens.size(0) == num_seqs,
+                "seq_lens must be a contiguous [num_seqs] int32 tensor")
+    dtype, cache_dtype = query.dtype, key_cache.dtype
+    torch_check(dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
+    torch_check(value_cache.dtype == cache_dtype, "key_cache and value_cache must share the same "
+                                                  "dtype")
+    torch_check(softcap >= 0 and softcap < float("inf"),
+                "softcap must be finite and not negative")
+    torch_check(window >= 0, "window must not be negative")
+    slopes = None
+    if alibi_slopes is not None:
+        torch_check(alibi_slopes.device == dev and alibi_slopes.dtype == torch.float32
+                    and alibi_slopes.dim() == 1 and alibi_slopes.size(0) == num_heads
+                    and alibi_slopes.is_contiguous(),
+                    "alibi_slopes must be a contiguous [num_heads] float32 tensor on the query's "
+                    "device")
+        slopes = alibi_slopes.data_ptr()
+    out = torch.empty(shape, dtype=dtype, device=dev)
+    max_blocks = block_tables.size(1)
+    if num_blocks == 0 or block_size == 0 or max_blocks == 0:
+        return out.zero_()  # no cache to read: every softmax is empty
+    if out.numel() == 0:
+        return out
+    with _lib.device_guard(dev):
+        nbytes = _scored_workspace_bytes(num_heads, num_kv_heads, head_dim, block_size, dtype,
+                                         cache_dtype, dev.index)
+        # Scratch of this call alone, from the stream's own pool (or the pool of
+        # the graph being captured): nothing in it outlives the call.
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.check(_lib.load().tlb_paged_attention_scored(
+            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+            key_scales.data_ptr() if key_scales is not None else None,
+            value_scales.data_ptr() if value_scales is not None else None,
+            block_tables.data_ptr(), seq_lens.data_ptr(), slopes, num_seqs, num_heads,
+            num_kv_heads, head_dim, num_blocks, block_size, max_blocks, q_stride[0], window,
+            scale, softcap, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype],
+            ws.data_ptr() if ws is not None else None, nbytes, 1 if overlap_prologue else 0,
+            _lib.stream_of(dev)))
+    return out
+
+
+def paged_attention_quantized(query: torch.Tensor, key_cache: torch.Tensor,
+                              value_cache: torch.Tensor, key_scales: torch.Tensor,
+                              value_scales: torch.Tensor, block_tables: torch.Tensor,
+                              seq_lens: torch.Tensor, scale: float, *, softcap: float = 0.0,
+                              alibi_slopes: torch.Tensor | None = None, window: int = 0,
+                              overlap_prologue: bool = False) -> torch.Tensor:
+    """Paged decode attention over 8-bit caches (not in the reference API).
+
+    As ``paged_attention``, with caches of float8_e4m3fn or int8 and the
+    float8_e8m0fnu scales [num_blocks, num_kv_heads, block_size] of their rows,
+    as ``cscr.cache.reshape_and_cache_quantized`` writes them. query
+    [num_seqs, num_heads, head_dim] in float16, bfloat16 or float32, its rows
+    possibly strided (a part of a fused projection); the result is dense.
+
+    ``softcap``, ``alibi_slopes`` and ``window`` as in ``paged_attention_biased``,
+    ``overlap_prologue`` as in ``paged_attention``.
+    """
+    torch_check(key_cache.dtype in _CACHE8_TYPES,
+                "key_cache must be float8_e4m3fn or int8")
+    rows = key_cache.shape[:-1]
+    torch_check(key_scales.dtype == torch.float8_e8m0fnu
+                and value_scales.dtype == torch.float8_e8m0fnu
+                and key_scales.shape == rows and value_scales.shape == rows
+                and key_scales.is_contiguous() and value_scales.is_contiguous()
+                and key_scales.device == query.device and value_scales.device == query.device,
+                "key_scales and value_scales must be contiguous float8_e8m0fnu tensors "
+                "[num_blocks, num_kv_heads, block_size] on the query's device")
+    return _paged_attention_scored(query, key_cache, value_cache, key_scales, value_scales,
+                                   block_tables, seq_lens, scale, softcap, alibi_slopes, window,
+                                   overlap_prologue)
+
+
+def paged_attention_biased(query: torch.Tensor, key_cache: torch.Tensor,
+                           value_cache: torch.Tensor, block_tables: torch.Tensor,
+                           seq_lens: torch.Tensor, scale: float, *, softcap: float = 0.0,
+                           alibi_slopes: torch.Tensor | None = None, window: int = 0,
+                           overlap_prologue: bool = False) -> torch.Tensor:
+    """Paged decode attention with capped, distance-biased or windowed scores
+    (not in the reference API).
+
+    As ``paged_attention``; the score of token j of a sequence of L tokens for
+    query head h is ``x = scale * (q . k_j)``, then
+    ``softcap * tanh(x / softcap)`` when ``softcap > 0``, plus
+    ``alibi_slopes[h] * (j - (L - 1))`` when ``alibi_slopes`` ([num_heads]
+    float32) is given; only the last ``window`` tokens are seen when
+    ``window > 0`` (their blocks alone are read). A sequence with no token
+    to see yields zeros.
+    """
+    torch_check(key_cache.dtype == query.dtype,
+                "query, key_cache and value_cache must share the same dtype")
+    return _paged_attention_scored(query, key_cache, value_cache, None, None, block_tables,
+                                   seq_lens, scale, softcap, alibi_slopes, window,
+                                   overlap_prologue)

@@ -12,6 +12,9 @@
 * ``write_kv_cache(key, value, positions, key_cache, value_cache,
   block_tables)`` is that write addressed exactly as the reference addresses
   it (block_tables[row, position // block_size]), without its host sync.
+* ``reshape_and_cache_quantized`` and ``dequantize_blocks`` (not in the
+  reference) write rows into 8-bit caches with a power-of-two scale each, and
+  read blocks of them back.
 """
 
 from __future__ import annotations
@@ -206,3 +209,130 @@ def write_kv_cache(key: torch.Tensor, value: torch.Tensor, positions: torch.Tens
             pos.data_ptr(), DTYPE_CODE[pos.dtype], bt.data_ptr(), bt.size(1), T, kvh, head_size,
             num_blocks, block_size, k2.stride(0), v2.stride(0), DTYPE_CODE[key_cache.dtype],
             _lib.stream_of(dev)))
+
+
+_CACHE8_TYPES = (torch.float8_e4m3fn, torch.int8)
+_FLOAT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def check_quantized_caches(key_cache: torch.Tensor, value_cache: torch.Tensor,
+                           key_scales: torch.Tensor, value_scales: torch.Tensor) -> None:
+    """The shapes and types of an 8-bit cache pair and its scales."""
+    torch_check(key_cache.is_cuda, "cache tensors must be CUDA tensors")
+    dev, shape = key_cache.device, key_cache.shape
+    torch_check(len(shape) == 4,
+                "key_cache must be [num_blocks, num_kv_heads, block_size, head_size]")
+    torch_check(value_cache.shape == shape, "value_cache must have the same shape as key_cache")
+    torch_check(key_cache.dtype in _CACHE8_TYPES, "key_cache must be float8_e4m3fn or int8")
+    torch_check(value_cache.dtype == key_cache.dtype,
+                "key_cache and value_cache must share the same dtype")
+    rows = shape[:-1]
+    torch_check(key_scales.dtype == torch.float8_e8m0fnu
+                and value_scales.dtype == torch.float8_e8m0fnu
+                and key_scales.shape == rows and value_scales.shape == rows,
+                "key_scales and value_scales must be float8_e8m0fnu tensors "
+                "[num_blocks, num_kv_heads, block_size]")
+    torch_check(key_cache.is_contiguous() and value_cache.is_contiguous()
+                and key_scales.is_contiguous() and value_scales.is_contiguous(),
+                "cache tensors must be contiguous")
+    torch_check(value_cache.device == dev and key_scales.device == dev
+                and value_scales.device == dev, "all tensors must be on the same CUDA device")
+
+
+def _token_rows(x: torch.Tensor, num_tokens: int, kvh: int, head_size: int, name: str) -> int:
+    """The stride between the tokens of x ([T, KVH, D] or [T, KVH * D] with each
+    token's heads contiguous)."""
+    if x.dim() == 3:
+        ok = x.shape == (num_tokens, kvh, head_size) and (kvh == 1 or x.stride(1) == head_size)
+    else:
+        ok = x.dim() == 2 and x.shape == (num_tokens, kvh * head_size)
+    torch_check(ok and (x.stride(-1) == 1 or x.numel() == 0),
+                f"{name} must be [num_tokens, num_kv_heads, head_size] or [num_tokens, "
+                "num_kv_heads * head_size] with each token's heads contiguous")
+    return x.stride(0)
+
+
+def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
+                                value_cache: torch.Tensor, key_scales: torch.Tensor,
+                                value_scales: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Quantise key/value rows [T, KVH, D] into 8-bit paged caches at slot_mapping.
+
+    key and value in float16, bfloat16 or float32 (one type), each token's heads
+    contiguous, any stride between tokens. The caches are float8_e4m3fn or int8
+    [num_blocks, KVH, block_size, D], the scales float8_e8m0fnu [num_blocks,
+    KVH, block_size]. A row's scale is the smallest power of two 2^E with
+    ``max|x| <= qmax * 2^E`` (qmax 448 or 127, E in [-126, 127], the maximum over
+    the finite values); its values are ``x / 2^E`` rounded to nearest even,
+    infinities saturated, NaN kept (float8_e4m3fn) or 0 (int8).
+
+    slot = block * block_size + offset; negative slots are skipped. The other
+    slots of a call must differ.
+    """
+    check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
+    dev = key_cache.device
+    torch_check(key.device == dev and value.device == dev and slot_mapping.device == dev,
+                "all tensors must be on the same CUDA device")
+    torch_check(key.dtype in _FLOAT_TYPES and value.dtype == key.dtype,
+                "key and value must share a dtype: float16, bfloat16 or float32")
+    torch_check(slot_mapping.dim() == 1 and slot_mapping.dtype in _INDEX_TYPES
+                and slot_mapping.is_contiguous(),
+                "slot_mapping must be a contiguous [num_tokens] int32 or int64 tensor")
+    num_blocks, kvh, block_size, head_size = key_cache.shape
+    T = slot_mapping.numel()
+    k_stride = _token_rows(key, T, kvh, head_size, "key")
+    v_stride = _token_rows(value, T, kvh, head_size, "value")
+    if T == 0 or key.numel() == 0:
+        return
+    with _lib.device_guard(dev):
+        _lib.check(_lib.load().tlb_reshape_and_cache_quantized(
+            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+            key_scales.data_ptr(), value_scales.data_ptr(), slot_mapping.data_ptr(),
+            DTYPE_CODE[slot_mapping.dtype], T, kvh, head_size, num_blocks, block_size, k_stride,
+            v_stride, DTYPE_CODE[key.dtype], DTYPE_CODE[key_cache.dtype], _lib.stream_of(dev)))
+
+
+def dequantize_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor,
+                      key_scales: torch.Tensor, value_scales: torch.Tensor,
+                      block_ids: torch.Tensor, dtype: torch.dtype,
+                      out: tuple[torch.Tensor, torch.Tensor] | None = None
+                      ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of blocks of 8-bit caches: (key blocks, value blocks), each
+    [N, KVH, block_size, D] of ``dtype`` (float16, bfloat16 or float32).
+
+    block_ids [N] int32 or int64; a negative id (a hole of a block table) yields
+    a block of zeros. A whole table can be passed as ``block_tables.view(-1)``:
+    the result is then a pool in which entry j of row s is block
+    ``s * max_blocks + j``, which ``paged_prefill_attention`` and
+    ``paged_attention`` read. ``out``: two tensors to fill instead of new ones.
+    """
+    check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
+    dev = key_cache.device
+    torch_check(block_ids.device == dev, "all tensors must be on the same CUDA device")
+    torch_check(block_ids.dim() == 1 and block_ids.dtype in _INDEX_TYPES
+                and block_ids.is_contiguous(),
+                "block_ids must be a contiguous [num_ids] int32 or int64 tensor")
+    torch_check(dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
+    num_blocks, kvh, block_size, head_size = key_cache.shape
+    n = block_ids.numel()
+    shape = (n, kvh, block_size, head_size)
+    if out is None:
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty(shape, dtype=dtype, device=dev)
+    else:
+        k, v = out
+        for t in out:
+            torch_check(t.shape == shape and t.dtype == dtype and t.device == dev
+                        and t.is_contiguous(),
+                        "out must be two contiguous [num_ids, num_kv_heads, block_size, head_size] "
+                        "tensors of dtype")
+    if k.numel() == 0:
+        return k, v
+    if num_blocks == 0:
+        return k.zero_(), v.zero_()
+    with _lib.device_guard(dev):
+        _lib.check(_lib.load().tlb_dequantize_blocks(
+            k.data_ptr(), v.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+            key_scales.data_ptr(), value_scales.data_ptr(), block_ids.data_ptr(),
+            DTYPE_CODE[block_ids.dtype], n, kvh, head_size, num_blocks, block_size,
+            DTYPE_CODE[dtype], DTYPE_CODE[key_cache.dtype], _lib.stream_of(dev)))
+    return k, v

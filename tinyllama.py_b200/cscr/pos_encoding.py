@@ -9,6 +9,9 @@ query as a new tensor and rotates ``key`` in place.
 ``rotary_embedding_neox_with_cache`` additionally writes the rotated key and
 the value into the paged KV cache in the same launch (the reference's RoPE
 followed by its KV write, attention.py:151-157).
+
+``qk_norm_rotary_embedding_neox`` and ``..._with_cache`` (not in the reference)
+normalise each query and key head in the same pass.
 """
 
 from __future__ import annotations
@@ -17,6 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import DTYPE_CODE, torch_check
+from .cache import _token_rows, check_quantized_caches
 
 _INDEX_TYPES = (torch.int32, torch.int64)
 
@@ -138,3 +142,146 @@ def rotary_embedding_neox_with_cache(postions: torch.Tensor, query: torch.Tensor
             DTYPE_CODE[query.dtype], 1 if overlap_previous else 0, _lib.stream_of(dev))
         _lib.check(rc)
     return out
+
+
+_CACHE8_TYPES = (torch.float8_e4m3fn, torch.int8)
+
+
+def _check_qk_norm(positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache):
+    dev, dtype = query.device, query.dtype
+    torch_check(query.is_cuda, "query must be a CUDA tensor")
+    torch_check(key.device == dev and positions.device == dev and cos_sin_cache.device == dev
+                and query_weight.device == dev and key_weight.device == dev,
+                "all tensors must be on the same CUDA device")
+    torch_check(dtype in (torch.float16, torch.bfloat16, torch.float32),
+                "dtype must be float16, bfloat16 or float32")
+    torch_check(key.dtype == dtype and cos_sin_cache.dtype == dtype
+                and query_weight.dtype == dtype and key_weight.dtype == dtype,
+                "query, key, cos_sin_cache and the weights must share a dtype")
+    torch_check(positions.dim() == 1 and positions.dtype in _INDEX_TYPES
+                and positions.is_contiguous(),
+                "positions must be a contiguous [num_tokens] int32 or int64 tensor")
+    num_tokens = positions.size(0)
+    torch_check(head_size > 0, "head_size must be positive")
+    for x, name in ((query, "query"), (key, "key")):
+        torch_check(x.dim() == 2 and x.size(0) == num_tokens and x.size(1) > 0
+                    and x.size(1) % head_size == 0 and x.stride(1) == 1,
+                    f"{name} must be [num_tokens, heads * head_size] with unit inner stride")
+    for w in (query_weight, key_weight):
+        torch_check(w.dim() == 1 and w.size(0) == head_size and w.is_contiguous(),
+                    "query_weight and key_weight must be contiguous [head_size] tensors")
+    torch_check(cos_sin_cache.dim() == 2 and cos_sin_cache.is_contiguous()
+                and cos_sin_cache.size(0) > 0,
+                "cos_sin_cache must be a contiguous [rows, rotary_dim] tensor")
+    rot_dim = cos_sin_cache.size(1)
+    torch_check(rot_dim > 0 and rot_dim % 2 == 0, "rotary dimension must be even and positive")
+    torch_check(rot_dim <= head_size, "rotary dimension must not exceed head_size")
+    torch_check(eps >= 0, "eps must not be negative")
+    return num_tokens, rot_dim
+
+
+def qk_norm_rotary_embedding_neox(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
+                                  query_weight: torch.Tensor, key_weight: torch.Tensor,
+                                  eps: float, head_size: int, cos_sin_cache: torch.Tensor
+                                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of each query and key head, then the NeoX rotation, in one pass.
+
+    For each head row x: ``y = x * rsqrt(mean(x^2) + eps) * weight``, then the
+    pairs (i, i + rotary_dim / 2) are rotated by their token's cos_sin_cache row;
+    fp32 math, one rounding. query [T, H * head_size] and key [T, KVH *
+    head_size], rows possibly strided (parts of a fused projection); weights
+    [head_size]. Returns new dense (query, key); the inputs are left as they are.
+    """
+    num_tokens, rot_dim = _check_qk_norm(positions, query, key, query_weight, key_weight, eps,
+                                         head_size, cos_sin_cache)
+    dev = query.device
+    q_out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+    k_out = torch.empty(key.shape, dtype=key.dtype, device=dev)
+    if num_tokens == 0:
+        return q_out, k_out
+    code = DTYPE_CODE[query.dtype]
+    with _lib.device_guard(dev):
+        _lib.check(_lib.load().tlb_qk_norm_rotary_embedding_neox(
+            q_out.data_ptr(), k_out.data_ptr(), positions.data_ptr(), DTYPE_CODE[positions.dtype],
+            query.data_ptr(), key.data_ptr(), None, query_weight.data_ptr(),
+            key_weight.data_ptr(), eps, None, None, None, None, None, 4, None, 0, num_tokens,
+            query.size(1) // head_size, key.size(1) // head_size, head_size,
+            cos_sin_cache.data_ptr(), cos_sin_cache.size(0), rot_dim, 0, 0, query.stride(0),
+            key.stride(0), 0, code, code, 0, _lib.stream_of(dev)))
+    return q_out, k_out
+
+
+def qk_norm_rotary_embedding_neox_with_cache(
+        positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+        query_weight: torch.Tensor, key_weight: torch.Tensor, eps: float,
+        key_cache: torch.Tensor, value_cache: torch.Tensor, slot_mapping: torch.Tensor | None,
+        head_size: int, cos_sin_cache: torch.Tensor, block_tables: torch.Tensor | None = None, *,
+        key_scales: torch.Tensor | None = None, value_scales: torch.Tensor | None = None,
+        overlap_previous: bool = False) -> torch.Tensor:
+    """``qk_norm_rotary_embedding_neox`` with the KV-cache write of the key and
+    the value in the same launch; returns the new query.
+
+    The key goes to its cache row only; ``key`` and ``value`` are left as they
+    are. value [T, KVH, head_size] or [T, KVH * head_size], rows possibly strided.
+    The caches [num_blocks, KVH, block_size, head_size] have the query dtype, or
+    are float8_e4m3fn or int8 with ``key_scales`` and ``value_scales``
+    (float8_e8m0fnu): then the stored rows are those that
+    ``cscr.cache.reshape_and_cache_quantized`` stores for the key as rounded to
+    the query dtype. Destinations and ``overlap_previous`` as in
+    ``rotary_embedding_neox_with_cache``; the slots of one call must differ.
+    """
+    num_tokens, rot_dim = _check_qk_norm(positions, query, key, query_weight, key_weight, eps,
+                                         head_size, cos_sin_cache)
+    dev, dtype = query.device, query.dtype
+    kvh = key.size(1) // head_size
+    cache_dtype = key_cache.dtype
+    ks_ptr = vs_ptr = None
+    if cache_dtype in _CACHE8_TYPES:
+        torch_check(key_scales is not None and value_scales is not None,
+                    "8-bit caches need key_scales and value_scales")
+        check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
+        ks_ptr, vs_ptr = key_scales.data_ptr(), value_scales.data_ptr()
+    else:
+        torch_check(key_scales is None and value_scales is None,
+                    "key_scales and value_scales belong to 8-bit caches")
+        torch_check(key_cache.dim() == 4 and value_cache.shape == key_cache.shape,
+                    "key_cache and value_cache must be [num_blocks, num_kv_heads, block_size, "
+                    "head_size]")
+        torch_check(cache_dtype == dtype and value_cache.dtype == dtype,
+                    "the caches must have the query dtype, or be float8_e4m3fn or int8")
+        torch_check(key_cache.is_contiguous() and value_cache.is_contiguous(),
+                    "key_cache and value_cache must be contiguous")
+    torch_check(key_cache.device == dev and value_cache.device == dev and value.device == dev,
+                "all tensors must be on the same CUDA device")
+    torch_check(key_cache.size(1) == kvh and key_cache.size(3) == head_size,
+                "cache heads / head_size must match key")
+    torch_check(value.dtype == dtype, "value must have the query dtype")
+    v_stride = _token_rows(value, num_tokens, kvh, head_size, "value")
+    if slot_mapping is not None:
+        torch_check(slot_mapping.device == dev and slot_mapping.dim() == 1
+                    and slot_mapping.size(0) == num_tokens
+                    and slot_mapping.dtype in _INDEX_TYPES and slot_mapping.is_contiguous(),
+                    "slot_mapping must be a contiguous [num_tokens] int32/int64 CUDA tensor")
+        slots, slot_code, tables, width = (slot_mapping.data_ptr(),
+                                           DTYPE_CODE[slot_mapping.dtype], None, 0)
+    else:
+        torch_check(block_tables is not None, "either slot_mapping or block_tables is required")
+        torch_check(block_tables.device == dev and block_tables.dim() == 2
+                    and block_tables.dtype == torch.int32 and block_tables.is_contiguous()
+                    and block_tables.size(0) >= num_tokens and block_tables.size(1) > 0,
+                    "block_tables must be a contiguous int32 CUDA tensor with a row per token")
+        slots, slot_code, tables, width = None, 4, block_tables.data_ptr(), block_tables.size(1)
+    q_out = torch.empty(query.shape, dtype=dtype, device=dev)
+    if num_tokens == 0:
+        return q_out
+    with _lib.device_guard(dev):
+        _lib.check(_lib.load().tlb_qk_norm_rotary_embedding_neox(
+            q_out.data_ptr(), None, positions.data_ptr(), DTYPE_CODE[positions.dtype],
+            query.data_ptr(), key.data_ptr(), value.data_ptr(), query_weight.data_ptr(),
+            key_weight.data_ptr(), eps, key_cache.data_ptr(), value_cache.data_ptr(), ks_ptr,
+            vs_ptr, slots, slot_code, tables, width, num_tokens, query.size(1) // head_size, kvh,
+            head_size, cos_sin_cache.data_ptr(), cos_sin_cache.size(0), rot_dim,
+            key_cache.size(0), key_cache.size(2), query.stride(0), key.stride(0), v_stride,
+            DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype], 1 if overlap_previous else 0,
+            _lib.stream_of(dev)))
+    return q_out

@@ -1,0 +1,371 @@
+// C ABI of the quantised-cache, query/key-norm and scored-attention operators:
+// argument checks, path choice and launches (contract in tinyllama_b200.h).
+#include <cstdarg>
+#include <cstdio>
+#include <initializer_list>
+
+#include "kernels.h"
+#include "tinyllama_b200.h"
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    tlb::set_last_error(buf);
+    return code;
+}
+int cuda_result(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return TLB_OK;
+    return fail(TLB_ERR_CUDA, "launching %s: %s (%s)", what, cudaGetErrorString(e),
+                cudaGetErrorName(e));
+}
+
+#define TLB_REQUIRE(cond, ...)                                           \
+    do {                                                                 \
+        if (!(cond)) return fail(TLB_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
+    } while (0)
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+bool is_float(int dtype) {
+    return dtype == TLB_FLOAT32 || dtype == TLB_FLOAT16 || dtype == TLB_BFLOAT16;
+}
+bool is_8bit(int dtype) { return dtype == TLB_FLOAT8_E4M3 || dtype == TLB_INT8; }
+bool is_index(int dtype) { return dtype == TLB_INT32 || dtype == TLB_INT64; }
+int elem_bytes(int dtype) { return dtype == TLB_FLOAT32 ? 4 : is_8bit(dtype) ? 1 : 2; }
+
+// 16-byte accesses: every listed pointer aligned, every stride a multiple of
+// 16 bytes.
+bool vec_ok(int dtype, std::initializer_list<const void*> ptrs,
+            std::initializer_list<int64_t> strides) {
+    for (const void* p : ptrs)
+        if (p && !aligned(p, 16)) return false;
+    for (int64_t s : strides)
+        if (s * elem_bytes(dtype) % 16) return false;
+    return true;
+}
+
+int cache_checks(const void* key_cache, const void* value_cache, int64_t num_tokens,
+                 int64_t num_kv_heads, int64_t head_size, int64_t num_blocks,
+                 int64_t block_size) {
+    TLB_REQUIRE(num_tokens >= 0, "num_tokens must not be negative");
+    TLB_REQUIRE(num_kv_heads > 0 && head_size > 0 && num_blocks > 0 && block_size > 0,
+                "cache sizes must be positive");
+    TLB_REQUIRE(num_tokens < (1ll << 40) && num_kv_heads < (1 << 16) && head_size < (1 << 16) &&
+                    block_size < (1 << 20) && num_blocks < (1ll << 31) &&
+                    num_kv_heads * block_size < (1ll << 31),
+                "sizes exceed the supported range");
+    TLB_REQUIRE(key_cache && value_cache, "cache pointers must not be null");
+    return TLB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tlb_reshape_and_cache_quantized(const void* key, const void* value, void* key_cache,
+                                    void* value_cache, void* key_scales, void* value_scales,
+                                    const void* slots, int slot_dtype, int64_t num_tokens,
+                                    int64_t num_kv_heads, int64_t head_size, int64_t num_blocks,
+                                    int64_t block_size, int64_t key_stride, int64_t value_stride,
+                                    int dtype, int cache_dtype, void* stream) {
+    TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
+    TLB_REQUIRE(is_8bit(cache_dtype), "cache dtype must be float8_e4m3 or int8");
+    if (int rc = cache_checks(key_cache, value_cache, num_tokens, num_kv_heads, head_size,
+                              num_blocks, block_size))
+        return rc;
+    TLB_REQUIRE(is_index(slot_dtype), "slot_mapping must be int32 or int64");
+    TLB_REQUIRE(key_scales && value_scales, "scale pointers must not be null");
+    if (num_tokens == 0) return TLB_OK;
+    TLB_REQUIRE(key && value && slots, "tensor pointers must not be null");
+    const int e = elem_bytes(dtype);
+    TLB_REQUIRE(aligned(key, e) && aligned(value, e),
+                "tensor pointers must be aligned to the element size");
+    tlb::QuantCacheParams p{};
+    p.key = key;
+    p.value = value;
+    p.key_cache = key_cache;
+    p.value_cache = value_cache;
+    p.key_scales = static_cast<uint8_t*>(key_scales);
+    p.value_scales = static_cast<uint8_t*>(value_scales);
+    p.slots = slots;
+    p.slots64 = slot_dtype == TLB_INT64;
+    p.num_tokens = num_tokens;
+    p.key_stride = key_stride;
+    p.value_stride = value_stride;
+    p.num_blocks = num_blocks;
+    p.num_kv_heads = (int)num_kv_heads;
+    p.head_size = (int)head_size;
+    p.block_size = (int)block_size;
+    // rows of the cache start at multiples of head_size bytes: 8-byte stores
+    const bool vec = head_size % 8 == 0 && vec_ok(dtype, {key, value, key_cache, value_cache},
+                                                  {key_stride, value_stride});
+    return cuda_result(tlb::launch_quantize_write(dtype, cache_dtype, p, vec,
+                                                  reinterpret_cast<cudaStream_t>(stream)),
+                       "reshape_and_cache_quantized");
+}
+
+int tlb_dequantize_blocks(void* key_out, void* value_out, const void* key_cache,
+                          const void* value_cache, const void* key_scales,
+                          const void* value_scales, const void* block_ids, int id_dtype,
+                          int64_t num_ids, int64_t num_kv_heads, int64_t head_size,
+                          int64_t num_blocks, int64_t block_size, int dtype, int cache_dtype,
+                          void* stream) {
+    TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
+    TLB_REQUIRE(is_8bit(cache_dtype), "cache dtype must be float8_e4m3 or int8");
+    if (int rc = cache_checks(key_cache, value_cache, num_ids, num_kv_heads, head_size, num_blocks,
+                              block_size))
+        return rc;
+    TLB_REQUIRE(is_index(id_dtype), "block_ids must be int32 or int64");
+    TLB_REQUIRE(key_scales && value_scales, "scale pointers must not be null");
+    if (num_ids == 0) return TLB_OK;
+    TLB_REQUIRE(key_out && value_out && block_ids, "tensor pointers must not be null");
+    const int e = elem_bytes(dtype);
+    TLB_REQUIRE(aligned(key_out, e) && aligned(value_out, e),
+                "tensor pointers must be aligned to the element size");
+    tlb::DequantParams p{};
+    p.key_out = key_out;
+    p.value_out = value_out;
+    p.key_cache = key_cache;
+    p.value_cache = value_cache;
+    p.key_scales = static_cast<const uint8_t*>(key_scales);
+    p.value_scales = static_cast<const uint8_t*>(value_scales);
+    p.ids = block_ids;
+    p.ids64 = id_dtype == TLB_INT64;
+    p.num_ids = num_ids;
+    p.num_blocks = num_blocks;
+    p.rows_per_block = (int)(num_kv_heads * block_size);
+    p.head_size = (int)head_size;
+    const bool vec =
+        head_size % 16 == 0 && vec_ok(dtype, {key_out, value_out, key_cache, value_cache}, {});
+    return cuda_result(tlb::launch_dequantize_blocks(dtype, cache_dtype, p, vec,
+                                                     reinterpret_cast<cudaStream_t>(stream)),
+                       "dequantize_blocks");
+}
+
+int tlb_qk_norm_rotary_embedding_neox(
+    void* query_out, void* key_out, const void* positions, int pos_dtype, const void* query,
+    const void* key, const void* value, const void* query_weight, const void* key_weight,
+    float eps, void* key_cache, void* value_cache, void* key_scales, void* value_scales,
+    const void* slots, int slot_dtype, const int32_t* block_tables, int64_t max_blocks_per_seq,
+    int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
+    const void* cos_sin_cache, int64_t cache_rows, int64_t rot_dim, int64_t num_blocks,
+    int64_t block_size, int64_t query_stride, int64_t key_stride, int64_t value_stride, int dtype,
+    int cache_dtype, unsigned flags, void* stream) {
+    TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
+    TLB_REQUIRE(is_index(pos_dtype), "positions must be int32 or int64");
+    TLB_REQUIRE((flags & ~TLB_ROPE_OVERLAP_PREVIOUS) == 0, "unknown flags");
+    TLB_REQUIRE(num_tokens >= 0 && num_heads > 0 && num_kv_heads > 0 && head_size > 0,
+                "sizes must be positive");
+    TLB_REQUIRE(num_tokens < (1ll << 40) && num_heads < (1 << 16) && num_kv_heads < (1 << 16) &&
+                    head_size < (1 << 16),
+                "sizes exceed the supported range");
+    TLB_REQUIRE(rot_dim > 0 && rot_dim % 2 == 0, "rotary dimension must be even and positive");
+    TLB_REQUIRE(rot_dim <= head_size, "rotary dimension must not exceed head_size");
+    TLB_REQUIRE(cache_rows > 0, "cos_sin_cache must have at least one row");
+    TLB_REQUIRE(eps >= 0.f, "eps must not be negative");
+    const bool with_cache = key_cache != nullptr;
+    if (with_cache) {
+        TLB_REQUIRE(cache_dtype == dtype || is_8bit(cache_dtype),
+                    "the caches must have the query dtype, or be float8_e4m3 or int8");
+        if (int rc = cache_checks(key_cache, value_cache, num_tokens, num_kv_heads, head_size,
+                                  num_blocks, block_size))
+            return rc;
+        TLB_REQUIRE(!is_8bit(cache_dtype) || (key_scales && value_scales),
+                    "8-bit caches need key_scales and value_scales");
+        if (slots) {
+            TLB_REQUIRE(is_index(slot_dtype), "slot_mapping must be int32 or int64");
+        } else {
+            TLB_REQUIRE(block_tables && max_blocks_per_seq > 0,
+                        "either slots or block_tables must be given");
+            TLB_REQUIRE(max_blocks_per_seq < (1ll << 31), "sizes exceed the supported range");
+        }
+    }
+    if (num_tokens == 0) return TLB_OK;
+    TLB_REQUIRE(query_out && query && key && positions && cos_sin_cache && query_weight &&
+                    key_weight && (with_cache ? value != nullptr : key_out != nullptr),
+                "tensor pointers must not be null");
+    const int e = elem_bytes(dtype);
+    for (const void* q : {(const void*)query_out, (const void*)key_out, query, key, value,
+                          query_weight, key_weight, cos_sin_cache})
+        TLB_REQUIRE(aligned(q, e), "tensor pointers must be aligned to the element size");
+    tlb::QuantCacheParams p{};
+    p.out = query_out;
+    p.key_out = key_out;
+    p.positions = positions;
+    p.positions64 = pos_dtype == TLB_INT64;
+    p.query = query;
+    p.key = key;
+    p.value = value;
+    p.query_weight = query_weight;
+    p.key_weight = key_weight;
+    p.cos_sin = cos_sin_cache;
+    p.key_cache = key_cache;
+    p.value_cache = value_cache;
+    p.key_scales = static_cast<uint8_t*>(key_scales);
+    p.value_scales = static_cast<uint8_t*>(value_scales);
+    p.slots = slots;
+    p.slots64 = slot_dtype == TLB_INT64;
+    p.block_tables = block_tables;
+    p.max_blocks = (int)max_blocks_per_seq;
+    p.cache_rows = cache_rows;
+    p.num_tokens = num_tokens;
+    p.query_stride = query_stride;
+    p.key_stride = key_stride;
+    p.value_stride = value_stride;
+    p.num_blocks = num_blocks;
+    p.num_heads = (int)num_heads;
+    p.num_kv_heads = (int)num_kv_heads;
+    p.head_size = (int)head_size;
+    p.rot_dim = (int)rot_dim;
+    p.block_size = with_cache ? (int)block_size : 1;
+    p.eps = eps;
+    p.overlap = (flags & TLB_ROPE_OVERLAP_PREVIOUS) != 0;
+    const bool vec = head_size % 16 == 0 && rot_dim % 16 == 0 &&
+                     vec_ok(dtype,
+                            {query_out, key_out, query, key, value, query_weight, key_weight,
+                             cos_sin_cache, key_cache, value_cache},
+                            {query_stride, key_stride, with_cache ? value_stride : 0});
+    return cuda_result(tlb::launch_qk_norm_rope(dtype, with_cache ? cache_dtype : dtype, p, vec,
+                                                reinterpret_cast<cudaStream_t>(stream)),
+                       "qk_norm_rotary_embedding_neox");
+}
+
+}  // extern "C"
+
+namespace {
+
+// Least cost points (tiles) of a warp's range before another CTA joins.
+constexpr int kMinCost = 1;
+
+int sm_count(int* sms) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+    return cuda_result(e, "paged attention (device query)");
+}
+
+}  // namespace
+
+extern "C" {
+
+int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t num_kv_heads,
+                                              int64_t head_dim, int64_t block_size, int dtype,
+                                              int cache_dtype, size_t* bytes_out) {
+    TLB_REQUIRE(bytes_out != nullptr, "bytes_out must not be null");
+    TLB_REQUIRE(num_heads > 0 && num_kv_heads > 0 && head_dim > 0 && block_size > 0,
+                "sizes must be positive");
+    TLB_REQUIRE(num_heads % num_kv_heads == 0, "num_heads must be divisible by num_kv_heads");
+    *bytes_out = 0;
+    if (!tlb::scored::fast_supported(dtype, cache_dtype, (int)head_dim, (int)block_size))
+        return TLB_OK;
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    *bytes_out =
+        tlb::scored::workspace_layout((int)(num_heads / num_kv_heads), (int)head_dim, sms).total;
+    return TLB_OK;
+}
+
+int tlb_paged_attention_scored(void* out, const void* query, const void* key_cache,
+                               const void* value_cache, const void* key_scales,
+                               const void* value_scales, const int32_t* block_tables,
+                               const int32_t* seq_lens, const float* alibi_slopes,
+                               int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                               int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                               int64_t max_blocks_per_seq, int64_t query_stride, int64_t window,
+                               float scale, float softcap, int dtype, int cache_dtype,
+                               void* workspace, size_t workspace_bytes, unsigned flags,
+                               void* stream) {
+    TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
+    TLB_REQUIRE(cache_dtype == dtype || is_8bit(cache_dtype),
+                "the caches must have the query dtype, or be float8_e4m3 or int8");
+    TLB_REQUIRE((flags & ~TLB_ATTN_OVERLAP_PROLOGUE) == 0, "unknown flags");
+    TLB_REQUIRE(num_seqs > 0, "query must contain at least one sequence");
+    TLB_REQUIRE(num_heads > 0 && num_kv_heads > 0 && head_dim > 0 && num_blocks > 0 &&
+                    block_size > 0 && max_blocks_per_seq > 0,
+                "sizes must be positive");
+    TLB_REQUIRE(num_heads % num_kv_heads == 0, "num_heads must be divisible by num_kv_heads");
+    TLB_REQUIRE(head_dim <= 1024, "head_dim must not exceed 1024");
+    TLB_REQUIRE(num_heads < (1 << 16) && num_seqs * num_heads < (1ll << 31) &&
+                    block_size < (1ll << 24) && max_blocks_per_seq < (1ll << 31) &&
+                    max_blocks_per_seq * block_size < (1ll << 31) - 64 && num_blocks < (1ll << 31),
+                "sizes exceed the supported range");
+    TLB_REQUIRE(window >= 0, "window must not be negative");
+    TLB_REQUIRE(softcap >= 0.f && softcap <= 3.0e38f, "softcap must be finite and not negative");
+    TLB_REQUIRE(out && query && key_cache && value_cache && block_tables && seq_lens,
+                "tensor pointers must not be null");
+    TLB_REQUIRE(!is_8bit(cache_dtype) || (key_scales && value_scales),
+                "8-bit caches need key_scales and value_scales");
+    const int e = elem_bytes(dtype), ce = elem_bytes(cache_dtype);
+    TLB_REQUIRE(aligned(query, e) && aligned(out, e) && aligned(key_cache, ce) &&
+                    aligned(value_cache, ce),
+                "tensor pointers must be aligned to the element size");
+    namespace sc = tlb::scored;
+    sc::Params p{};
+    p.out = out;
+    p.query = query;
+    p.key_cache = key_cache;
+    p.value_cache = value_cache;
+    p.key_scales = static_cast<const uint8_t*>(key_scales);
+    p.value_scales = static_cast<const uint8_t*>(value_scales);
+    p.block_tables = block_tables;
+    p.seq_lens = seq_lens;
+    p.alibi_slopes = alibi_slopes;
+    p.num_blocks = num_blocks;
+    p.query_stride = query_stride;
+    p.num_seqs = (int)num_seqs;
+    p.num_heads = (int)num_heads;
+    p.num_kv_heads = (int)num_kv_heads;
+    p.group = (int)(num_heads / num_kv_heads);
+    p.unit_heads = sc::unit_heads_of(p.group);
+    p.head_chunks = (p.group + p.unit_heads - 1) / p.unit_heads;
+    p.units_per_seq = p.num_kv_heads * p.head_chunks;
+    p.head_dim = (int)head_dim;
+    p.block_size = (int)block_size;
+    p.block_shift = -1;
+    for (int i = 0; i < 24; ++i)
+        if (block_size == (1ll << i)) p.block_shift = i;
+    p.max_blocks = (int)max_blocks_per_seq;
+    p.max_tokens = (int)(max_blocks_per_seq * block_size);
+    p.window = window < p.max_tokens ? (int)window : 0;
+    p.min_cost = kMinCost;
+    p.scale = scale;
+    p.cap_log2 = softcap * 1.4426950408889634f;
+    p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    // The tensor-core kernel copies 16-byte pieces of rows and 4-byte pieces of
+    // scales, and numbers cache rows in 32 bits.
+    const bool fast =
+        sc::fast_supported(dtype, cache_dtype, (int)head_dim, (int)block_size) &&
+        aligned(query, 16) && query_stride % 8 == 0 && aligned(key_cache, 16) &&
+        aligned(value_cache, 16) && aligned(key_scales, 4) && aligned(value_scales, 4) &&
+        num_blocks * num_kv_heads < (1ll << 32) / block_size;
+    if (!fast)
+        return cuda_result(sc::launch_generic(dtype, cache_dtype, p, st), "paged attention");
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    const int tt = sc::tile_tokens(cache_dtype);
+    const long long seen = p.window > 0 ? p.window + tt : p.max_tokens;
+    const long long tiles = (seen + tt - 1) / tt * p.units_per_seq * num_seqs;
+    const int ctas = sc::ctas_for(tiles, sms, kMinCost);
+    const sc::Workspace w = sc::workspace_layout(p.group, p.head_dim, ctas);
+    if (workspace == nullptr || workspace_bytes < w.total || !aligned(workspace, 16))
+        return fail(TLB_ERR_WORKSPACE,
+                    "this call needs a 16-byte aligned workspace of %zu bytes (got %zu)", w.total,
+                    workspace_bytes);
+    char* ws = static_cast<char*>(workspace);
+    p.warp_partials = reinterpret_cast<float4*>(ws + w.warp_partials);
+    p.cta_partials = reinterpret_cast<float4*>(ws + w.cta_partials);
+    p.cta_ml = reinterpret_cast<float2*>(ws + w.cta_ml);
+    p.cta_ids = reinterpret_cast<int2*>(ws + w.cta_ids);
+    const bool overlap = (flags & TLB_ATTN_OVERLAP_PROLOGUE) != 0;
+    cudaError_t err = cache_dtype == TLB_FLOAT8_E4M3 ? sc::launch_e4m3(dtype, p, ctas, overlap, st)
+                      : cache_dtype == TLB_INT8      ? sc::launch_int8(dtype, p, ctas, overlap, st)
+                                                : sc::launch_16bit(dtype, p, ctas, overlap, st);
+    return cuda_result(err, "paged attention");
+}
+
+}  // extern "C"

@@ -179,6 +179,124 @@ cudaError_t launch_prefill_attention(int dtype, int head_dim, void* out, const v
 // or a 64-row part of one), 0 when the block size needs the cp.async loader.
 int prefill_box_rows(int block_size);
 
+// ------------------------------------------------- quantised cache rows
+// Arguments of the quantising cache write and of the query / key norm with
+// rotation (the fields its name does not need stay null).
+struct QuantCacheParams {
+    void* out;                 // normed, rotated query [tokens, heads, D]
+    void* key_out;             // the key likewise, when no cache is written
+    const void* positions;
+    const void* query;
+    const void* key;
+    const void* value;
+    const void* query_weight;  // [D]
+    const void* key_weight;
+    const void* cos_sin;
+    void* key_cache;
+    void* value_cache;
+    uint8_t* key_scales;       // exponent bytes [blocks, kv_heads, block_size] (8-bit caches)
+    uint8_t* value_scales;
+    const void* slots;         // slot mapping, or null with block_tables
+    const int32_t* block_tables;
+    long long cache_rows;
+    long long num_tokens;
+    long long query_stride, key_stride, value_stride;
+    long long num_blocks;
+    int max_blocks;
+    int num_heads;
+    int num_kv_heads;
+    int head_size;
+    int rot_dim;
+    int block_size;
+    float eps;
+    bool positions64, slots64;
+    bool overlap;              // launched with programmatic stream serialization
+};
+struct DequantParams {
+    void* key_out;
+    void* value_out;
+    const void* key_cache;
+    const void* value_cache;
+    const uint8_t* key_scales;
+    const uint8_t* value_scales;
+    const void* ids;
+    long long num_ids;
+    long long num_blocks;
+    int rows_per_block;        // kv_heads * block_size
+    int head_size;
+    bool ids64;
+};
+// `vec`: pointers, strides and row widths allow 16-byte accesses.
+cudaError_t launch_quantize_write(int dtype, int cache_dtype, const QuantCacheParams& p, bool vec,
+                                  cudaStream_t stream);
+cudaError_t launch_dequantize_blocks(int out_dtype, int cache_dtype, const DequantParams& p,
+                                     bool vec, cudaStream_t stream);
+// cache_dtype: an 8-bit type, or the dtype itself (also when no cache is written).
+cudaError_t launch_qk_norm_rope(int dtype, int cache_dtype, const QuantCacheParams& p, bool vec,
+                                cudaStream_t stream);
+
+// ------------------------------------------------- scored decode attention
+namespace scored {
+
+struct Params {
+    void* out;
+    const void* query;
+    const void* key_cache;
+    const void* value_cache;
+    const uint8_t* key_scales;    // exponent bytes, null for 16-bit / fp32 caches
+    const uint8_t* value_scales;
+    const int32_t* block_tables;
+    const int32_t* seq_lens;
+    const float* alibi_slopes;    // [num_heads] or null
+    float4* warp_partials;        // [ctas][warps][fragments]
+    float4* cta_partials;         // [2 * ctas][fragments]
+    float2* cta_ml;               // [2 * ctas][unit heads padded] (reference, sum)
+    int2* cta_ids;                // [2 * ctas] (unit or -1, flags)
+    long long num_blocks;
+    long long query_stride;       // elements between sequences' query rows
+    int num_seqs;
+    int num_heads;
+    int num_kv_heads;
+    int group;                    // query heads per kv head
+    int unit_heads;               // query heads of a unit: min(group, 16)
+    int head_chunks;              // units per kv head
+    int units_per_seq;
+    int head_dim;
+    int block_size;
+    int block_shift;              // log2(block_size), -1 when it is no power of two
+    int max_blocks;
+    int max_tokens;               // max_blocks * block_size
+    int window;                   // tokens the query sees, 0: all
+    int min_cost;                 // least cost points of a warp's range
+    float scale;
+    float cap_log2;               // softcap * log2(e), 0: none
+    float inv_cap;
+
+    __host__ __device__ int block_of(int pos) const {
+        return block_shift >= 0 ? pos >> block_shift : pos / block_size;
+    }
+};
+
+// Whether the tensor-core kernel serves these (aligned tensors assumed).
+bool fast_supported(int dtype, int cache_dtype, int head_dim, int block_size);
+// Bytes of the four workspace arrays for `ctas` CTAs.
+struct Workspace {
+    size_t warp_partials, cta_partials, cta_ml, cta_ids, total;
+};
+Workspace workspace_layout(int group, int head_dim, int ctas);
+int unit_heads_of(int group);
+// Tokens of a tile; CTAs worth launching for at most `max_tiles` tiles.
+int tile_tokens(int cache_dtype);
+int ctas_for(long long max_tiles, int sms, int min_cost);
+
+cudaError_t launch_e4m3(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream);
+cudaError_t launch_int8(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream);
+cudaError_t launch_16bit(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream);
+// Any shape and type, one CTA per (sequence, query head).
+cudaError_t launch_generic(int dtype, int cache_dtype, const Params& p, cudaStream_t stream);
+
+}  // namespace scored
+
 // ------------------------------------------------------------ block copies
 constexpr int kCopyMaxCaches = 128;
 constexpr int kCopyMaxPairs = 1024;

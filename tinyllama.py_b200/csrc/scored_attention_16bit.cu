@@ -1,0 +1,15 @@
+// Decode attention with capped, biased or windowed scores over 16-bit caches
+// (scored_attention.cuh).
+#include "scored_attention.cuh"
+
+namespace tlb {
+namespace scored {
+
+cudaError_t launch_16bit(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream) {
+    return dtype == TLB_BFLOAT16
+               ? launch_fast_shape<__nv_bfloat16, __nv_bfloat16>(p, p.head_dim, ctas, overlap, stream)
+               : launch_fast_shape<__half, __half>(p, p.head_dim, ctas, overlap, stream);
+}
+
+}  // namespace scored
+}  // namespace tlb

@@ -1,0 +1,14 @@
+// Decode attention over int8 caches (scored_attention.cuh).
+#include "scored_attention.cuh"
+
+namespace tlb {
+namespace scored {
+
+cudaError_t launch_int8(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream) {
+    return dtype == TLB_BFLOAT16
+               ? launch_fast_shape<__nv_bfloat16, int8_t>(p, p.head_dim, ctas, overlap, stream)
+               : launch_fast_shape<__half, int8_t>(p, p.head_dim, ctas, overlap, stream);
+}
+
+}  // namespace scored
+}  // namespace tlb
