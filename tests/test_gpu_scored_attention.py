@@ -261,6 +261,24 @@ def test_two_captured_graphs_run_at_once():
     assert bool((outs[0] == 0).all())
 
 
+@pytest.mark.parametrize("kind", [E4M3, BF16], ids=short)
+def test_a_wait_that_gives_up_is_reported(kind):
+    """With no probes allowed every tile wait gives up: the kernel ends, the status
+    says so, and the next call is whole."""
+    c = Case([3000, 40, 700], 16, 2, 128, 16, BF16, kind, seed=16)
+    want = c.run()
+    torch.cuda.synchronize()
+    try:
+        _lib.set_wait_limit(0)
+        c.run()
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_wait_limit(_lib.WAIT_LIMIT_DEFAULT)
+    assert _lib.device_status() == 0x10
+    assert torch.equal(c.run(), want)
+    assert _lib.device_status() == 0
+
+
 def test_refusals():
     c = Case([10], 4, 2, 64, 16, F16, INT8)
     with pytest.raises(RuntimeError, match="alibi_slopes"):

@@ -205,6 +205,8 @@ WsLayout ws_layout(int64_t num_seqs, int64_t num_kv_heads, int64_t head_dim, int
 }  // namespace
 
 void tlb::set_last_error(const char* msg) { g_last_error = msg ? msg : ""; }
+void* tlb::tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
+unsigned tlb::attention_wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }
 
 extern "C" {
 

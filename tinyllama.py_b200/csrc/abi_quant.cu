@@ -4,6 +4,8 @@
 #include <cstdio>
 #include <initializer_list>
 
+#include <cudaTypedefs.h>
+
 #include "kernels.h"
 #include "tinyllama_b200.h"
 
@@ -241,6 +243,27 @@ namespace {
 // Least cost points (tiles) of a warp's range before another CTA joins.
 constexpr int kMinCost = 1;
 
+// A cache as a 2-D tensor of bytes-or-halves {head_dim, rows}, read in boxes of
+// {128 bytes or a whole shorter row, 2^box_shift rows}. Encoded for each call
+// (under a microsecond): nothing is kept by address.
+int cache_map(const void* base, int64_t rows, int head_dim, int bytes, int box_shift,
+              CUtensorMap* out) {
+    auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tlb::tensor_map_encoder());
+    if (fn == nullptr) return fail(TLB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const int row = head_dim * bytes, column = row < 128 ? row : 128;
+    cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)row};
+    cuuint32_t box[2] = {(cuuint32_t)(column / bytes), 1u << box_shift};
+    cuuint32_t steps[2] = {1, 1};
+    CUresult r = fn(out, bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                    2, const_cast<void*>(base), dims, strides, box, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    column == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(TLB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return TLB_OK;
+}
+
 int sm_count(int* sms) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -336,21 +359,22 @@ int tlb_paged_attention_scored(void* out, const void* query, const void* key_cac
     p.cap_log2 = softcap * 1.4426950408889634f;
     p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    // The tensor-core kernel copies 16-byte pieces of rows and 4-byte pieces of
-    // scales, and numbers cache rows in 32 bits.
+    // The tensor-core kernel copies rows by TMA, whose coordinates are 32-bit
+    // and whose base is 16-byte aligned, and scales four bytes at a time, and
+    // numbers the tiles of a call (with their charges) in 31 bits.
+    const int tt = sc::tile_tokens((int)head_dim * ce);
+    const long long seen = p.window > 0 ? (long long)p.window + tt : p.max_tokens;
+    const long long tiles = (seen + tt - 1) / tt * p.units_per_seq * num_seqs;
     const bool fast =
         sc::fast_supported(dtype, cache_dtype, (int)head_dim, (int)block_size) &&
         aligned(query, 16) && query_stride % 8 == 0 && aligned(key_cache, 16) &&
         aligned(value_cache, 16) && aligned(key_scales, 4) && aligned(value_scales, 4) &&
-        num_blocks * num_kv_heads < (1ll << 32) / block_size;
+        num_blocks * num_kv_heads < (1ll << 31) / block_size && tiles < (1ll << 30);
     if (!fast)
         return cuda_result(sc::launch_generic(dtype, cache_dtype, p, st), "paged attention");
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
-    const int tt = sc::tile_tokens(cache_dtype);
-    const long long seen = p.window > 0 ? p.window + tt : p.max_tokens;
-    const long long tiles = (seen + tt - 1) / tt * p.units_per_seq * num_seqs;
-    const int ctas = sc::ctas_for(tiles, sms, kMinCost);
+    const int ctas = sc::ctas_for(tiles, p.group, sms, kMinCost);
     const sc::Workspace w = sc::workspace_layout(p.group, p.head_dim, ctas);
     if (workspace == nullptr || workspace_bytes < w.total || !aligned(workspace, 16))
         return fail(TLB_ERR_WORKSPACE,
@@ -362,9 +386,16 @@ int tlb_paged_attention_scored(void* out, const void* query, const void* key_cac
     p.cta_ml = reinterpret_cast<float2*>(ws + w.cta_ml);
     p.cta_ids = reinterpret_cast<int2*>(ws + w.cta_ids);
     const bool overlap = (flags & TLB_ATTN_OVERLAP_PROLOGUE) != 0;
-    cudaError_t err = cache_dtype == TLB_FLOAT8_E4M3 ? sc::launch_e4m3(dtype, p, ctas, overlap, st)
-                      : cache_dtype == TLB_INT8      ? sc::launch_int8(dtype, p, ctas, overlap, st)
-                                                : sc::launch_16bit(dtype, p, ctas, overlap, st);
+    p.box_shift = sc::box_shift_of(p.block_size, tt);
+    p.wait_limit = tlb::attention_wait_limit();
+    CUtensorMap tk, tv;
+    const int64_t rows = num_blocks * num_kv_heads * block_size;
+    if (int rc = cache_map(key_cache, rows, p.head_dim, ce, p.box_shift, &tk)) return rc;
+    if (int rc = cache_map(value_cache, rows, p.head_dim, ce, p.box_shift, &tv)) return rc;
+    auto launch = cache_dtype == TLB_FLOAT8_E4M3 ? sc::launch_e4m3
+                  : cache_dtype == TLB_INT8      ? sc::launch_int8
+                                                 : sc::launch_16bit;
+    const cudaError_t err = launch(dtype, p, tk, tv, ctas, overlap, st);
     return cuda_result(err, "paged attention");
 }
 

@@ -10,6 +10,11 @@ namespace tlb {
 // Message returned by tlb_last_error() on this thread (defined in abi.cu).
 void set_last_error(const char* msg);
 
+// The driver's tensor-map encoder (null when it has none) and the probe limit
+// that tlb_attention_set_wait_limit holds (abi.cu).
+void* tensor_map_encoder();
+unsigned attention_wait_limit();
+
 // The argument checks and path choice of tlb_paged_attention, without
 // launching (abi.cu). On TLB_OK, `total` is the workspace the call will use
 // and `zeroed` the prefix that must be zero when it starts; both are 0 when
@@ -238,6 +243,12 @@ cudaError_t launch_qk_norm_rope(int dtype, int cache_dtype, const QuantCachePara
 // ------------------------------------------------- scored decode attention
 namespace scored {
 
+// Warps of a CTA for units of up to `heads` (8 or 16) query heads: their output
+// and query fragments take 168 registers a thread for 8 heads, 255 for 16.
+constexpr int warps_for(int heads) { return heads <= 8 ? 12 : 8; }
+// Tokens of a tile for rows of `bytes`: 4 KB of keys.
+constexpr int tile_tokens(int bytes) { return 4096 / bytes; }
+
 struct Params {
     void* out;
     const void* query;
@@ -268,6 +279,8 @@ struct Params {
     int max_tokens;               // max_blocks * block_size
     int window;                   // tokens the query sees, 0: all
     int min_cost;                 // least cost points of a warp's range
+    int box_shift;                // log2 of the cache rows a TMA box holds
+    unsigned wait_limit;          // mbarrier probes before a wait gives up
     float scale;
     float cap_log2;               // softcap * log2(e), 0: none
     float inv_cap;
@@ -285,13 +298,18 @@ struct Workspace {
 };
 Workspace workspace_layout(int group, int head_dim, int ctas);
 int unit_heads_of(int group);
-// Tokens of a tile; CTAs worth launching for at most `max_tiles` tiles.
-int tile_tokens(int cache_dtype);
-int ctas_for(long long max_tiles, int sms, int min_cost);
+// CTAs worth launching for at most `max_tiles` tiles.
+int ctas_for(long long max_tiles, int group, int sms, int min_cost);
+// log2 of the rows of a TMA box: the largest power of two that divides a block
+// and a tile.
+int box_shift_of(int block_size, int tile);
 
-cudaError_t launch_e4m3(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream);
-cudaError_t launch_int8(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream);
-cudaError_t launch_16bit(int dtype, const Params& p, int ctas, bool overlap, cudaStream_t stream);
+cudaError_t launch_e4m3(int dtype, const Params& p, const CUtensorMap& map_k,
+                        const CUtensorMap& map_v, int ctas, bool overlap, cudaStream_t stream);
+cudaError_t launch_int8(int dtype, const Params& p, const CUtensorMap& map_k,
+                        const CUtensorMap& map_v, int ctas, bool overlap, cudaStream_t stream);
+cudaError_t launch_16bit(int dtype, const Params& p, const CUtensorMap& map_k,
+                         const CUtensorMap& map_v, int ctas, bool overlap, cudaStream_t stream);
 // Any shape and type, one CTA per (sequence, query head).
 cudaError_t launch_generic(int dtype, int cache_dtype, const Params& p, cudaStream_t stream);
 

@@ -1,6 +1,6 @@
 // Decode attention with scored tokens: the path choice's helpers and the kernel
 // for the shapes and types that the tensor-core kernel does not serve (fp32,
-// head dims other than 64 and 128, block sizes that are no multiple of four,
+// head dims other than 64 and 128, block sizes that are no multiple of eight,
 // unaligned tensors).
 #include "scored_attention.cuh"
 
@@ -8,6 +8,8 @@ namespace tlb {
 namespace scored {
 
 namespace {
+
+constexpr int kWarps = 8, kThreads = 256;
 
 // One CTA per (sequence, query head): eight warps take tokens in turn, a lane
 // holds the dims lane + 32 i, everything in fp32. Same scores as the tensor-core
@@ -122,17 +124,19 @@ cudaError_t generic_t(int cache_dtype, const Params& p, cudaStream_t st) {
 bool fast_supported(int dtype, int cache_dtype, int head_dim, int block_size) {
     return (dtype == TLB_FLOAT16 || dtype == TLB_BFLOAT16) &&
            (cache_dtype == dtype || cache_dtype == TLB_INT8 || cache_dtype == TLB_FLOAT8_E4M3) &&
-           (head_dim == 64 || head_dim == 128) && block_size % 4 == 0;
+           (head_dim == 64 || head_dim == 128) && block_size % 8 == 0;
 }
 
 int unit_heads_of(int group) { return group < 16 ? group : 16; }
 
-int tile_tokens(int cache_dtype) {
-    return cache_dtype == TLB_INT8 || cache_dtype == TLB_FLOAT8_E4M3 ? 32 : 16;
+int box_shift_of(int block_size, int tile) {
+    int n = 3;
+    while ((2 << n) <= tile && block_size % (2 << n) == 0) ++n;
+    return n;
 }
 
-int ctas_for(long long max_tiles, int sms, int min_cost) {
-    const long long per = (long long)kWarps * min_cost;
+int ctas_for(long long max_tiles, int group, int sms, int min_cost) {
+    const long long per = (long long)warps_for(unit_heads_of(group)) * min_cost;
     const long long n = (max_tiles + per - 1) / per;
     return (int)(n < 1 ? 1 : n < sms ? n : sms);
 }
@@ -142,7 +146,7 @@ Workspace workspace_layout(int group, int head_dim, int ctas) {
     const size_t frags = (size_t)heads / 8 * (head_dim / 16) * 32 * sizeof(float4);
     Workspace w;
     w.warp_partials = 0;
-    w.cta_partials = (size_t)ctas * kWarps * frags;
+    w.cta_partials = (size_t)ctas * warps_for(heads) * frags;
     w.cta_ml = w.cta_partials + 2 * (size_t)ctas * frags;
     w.cta_ids = w.cta_ml + 2 * (size_t)ctas * heads * sizeof(float2);
     w.total = w.cta_ids + 2 * (size_t)ctas * sizeof(int2);

@@ -10,13 +10,14 @@
 //
 // What bounds it: the stream of cache rows (two flops a byte and query head),
 // so the work is laid out for bytes in flight and even ranges:
-//  * A tile is kTT tokens of one (sequence, kv head): 32 rows of 8-bit values
-//    or 16 of 16-bit ones, 8 KB of keys and values at head_dim 128. The tiles
+//  * A tile is kTT tokens of one (sequence, kv head), 8 KB of keys and values:
+//    16 to 64 rows by their width. The tiles
 //    of all units, with a charge of kUnitCost tiles for starting a unit, form
 //    one line, cut evenly over all warps of the grid (one CTA of 8 warps per
-//    SM). Each warp streams its contiguous part through a ring of its own
-//    (24 KB, cp.async) and never waits for another warp, so units of any mix
-//    of lengths keep every SM busy and a short sequence costs one warp one tile.
+//    SM, kWarps of them each). Each warp streams its contiguous part through a
+//    ring of its own (TMA boxes of a block's rows, scale bytes by cp.async) and
+//    never waits for another warp, so units of any mix of lengths keep every SM
+//    busy and a short sequence costs one warp one tile.
 //  * S^T = K Q^T and O^T += V^T P^T with mma.m16n8k16: the tokens (then the
 //    dims) fill m = 16 and the query heads of the kv head n = 8, so a group of
 //    8 wastes nothing; 8-bit values become fp16 in registers, exactly. bf16
@@ -44,9 +45,6 @@
 namespace tlb {
 namespace scored {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kRingBytes = 24576;  // per warp
 constexpr int kUnitCost = 1;       // tiles charged for starting a unit
 constexpr float kLazy = 8.f;       // log2 of how far a score may pass the reference
 constexpr float kLog2e = 1.4426950408889634f;
@@ -61,12 +59,16 @@ template <typename QT, typename CT, int D, int NT>
 struct Cfg {
     static constexpr int kBytes = sizeof(CT);
     static constexpr bool kQ8 = kBytes == 1;
-    static constexpr int kTT = kQ8 ? 32 : 16;       // tokens per tile
     static constexpr int kRow = D * kBytes;         // bytes per row
+    static constexpr int kTT = tile_tokens(kRow);   // tokens per tile
     static constexpr int kChunks = kRow / 16;
     static constexpr int kHalfStage = kTT * kRow;   // K (or V) bytes of a stage
     static constexpr int kStage = 2 * kHalfStage;
-    static constexpr int kStages = kRingBytes / kStage;
+    static constexpr int kWarps = warps_for(8 * NT);
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kStages = kWarps > 8 ? 2 : 3;
+    static constexpr int kRingBytes = kStages * kStage;  // per warp
+    static constexpr int kColumns = kRow > 128 ? 2 : 1;  // 128-byte columns of a row
     static constexpr int kGroup = 8 * NT;           // heads per unit
     static constexpr int kTiles = D / 16;           // dim tiles
     // float4 fragments of a partial: [nt][dim tile][lane]
@@ -76,32 +78,37 @@ struct Cfg {
     static constexpr bool kSplit = !(kQ8 && std::is_same<QT, __nv_bfloat16>::value);
     // weights are held 2^kLift above the reference where they are fp16
     static constexpr int kLift = kQ8 || std::is_same<QT, __half>::value ? 7 : 0;
-    // shared memory: rings, tile headers, scale bytes, partial (m, l), ids, prefix
-    static constexpr int kHdrOff = kWarps * kRingBytes;
+    // Partials of pieces that end inside a warp's range: the first kParts of a
+    // CTA in shared memory, others in the workspace.
+    static constexpr int kPartBytes = kFrags * 16;
+    static constexpr int kParts = 24576 / kPartBytes;
+    // shared memory
+    static constexpr int kPartOff = kWarps * kRingBytes;
+    static constexpr int kBarOff = kPartOff + kParts * kPartBytes;
+    static constexpr int kHdrOff = kBarOff + (kWarps * kStages * 8 + 15) / 16 * 16;
     static constexpr int kScaleOff = kHdrOff + kWarps * kStages * 16;
-    static constexpr int kMlOff = kScaleOff + (kQ8 ? kWarps * kStages * 64 : 0);
-    static constexpr int kUnitOff = kMlOff + 2 * kWarps * kGroup * 8;
-    static constexpr int kPrefixOff = kUnitOff + 2 * kWarps * 8;
-    static constexpr int kSmem = kPrefixOff + (kThreads + 1) * 8 + 64;
+    static constexpr int kMlOff = kScaleOff + (kQ8 ? kWarps * kStages * 2 * kTT : 0);
+    static constexpr int kWeightOff = kMlOff + 2 * kWarps * kGroup * 8;
+    static constexpr int kUnitOff = kWeightOff + 2 * kWarps * kGroup * 4;
+    static constexpr int kPrefixOff = kUnitOff + 2 * kWarps * 16;
+    static constexpr int kSmem = kPrefixOff + (kThreads + kWarps) * 4 + 1024;  // + alignment slack
+    static_assert(kSmem <= 232448, "one CTA per SM");
 };
 
-// Byte offset of 16-byte chunk c of row r in a tile: rows of a 128-byte line
-// are xor-swizzled so that ldmatrix's eight rows of one chunk hit all banks.
-template <int CH>
+// Byte offset of 16-byte chunk c of row r in a tile, as the TMA boxes leave it:
+// rows of 128 bytes with 128-byte swizzle, 256-byte rows as two such columns,
+// 64-byte rows two to a line with 64-byte swizzle. ldmatrix's eight rows of one
+// chunk then hit all banks.
+template <int CH, int TT>
 __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
-    if constexpr (CH == 4) {  // two 64-byte rows per line
+    if constexpr (CH == 4) {
         const int line = r >> 1;
         return (uint32_t)(line * 128 + (((((r & 1) << 2) | c) ^ (line & 3)) << 4));
     } else {
-        return (uint32_t)(r * CH * 16 + ((c ^ (r & 7)) << 4));
+        return (uint32_t)((c >> 3) * TT * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
     }
 }
 
-__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-                 "l"(reinterpret_cast<uint64_t>(src)), "r"(on ? 16 : 0)
-                 : "memory");
-}
 __device__ __forceinline__ void cp_async_4_zfill(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst),
                  "l"(reinterpret_cast<uint64_t>(src)), "r"(on ? 4 : 0)
@@ -124,8 +131,10 @@ template <typename C> __device__ __forceinline__ void widen_row(uint32_t x, uint
 // 16-bit ldmatrix leaves them -> the token pairs of dim 2g and of dim 2g + 1.
 template <typename C> __device__ __forceinline__ void widen_col(uint32_t x, uint32_t& a, uint32_t& b);
 template <> __device__ __forceinline__ void widen_row<E4M3>(uint32_t x, uint32_t& a, uint32_t& b) {
-    a = e4m3x2_to_half2(x);
-    b = e4m3x2_to_half2(x >> 16);
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(x));
 }
 template <> __device__ __forceinline__ void widen_col<E4M3>(uint32_t x, uint32_t& a, uint32_t& b) {
     widen_row<E4M3>(__byte_perm(x, 0, 0x3120), a, b);
@@ -169,6 +178,11 @@ struct ScoreMod {
 // (-inf: an empty partial).
 __device__ __forceinline__ float piece_weight(float m, float M) {
     return m == -INFINITY ? 0.f : ex2(m - M);
+}
+
+// 1 / the sum of weights; 0 for an empty softmax (NaN stays NaN).
+__device__ __forceinline__ float inverse(float sum) {
+    return sum > 0.f || sum != sum ? __fdividef(1.f, sum) : 0.f;
 }
 
 // Unit u: sequence, kv head and chunk of its query heads.
@@ -218,58 +232,78 @@ __device__ __forceinline__ Span span_of(int s, const Params& p) {
 }
 
 template <typename QT, typename CT, int D, int NT>
-__global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Params p) {
+__global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
+    scored_attention_kernel(const __grid_constant__ CUtensorMap map_k,
+                            const __grid_constant__ CUtensorMap map_v, const Params p) {
     using F = Cfg<QT, CT, D, NT>;
     // element type of the matrix products: 8-bit values become fp16
     using MT = typename std::conditional<F::kQ8, __half, QT>::type;
     constexpr int TT = F::kTT, CH = F::kChunks, ST = F::kStages, G = F::kGroup;
+    constexpr int W = F::kWarps, THREADS = F::kThreads;
     constexpr int MT_TILES = TT / 16;  // 16-token tiles of a stage
-    extern __shared__ __align__(1024) unsigned char smem[];
+    // the swizzled boxes need a 1024-byte aligned base, which nothing promises
+    // of the dynamic array itself
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_base = smem_u32(smem_raw);
+    uint8_t* smem = smem_raw + (((raw_base + 1023u) & ~1023u) - raw_base);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
     int4* hdr = reinterpret_cast<int4*>(smem + F::kHdrOff) + warp * ST;
-    uint8_t* sc = smem + F::kScaleOff + warp * ST * 64;
-    float2* ml = reinterpret_cast<float2*>(smem + F::kMlOff);       // [2 W][G] (m, l)
-    int2* ids = reinterpret_cast<int2*>(smem + F::kUnitOff);        // [2 W] (unit, flags)
-    long long* pre = reinterpret_cast<long long*>(smem + F::kPrefixOff);
-    __shared__ long long wsum[kWarps];
+    uint8_t* sc = smem + F::kScaleOff + warp * ST * 2 * TT;
+    float2* ml = reinterpret_cast<float2*>(smem + F::kMlOff);      // [2 W][G] (m, l)
+    float* wt = reinterpret_cast<float*>(smem + F::kWeightOff);    // [2 W][G] joint weights
+    int4* ids = reinterpret_cast<int4*>(smem + F::kUnitOff);       // [2 W] (unit, flags, part)
+    int* pre = reinterpret_cast<int*>(smem + F::kPrefixOff);       // [THREADS] cost before, in warp
+    int* wsum = pre + THREADS;                                     // [W] cost of a warp's threads
+    __shared__ int parts_used;
+    const uint32_t bars = smem_u32(smem + F::kBarOff) + warp * ST * 8;
+    const uint32_t ring = smem_u32(smem) + warp * F::kRingBytes;
 
     grid_launch_dependents();
     // ---- cost line: thread i holds the sequences [i * per, (i + 1) * per)
-    auto tiles_of = [&](int s) {
+    auto cost_of = [&](int s) {
         const Span sp = span_of(s, p);
-        return sp.len > 0 ? (sp.len + TT - 1) / TT - sp.first / TT : 0;
+        return sp.len > 0
+                   ? ((sp.len + TT - 1) / TT - sp.first / TT + kUnitCost) * p.units_per_seq : 0;
     };
-    const int per = (p.num_seqs + kThreads - 1) / kThreads;
+    const int per = (p.num_seqs + THREADS - 1) / THREADS;
     {
-        long long mine = 0;
-        for (int s = tid * per; s < min((tid + 1) * per, p.num_seqs); ++s) {
-            const int n = tiles_of(s);
-            if (n > 0) mine += (long long)(n + kUnitCost) * p.units_per_seq;
-        }
-        long long inc = mine;
+        int mine = 0;
+        for (int s = tid * per; s < min((tid + 1) * per, p.num_seqs); ++s) mine += cost_of(s);
+        int inc = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
+        pre[tid] = inc - mine;
         if (lane == 31) wsum[warp] = inc;
-        __syncthreads();
-        long long before = 0;
-        for (int w = 0; w < warp; ++w) before += wsum[w];
-        pre[tid] = before + inc - mine;
-        if (tid == kThreads - 1) pre[kThreads] = before + inc;
-        if (tid < 2 * kWarps) ids[tid] = make_int2(-1, 0);
+        if (lane < 2) ids[2 * warp + lane] = make_int4(-1, 0, 0, 0);
+        if (tid == 0) parts_used = 0;
+        if (lane == 0) {
+            prefetch_tensormap(&map_k);
+            prefetch_tensormap(&map_v);
+            for (int i = 0; i < ST; ++i) mbar_init(bars + 8 * i, 1);
+            fence_mbar_init();
+        }
         __syncthreads();
     }
-    const long long total = pre[kThreads];
-    // CTAs that take part: at least kMinTiles tiles' cost per warp
-    const long long want = (total + kWarps * p.min_cost - 1) / (kWarps * p.min_cost);
-    const long long nw = (long long)kWarps * max(1ll, min((long long)gridDim.x, want));
-    const long long wi = (long long)blockIdx.x * kWarps + warp;
+    // lane i: cost before warp i's threads
+    const int own = lane < W ? wsum[lane] : 0;
+    int before = own;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    const unsigned total = __shfl_sync(0xffffffffu, before, W - 1);
+    before -= own;
+    // CTAs that take part: at least min_cost tiles' cost per warp
+    const unsigned nw = W * max(1u, min(gridDim.x, (total + W * p.min_cost - 1) / (W * p.min_cost)));
+    const unsigned wi = blockIdx.x * W + warp;
 
     // ---- cursor of the tile loads
-    int seq = 0, sub = 0, tile = 0, tile_begin = 0, tile_end = 0;
+    int seq = 0, kvh = 0, chunk = 0, tile = 0, tile_begin = 0, tile_end = 0;
     int rel = 0, lim = 0;  // cost points from this warp's range start
     Span span{0, 0};
     auto enter_seq = [&](int s) {
@@ -280,88 +314,99 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
     };
     bool fresh = true;  // next tile starts a piece
     if (wi < nw) {
-        const long long a = total * wi / nw, b = total * (wi + 1) / nw;
-        lim = (int)(b - a);
+        // the range [total * wi / nw, total * (wi + 1) / nw) in 32 bits
+        const unsigned q = total / nw, r = total - q * nw;
+        const unsigned a = q * wi + r * wi / nw;
+        lim = (int)(q * (wi + 1) + r * (wi + 1) / nw - a);
         if (lim > 0) {
-            // the sequence whose costs hold point a
-            int lo = 0, hi = kThreads;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (pre[mid] <= a) lo = mid; else hi = mid;
-            }
-            long long at = pre[lo];
-            int s = lo * per;
-            long long cost;
+            // the sequence whose costs hold point a: the last thread whose cost
+            // before it is at most a (an empty one shares its number with the next)
+            const int w = 31 - __clz(__ballot_sync(0xffffffffu, lane < W && (unsigned)before <= a));
+            const unsigned mine = __shfl_sync(0xffffffffu, before, w) + pre[w * 32 + lane];
+            const int i = 31 - __clz(__ballot_sync(0xffffffffu, mine <= a));
+            unsigned at = a - __shfl_sync(0xffffffffu, mine, i);  // a's place from there
+            int s = (w * 32 + i) * per;
             while (true) {
-                const int n = tiles_of(s);
-                cost = n > 0 ? (long long)(n + kUnitCost) * p.units_per_seq : 0;
-                if (a < at + cost) break;
-                at += cost;
+                const unsigned cost = cost_of(s);
+                if (at < cost) break;
+                at -= cost;
                 ++s;
             }
             enter_seq(s);
-            const int unit_cost = tile_end - tile_begin + kUnitCost;
-            sub = (int)((a - at) / unit_cost);
-            const int off = (int)((a - at) - (long long)sub * unit_cost);
+            const unsigned unit_cost = tile_end - tile_begin + kUnitCost;
+            const int sub = at / unit_cost;
+            const int off = at - sub * unit_cost;
+            kvh = p.head_chunks == 1 ? sub : sub / p.head_chunks;
+            chunk = sub - kvh * p.head_chunks;
             // a unit's tiles sit at the end of its cost points
             const int skip = max(off - kUnitCost, 0);
             tile = tile_begin + skip;
             rel = skip + kUnitCost - off;
         }
     }
-    int bid_next = -1;
+    // Boxes of a tile: box_rows rows (a block or a part of one) each. Lane i
+    // holds the block id of box i of the next tile, and its offset in the block.
+    const int shift = p.box_shift, boxes = TT >> shift;
+    const int32_t* table = p.block_tables + (long long)seq * p.max_blocks;
+    int bid_next = -1, off_next = 0;
     auto fetch_bid = [&]() {
-        // this lane's token of the next tile (tokens of its group of four that
-        // are all outside the context read no table)
         bid_next = -1;
-        if (rel < lim) {
-            const int pos = tile * TT + (lane & (TT - 1));
-            if ((pos & ~3) < span.len)
-                bid_next = p.block_tables[(long long)seq * p.max_blocks + p.block_of(pos)];
+        const int pos = tile * TT + (lane << shift);
+        // a box past the context's end reads no table
+        if (rel < lim && lane < boxes && pos < span.len) {
+            const int b = p.block_of(pos);
+            bid_next = table[b];
+            off_next = pos - b * p.block_size;
         }
     };
-    const unsigned char* kc = reinterpret_cast<const unsigned char*>(p.key_cache);
-    const unsigned char* vc = reinterpret_cast<const unsigned char*>(p.value_cache);
-    const uint32_t ring = smem_u32(smem) + warp * kRingBytes;
+    const uint64_t policy = l2_policy_evict_first();
 
     auto load_tile = [&](int slot) {
         if (rel < lim) {
-            const int r0 = lane & (TT - 1);
-            const int pos = tile * TT + r0;
+            const int pos0 = tile * TT;
             const int bid = bid_next;
-            const bool in_pool = bid >= 0 && bid < p.num_blocks;
-            const bool in_span = pos >= span.first && pos < span.len;
-            if (in_span && bid >= p.num_blocks) flag_status(TLB_STATUS_BAD_BLOCK_ID);
-            const int kvh = sub / p.head_chunks;
-            const uint32_t row = in_pool ? ((uint32_t)bid * p.num_kv_heads + kvh) * p.block_size +
-                                               (pos - p.block_of(pos) * p.block_size)
-                                         : 0u;
-            uint32_t mask = __ballot_sync(0xffffffffu, in_pool && in_span);
-            if constexpr (TT == 16) mask &= 0xffffu;
-            const uint32_t base = ring + slot * F::kStage;
-            constexpr int RPI = 32 / CH;  // rows per instruction
-            const int cc = lane & (CH - 1);
+            const int lo = max(span.first - pos0, 0), hi = min(span.len - pos0, TT);
+            // boxes with a token in the span and a block of the pool
+            const int row0 = lane << shift;
+            const bool overlaps = lane < boxes && row0 < hi && row0 + (1 << shift) > lo;
+            const bool on = overlaps && bid >= 0 && bid < p.num_blocks;
+            if (overlaps && bid >= p.num_blocks) flag_status(TLB_STATUS_BAD_BLOCK_ID);
+            const uint32_t box_mask = __ballot_sync(0xffffffffu, on);
+            // first cache row of this lane's box
+            const int row = on ? (bid * p.num_kv_heads + kvh) * p.block_size + off_next : 0;
+            const uint32_t bar = bars + 8 * slot;
+            if (lane == 0)
+                mbar_arrive_expect_tx(bar, (uint32_t)__popc(box_mask) * 2u * F::kRow << shift);
+            __syncwarp();
+            uint32_t dst = ring + slot * F::kStage;
+            for (int i = 0; i < boxes; ++i) {
+                const int y = __shfl_sync(0xffffffffu, row, i);
+                if (((box_mask >> i) & 1) && elect_one()) {
 #pragma unroll
-            for (int i = 0; i < TT / RPI; ++i) {
-                const int r = i * RPI + lane / CH;
-                const uint64_t off = (uint64_t)__shfl_sync(0xffffffffu, row, r) * F::kRow + cc * 16;
-                const bool on = (mask >> r) & 1;
-                const uint32_t dst = base + tile_offset<CH>(r, cc);
-                cp_async_16_zfill(dst, kc + off, on);
-                cp_async_16_zfill(dst + F::kHalfStage, vc + off, on);
+                    for (int c = 0; c < F::kColumns; ++c) {
+                        const int x = c * (128 / F::kBytes);
+                        tma_load_2d(dst + c * TT * 128, &map_k, x, y, bar, policy);
+                        tma_load_2d(dst + c * TT * 128 + F::kHalfStage, &map_v, x, y, bar, policy);
+                    }
+                }
+                dst += (F::kRow < 128 ? F::kRow : 128) << shift;
             }
             if constexpr (F::kQ8) {
-                // lanes 0-7: four key scales each, lanes 8-15: value scales
-                const uint32_t srow = __shfl_sync(0xffffffffu, row, 4 * (lane & 7));
-                const bool on = (mask >> (4 * (lane & 7))) & 15;
-                if (lane < 16)
-                    cp_async_4_zfill(smem_u32(sc) + slot * 64 + lane * 4,
-                                     (lane < 8 ? p.key_scales : p.value_scales) + srow, on);
+                // four key scales each for the first TT / 4 lanes, value scales next
+                const int tok = 4 * (lane & (TT / 4 - 1)), box = tok >> shift;
+                const int srow = __shfl_sync(0xffffffffu, row, box) + tok - (box << shift);
+                if (lane < TT / 2)
+                    cp_async_4_zfill(smem_u32(sc) + slot * 2 * TT + lane * 4,
+                                     (lane < TT / 4 ? p.key_scales : p.value_scales) + srow,
+                                     (box_mask >> box) & 1);
+                cp_async_commit();
             }
             int flags = (fresh ? kFirst : 0) | (tile == tile_begin ? kUnitBegin : 0) |
                         (tile + 1 == tile_end ? kUnitEnd : 0);
-            const int u = seq * p.units_per_seq + sub;
-            const int pos0 = tile * TT;
+            const int u = seq * p.units_per_seq + kvh * p.head_chunks + chunk;
+            // every token seen: box_mask 0 stands for it
+            const uint32_t seen = box_mask == (1u << boxes) - 1u && lo == 0 && hi == TT
+                                      ? 0u : 1u << 31 | box_mask << 16 | hi << 8 | lo;
             // advance
             fresh = false;
             ++tile;
@@ -369,23 +414,36 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
             if (tile == tile_end) {
                 fresh = true;
                 rel += kUnitCost;
-                if (++sub == p.units_per_seq) {
-                    sub = 0;
-                    if (rel < lim) {
-                        int s = seq + 1;
-                        while (s < p.num_seqs && tiles_of(s) == 0) ++s;
-                        if (s < p.num_seqs) enter_seq(s); else lim = rel;
+                if (++chunk == p.head_chunks) {
+                    chunk = 0;
+                    if (++kvh == p.num_kv_heads) {
+                        kvh = 0;
+                        if (rel < lim) {
+                            int s = seq + 1;
+                            while (s < p.num_seqs && cost_of(s) == 0) ++s;
+                            if (s < p.num_seqs) {
+                                enter_seq(s);
+                                table = p.block_tables + (long long)seq * p.max_blocks;
+                            } else {
+                                lim = rel;
+                            }
+                        }
                     }
                 }
                 tile = tile_begin;
             }
             if (fresh || rel >= lim) flags |= kLast;
-            if (lane == 0) hdr[slot] = make_int4((int)mask, pos0, u, flags);
+            if (lane == 0) hdr[slot] = make_int4((int)seen, pos0, u, flags);
             fetch_bid();
-        } else if (lane == 0) {
-            hdr[slot] = make_int4(0, 0, -1, 0);
+        } else {
+            if (lane == 0) hdr[slot] = make_int4(0, 0, -1, 0);
+            if constexpr (F::kQ8) cp_async_commit();
         }
-        cp_async_commit();
+    };
+    // whether token t of a tile that is not all seen is
+    auto is_seen = [&](uint32_t seen, int t) {
+        return t >= (int)(seen & 255) && t < (int)((seen >> 8) & 255) &&
+               ((seen >> 16) >> (t >> shift)) & 1;
     };
 
     fetch_bid();
@@ -401,20 +459,16 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
     Unit un{0, 0, 0, 0};
     const ScoreMod mod{p.cap_log2, p.inv_cap, p.alibi_slopes != nullptr};
     QT* out = reinterpret_cast<QT*>(p.out);
-    float4* part_a = p.warp_partials + ((long long)blockIdx.x * kWarps + warp) * F::kFrags;
+    float4* part_a = p.warp_partials + ((long long)blockIdx.x * W + warp) * F::kFrags;
 
     int slot = 0;
+    uint32_t parity = 0;
+    bool failed = false;
     while (true) {
-        {
-            int next = slot + ST - 1;
-            if (next >= ST) next -= ST;
-            load_tile(next);
-        }
-        cp_async_wait<ST - 1>();
+        load_tile(slot == 0 ? ST - 1 : slot - 1);
         __syncwarp();
         const int4 h = hdr[slot];
         if (h.z < 0) break;
-        const uint32_t mask = (uint32_t)h.x;
         if (h.w & kFirst) {
             piece_flags = h.w & kUnitBegin;
             un = unit_of(h.z, p);
@@ -425,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
                 const bool there = head < un.heads;
                 const QT* q = reinterpret_cast<const QT*>(p.query) +
                               (long long)un.s * p.query_stride + (long long)(un.head0 + head) * D;
-                float scale_q = p.scale;
+                float scale_q = p.cap_log2 > 0.f ? p.scale : p.scale * kLog2e;
                 if constexpr (F::kQ8) {
                     uint2 raw[F::kTiles];
                     uint32_t top = 0;
@@ -479,6 +533,27 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
             }
         }
         const uint32_t kbase = ring + slot * F::kStage, vbase = kbase + F::kHalfStage;
+        // the tile's rows (bounded: see TLB_STATUS_WAIT_TIMEOUT) and scales
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(bars + 8 * slot, parity, p.wait_limit))) {
+            failed = true;
+            break;
+        }
+        if constexpr (F::kQ8) {
+            cp_async_wait<ST - 1>();
+            __syncwarp();
+        }
+        const uint32_t seen = (uint32_t)h.x;
+        const bool full = seen == 0;
+        if (!full) {
+            // value rows that are not seen may hold anything (0 * NaN): zeros
+            for (int i = lane; i < TT * CH; i += 32)
+                if (!is_seen(seen, i / CH))
+                    *reinterpret_cast<uint4*>(smem + (vbase - smem_u32(smem)) +
+                                              tile_offset<CH, TT>(i / CH, i % CH)) =
+                        make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();  // before a later copy into this slot
+            __syncwarp();
+        }
 
         // ---- S^T = K Q^T
         float s[NT][MT_TILES][4];
@@ -496,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
 #pragma unroll
                     for (int mt = 0; mt < MT_TILES; ++mt) {
                         uint32_t r0, r1, r2, r3;
-                        ldsm_x4(kbase + tile_offset<CH>(mt * 16 + lr, c + lc), r0, r1, r2, r3);
+                        ldsm_x4(kbase + tile_offset<CH, TT>(mt * 16 + lr, c + lc), r0, r1, r2, r3);
                         uint32_t a[4], b[4];
                         widen_row<CT>(r0, a[0], a[2]);
                         widen_row<CT>(r1, a[1], a[3]);
@@ -514,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
 #pragma unroll
                     for (int mt = 0; mt < MT_TILES; ++mt) {
                         uint32_t a[4];
-                        ldsm_x4(kbase + tile_offset<CH>(mt * 16 + lr, 2 * c + lc), a[0], a[1], a[2],
+                        ldsm_x4(kbase + tile_offset<CH, TT>(mt * 16 + lr, 2 * c + lc), a[0], a[1], a[2],
                                 a[3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
@@ -523,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
             }
         }
 
-        // ---- scores in log2 units, weights
+        // ---- scores in log2 units
         float ev[MT_TILES][2];
 #pragma unroll
         for (int mt = 0; mt < MT_TILES; ++mt)
@@ -531,27 +606,52 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
             for (int r = 0; r < 2; ++r) {
                 const int tok = mt * 16 + r * 8 + g;
                 float ks = 1.f;
+                ev[mt][r] = 0.f;
                 if constexpr (F::kQ8) {
-                    ks = scale_value(sc[slot * 64 + tok]);
-                    ev[mt][r] = (float)((int)sc[slot * 64 + 32 + tok] - 127);
-                } else {
-                    ev[mt][r] = 0.f;
+                    ks = scale_value(sc[slot * 2 * TT + tok]);
+                    // byte - 127, through the mantissa of 2^23
+                    ev[mt][r] = __uint_as_float(0x4b000000u | sc[slot * 2 * TT + TT + tok]) - 8388735.f;
                 }
-                const bool seen = (mask >> tok) & 1;
-                const float back = (float)(h.y + tok - last_pos);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
+                    for (int e = 0; e < 2; ++e)
                         // the two scales first: the product of the stored
                         // values is of moderate size, so nothing overflows
                         // that the score itself does not
-                        float x = s[nt][mt][2 * r + e] * (ks * qs[nt][e]);
-                        x = p.cap_log2 > 0.f ? mod.cap(x) : x * kLog2e;
-                        x = fmaf(slope[nt][e], back, x);
-                        s[nt][mt][2 * r + e] = seen ? x : -INFINITY;
-                    }
+                        s[nt][mt][2 * r + e] *= F::kQ8 ? ks * qs[nt][e] : qs[nt][e];
             }
+        if (p.cap_log2 > 0.f) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int mt = 0; mt < MT_TILES; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nt][mt][e] = mod.cap(s[nt][mt][e]);
+        }
+        if (mod.alibi) {
+            const float back = (float)(h.y + g - last_pos);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int mt = 0; mt < MT_TILES; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[nt][mt][e] = fmaf(slope[nt][e & 1], back + (float)(mt * 16 + (e >> 1) * 8),
+                                            s[nt][mt][e]);
+        }
+        if (!full) {
+#pragma unroll
+            for (int mt = 0; mt < MT_TILES; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool on = is_seen(seen, mt * 16 + (e >> 1) * 8 + g);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        s[nt][mt][e] = on ? s[nt][mt][e] : -INFINITY;
+                }
+        }
+        // ---- weights
         bool over = false;
         float cm[NT][2], cv[NT][2];
 #pragma unroll
@@ -639,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
 #pragma unroll
                     for (int c = 0; c < F::kTiles; c += 2) {
                         uint32_t r0, r1, r2, r3;
-                        ldsm_x4_trans(vbase + tile_offset<CH>(mt * 16 + lr, c + lc), r0, r1, r2, r3);
+                        ldsm_x4_trans(vbase + tile_offset<CH, TT>(mt * 16 + lr, c + lc), r0, r1, r2, r3);
                         uint32_t a[4], b[4];
                         widen_col<CT>(r0, a[0], a[1]);
                         widen_col<CT>(r1, a[2], a[3]);
@@ -660,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
                     for (int c = 0; c < F::kTiles; ++c) {
                         // (tokens 0-7, dims 0-7), (tokens 8-15, dims 0-7), then dims 8-15
                         uint32_t a[4];
-                        ldsm_x4_trans(vbase + tile_offset<CH>(mt * 16 + lr, 2 * c + lc), a[0], a[2],
+                        ldsm_x4_trans(vbase + tile_offset<CH, TT>(mt * 16 + lr, 2 * c + lc), a[0], a[2],
                                       a[1], a[3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
@@ -676,14 +776,18 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
             piece_flags |= h.w & kUnitEnd;
             const bool whole = piece_flags == (kUnitBegin | kUnitEnd);
             // the last piece of the range stays in shared memory (the ring is
-            // free: every load has landed), an earlier one goes to the workspace
-            const bool end = rel >= lim && hdr[slot + 1 == ST ? 0 : slot + 1].z < 0;
+            // free: no tile follows), an earlier one goes to the workspace
+            const bool end = hdr[slot + 1 == ST ? 0 : slot + 1].z < 0;
             const int entry = 2 * warp + (end ? 1 : 0);
-            if (end && !whole) {
-                cp_async_wait<0>();
-                __syncwarp();
+            int part = 0;
+            float4* dst = reinterpret_cast<float4*>(smem + warp * F::kRingBytes);
+            if (!end && !whole) {
+                if (lane == 0) part = atomicAdd(&parts_used, 1);
+                part = __shfl_sync(0xffffffffu, part, 0);
+                dst = part < F::kParts
+                          ? reinterpret_cast<float4*>(smem + F::kPartOff + part * F::kPartBytes)
+                          : part_a;
             }
-            float4* dst = end ? reinterpret_cast<float4*>(smem + warp * kRingBytes) : part_a;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float inv[2], fac[2];
@@ -696,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
                     fac[e] = !F::kQ8                  ? 1.f / (1 << F::kLift)
                              : mv[nt][e] == -INFINITY ? 0.f
                                                       : ex2(mv[nt][e] - m[nt][e] - F::kLift);
-                    inv[e] = sum > 0.f || sum != sum ? __fdividef(1.f, sum) : 0.f;
+                    inv[e] = inverse(sum);
                     if (!whole && g == 0)
                         ml[entry * G + nt * 8 + 2 * t4 + e] = make_float2(m[nt][e], sum);
                 }
@@ -710,88 +814,106 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
                         dst[(nt * F::kTiles + i) * 32 + lane] = v;
                 }
             }
-            if (!whole && lane == 0) ids[entry] = make_int2(h.z, piece_flags);
+            if (!whole && lane == 0) ids[entry] = make_int4(h.z, piece_flags, part, 0);
         }
         __syncwarp();
-        if (++slot == ST) slot = 0;
+        if (++slot == ST) {
+            slot = 0;
+            parity ^= 1;
+        }
     }
-    cp_async_wait<0>();
+    if (failed) {
+        // a copy did not arrive in time: report it, give the copies in flight
+        // (this slot's and the following ones') the same time to land, and stop
+        if (lane == 0) {
+            flag_status(TLB_STATUS_WAIT_TIMEOUT);
+            ids[2 * warp] = ids[2 * warp + 1] = make_int4(-1, 0, 0, 0);
+        }
+        for (int i = 0; i < ST; ++i) {
+            if (hdr[slot].z >= 0) mbar_wait_bounded(bars + 8 * slot, parity, kWaitLimit);
+            if (++slot == ST) {
+                slot = 0;
+                parity ^= 1;
+            }
+        }
+    }
+    if constexpr (F::kQ8) cp_async_wait<0>();
     __syncthreads();
 
-    // ---- join the CTA's partials, in range order
-    {
-        const int slot0 = 2 * blockIdx.x;
+    // ---- join the CTA's partials, in range order (entry 2 w: the piece that
+    // ended inside warp w's range, 2 w + 1: the last piece of its range)
+    const uint32_t there = __ballot_sync(0xffffffffu, lane < 2 * W && ids[lane < 2 * W ? lane : 0].x >= 0);
+    if (there) {
+        // weights of all entries: one thread for each entry and head
+        for (int i = tid; i < 2 * W * G; i += THREADS) {
+            const int e = i / G, h = i - e * G, u = ids[e].x;
+            if (u < 0) continue;
+            float M = -INFINITY;
+            for (uint32_t k = there; k; k &= k - 1) {
+                const int x = __ffs(k) - 1;
+                if (ids[x].x == u) M = fmaxf(M, ml[x * G + h].x);
+            }
+            wt[i] = piece_weight(ml[i].x, M);
+        }
+        __syncthreads();
         int2 left = make_int2(-1, 0), right = make_int2(-1, 0);
-        int e0 = 0;
-        while (e0 < 2 * kWarps) {
-            if (ids[e0].x < 0) {
-                ++e0;
-                continue;
-            }
-            const int u = ids[e0].x;
-            int flags = ids[e0].y, e1 = e0 + 1;
-            for (; e1 < 2 * kWarps; ++e1) {
-                if (ids[e1].x < 0) continue;
-                if (ids[e1].x != u) break;
-                flags |= ids[e1].y;
-            }
-            const bool whole = flags == (kUnitBegin | kUnitEnd);
-            const int side = (flags & kUnitBegin) ? 1 : 0;
-            if (!whole) {
-                if (side) right = make_int2(u, flags); else left = make_int2(u, flags);
-            }
-            const Unit w = unit_of(u, p);
-            for (int f = tid; f < F::kFrags; f += kThreads) {
-                const int nt = f / (F::kTiles * 32), fl = f & 31;
-                const int h0 = nt * 8 + 2 * (fl & 3);
-                float M0 = -INFINITY, M1 = -INFINITY;
-                for (int e = e0; e < e1; ++e) {
-                    if (ids[e].x < 0) continue;
-                    M0 = fmaxf(M0, ml[e * G + h0].x);
-                    M1 = fmaxf(M1, ml[e * G + h0 + 1].x);
-                }
-                float L0 = 0.f, L1 = 0.f;
+        for (int f = tid; f < F::kFrags; f += THREADS) {
+            const int nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles, fl = f & 31;
+            const int h0 = nt * 8 + 2 * (fl & 3);
+            for (uint32_t k = there; k;) {
+                const int u = ids[__ffs(k) - 1].x;
+                int flags = 0;
+                float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int e = e0; e < e1; ++e) {
-                    if (ids[e].x < 0) continue;
-                    const float2 a = ml[e * G + h0], b = ml[e * G + h0 + 1];
-                    const float w0 = piece_weight(a.x, M0), w1 = piece_weight(b.x, M1);
-                    const float4* src = (e & 1) ? reinterpret_cast<const float4*>(
-                                                      smem + (e >> 1) * kRingBytes)
-                                                : p.warp_partials + ((long long)blockIdx.x * kWarps +
-                                                                     (e >> 1)) * F::kFrags;
+                for (; k; k &= k - 1) {
+                    const int e = __ffs(k) - 1;
+                    const int4 id = ids[e];
+                    if (id.x != u) break;
+                    flags |= id.y;
+                    const float4* src =
+                        (e & 1) ? reinterpret_cast<const float4*>(smem + (e >> 1) * F::kRingBytes)
+                        : id.z < F::kParts
+                            ? reinterpret_cast<const float4*>(smem + F::kPartOff +
+                                                              id.z * F::kPartBytes)
+                            : p.warp_partials + ((long long)blockIdx.x * W + (e >> 1)) * F::kFrags;
                     const float4 v = src[f];
-                    L0 += w0 * a.y;
-                    L1 += w1 * b.y;
-                    acc.x += w0 * v.x;
-                    acc.y += w1 * v.y;
-                    acc.z += w0 * v.z;
-                    acc.w += w1 * v.w;
+                    const float2 w = *reinterpret_cast<const float2*>(wt + e * G + h0);
+                    const float4 m2 = *reinterpret_cast<const float4*>(ml + e * G + h0);
+                    M0 = fmaxf(M0, m2.x);
+                    M1 = fmaxf(M1, m2.z);
+                    L0 += w.x * m2.y;
+                    L1 += w.y * m2.w;
+                    acc.x += w.x * v.x;
+                    acc.y += w.y * v.y;
+                    acc.z += w.x * v.z;
+                    acc.w += w.y * v.w;
                 }
-                if (whole) {
-                    write_frag<QT, F::kQ8>(out, p, w, D, nt, (f >> 5) % F::kTiles, fl, acc,
-                                           L0 > 0.f || L0 != L0 ? __fdividef(1.f, L0) : 0.f,
-                                           L1 > 0.f || L1 != L1 ? __fdividef(1.f, L1) : 0.f);
+                if (flags == (kUnitBegin | kUnitEnd)) {
+                    write_frag<QT, F::kQ8>(out, p, unit_of(u, p), D, nt, i, fl, acc, inverse(L0),
+                                           inverse(L1));
                 } else {
-                    p.cta_partials[(long long)(slot0 + side) * F::kFrags + f] = acc;
-                    if ((f >> 5) % F::kTiles == 0 && fl < 4) {
-                        p.cta_ml[(slot0 + side) * G + h0] = make_float2(M0, L0);
-                        p.cta_ml[(slot0 + side) * G + h0 + 1] = make_float2(M1, L1);
-                    }
+                    const int side = (flags & kUnitBegin) ? 1 : 0;
+                    const int at = 2 * blockIdx.x + side;
+                    if (side) right = make_int2(u, flags); else left = make_int2(u, flags);
+                    p.cta_partials[(long long)at * F::kFrags + f] = acc;
+                    if (i == 0 && fl < 4)
+                        *reinterpret_cast<float4*>(p.cta_ml + at * G + h0) =
+                            make_float4(M0, L0, M1, L1);
                 }
             }
-            e0 = e1;
         }
         if (tid == 0) {
-            p.cta_ids[slot0] = left;
-            p.cta_ids[slot0 + 1] = right;
+            p.cta_ids[2 * blockIdx.x] = left;
+            p.cta_ids[2 * blockIdx.x + 1] = right;
         }
+    } else if (tid == 0) {
+        p.cta_ids[2 * blockIdx.x] = p.cta_ids[2 * blockIdx.x + 1] = make_int2(-1, 0);
     }
     // ---- sequences with no token: zeros
     for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
         if (p.seq_lens[s] > p.max_tokens && tid == 0) flag_status(TLB_STATUS_SEQ_TOO_LONG);
-        if (tiles_of(s) == 0)
-            for (int i = tid; i < p.num_heads * D; i += kThreads)
+        if (p.seq_lens[s] <= 0)
+            for (int i = tid; i < p.num_heads * D; i += THREADS)
                 out[(long long)s * p.num_heads * D + i] = Elem<QT>::from_f(0.f);
     }
 }
@@ -799,7 +921,9 @@ __global__ void __launch_bounds__(kThreads, 1) scored_attention_kernel(const Par
 // Units that several CTAs share: CTA c takes the unit whose first partial is
 // c's right one; its others are the left partials of the CTAs after c, up to
 // the one that holds the unit's end. blockIdx.y takes a quarter of the
-// fragments; the threads split the partials of a fragment between them.
+// fragments; the threads split the partials of a fragment between them. What
+// the first 32 partials need is loaded before their number is known, so a
+// short join waits for memory once.
 constexpr int kJoinParts = 4;
 
 template <typename QT, bool Q8, int D, int NT>
@@ -807,29 +931,42 @@ __global__ void __launch_bounds__(256) scored_join_kernel(const Params p, int ct
     constexpr int kTiles = D / 16, kFrags = NT * kTiles * 32, G = 8 * NT;
     constexpr int P = kFrags / kJoinParts;  // fragments of this block
     constexpr int LANES = 256 / P;          // threads per fragment
-    static_assert(P <= 256 && 256 % P == 0, "fragments split over the block");
-    __shared__ int last_s;
+    static_assert(P <= 256 && 256 % P == 0 && G % 8 == 0, "fragments split over the block");
     __shared__ float sM[G], sL[G];
     __shared__ float4 red[256];
     const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int f = blockIdx.y * P + tid % P, part = tid / P;
+    auto slot = [&](int i) { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
     grid_dependency_wait();
     const int2 id = p.cta_ids[2 * c + 1];
+    const bool in = c + lane < ctas;
+    const int2 next = in && lane > 0 ? p.cta_ids[2 * (c + lane)] : make_int2(-1, 0);
+    float2 mine[G / 8];
+#pragma unroll
+    for (int i = 0; i < G / 8; ++i)
+        mine[i] = in ? p.cta_ml[slot(lane) * G + warp + 8 * i] : make_float2(-INFINITY, 0.f);
+    const float4 v0 = c + part < ctas ? p.cta_partials[(long long)slot(part) * kFrags + f]
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
     if (id.x < 0) return;
-    if (tid == 0) last_s = ctas;
-    __syncthreads();
-    for (int i = c + 1 + tid; i < ctas; i += 256)
-        if (p.cta_ids[2 * i].x == id.x && (p.cta_ids[2 * i].y & kUnitEnd)) atomicMin(&last_s, i);
-    __syncthreads();
-    const int n = min(last_s, ctas - 1) - c + 1;  // partials
-    auto slot = [&](int i) { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
-    for (int h = warp; h < G; h += 8) {
-        float M = -INFINITY;
-        for (int i = lane; i < n; i += 32) M = fmaxf(M, p.cta_ml[slot(i) * G + h].x);
+    // partials of the unit
+    uint32_t ends = __ballot_sync(0xffffffffu, next.x == id.x && (next.y & kUnitEnd));
+    int n = __ffs(ends);
+    for (int i0 = 32; n == 0 && c + i0 < ctas; i0 += 32) {
+        const int2 more = c + i0 + lane < ctas ? p.cta_ids[2 * (c + i0 + lane)] : make_int2(-1, 0);
+        ends = __ballot_sync(0xffffffffu, more.x == id.x && (more.y & kUnitEnd));
+        if (ends) n = i0 + __ffs(ends);
+    }
+    if (n == 0) return;  // a wait gave up: the status word says so
+#pragma unroll
+    for (int i = 0; i < G / 8; ++i) {
+        const int h = warp + 8 * i;
+        float M = lane < n ? mine[i].x : -INFINITY;
+        for (int k = lane + 32; k < n; k += 32) M = fmaxf(M, p.cta_ml[slot(k) * G + h].x);
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        float L = 0.f;
-        for (int i = lane; i < n; i += 32) {
-            const float2 v = p.cta_ml[slot(i) * G + h];
+        float L = lane < n ? piece_weight(mine[i].x, M) * mine[i].y : 0.f;
+        for (int k = lane + 32; k < n; k += 32) {
+            const float2 v = p.cta_ml[slot(k) * G + h];
             L += piece_weight(v.x, M) * v.y;
         }
 #pragma unroll
@@ -840,15 +977,14 @@ __global__ void __launch_bounds__(256) scored_join_kernel(const Params p, int ct
         }
     }
     __syncthreads();
-    const int f = blockIdx.y * P + tid % P, part = tid / P;
     const int nt = f / (kTiles * 32), fl = f & 31, h0 = nt * 8 + 2 * (fl & 3);
     const float M0 = sM[h0], M1 = sM[h0 + 1];
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int i = part; i < n; i += LANES) {
-        const float4 v = p.cta_partials[(long long)slot(i) * kFrags + f];
-        const float w0 = piece_weight(p.cta_ml[slot(i) * G + h0].x, M0);
-        const float w1 = piece_weight(p.cta_ml[slot(i) * G + h0 + 1].x, M1);
+        const float4 v = i == part ? v0 : p.cta_partials[(long long)slot(i) * kFrags + f];
+        const float4 w = *reinterpret_cast<const float4*>(p.cta_ml + slot(i) * G + h0);
+        const float w0 = piece_weight(w.x, M0), w1 = piece_weight(w.z, M1);
         acc.x += w0 * v.x;
         acc.y += w1 * v.y;
         acc.z += w0 * v.z;
@@ -864,16 +1000,14 @@ __global__ void __launch_bounds__(256) scored_join_kernel(const Params p, int ct
             acc.z += v.z;
             acc.w += v.w;
         }
-        const float L0 = sL[h0], L1 = sL[h0 + 1];
         write_frag<QT, Q8>(reinterpret_cast<QT*>(p.out), p, unit_of(id.x, p), D, nt,
-                           (f >> 5) % kTiles, fl, acc,
-                           L0 > 0.f || L0 != L0 ? __fdividef(1.f, L0) : 0.f,
-                           L1 > 0.f || L1 != L1 ? __fdividef(1.f, L1) : 0.f);
+                           (f >> 5) % kTiles, fl, acc, inverse(sL[h0]), inverse(sL[h0 + 1]));
     }
 }
 
 template <typename QT, typename CT, int D, int NT>
-cudaError_t launch_fast(const Params& p, int ctas, bool overlap, cudaStream_t st) {
+cudaError_t launch_fast(const Params& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                        int ctas, bool overlap, cudaStream_t st) {
     using F = Cfg<QT, CT, D, NT>;
     auto kern = scored_attention_kernel<QT, CT, D, NT>;
     cudaError_t e =
@@ -884,12 +1018,12 @@ cudaError_t launch_fast(const Params& p, int ctas, bool overlap, cudaStream_t st
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(F::kThreads);
     cfg.dynamicSmemBytes = F::kSmem;
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = overlap ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, p);
+    e = cudaLaunchKernelEx(&cfg, kern, map_k, map_v, p);
     if (e != cudaSuccess || ctas == 1) return e;
     cfg.gridDim = dim3(ctas, kJoinParts);
     cfg.blockDim = dim3(256);
@@ -899,13 +1033,13 @@ cudaError_t launch_fast(const Params& p, int ctas, bool overlap, cudaStream_t st
 }
 
 template <typename QT, typename CT>
-cudaError_t launch_fast_shape(const Params& p, int head_dim, int ctas, bool overlap,
-                              cudaStream_t st) {
-    if (head_dim == 128)
-        return p.unit_heads <= 8 ? launch_fast<QT, CT, 128, 1>(p, ctas, overlap, st)
-                                 : launch_fast<QT, CT, 128, 2>(p, ctas, overlap, st);
-    return p.unit_heads <= 8 ? launch_fast<QT, CT, 64, 1>(p, ctas, overlap, st)
-                             : launch_fast<QT, CT, 64, 2>(p, ctas, overlap, st);
+cudaError_t launch_fast_shape(const Params& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                              int ctas, bool overlap, cudaStream_t st) {
+    if (p.head_dim == 128)
+        return p.unit_heads <= 8 ? launch_fast<QT, CT, 128, 1>(p, map_k, map_v, ctas, overlap, st)
+                                 : launch_fast<QT, CT, 128, 2>(p, map_k, map_v, ctas, overlap, st);
+    return p.unit_heads <= 8 ? launch_fast<QT, CT, 64, 1>(p, map_k, map_v, ctas, overlap, st)
+                             : launch_fast<QT, CT, 64, 2>(p, map_k, map_v, ctas, overlap, st);
 }
 
 }  // namespace scored
