@@ -317,3 +317,14 @@ def test_pool_past_32_bit_byte_offsets():
                                       vs.view(torch.float8_e8m0fnu), tables, small.lens,
                                       small.scale)
     assert torch.equal(out, small.run())
+
+
+@pytest.mark.parametrize("dtype,kind", PAIRS, ids=short)
+@pytest.mark.parametrize("d,h,kvh", [(64, 16, 2), (128, 16, 2), (128, 24, 2)])
+def test_few_short_units(d, h, kvh, dtype, kind):
+    """Batches whose units are taken whole by a CTA, and the first ones that are
+    not (the longest is one tile past the limit for its width)."""
+    for longest in (1, 95, 192, 193, 384, 385, 768, 769, 1536, 1537):
+        c = Case([longest, 0, 1, longest // 2, 17], h, kvh, d, 8, dtype, kind, seed=17)
+        c.tables = c.tables[:, :-1].contiguous()  # no spare column: the limit is exact
+        c.check(c.run())

@@ -374,7 +374,11 @@ int tlb_paged_attention_scored(void* out, const void* query, const void* key_cac
         return cuda_result(sc::launch_generic(dtype, cache_dtype, p, st), "paged attention");
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
-    const int ctas = sc::ctas_for(tiles, p.group, sms, kMinCost);
+    const long long units = (long long)p.units_per_seq * num_seqs;
+    const long long unit_tiles = tiles / units;
+    p.aligned = units <= sms &&
+                unit_tiles <= (long long)sc::kAlignedTiles * sc::warps_for(p.unit_heads);
+    const int ctas = p.aligned ? (int)units : sc::ctas_for(tiles, p.group, sms, kMinCost);
     const sc::Workspace w = sc::workspace_layout(p.group, p.head_dim, ctas);
     if (workspace == nullptr || workspace_bytes < w.total || !aligned(workspace, 16))
         return fail(TLB_ERR_WORKSPACE,

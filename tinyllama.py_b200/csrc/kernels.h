@@ -249,6 +249,9 @@ constexpr int warps_for(int heads) { return heads <= 8 ? 12 : 8; }
 // Tokens of a tile for rows of `bytes`: 4 KB of keys.
 constexpr int tile_tokens(int bytes) { return 4096 / bytes; }
 
+// Most tiles of a unit for each warp of a CTA that takes it whole.
+constexpr int kAlignedTiles = 2;
+
 struct Params {
     void* out;
     const void* query;
@@ -279,6 +282,7 @@ struct Params {
     int max_tokens;               // max_blocks * block_size
     int window;                   // tokens the query sees, 0: all
     int min_cost;                 // least cost points of a warp's range
+    bool aligned;                 // a CTA takes one whole unit
     int box_shift;                // log2 of the cache rows a TMA box holds
     unsigned wait_limit;          // mbarrier probes before a wait gives up
     float scale;

@@ -31,6 +31,9 @@
 //    so w_j fits fp16 whatever the scales of the rows are. fp16 weights are
 //    held 2^7 higher (up to 2^15 with the lazy reference), so that what
 //    fp16 rounds by 2^-25 below its normal range is 2^-32 of the reference.
+//  * Where there are no more units than SMs and none has more than
+//    kAlignedTiles tiles a warp, a CTA takes a whole unit instead: even ranges
+//    would gain little, and no scan, no second kernel is needed.
 //  * A unit cut by range ends leaves fp32 partials: warps of one CTA join
 //    theirs in shared memory, CTAs through the workspace in a second small
 //    kernel (programmatic launch). The order of every sum is fixed: results
@@ -89,7 +92,7 @@ struct Cfg {
     static constexpr int kScaleOff = kHdrOff + kWarps * kStages * 16;
     static constexpr int kMlOff = kScaleOff + (kQ8 ? kWarps * kStages * 2 * kTT : 0);
     static constexpr int kWeightOff = kMlOff + 2 * kWarps * kGroup * 8;
-    static constexpr int kUnitOff = kWeightOff + 2 * kWarps * kGroup * 4;
+    static constexpr int kUnitOff = kWeightOff + 2 * kWarps * kGroup * 8;
     static constexpr int kPrefixOff = kUnitOff + 2 * kWarps * 16;
     static constexpr int kSmem = kPrefixOff + (kThreads + kWarps) * 4 + 1024;  // + alignment slack
     static_assert(kSmem <= 232448, "one CTA per SM");
@@ -185,6 +188,14 @@ __device__ __forceinline__ float inverse(float sum) {
     return sum > 0.f || sum != sum ? __fdividef(1.f, sum) : 0.f;
 }
 
+// Largest x of the lanes in `mask`, each of which calls this with its own set.
+__device__ __forceinline__ float max_of(uint32_t mask, float x) {
+    // as integers of the same order (NaN above or below all numbers)
+    const int b = __float_as_int(x);
+    const int m = __reduce_max_sync(mask, b ^ ((b >> 31) & 0x7fffffff));
+    return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
+}
+
 // Unit u: sequence, kv head and chunk of its query heads.
 struct Unit {
     int s, kvh, head0, heads;
@@ -251,7 +262,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     int4* hdr = reinterpret_cast<int4*>(smem + F::kHdrOff) + warp * ST;
     uint8_t* sc = smem + F::kScaleOff + warp * ST * 2 * TT;
     float2* ml = reinterpret_cast<float2*>(smem + F::kMlOff);      // [2 W][G] (m, l)
-    float* wt = reinterpret_cast<float*>(smem + F::kWeightOff);    // [2 W][G] joint weights
+    float2* wl = reinterpret_cast<float2*>(smem + F::kWeightOff);  // [2 W][G] joint weight, times l
     int4* ids = reinterpret_cast<int4*>(smem + F::kUnitOff);       // [2 W] (unit, flags, part)
     int* pre = reinterpret_cast<int*>(smem + F::kPrefixOff);       // [THREADS] cost before, in warp
     int* wsum = pre + THREADS;                                     // [W] cost of a warp's threads
@@ -266,42 +277,14 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
         return sp.len > 0
                    ? ((sp.len + TT - 1) / TT - sp.first / TT + kUnitCost) * p.units_per_seq : 0;
     };
-    const int per = (p.num_seqs + THREADS - 1) / THREADS;
-    {
-        int mine = 0;
-        for (int s = tid * per; s < min((tid + 1) * per, p.num_seqs); ++s) mine += cost_of(s);
-        int inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        pre[tid] = inc - mine;
-        if (lane == 31) wsum[warp] = inc;
-        if (lane < 2) ids[2 * warp + lane] = make_int4(-1, 0, 0, 0);
-        if (tid == 0) parts_used = 0;
-        if (lane == 0) {
-            prefetch_tensormap(&map_k);
-            prefetch_tensormap(&map_v);
-            for (int i = 0; i < ST; ++i) mbar_init(bars + 8 * i, 1);
-            fence_mbar_init();
-        }
-        __syncthreads();
+    if (lane < 2) ids[2 * warp + lane] = make_int4(-1, 0, 0, 0);
+    if (tid == 0) parts_used = 0;
+    if (lane == 0) {
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
+        for (int i = 0; i < ST; ++i) mbar_init(bars + 8 * i, 1);
+        fence_mbar_init();
     }
-    // lane i: cost before warp i's threads
-    const int own = lane < W ? wsum[lane] : 0;
-    int before = own;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
-    }
-    const unsigned total = __shfl_sync(0xffffffffu, before, W - 1);
-    before -= own;
-    // CTAs that take part: at least min_cost tiles' cost per warp
-    const unsigned nw = W * max(1u, min(gridDim.x, (total + W * p.min_cost - 1) / (W * p.min_cost)));
-    const unsigned wi = blockIdx.x * W + warp;
-
     // ---- cursor of the tile loads
     int seq = 0, kvh = 0, chunk = 0, tile = 0, tile_begin = 0, tile_end = 0;
     int rel = 0, lim = 0;  // cost points from this warp's range start
@@ -313,35 +296,75 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
         tile_end = (span.len + TT - 1) / TT;
     };
     bool fresh = true;  // next tile starts a piece
-    if (wi < nw) {
-        // the range [total * wi / nw, total * (wi + 1) / nw) in 32 bits
-        const unsigned q = total / nw, r = total - q * nw;
-        const unsigned a = q * wi + r * wi / nw;
-        lim = (int)(q * (wi + 1) + r * (wi + 1) / nw - a);
-        if (lim > 0) {
-            // the sequence whose costs hold point a: the last thread whose cost
-            // before it is at most a (an empty one shares its number with the next)
-            const int w = 31 - __clz(__ballot_sync(0xffffffffu, lane < W && (unsigned)before <= a));
-            const unsigned mine = __shfl_sync(0xffffffffu, before, w) + pre[w * 32 + lane];
-            const int i = 31 - __clz(__ballot_sync(0xffffffffu, mine <= a));
-            unsigned at = a - __shfl_sync(0xffffffffu, mine, i);  // a's place from there
-            int s = (w * 32 + i) * per;
-            while (true) {
-                const unsigned cost = cost_of(s);
-                if (at < cost) break;
-                at -= cost;
-                ++s;
+    if (p.aligned) {
+        // one unit for each CTA, its tiles cut evenly over the warps
+        const int s = blockIdx.x / p.units_per_seq, sub = blockIdx.x - s * p.units_per_seq;
+        enter_seq(s);
+        kvh = sub / p.head_chunks;
+        chunk = sub - kvh * p.head_chunks;
+        const int n = tile_end - tile_begin;
+        tile = tile_begin + n * warp / W;
+        lim = tile_begin + n * (warp + 1) / W - tile;
+        __syncthreads();
+    } else {
+        const int per = (p.num_seqs + THREADS - 1) / THREADS;
+        int mine = 0;
+        for (int s = tid * per; s < min((tid + 1) * per, p.num_seqs); ++s) mine += cost_of(s);
+        int inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        pre[tid] = inc - mine;
+        if (lane == 31) wsum[warp] = inc;
+        __syncthreads();
+        // lane i: cost before warp i's threads
+        const int own = lane < W ? wsum[lane] : 0;
+        int before = own;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += v;
+        }
+        const unsigned total = __shfl_sync(0xffffffffu, before, W - 1);
+        before -= own;
+        // CTAs that take part: at least min_cost tiles' cost per warp
+        const unsigned least = W * p.min_cost;
+        const unsigned nw = W * max(1u, min(gridDim.x, (total + least - 1) / least));
+        const unsigned wi = blockIdx.x * W + warp;
+        if (wi < nw) {
+            // the range [total * wi / nw, total * (wi + 1) / nw) in 32 bits
+            const unsigned q = total / nw, r = total - q * nw;
+            const unsigned a = q * wi + r * wi / nw;
+            lim = (int)(q * (wi + 1) + r * (wi + 1) / nw - a);
+            if (lim > 0) {
+                // the sequence whose costs hold point a: the last thread whose
+                // cost before it is at most a (an empty one shares its number
+                // with the next)
+                const int w =
+                    31 - __clz(__ballot_sync(0xffffffffu, lane < W && (unsigned)before <= a));
+                const unsigned at_lane = __shfl_sync(0xffffffffu, before, w) + pre[w * 32 + lane];
+                const int i = 31 - __clz(__ballot_sync(0xffffffffu, at_lane <= a));
+                unsigned at = a - __shfl_sync(0xffffffffu, at_lane, i);  // a's place from there
+                int s = (w * 32 + i) * per;
+                while (true) {
+                    const unsigned cost = cost_of(s);
+                    if (at < cost) break;
+                    at -= cost;
+                    ++s;
+                }
+                enter_seq(s);
+                const unsigned unit_cost = tile_end - tile_begin + kUnitCost;
+                const int sub = at / unit_cost;
+                const int off = at - sub * unit_cost;
+                kvh = p.head_chunks == 1 ? sub : sub / p.head_chunks;
+                chunk = sub - kvh * p.head_chunks;
+                // a unit's tiles sit at the end of its cost points
+                const int skip = max(off - kUnitCost, 0);
+                tile = tile_begin + skip;
+                rel = skip + kUnitCost - off;
             }
-            enter_seq(s);
-            const unsigned unit_cost = tile_end - tile_begin + kUnitCost;
-            const int sub = at / unit_cost;
-            const int off = at - sub * unit_cost;
-            kvh = p.head_chunks == 1 ? sub : sub / p.head_chunks;
-            chunk = sub - kvh * p.head_chunks;
-            // a unit's tiles sit at the end of its cost points
-            const int skip = max(off - kUnitCost, 0);
-            tile = tile_begin + skip;
-            rel = skip + kUnitCost - off;
         }
     }
     // Boxes of a tile: box_rows rows (a block or a part of one) each. Lane i
@@ -448,8 +471,6 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
 
     fetch_bid();
     grid_dependency_wait();
-#pragma unroll
-    for (int i = 0; i < ST - 1; ++i) load_tile(i);
 
     // ---- state of the piece in flight
     uint32_t qf[NT][F::kTiles][2];
@@ -464,8 +485,13 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     int slot = 0;
     uint32_t parity = 0;
     bool failed = false;
+    int ahead = 0;  // tiles loaded before the first is used
     while (true) {
-        load_tile(slot == 0 ? ST - 1 : slot - 1);
+        load_tile(ahead < ST - 1 ? ahead : slot == 0 ? ST - 1 : slot - 1);
+        if (ahead < ST - 1) {
+            ++ahead;
+            continue;
+        }
         __syncwarp();
         const int4 h = hdr[slot];
         if (h.z < 0) break;
@@ -840,74 +866,86 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     if constexpr (F::kQ8) cp_async_wait<0>();
     __syncthreads();
 
-    // ---- join the CTA's partials, in range order (entry 2 w: the piece that
-    // ended inside warp w's range, 2 w + 1: the last piece of its range)
-    const uint32_t there = __ballot_sync(0xffffffffu, lane < 2 * W && ids[lane < 2 * W ? lane : 0].x >= 0);
+    // ---- join the CTA's partials, in range order. Lane e of every warp holds
+    // entry e: the piece that ended inside warp e / 2's range (even e) or was
+    // the last of its range (odd e).
+    const int4 mine = lane < 2 * W ? ids[lane] : make_int4(-1, 0, 0, 0);
+    const uint32_t run = __match_any_sync(0xffffffffu, mine.x);  // entries of the same unit
+    uint32_t there = __ballot_sync(0xffffffffu, mine.x >= 0);
+    int2 left = make_int2(-1, 0), right = make_int2(-1, 0);
     if (there) {
-        // weights of all entries: one thread for each entry and head
-        for (int i = tid; i < 2 * W * G; i += THREADS) {
-            const int e = i / G, h = i - e * G, u = ids[e].x;
-            if (u < 0) continue;
-            float M = -INFINITY;
-            for (uint32_t k = there; k; k &= k - 1) {
-                const int x = __ffs(k) - 1;
-                if (ids[x].x == u) M = fmaxf(M, ml[x * G + h].x);
+        // weights of the entries, a warp for each head
+        if (mine.x >= 0)
+            for (int h = warp; h < G; h += W) {
+                const float2 v = ml[lane * G + h];
+                const float M = max_of(run, v.x);
+                const float w = piece_weight(v.x, M);
+                wl[lane * G + h] = make_float2(w, w * v.y);
+                ml[lane * G + h].x = M;
             }
-            wt[i] = piece_weight(ml[i].x, M);
-        }
         __syncthreads();
-        int2 left = make_int2(-1, 0), right = make_int2(-1, 0);
-        for (int f = tid; f < F::kFrags; f += THREADS) {
-            const int nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles, fl = f & 31;
-            const int h0 = nt * 8 + 2 * (fl & 3);
-            for (uint32_t k = there; k;) {
-                const int u = ids[__ffs(k) - 1].x;
-                int flags = 0;
-                float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+        // byte offset of the entry's partial in shared memory, -1: workspace
+        const int from = (lane & 1) ? (lane >> 1) * F::kRingBytes
+                         : mine.z < F::kParts ? F::kPartOff + mine.z * F::kPartBytes : -1;
+        while (there) {
+            const int e0 = __ffs(there) - 1;
+            uint32_t k = __shfl_sync(0xffffffffu, run, e0);
+            const int u = __shfl_sync(0xffffffffu, mine.x, e0);
+            const int flags = __reduce_or_sync(0xffffffffu, (k >> lane) & 1 ? mine.y : 0);
+            there &= ~k;
+            const uint32_t entries = k;
+            const bool whole = flags == (kUnitBegin | kUnitEnd);
+            const int side = (flags & kUnitBegin) ? 1 : 0, at = 2 * blockIdx.x + side;
+            if (!whole) {
+                if (side) right = make_int2(u, flags); else left = make_int2(u, flags);
+            }
+            const Unit un_k = unit_of(u, p);
+            for (int f0 = warp * 32; f0 < F::kFrags; f0 += THREADS) {
+                const int f = f0 + lane, nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles;
+                const int h0 = nt * 8 + 2 * (lane & 3);
+                float L0 = 0.f, L1 = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (; k; k &= k - 1) {
-                    const int e = __ffs(k) - 1;
-                    const int4 id = ids[e];
-                    if (id.x != u) break;
-                    flags |= id.y;
-                    const float4* src =
-                        (e & 1) ? reinterpret_cast<const float4*>(smem + (e >> 1) * F::kRingBytes)
-                        : id.z < F::kParts
-                            ? reinterpret_cast<const float4*>(smem + F::kPartOff +
-                                                              id.z * F::kPartBytes)
-                            : p.warp_partials + ((long long)blockIdx.x * W + (e >> 1)) * F::kFrags;
-                    const float4 v = src[f];
-                    const float2 w = *reinterpret_cast<const float2*>(wt + e * G + h0);
-                    const float4 m2 = *reinterpret_cast<const float4*>(ml + e * G + h0);
-                    M0 = fmaxf(M0, m2.x);
-                    M1 = fmaxf(M1, m2.z);
-                    L0 += w.x * m2.y;
-                    L1 += w.y * m2.w;
-                    acc.x += w.x * v.x;
-                    acc.y += w.y * v.y;
-                    acc.z += w.x * v.z;
-                    acc.w += w.y * v.w;
+                for (k = entries; k;) {
+                    // four entries' loads in flight
+                    float4 v[4], w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        v[j] = w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (k) {
+                            const int e = __ffs(k) - 1;
+                            k &= k - 1;
+                            const int off = __shfl_sync(0xffffffffu, from, e);
+                            v[j] = off >= 0 ? reinterpret_cast<const float4*>(smem + off)[f]
+                                            : p.warp_partials[((long long)blockIdx.x * W + (e >> 1)) *
+                                                                  F::kFrags + f];
+                            w[j] = *reinterpret_cast<const float4*>(wl + e * G + h0);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        acc.x += w[j].x * v[j].x;
+                        acc.y += w[j].z * v[j].y;
+                        acc.z += w[j].x * v[j].z;
+                        acc.w += w[j].z * v[j].w;
+                        L0 += w[j].y;
+                        L1 += w[j].w;
+                    }
                 }
-                if (flags == (kUnitBegin | kUnitEnd)) {
-                    write_frag<QT, F::kQ8>(out, p, unit_of(u, p), D, nt, i, fl, acc, inverse(L0),
+                if (whole) {
+                    write_frag<QT, F::kQ8>(out, p, un_k, D, nt, i, lane, acc, inverse(L0),
                                            inverse(L1));
                 } else {
-                    const int side = (flags & kUnitBegin) ? 1 : 0;
-                    const int at = 2 * blockIdx.x + side;
-                    if (side) right = make_int2(u, flags); else left = make_int2(u, flags);
                     p.cta_partials[(long long)at * F::kFrags + f] = acc;
-                    if (i == 0 && fl < 4)
+                    if (i == 0 && lane < 4)
                         *reinterpret_cast<float4*>(p.cta_ml + at * G + h0) =
-                            make_float4(M0, L0, M1, L1);
+                            make_float4(ml[e0 * G + h0].x, L0, ml[e0 * G + h0 + 1].x, L1);
                 }
             }
         }
-        if (tid == 0) {
-            p.cta_ids[2 * blockIdx.x] = left;
-            p.cta_ids[2 * blockIdx.x + 1] = right;
-        }
-    } else if (tid == 0) {
-        p.cta_ids[2 * blockIdx.x] = p.cta_ids[2 * blockIdx.x + 1] = make_int2(-1, 0);
+    }
+    if (tid == 0 && !p.aligned) {
+        p.cta_ids[2 * blockIdx.x] = left;
+        p.cta_ids[2 * blockIdx.x + 1] = right;
     }
     // ---- sequences with no token: zeros
     for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
@@ -1024,7 +1062,7 @@ cudaError_t launch_fast(const Params& p, const CUtensorMap& map_k, const CUtenso
     cfg.attrs = attr;
     cfg.numAttrs = overlap ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, kern, map_k, map_v, p);
-    if (e != cudaSuccess || ctas == 1) return e;
+    if (e != cudaSuccess || p.aligned) return e;
     cfg.gridDim = dim3(ctas, kJoinParts);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
