@@ -485,13 +485,16 @@ TLB_API int tlb_qk_norm_rotary_embedding_neox(
  *   alibi_slopes : [num_heads] float or NULL
  *   cache_dtype  : dtype, or TLB_FLOAT8_E4M3 / TLB_INT8 with scales
  * `workspace`: device scratch of the size that the _workspace_size call gives
- * for these shapes on this device (16-byte aligned; may be uninitialised, holds
- * nothing between calls; NULL when the size is 0). Calls that overlap in time
- * need separate buffers. flags: TLB_ATTN_OVERLAP_PROLOGUE as above.
+ * for these shapes on this device (16-byte aligned; NULL when the size is 0).
+ * Its first zeroed_out bytes (arrival counters) must be zero when the call
+ * starts and are zero again when it ends, the rest may hold anything: calls on
+ * one stream can share a buffer, calls that overlap in time need separate
+ * ones. The zeroed size depends on the device alone. After TLB_STATUS_WAIT_TIMEOUT
+ * the caller zeroes it again. flags: TLB_ATTN_OVERLAP_PROLOGUE as above.
  * ---------------------------------------------------------------------- */
 TLB_API int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t num_kv_heads,
                         int64_t head_dim, int64_t block_size, int dtype,
-                        int cache_dtype, size_t* bytes_out);
+                        int cache_dtype, size_t* bytes_out, size_t* zeroed_out);
 
 TLB_API int tlb_paged_attention_scored(void* out, const void* query, const void* key_cache,
                         const void* value_cache, const void* key_scales,

@@ -53,6 +53,8 @@ def invalidate_workspaces(device_index: int) -> None:
     for (dev, _stream), ws in _workspaces.items():
         if dev == device_index:
             ws.clean = 0
+    for key in [k for k in _scored_workspaces if k[0] == device_index]:
+        del _scored_workspaces[key]
 
 
 def workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -292,45 +294,59 @@ def paged_prefill_attention(query: torch.Tensor, key_cache: torch.Tensor,
 
 
 _CACHE8_TYPES = (torch.float8_e4m3fn, torch.int8)
-_scored_ws_sizes: dict[tuple, int] = {}
+_scored_ws_sizes: dict[tuple, tuple[int, int]] = {}
+# (device index, stream handle) -> scratch whose counter prefix is zero between calls
+_scored_workspaces: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _scored_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int, block_size: int,
-                            dtype: torch.dtype, cache_dtype: torch.dtype,
-                            device_index: int) -> int:
-    key = (num_heads, num_kv_heads, head_dim, block_size, dtype, cache_dtype, device_index)
+def _scored_workspace_bytes(*key) -> tuple[int, int]:
+    """(total bytes, zero-at-rest prefix bytes) for (num_heads, num_kv_heads,
+    head_dim, block_size, dtype, cache dtype, device index)."""
     n = _scored_ws_sizes.get(key)
     if n is None:
-        size = ctypes.c_size_t(0)
-        _lib.check(_lib.load().tlb_paged_attention_scored_workspace_size(
-            num_heads, num_kv_heads, head_dim, block_size, DTYPE_CODE[dtype],
-            DTYPE_CODE[cache_dtype], ctypes.byref(size)))
-        n = _scored_ws_sizes[key] = size.value
+        total, zeroed = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        with _lib.device_guard(torch.device("cuda", key[-1])):
+            _lib.check(_lib.load().tlb_paged_attention_scored_workspace_size(
+                *key[:4], DTYPE_CODE[key[4]], DTYPE_CODE[key[5]], ctypes.byref(total),
+                ctypes.byref(zeroed)))
+        n = _scored_ws_sizes[key] = (total.value, zeroed.value)
     return n
 
 
-def _paged_attention_scored(query, key_cache, value_cache, key_scales, value_scales, block_tables,
-                            seq_lens, scale, softcap, alibi_slopes, window, overlap_prologue):
-    """Checks shared by the two entry points below, and the launch."""
-    dev = query.device
-    shape, cshape = query.shape, key_cache.shape
+def _scored_workspace(query: torch.Tensor, index: int, nbytes: int, zeroed: int) -> torch.Tensor:
+    """Scratch of a call: the stream's own, or while the stream is captured one
+    of the graph's (zeroed in the graph), so that graphs replayed together share
+    none."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = query.new_empty(nbytes, dtype=torch.uint8)
+        ws[:zeroed].zero_()
+        return ws
+    key = (index, _lib.stream_of(query.device))
+    ws = _scored_workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _scored_workspaces[key] = query.new_zeros(max(nbytes, 1 << 23), dtype=torch.uint8)
+    return ws
+
+
+def _check_scored(query, key_cache, value_cache, block_tables, seq_lens, softcap, alibi_slopes,
+                  window):
+    """The checks of ``_paged_attention_scored`` one by one, for their messages."""
     torch_check(query.is_cuda, "query must be a CUDA tensor")
+    dev = query.device
     torch_check(key_cache.device == dev and value_cache.device == dev
                 and block_tables.device == dev and seq_lens.device == dev,
                 "all tensors must be on the same CUDA device")
-    torch_check(len(shape) == 3, "query must be [num_seqs, num_heads, head_dim]")
-    torch_check(len(cshape) == 4,
+    torch_check(query.dim() == 3, "query must be [num_seqs, num_heads, head_dim]")
+    torch_check(key_cache.dim() == 4,
                 "key_cache must be [num_blocks, num_kv_heads, block_size, head_dim]")
-    torch_check(value_cache.shape == cshape, "value_cache must have the same shape as key_cache")
-    num_seqs, num_heads, head_dim = shape
-    num_blocks, num_kv_heads, block_size, cache_head_dim = cshape
+    torch_check(value_cache.shape == key_cache.shape,
+                "value_cache must have the same shape as key_cache")
+    num_seqs, num_heads, head_dim = query.shape
     torch_check(num_seqs > 0, "query must contain at least one sequence")
-    torch_check(head_dim == cache_head_dim, "query head_dim must match the cache head_dim")
-    torch_check(head_dim <= 1024, "head_dim must not exceed 1024")
-    torch_check(num_kv_heads > 0 and num_heads % num_kv_heads == 0,
+    torch_check(head_dim == key_cache.size(3), "query head_dim must match the cache head_dim")
+    torch_check(key_cache.size(1) > 0 and num_heads % key_cache.size(1) == 0,
                 "num_heads must be divisible by num_kv_heads")
-    q_stride = query.stride()
-    torch_check(q_stride[2] == 1 and q_stride[1] == head_dim,
+    torch_check(query.stride(2) == 1 and query.stride(1) == head_dim,
                 "query must hold each sequence's heads contiguously")
     torch_check(key_cache.is_contiguous() and value_cache.is_contiguous(),
                 "key_cache and value_cache must be contiguous")
@@ -340,42 +356,62 @@ def _paged_attention_scored(query, key_cache, value_cache, key_scales, value_sca
     torch_check(seq_lens.dim() == 1 and seq_lens.dtype == torch.int32 and seq_lens.is_contiguous()
                 and seq_lens.size(0) == num_seqs,
                 "seq_lens must be a contiguous [num_seqs] int32 tensor")
-    dtype, cache_dtype = query.dtype, key_cache.dtype
-    torch_check(dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
-    torch_check(value_cache.dtype == cache_dtype, "key_cache and value_cache must share the same "
-                                                  "dtype")
-    torch_check(softcap >= 0 and softcap < float("inf"),
-                "softcap must be finite and not negative")
+    torch_check(query.dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
+    torch_check(value_cache.dtype == key_cache.dtype,
+                "key_cache and value_cache must share the same dtype")
+    torch_check(0 <= softcap < float("inf"), "softcap must be finite and not negative")
     torch_check(window >= 0, "window must not be negative")
-    slopes = None
-    if alibi_slopes is not None:
-        torch_check(alibi_slopes.device == dev and alibi_slopes.dtype == torch.float32
+    torch_check(alibi_slopes is None
+                or (alibi_slopes.device == dev and alibi_slopes.dtype == torch.float32
                     and alibi_slopes.dim() == 1 and alibi_slopes.size(0) == num_heads
-                    and alibi_slopes.is_contiguous(),
-                    "alibi_slopes must be a contiguous [num_heads] float32 tensor on the query's "
-                    "device")
-        slopes = alibi_slopes.data_ptr()
-    out = torch.empty(shape, dtype=dtype, device=dev)
-    max_blocks = block_tables.size(1)
-    if num_blocks == 0 or block_size == 0 or max_blocks == 0:
+                    and alibi_slopes.is_contiguous()),
+                "alibi_slopes must be a contiguous [num_heads] float32 tensor on the query's "
+                "device")
+    raise RuntimeError("paged attention: unsupported arguments")
+
+
+def _paged_attention_scored(query, key_cache, value_cache, key_scales, value_scales, block_tables,
+                            seq_lens, scale, softcap, alibi_slopes, window, overlap_prologue):
+    """The launch shared by the two entry points below. Their checks are one
+    expression (a call's host time counts in a decode step); a call that fails
+    it goes through ``_check_scored`` for the message."""
+    index = query.get_device()
+    shape, cshape, tshape = query.shape, key_cache.shape, block_tables.shape
+    dtype, cache_dtype, strides = query.dtype, key_cache.dtype, query.stride()
+    if not (index >= 0 and len(shape) == 3 and len(cshape) == 4 and len(tshape) == 2
+            and shape[0] > 0 and cshape[1] > 0 and shape[1] % cshape[1] == 0
+            and shape[2] == cshape[3] and strides[2] == 1 and strides[1] == shape[2]
+            and value_cache.shape == cshape and value_cache.dtype == cache_dtype
+            and dtype in _FLOAT_TYPES and tshape[0] == shape[0]
+            and seq_lens.shape == shape[:1] and block_tables.dtype == torch.int32
+            and seq_lens.dtype == torch.int32 and key_cache.is_contiguous()
+            and value_cache.is_contiguous() and block_tables.is_contiguous()
+            and seq_lens.is_contiguous() and key_cache.get_device() == index
+            and value_cache.get_device() == index and block_tables.get_device() == index
+            and seq_lens.get_device() == index and 0 <= softcap < float("inf") and window >= 0
+            and (alibi_slopes is None
+                 or (alibi_slopes.get_device() == index and alibi_slopes.dtype == torch.float32
+                     and alibi_slopes.shape == shape[1:2] and alibi_slopes.is_contiguous()))):
+        _check_scored(query, key_cache, value_cache, block_tables, seq_lens, softcap, alibi_slopes,
+                      window)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    num_blocks, num_kv_heads, block_size, head_dim = cshape
+    if num_blocks == 0 or block_size == 0 or tshape[1] == 0:
         return out.zero_()  # no cache to read: every softmax is empty
     if out.numel() == 0:
         return out
-    with _lib.device_guard(dev):
-        nbytes = _scored_workspace_bytes(num_heads, num_kv_heads, head_dim, block_size, dtype,
-                                         cache_dtype, dev.index)
-        # Scratch of this call alone, from the stream's own pool (or the pool of
-        # the graph being captured): nothing in it outlives the call.
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.check(_lib.load().tlb_paged_attention_scored(
-            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-            key_scales.data_ptr() if key_scales is not None else None,
-            value_scales.data_ptr() if value_scales is not None else None,
-            block_tables.data_ptr(), seq_lens.data_ptr(), slopes, num_seqs, num_heads,
-            num_kv_heads, head_dim, num_blocks, block_size, max_blocks, q_stride[0], window,
-            scale, softcap, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype],
-            ws.data_ptr() if ws is not None else None, nbytes, 1 if overlap_prologue else 0,
-            _lib.stream_of(dev)))
+    nbytes, zeroed = _scored_workspace_bytes(shape[1], num_kv_heads, head_dim, block_size, dtype,
+                                             cache_dtype, index)
+    ws = _scored_workspace(query, index, nbytes, zeroed).data_ptr() if nbytes else None
+    _lib.launch("tlb_paged_attention_scored", index, out.data_ptr(), query.data_ptr(),
+                key_cache.data_ptr(), value_cache.data_ptr(),
+                None if key_scales is None else key_scales.data_ptr(),
+                None if value_scales is None else value_scales.data_ptr(),
+                block_tables.data_ptr(), seq_lens.data_ptr(),
+                None if alibi_slopes is None else alibi_slopes.data_ptr(), shape[0], shape[1],
+                num_kv_heads, head_dim, num_blocks, block_size, tshape[1], strides[0], window,
+                scale, softcap, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype], ws, nbytes,
+                1 if overlap_prologue else 0)
     return out
 
 
@@ -398,14 +434,13 @@ def paged_attention_quantized(query: torch.Tensor, key_cache: torch.Tensor,
     """
     torch_check(key_cache.dtype in _CACHE8_TYPES,
                 "key_cache must be float8_e4m3fn or int8")
-    rows = key_cache.shape[:-1]
-    torch_check(key_scales.dtype == torch.float8_e8m0fnu
-                and value_scales.dtype == torch.float8_e8m0fnu
-                and key_scales.shape == rows and value_scales.shape == rows
-                and key_scales.is_contiguous() and value_scales.is_contiguous()
-                and key_scales.device == query.device and value_scales.device == query.device,
-                "key_scales and value_scales must be contiguous float8_e8m0fnu tensors "
-                "[num_blocks, num_kv_heads, block_size] on the query's device")
+    rows, index = key_cache.shape[:3], query.get_device()
+    for s in (key_scales, value_scales):
+        if not (s.dtype == torch.float8_e8m0fnu and s.shape == rows and s.is_contiguous()
+                and s.get_device() == index):
+            raise RuntimeError("key_scales and value_scales must be contiguous float8_e8m0fnu "
+                               "tensors [num_blocks, num_kv_heads, block_size] on the query's "
+                               "device")
     return _paged_attention_scored(query, key_cache, value_cache, key_scales, value_scales,
                                    block_tables, seq_lens, scale, softcap, alibi_slopes, window,
                                    overlap_prologue)

@@ -216,17 +216,18 @@ _FLOAT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def check_quantized_caches(key_cache: torch.Tensor, value_cache: torch.Tensor,
-                           key_scales: torch.Tensor, value_scales: torch.Tensor) -> None:
-    """The shapes and types of an 8-bit cache pair and its scales."""
-    torch_check(key_cache.is_cuda, "cache tensors must be CUDA tensors")
-    dev, shape = key_cache.device, key_cache.shape
+                           key_scales: torch.Tensor, value_scales: torch.Tensor) -> int:
+    """The shapes and types of an 8-bit cache pair and its scales; returns their
+    device index."""
+    index, shape = key_cache.get_device(), key_cache.shape
+    torch_check(index >= 0, "cache tensors must be CUDA tensors")
     torch_check(len(shape) == 4,
                 "key_cache must be [num_blocks, num_kv_heads, block_size, head_size]")
     torch_check(value_cache.shape == shape, "value_cache must have the same shape as key_cache")
     torch_check(key_cache.dtype in _CACHE8_TYPES, "key_cache must be float8_e4m3fn or int8")
     torch_check(value_cache.dtype == key_cache.dtype,
                 "key_cache and value_cache must share the same dtype")
-    rows = shape[:-1]
+    rows = shape[:3]
     torch_check(key_scales.dtype == torch.float8_e8m0fnu
                 and value_scales.dtype == torch.float8_e8m0fnu
                 and key_scales.shape == rows and value_scales.shape == rows,
@@ -235,21 +236,24 @@ def check_quantized_caches(key_cache: torch.Tensor, value_cache: torch.Tensor,
     torch_check(key_cache.is_contiguous() and value_cache.is_contiguous()
                 and key_scales.is_contiguous() and value_scales.is_contiguous(),
                 "cache tensors must be contiguous")
-    torch_check(value_cache.device == dev and key_scales.device == dev
-                and value_scales.device == dev, "all tensors must be on the same CUDA device")
+    torch_check(value_cache.get_device() == index and key_scales.get_device() == index
+                and value_scales.get_device() == index,
+                "all tensors must be on the same CUDA device")
+    return index
 
 
-def _token_rows(x: torch.Tensor, num_tokens: int, kvh: int, head_size: int, name: str) -> int:
-    """The stride between the tokens of x ([T, KVH, D] or [T, KVH * D] with each
-    token's heads contiguous)."""
-    if x.dim() == 3:
-        ok = x.shape == (num_tokens, kvh, head_size) and (kvh == 1 or x.stride(1) == head_size)
+def token_stride(x: torch.Tensor, num_tokens: int, kvh: int, head_size: int, name: str) -> int:
+    """The stride between the tokens of x: [T, KVH, D] or [T, KVH * D] with each
+    token's heads contiguous."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) == 3:
+        ok = shape == (num_tokens, kvh, head_size) and (kvh == 1 or strides[1] == head_size)
     else:
-        ok = x.dim() == 2 and x.shape == (num_tokens, kvh * head_size)
-    torch_check(ok and (x.stride(-1) == 1 or x.numel() == 0),
-                f"{name} must be [num_tokens, num_kv_heads, head_size] or [num_tokens, "
-                "num_kv_heads * head_size] with each token's heads contiguous")
-    return x.stride(0)
+        ok = shape == (num_tokens, kvh * head_size)
+    if not (ok and (strides[-1] == 1 or 0 in shape)):
+        raise RuntimeError(f"{name} must be [num_tokens, num_kv_heads, head_size] or [num_tokens, "
+                           "num_kv_heads * head_size] with each token's heads contiguous")
+    return strides[0]
 
 
 def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
@@ -268,27 +272,27 @@ def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cach
     slot = block * block_size + offset; negative slots are skipped. The other
     slots of a call must differ.
     """
-    check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
-    dev = key_cache.device
-    torch_check(key.device == dev and value.device == dev and slot_mapping.device == dev,
+    index = check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
+    torch_check(key.get_device() == index and value.get_device() == index
+                and slot_mapping.get_device() == index,
                 "all tensors must be on the same CUDA device")
-    torch_check(key.dtype in _FLOAT_TYPES and value.dtype == key.dtype,
+    dtype, slot_dtype = key.dtype, slot_mapping.dtype
+    torch_check(dtype in _FLOAT_TYPES and value.dtype == dtype,
                 "key and value must share a dtype: float16, bfloat16 or float32")
-    torch_check(slot_mapping.dim() == 1 and slot_mapping.dtype in _INDEX_TYPES
+    torch_check(slot_mapping.dim() == 1 and slot_dtype in _INDEX_TYPES
                 and slot_mapping.is_contiguous(),
                 "slot_mapping must be a contiguous [num_tokens] int32 or int64 tensor")
     num_blocks, kvh, block_size, head_size = key_cache.shape
-    T = slot_mapping.numel()
-    k_stride = _token_rows(key, T, kvh, head_size, "key")
-    v_stride = _token_rows(value, T, kvh, head_size, "value")
-    if T == 0 or key.numel() == 0:
+    T = slot_mapping.size(0)
+    k_stride = token_stride(key, T, kvh, head_size, "key")
+    v_stride = token_stride(value, T, kvh, head_size, "value")
+    if T == 0 or kvh * head_size == 0:
         return
-    with _lib.device_guard(dev):
-        _lib.check(_lib.load().tlb_reshape_and_cache_quantized(
-            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-            key_scales.data_ptr(), value_scales.data_ptr(), slot_mapping.data_ptr(),
-            DTYPE_CODE[slot_mapping.dtype], T, kvh, head_size, num_blocks, block_size, k_stride,
-            v_stride, DTYPE_CODE[key.dtype], DTYPE_CODE[key_cache.dtype], _lib.stream_of(dev)))
+    _lib.launch("tlb_reshape_and_cache_quantized", index, key.data_ptr(), value.data_ptr(),
+                key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+                value_scales.data_ptr(), slot_mapping.data_ptr(), DTYPE_CODE[slot_dtype], T, kvh,
+                head_size, num_blocks, block_size, k_stride, v_stride, DTYPE_CODE[dtype],
+                DTYPE_CODE[key_cache.dtype])
 
 
 def dequantize_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -305,34 +309,31 @@ def dequantize_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor,
     ``s * max_blocks + j``, which ``paged_prefill_attention`` and
     ``paged_attention`` read. ``out``: two tensors to fill instead of new ones.
     """
-    check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
-    dev = key_cache.device
-    torch_check(block_ids.device == dev, "all tensors must be on the same CUDA device")
+    index = check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
+    torch_check(block_ids.get_device() == index, "all tensors must be on the same CUDA device")
     torch_check(block_ids.dim() == 1 and block_ids.dtype in _INDEX_TYPES
                 and block_ids.is_contiguous(),
                 "block_ids must be a contiguous [num_ids] int32 or int64 tensor")
     torch_check(dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
     num_blocks, kvh, block_size, head_size = key_cache.shape
-    n = block_ids.numel()
+    n = block_ids.size(0)
     shape = (n, kvh, block_size, head_size)
     if out is None:
-        k = torch.empty(shape, dtype=dtype, device=dev)
-        v = torch.empty(shape, dtype=dtype, device=dev)
+        k = key_cache.new_empty(shape, dtype=dtype)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for t in out:
-            torch_check(t.shape == shape and t.dtype == dtype and t.device == dev
+            torch_check(t.shape == shape and t.dtype == dtype and t.get_device() == index
                         and t.is_contiguous(),
                         "out must be two contiguous [num_ids, num_kv_heads, block_size, head_size] "
                         "tensors of dtype")
-    if k.numel() == 0:
+    if n * kvh * block_size * head_size == 0:
         return k, v
     if num_blocks == 0:
         return k.zero_(), v.zero_()
-    with _lib.device_guard(dev):
-        _lib.check(_lib.load().tlb_dequantize_blocks(
-            k.data_ptr(), v.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-            key_scales.data_ptr(), value_scales.data_ptr(), block_ids.data_ptr(),
-            DTYPE_CODE[block_ids.dtype], n, kvh, head_size, num_blocks, block_size,
-            DTYPE_CODE[dtype], DTYPE_CODE[key_cache.dtype], _lib.stream_of(dev)))
+    _lib.launch("tlb_dequantize_blocks", index, k.data_ptr(), v.data_ptr(), key_cache.data_ptr(),
+                value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+                block_ids.data_ptr(), DTYPE_CODE[block_ids.dtype], n, kvh, head_size, num_blocks,
+                block_size, DTYPE_CODE[dtype], DTYPE_CODE[key_cache.dtype])
     return k, v

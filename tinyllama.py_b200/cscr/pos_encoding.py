@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import DTYPE_CODE, torch_check
-from .cache import _token_rows, check_quantized_caches
+from .cache import check_quantized_caches, token_stride
 
 _INDEX_TYPES = (torch.int32, torch.int64)
 
@@ -145,39 +145,46 @@ def rotary_embedding_neox_with_cache(postions: torch.Tensor, query: torch.Tensor
 
 
 _CACHE8_TYPES = (torch.float8_e4m3fn, torch.int8)
+_FLOAT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def _check_qk_norm(positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache):
-    dev, dtype = query.device, query.dtype
-    torch_check(query.is_cuda, "query must be a CUDA tensor")
-    torch_check(key.device == dev and positions.device == dev and cos_sin_cache.device == dev
-                and query_weight.device == dev and key_weight.device == dev,
+    """Checks shared by the two entry points below: (device index, tokens, query
+    stride, key stride, table shape)."""
+    index, dtype = query.get_device(), query.dtype
+    torch_check(index >= 0, "query must be a CUDA tensor")
+    torch_check(key.get_device() == index and positions.get_device() == index
+                and cos_sin_cache.get_device() == index and query_weight.get_device() == index
+                and key_weight.get_device() == index,
                 "all tensors must be on the same CUDA device")
-    torch_check(dtype in (torch.float16, torch.bfloat16, torch.float32),
-                "dtype must be float16, bfloat16 or float32")
+    torch_check(dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
     torch_check(key.dtype == dtype and cos_sin_cache.dtype == dtype
                 and query_weight.dtype == dtype and key_weight.dtype == dtype,
                 "query, key, cos_sin_cache and the weights must share a dtype")
-    torch_check(positions.dim() == 1 and positions.dtype in _INDEX_TYPES
-                and positions.is_contiguous(),
+    pshape = positions.shape
+    torch_check(len(pshape) == 1 and positions.dtype in _INDEX_TYPES and positions.is_contiguous(),
                 "positions must be a contiguous [num_tokens] int32 or int64 tensor")
-    num_tokens = positions.size(0)
     torch_check(head_size > 0, "head_size must be positive")
-    for x, name in ((query, "query"), (key, "key")):
-        torch_check(x.dim() == 2 and x.size(0) == num_tokens and x.size(1) > 0
-                    and x.size(1) % head_size == 0 and x.stride(1) == 1,
-                    f"{name} must be [num_tokens, heads * head_size] with unit inner stride")
-    for w in (query_weight, key_weight):
-        torch_check(w.dim() == 1 and w.size(0) == head_size and w.is_contiguous(),
-                    "query_weight and key_weight must be contiguous [head_size] tensors")
-    torch_check(cos_sin_cache.dim() == 2 and cos_sin_cache.is_contiguous()
-                and cos_sin_cache.size(0) > 0,
+    strides = []
+    for x in (query, key):
+        shape, stride = x.shape, x.stride()
+        if not (len(shape) == 2 and shape[0] == pshape[0] and shape[1] > 0
+                and shape[1] % head_size == 0 and stride[1] == 1):
+            raise RuntimeError("query and key must be [num_tokens, heads * head_size] with unit "
+                               "inner stride")
+        strides.append(stride[0])
+    wshape = (head_size,)
+    torch_check(query_weight.shape == wshape and key_weight.shape == wshape
+                and query_weight.is_contiguous() and key_weight.is_contiguous(),
+                "query_weight and key_weight must be contiguous [head_size] tensors")
+    tshape = cos_sin_cache.shape
+    torch_check(len(tshape) == 2 and tshape[0] > 0 and cos_sin_cache.is_contiguous(),
                 "cos_sin_cache must be a contiguous [rows, rotary_dim] tensor")
-    rot_dim = cos_sin_cache.size(1)
+    rot_dim = tshape[1]
     torch_check(rot_dim > 0 and rot_dim % 2 == 0, "rotary dimension must be even and positive")
     torch_check(rot_dim <= head_size, "rotary dimension must not exceed head_size")
     torch_check(eps >= 0, "eps must not be negative")
-    return num_tokens, rot_dim
+    return index, pshape[0], strides[0], strides[1], tshape
 
 
 def qk_norm_rotary_embedding_neox(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
@@ -192,22 +199,19 @@ def qk_norm_rotary_embedding_neox(positions: torch.Tensor, query: torch.Tensor, 
     head_size], rows possibly strided (parts of a fused projection); weights
     [head_size]. Returns new dense (query, key); the inputs are left as they are.
     """
-    num_tokens, rot_dim = _check_qk_norm(positions, query, key, query_weight, key_weight, eps,
-                                         head_size, cos_sin_cache)
-    dev = query.device
-    q_out = torch.empty(query.shape, dtype=query.dtype, device=dev)
-    k_out = torch.empty(key.shape, dtype=key.dtype, device=dev)
+    index, num_tokens, q_stride, k_stride, (rows, rot_dim) = _check_qk_norm(
+        positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache)
+    q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
     if num_tokens == 0:
         return q_out, k_out
     code = DTYPE_CODE[query.dtype]
-    with _lib.device_guard(dev):
-        _lib.check(_lib.load().tlb_qk_norm_rotary_embedding_neox(
-            q_out.data_ptr(), k_out.data_ptr(), positions.data_ptr(), DTYPE_CODE[positions.dtype],
-            query.data_ptr(), key.data_ptr(), None, query_weight.data_ptr(),
-            key_weight.data_ptr(), eps, None, None, None, None, None, 4, None, 0, num_tokens,
-            query.size(1) // head_size, key.size(1) // head_size, head_size,
-            cos_sin_cache.data_ptr(), cos_sin_cache.size(0), rot_dim, 0, 0, query.stride(0),
-            key.stride(0), 0, code, code, 0, _lib.stream_of(dev)))
+    _lib.launch("tlb_qk_norm_rotary_embedding_neox", index, q_out.data_ptr(), k_out.data_ptr(),
+                positions.data_ptr(), DTYPE_CODE[positions.dtype], query.data_ptr(),
+                key.data_ptr(), None, query_weight.data_ptr(), key_weight.data_ptr(), eps, None,
+                None, None, None, None, 4, None, 0, num_tokens, query.size(1) // head_size,
+                key.size(1) // head_size, head_size, cos_sin_cache.data_ptr(), rows, rot_dim, 0, 0,
+                q_stride, k_stride, 0, code, code, 0)
     return q_out, k_out
 
 
@@ -230,58 +234,57 @@ def qk_norm_rotary_embedding_neox_with_cache(
     the query dtype. Destinations and ``overlap_previous`` as in
     ``rotary_embedding_neox_with_cache``; the slots of one call must differ.
     """
-    num_tokens, rot_dim = _check_qk_norm(positions, query, key, query_weight, key_weight, eps,
-                                         head_size, cos_sin_cache)
-    dev, dtype = query.device, query.dtype
+    index, num_tokens, q_stride, k_stride, (rows, rot_dim) = _check_qk_norm(
+        positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache)
+    dtype, cache_dtype, cshape = query.dtype, key_cache.dtype, key_cache.shape
     kvh = key.size(1) // head_size
-    cache_dtype = key_cache.dtype
     ks_ptr = vs_ptr = None
     if cache_dtype in _CACHE8_TYPES:
         torch_check(key_scales is not None and value_scales is not None,
                     "8-bit caches need key_scales and value_scales")
-        check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
+        cache_index = check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
         ks_ptr, vs_ptr = key_scales.data_ptr(), value_scales.data_ptr()
     else:
         torch_check(key_scales is None and value_scales is None,
                     "key_scales and value_scales belong to 8-bit caches")
-        torch_check(key_cache.dim() == 4 and value_cache.shape == key_cache.shape,
+        torch_check(len(cshape) == 4 and value_cache.shape == cshape,
                     "key_cache and value_cache must be [num_blocks, num_kv_heads, block_size, "
                     "head_size]")
         torch_check(cache_dtype == dtype and value_cache.dtype == dtype,
                     "the caches must have the query dtype, or be float8_e4m3fn or int8")
         torch_check(key_cache.is_contiguous() and value_cache.is_contiguous(),
                     "key_cache and value_cache must be contiguous")
-    torch_check(key_cache.device == dev and value_cache.device == dev and value.device == dev,
+        cache_index = key_cache.get_device()
+        torch_check(value_cache.get_device() == cache_index,
+                    "all tensors must be on the same CUDA device")
+    torch_check(cache_index == index and value.get_device() == index,
                 "all tensors must be on the same CUDA device")
-    torch_check(key_cache.size(1) == kvh and key_cache.size(3) == head_size,
+    torch_check(cshape[1] == kvh and cshape[3] == head_size,
                 "cache heads / head_size must match key")
     torch_check(value.dtype == dtype, "value must have the query dtype")
-    v_stride = _token_rows(value, num_tokens, kvh, head_size, "value")
+    v_stride = token_stride(value, num_tokens, kvh, head_size, "value")
     if slot_mapping is not None:
-        torch_check(slot_mapping.device == dev and slot_mapping.dim() == 1
-                    and slot_mapping.size(0) == num_tokens
+        torch_check(slot_mapping.get_device() == index and slot_mapping.shape == (num_tokens,)
                     and slot_mapping.dtype in _INDEX_TYPES and slot_mapping.is_contiguous(),
                     "slot_mapping must be a contiguous [num_tokens] int32/int64 CUDA tensor")
         slots, slot_code, tables, width = (slot_mapping.data_ptr(),
                                            DTYPE_CODE[slot_mapping.dtype], None, 0)
     else:
         torch_check(block_tables is not None, "either slot_mapping or block_tables is required")
-        torch_check(block_tables.device == dev and block_tables.dim() == 2
+        torch_check(block_tables.get_device() == index and block_tables.dim() == 2
                     and block_tables.dtype == torch.int32 and block_tables.is_contiguous()
                     and block_tables.size(0) >= num_tokens and block_tables.size(1) > 0,
                     "block_tables must be a contiguous int32 CUDA tensor with a row per token")
         slots, slot_code, tables, width = None, 4, block_tables.data_ptr(), block_tables.size(1)
-    q_out = torch.empty(query.shape, dtype=dtype, device=dev)
+    q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if num_tokens == 0:
         return q_out
-    with _lib.device_guard(dev):
-        _lib.check(_lib.load().tlb_qk_norm_rotary_embedding_neox(
-            q_out.data_ptr(), None, positions.data_ptr(), DTYPE_CODE[positions.dtype],
-            query.data_ptr(), key.data_ptr(), value.data_ptr(), query_weight.data_ptr(),
-            key_weight.data_ptr(), eps, key_cache.data_ptr(), value_cache.data_ptr(), ks_ptr,
-            vs_ptr, slots, slot_code, tables, width, num_tokens, query.size(1) // head_size, kvh,
-            head_size, cos_sin_cache.data_ptr(), cos_sin_cache.size(0), rot_dim,
-            key_cache.size(0), key_cache.size(2), query.stride(0), key.stride(0), v_stride,
-            DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype], 1 if overlap_previous else 0,
-            _lib.stream_of(dev)))
+    _lib.launch("tlb_qk_norm_rotary_embedding_neox", index, q_out.data_ptr(), None,
+                positions.data_ptr(), DTYPE_CODE[positions.dtype], query.data_ptr(),
+                key.data_ptr(), value.data_ptr(), query_weight.data_ptr(), key_weight.data_ptr(),
+                eps, key_cache.data_ptr(), value_cache.data_ptr(), ks_ptr, vs_ptr, slots,
+                slot_code, tables, width, num_tokens, query.size(1) // head_size, kvh, head_size,
+                cos_sin_cache.data_ptr(), rows, rot_dim, cshape[0], cshape[2], q_stride, k_stride,
+                v_stride, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype],
+                1 if overlap_previous else 0)
     return q_out

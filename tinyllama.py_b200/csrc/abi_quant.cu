@@ -240,9 +240,6 @@ int tlb_qk_norm_rotary_embedding_neox(
 
 namespace {
 
-// Least cost points (tiles) of a warp's range before another CTA joins.
-constexpr int kMinCost = 1;
-
 // A cache as a 2-D tensor of bytes-or-halves {head_dim, rows}, read in boxes of
 // {128 bytes or a whole shorter row, 2^box_shift rows}. Encoded for each call
 // (under a microsecond): nothing is kept by address.
@@ -277,18 +274,22 @@ extern "C" {
 
 int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t num_kv_heads,
                                               int64_t head_dim, int64_t block_size, int dtype,
-                                              int cache_dtype, size_t* bytes_out) {
-    TLB_REQUIRE(bytes_out != nullptr, "bytes_out must not be null");
+                                              int cache_dtype, size_t* bytes_out,
+                                              size_t* zeroed_out) {
+    TLB_REQUIRE(bytes_out != nullptr && zeroed_out != nullptr,
+                "bytes_out and zeroed_out must not be null");
     TLB_REQUIRE(num_heads > 0 && num_kv_heads > 0 && head_dim > 0 && block_size > 0,
                 "sizes must be positive");
     TLB_REQUIRE(num_heads % num_kv_heads == 0, "num_heads must be divisible by num_kv_heads");
-    *bytes_out = 0;
+    *bytes_out = *zeroed_out = 0;
     if (!tlb::scored::fast_supported(dtype, cache_dtype, (int)head_dim, (int)block_size))
         return TLB_OK;
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
-    *bytes_out =
-        tlb::scored::workspace_layout((int)(num_heads / num_kv_heads), (int)head_dim, sms).total;
+    const tlb::scored::Workspace w =
+        tlb::scored::workspace_layout((int)(num_heads / num_kv_heads), (int)head_dim, sms);
+    *bytes_out = w.total;
+    *zeroed_out = w.counters_end;
     return TLB_OK;
 }
 
@@ -354,7 +355,6 @@ int tlb_paged_attention_scored(void* out, const void* query, const void* key_cac
     p.max_blocks = (int)max_blocks_per_seq;
     p.max_tokens = (int)(max_blocks_per_seq * block_size);
     p.window = window < p.max_tokens ? (int)window : 0;
-    p.min_cost = kMinCost;
     p.scale = scale;
     p.cap_log2 = softcap * 1.4426950408889634f;
     p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
@@ -376,19 +376,23 @@ int tlb_paged_attention_scored(void* out, const void* query, const void* key_cac
     if (int rc = sm_count(&sms)) return rc;
     const long long units = (long long)p.units_per_seq * num_seqs;
     const long long unit_tiles = tiles / units;
-    p.aligned = units <= sms &&
-                unit_tiles <= (long long)sc::kAlignedTiles * sc::warps_for(p.unit_heads);
-    const int ctas = p.aligned ? (int)units : sc::ctas_for(tiles, p.group, sms, kMinCost);
-    const sc::Workspace w = sc::workspace_layout(p.group, p.head_dim, ctas);
+    const int warps = sc::warps_for(p.unit_heads);
+    p.aligned = units <= sms && unit_tiles <= (long long)sc::kAlignedTiles * warps;
+    const int ctas = p.aligned ? (int)units : sc::ctas_for(units, unit_tiles, p.group, sms);
+    // ceil(2^64 / warps)
+    p.inv_warps = ~0ull / (unsigned long long)(ctas * warps) + 1;
+    // laid out for the whole device whatever the grid: the counters' place, which
+    // is zero between calls, is the same for every call
+    const sc::Workspace w = sc::workspace_layout(p.group, p.head_dim, sms);
     if (workspace == nullptr || workspace_bytes < w.total || !aligned(workspace, 16))
         return fail(TLB_ERR_WORKSPACE,
                     "this call needs a 16-byte aligned workspace of %zu bytes (got %zu)", w.total,
                     workspace_bytes);
     char* ws = static_cast<char*>(workspace);
+    p.counters = reinterpret_cast<unsigned*>(ws);
     p.warp_partials = reinterpret_cast<float4*>(ws + w.warp_partials);
     p.cta_partials = reinterpret_cast<float4*>(ws + w.cta_partials);
     p.cta_ml = reinterpret_cast<float2*>(ws + w.cta_ml);
-    p.cta_ids = reinterpret_cast<int2*>(ws + w.cta_ids);
     const bool overlap = (flags & TLB_ATTN_OVERLAP_PROLOGUE) != 0;
     p.box_shift = sc::box_shift_of(p.block_size, tt);
     p.wait_limit = tlb::attention_wait_limit();

@@ -249,6 +249,9 @@ constexpr int warps_for(int heads) { return heads <= 8 ? 12 : 8; }
 // Tokens of a tile for rows of `bytes`: 4 KB of keys.
 constexpr int tile_tokens(int bytes) { return 4096 / bytes; }
 
+// CTAs that share a unit on average, at most: the last of them sums all their
+// partials.
+constexpr int kMaxShares = 32;
 // Most tiles of a unit for each warp of a CTA that takes it whole.
 constexpr int kAlignedTiles = 2;
 
@@ -265,7 +268,7 @@ struct Params {
     float4* warp_partials;        // [ctas][warps][fragments]
     float4* cta_partials;         // [2 * ctas][fragments]
     float2* cta_ml;               // [2 * ctas][unit heads padded] (reference, sum)
-    int2* cta_ids;                // [2 * ctas] (unit or -1, flags)
+    unsigned* counters;           // [ctas] arrivals at the unit that begins in a CTA, zero at rest
     long long num_blocks;
     long long query_stride;       // elements between sequences' query rows
     int num_seqs;
@@ -281,7 +284,7 @@ struct Params {
     int max_blocks;
     int max_tokens;               // max_blocks * block_size
     int window;                   // tokens the query sees, 0: all
-    int min_cost;                 // least cost points of a warp's range
+    unsigned long long inv_warps; // ceil(2^64 / warps of the grid)
     bool aligned;                 // a CTA takes one whole unit
     int box_shift;                // log2 of the cache rows a TMA box holds
     unsigned wait_limit;          // mbarrier probes before a wait gives up
@@ -296,14 +299,14 @@ struct Params {
 
 // Whether the tensor-core kernel serves these (aligned tensors assumed).
 bool fast_supported(int dtype, int cache_dtype, int head_dim, int block_size);
-// Bytes of the four workspace arrays for `ctas` CTAs.
+// Offsets of the workspace arrays for `ctas` CTAs; the counters come first.
 struct Workspace {
-    size_t warp_partials, cta_partials, cta_ml, cta_ids, total;
+    size_t counters_end, warp_partials, cta_partials, cta_ml, total;
 };
 Workspace workspace_layout(int group, int head_dim, int ctas);
 int unit_heads_of(int group);
-// CTAs worth launching for at most `max_tiles` tiles.
-int ctas_for(long long max_tiles, int group, int sms, int min_cost);
+// CTAs worth launching for `units` units with at most `unit_tiles` tiles each.
+int ctas_for(long long units, long long unit_tiles, int group, int sms);
 // log2 of the rows of a TMA box: the largest power of two that divides a block
 // and a tile.
 int box_shift_of(int block_size, int tile);

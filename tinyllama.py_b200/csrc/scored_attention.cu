@@ -135,21 +135,22 @@ int box_shift_of(int block_size, int tile) {
     return n;
 }
 
-int ctas_for(long long max_tiles, int group, int sms, int min_cost) {
-    const long long per = (long long)warps_for(unit_heads_of(group)) * min_cost;
-    const long long n = (max_tiles + per - 1) / per;
-    return (int)(n < 1 ? 1 : n < sms ? n : sms);
+int ctas_for(long long units, long long unit_tiles, int group, int sms) {
+    const int warps = warps_for(unit_heads_of(group));
+    const long long n = (units * unit_tiles + warps - 1) / warps;
+    const long long cap = units < sms ? units * kMaxShares < sms ? units * kMaxShares : sms : sms;
+    return (int)(n < 1 ? 1 : n < cap ? n : cap);
 }
 
 Workspace workspace_layout(int group, int head_dim, int ctas) {
     const int heads = unit_heads_of(group) <= 8 ? 8 : 16;
     const size_t frags = (size_t)heads / 8 * (head_dim / 16) * 32 * sizeof(float4);
     Workspace w;
-    w.warp_partials = 0;
-    w.cta_partials = (size_t)ctas * warps_for(heads) * frags;
+    w.counters_end = ((size_t)ctas * sizeof(unsigned) + 255) / 256 * 256;
+    w.warp_partials = w.counters_end;
+    w.cta_partials = w.warp_partials + (size_t)ctas * warps_for(heads) * frags;
     w.cta_ml = w.cta_partials + 2 * (size_t)ctas * frags;
-    w.cta_ids = w.cta_ml + 2 * (size_t)ctas * heads * sizeof(float2);
-    w.total = w.cta_ids + 2 * (size_t)ctas * sizeof(int2);
+    w.total = w.cta_ml + 2 * (size_t)ctas * heads * sizeof(float2);
     return w;
 }
 

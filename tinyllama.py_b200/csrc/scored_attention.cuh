@@ -33,13 +33,14 @@
 //    fp16 rounds by 2^-25 below its normal range is 2^-32 of the reference.
 //  * Where there are no more units than SMs and none has more than
 //    kAlignedTiles tiles a warp, a CTA takes a whole unit instead: even ranges
-//    would gain little, and no scan, no second kernel is needed.
+//    would gain little, and neither a scan nor a joining of CTAs is needed.
 //  * A unit cut by range ends leaves fp32 partials: warps of one CTA join
-//    theirs in shared memory, CTAs through the workspace in a second small
-//    kernel (programmatic launch). The order of every sum is fixed: results
-//    are the same bits on every run. Nothing in the workspace outlives a call.
+//    theirs in shared memory, CTAs through the workspace: the last CTA to
+//    publish its partial sums them all. The order of every sum is fixed, so
+//    results are the same bits on every run.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "kernels.h"
@@ -52,11 +53,13 @@ constexpr int kUnitCost = 1;       // tiles charged for starting a unit
 constexpr float kLazy = 8.f;       // log2 of how far a score may pass the reference
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Flags of a tile and, or-ed over a piece, of a partial.
+// Flags of a tile and, or-ed over a piece, of a partial. Above them the unit's
+// number of query heads (bits 4-8) and, in a tile's header, its first one.
 constexpr int kFirst = 1;      // first tile of a piece in this warp's range
 constexpr int kLast = 2;       // last tile of a piece in this warp's range
 constexpr int kUnitBegin = 4;  // first tile of its unit
 constexpr int kUnitEnd = 8;    // last tile of its unit
+constexpr int kHeadsShift = 4, kHeadsMask = 31 << kHeadsShift, kHead0Shift = 9;
 
 template <typename QT, typename CT, int D, int NT>
 struct Cfg {
@@ -93,7 +96,8 @@ struct Cfg {
     static constexpr int kMlOff = kScaleOff + (kQ8 ? kWarps * kStages * 2 * kTT : 0);
     static constexpr int kWeightOff = kMlOff + 2 * kWarps * kGroup * 8;
     static constexpr int kUnitOff = kWeightOff + 2 * kWarps * kGroup * 8;
-    static constexpr int kPrefixOff = kUnitOff + 2 * kWarps * 16;
+    static constexpr int kPointOff = kUnitOff + 2 * kWarps * 16;
+    static constexpr int kPrefixOff = kPointOff + (2 * kWarps * 8 + kWarps * kStages * 4 + 15) / 16 * 16;
     static constexpr int kSmem = kPrefixOff + (kThreads + kWarps) * 4 + 1024;  // + alignment slack
     static_assert(kSmem <= 232448, "one CTA per SM");
 };
@@ -196,38 +200,28 @@ __device__ __forceinline__ float max_of(uint32_t mask, float x) {
     return __int_as_float(m ^ ((m >> 31) & 0x7fffffff));
 }
 
-// Unit u: sequence, kv head and chunk of its query heads.
-struct Unit {
-    int s, kvh, head0, heads;
-};
-__device__ __forceinline__ Unit unit_of(int u, const Params& p) {
-    Unit r;
-    r.s = u / p.units_per_seq;
-    const int sub = u - r.s * p.units_per_seq;
-    r.kvh = sub / p.head_chunks;
-    const int hc = sub - r.kvh * p.head_chunks;
-    const int first = hc * p.unit_heads;
-    r.heads = min(p.unit_heads, p.group - first);
-    r.head0 = r.kvh * p.group + first;
-    return r;
-}
-
-// One fragment (dim tile i, lane) of a unit's output: (v.x, v.y) are heads
-// 2t, 2t + 1 of one dim, (v.z, v.w) of another: with 8-bit values the next
-// dim (dims 2g, 2g + 1 of the tile), otherwise dims g and g + 8.
-template <typename QT, bool Q8>
-__device__ __forceinline__ void write_frag(QT* out, const Params& p, const Unit& u, int D, int nt,
-                                           int i, int lane, float4 v, float inv0, float inv1) {
+// One fragment (dim tile i, lane) of a unit's output, whose first head is row
+// `row` of the [sequences * heads] output: (v.x, v.y) are heads 2t, 2t + 1 of
+// one dim, (v.z, v.w) of another: with 8-bit values the next dim (dims 2g,
+// 2g + 1 of the tile), otherwise dims g and g + 8.
+template <typename QT, bool Q8, int D>
+__device__ __forceinline__ void write_frag(void* out, int row, int heads, int nt, int i, int lane,
+                                           float4 v, float inv0, float inv1) {
     const int g = lane >> 2, h = nt * 8 + 2 * (lane & 3);
-    const int d0 = 16 * i + (Q8 ? 2 * g : g), d1 = Q8 ? d0 + 1 : d0 + 8;
-    QT* o = out + ((long long)u.s * p.num_heads + u.head0 + h) * D;
-    if (h < u.heads) {
-        o[d0] = Elem<QT>::from_f(v.x * inv0);
-        o[d1] = Elem<QT>::from_f(v.z * inv0);
-    }
-    if (h + 1 < u.heads) {
-        o[D + d0] = Elem<QT>::from_f(v.y * inv1);
-        o[D + d1] = Elem<QT>::from_f(v.w * inv1);
+    const int d0 = 16 * i + (Q8 ? 2 * g : g);
+    QT* o = reinterpret_cast<QT*>(out) + (long long)(row + h) * D + d0;
+    if constexpr (Q8) {
+        if (h < heads) *reinterpret_cast<uint32_t*>(o) = pack2<QT>(v.x * inv0, v.z * inv0);
+        if (h + 1 < heads) *reinterpret_cast<uint32_t*>(o + D) = pack2<QT>(v.y * inv1, v.w * inv1);
+    } else {
+        if (h < heads) {
+            o[0] = Elem<QT>::from_f(v.x * inv0);
+            o[8] = Elem<QT>::from_f(v.z * inv0);
+        }
+        if (h + 1 < heads) {
+            o[D] = Elem<QT>::from_f(v.y * inv1);
+            o[D + 8] = Elem<QT>::from_f(v.w * inv1);
+        }
     }
 }
 
@@ -263,10 +257,13 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     uint8_t* sc = smem + F::kScaleOff + warp * ST * 2 * TT;
     float2* ml = reinterpret_cast<float2*>(smem + F::kMlOff);      // [2 W][G] (m, l)
     float2* wl = reinterpret_cast<float2*>(smem + F::kWeightOff);  // [2 W][G] joint weight, times l
-    int4* ids = reinterpret_cast<int4*>(smem + F::kUnitOff);       // [2 W] (unit, flags, part)
+    int4* ids = reinterpret_cast<int4*>(smem + F::kUnitOff);       // [2 W] (row, flags, part)
+    int2* points = reinterpret_cast<int2*>(smem + F::kPointOff);   // [2 W] a unit's (first cost point, tiles)
+    int* hdr_point = reinterpret_cast<int*>(points + 2 * W) + warp * ST;  // first cost point
     int* pre = reinterpret_cast<int*>(smem + F::kPrefixOff);       // [THREADS] cost before, in warp
     int* wsum = pre + THREADS;                                     // [W] cost of a warp's threads
     __shared__ int parts_used;
+    __shared__ bool last_cta[2];
     const uint32_t bars = smem_u32(smem + F::kBarOff) + warp * ST * 8;
     const uint32_t ring = smem_u32(smem) + warp * F::kRingBytes;
 
@@ -288,6 +285,15 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     // ---- cursor of the tile loads
     int seq = 0, kvh = 0, chunk = 0, tile = 0, tile_begin = 0, tile_end = 0;
     int rel = 0, lim = 0;  // cost points from this warp's range start
+    unsigned total = 0, range0 = 0;  // cost points of the line, and where this range starts
+    // cost point at which warp w of the grid starts: total * w / nw, nw = W * gridDim.x,
+    // by multiplication with ceil(2^64 / nw): exact below 2^64 / nw. Lines shorter
+    // than nw go to the first warps, a point each: every CTA up to a unit's last
+    // one then holds a part of it.
+    auto start_of = [&](unsigned w) {
+        return total < W * gridDim.x ? min(w, total)
+                                     : (unsigned)__umul64hi((unsigned long long)total * w, p.inv_warps);
+    };
     Span span{0, 0};
     auto enter_seq = [&](int s) {
         seq = s;
@@ -327,17 +333,12 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
             const int v = __shfl_up_sync(0xffffffffu, before, o);
             if (lane >= o) before += v;
         }
-        const unsigned total = __shfl_sync(0xffffffffu, before, W - 1);
+        total = __shfl_sync(0xffffffffu, before, W - 1);
         before -= own;
-        // CTAs that take part: at least min_cost tiles' cost per warp
-        const unsigned least = W * p.min_cost;
-        const unsigned nw = W * max(1u, min(gridDim.x, (total + least - 1) / least));
         const unsigned wi = blockIdx.x * W + warp;
-        if (wi < nw) {
-            // the range [total * wi / nw, total * (wi + 1) / nw) in 32 bits
-            const unsigned q = total / nw, r = total - q * nw;
-            const unsigned a = q * wi + r * wi / nw;
-            lim = (int)(q * (wi + 1) + r * (wi + 1) / nw - a);
+        {
+            const unsigned a = range0 = start_of(wi);
+            lim = (int)(start_of(wi + 1) - a);
             if (lim > 0) {
                 // the sequence whose costs hold point a: the last thread whose
                 // cost before it is at most a (an empty one shares its number
@@ -356,8 +357,17 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                 }
                 enter_seq(s);
                 const unsigned unit_cost = tile_end - tile_begin + kUnitCost;
-                const int sub = at / unit_cost;
-                const int off = at - sub * unit_cost;
+                // at / unit_cost: the quotient is below 2^16, so the estimate is
+                // off by one at most
+                int sub = (int)__fdividef((float)at, (float)unit_cost);
+                int off = (int)(at - sub * unit_cost);
+                if (off < 0) {
+                    --sub;
+                    off += unit_cost;
+                } else if (off >= (int)unit_cost) {
+                    ++sub;
+                    off -= unit_cost;
+                }
                 kvh = p.head_chunks == 1 ? sub : sub / p.head_chunks;
                 chunk = sub - kvh * p.head_chunks;
                 // a unit's tiles sit at the end of its cost points
@@ -424,9 +434,13 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                                      (box_mask >> box) & 1);
                 cp_async_commit();
             }
+            const int in_group = chunk * p.unit_heads;
             int flags = (fresh ? kFirst : 0) | (tile == tile_begin ? kUnitBegin : 0) |
-                        (tile + 1 == tile_end ? kUnitEnd : 0);
-            const int u = seq * p.units_per_seq + kvh * p.head_chunks + chunk;
+                        (tile + 1 == tile_end ? kUnitEnd : 0) |
+                        min(p.unit_heads, p.group - in_group) << kHeadsShift |
+                        (kvh * p.group + in_group) << kHead0Shift;
+            const int u = seq;
+            const int point = (int)range0 + rel - (tile - tile_begin);
             // every token seen: box_mask 0 stands for it
             const uint32_t seen = box_mask == (1u << boxes) - 1u && lo == 0 && hi == TT
                                       ? 0u : 1u << 31 | box_mask << 16 | hi << 8 | lo;
@@ -456,7 +470,10 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                 tile = tile_begin;
             }
             if (fresh || rel >= lim) flags |= kLast;
-            if (lane == 0) hdr[slot] = make_int4((int)seen, pos0, u, flags);
+            if (lane == 0) {
+                hdr[slot] = make_int4((int)seen, pos0, u, flags);
+                hdr_point[slot] = point;
+            }
             fetch_bid();
         } else {
             if (lane == 0) hdr[slot] = make_int4(0, 0, -1, 0);
@@ -472,12 +489,22 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     fetch_bid();
     grid_dependency_wait();
 
+    // the CTA whose ranges hold cost point x
+    auto cta_of = [&](int x) {
+        int c = total < W * gridDim.x
+                    ? x / W
+                    : min((int)(__fdividef((float)x, (float)total) * gridDim.x), (int)gridDim.x - 1);
+        while (c > 0 && start_of(c * W) > (unsigned)x) --c;
+        while (start_of((c + 1) * W) <= (unsigned)x) ++c;
+        return c;
+    };
+
     // ---- state of the piece in flight
     uint32_t qf[NT][F::kTiles][2];
     float o[NT][F::kTiles][4];
     float m[NT][2], mv[NT][2], l[NT][2], qs[NT][2], slope[NT][2];
     int piece_flags = 0, last_pos = 0;
-    Unit un{0, 0, 0, 0};
+    int row = 0, heads = 0;  // output row of the unit's first head, its heads
     const ScoreMod mod{p.cap_log2, p.inv_cap, p.alibi_slopes != nullptr};
     QT* out = reinterpret_cast<QT*>(p.out);
     float4* part_a = p.warp_partials + ((long long)blockIdx.x * W + warp) * F::kFrags;
@@ -496,15 +523,17 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
         const int4 h = hdr[slot];
         if (h.z < 0) break;
         if (h.w & kFirst) {
-            piece_flags = h.w & kUnitBegin;
-            un = unit_of(h.z, p);
-            last_pos = min(max(p.seq_lens[un.s], 0), p.max_tokens) - 1;
+            piece_flags = h.w & (kUnitBegin | kHeadsMask);
+            heads = (h.w & kHeadsMask) >> kHeadsShift;
+            const int head0 = h.w >> kHead0Shift;
+            row = h.z * p.num_heads + head0;
+            last_pos = min(max(p.seq_lens[h.z], 0), p.max_tokens) - 1;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int head = nt * 8 + g;
-                const bool there = head < un.heads;
+                const bool there = head < heads;
                 const QT* q = reinterpret_cast<const QT*>(p.query) +
-                              (long long)un.s * p.query_stride + (long long)(un.head0 + head) * D;
+                              h.z * p.query_stride + (long long)(head0 + head) * D;
                 float scale_q = p.cap_log2 > 0.f ? p.scale : p.scale * kLog2e;
                 if constexpr (F::kQ8) {
                     uint2 raw[F::kTiles];
@@ -547,8 +576,8 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                     // this lane's score columns are heads 2 t4 + e
                     qs[nt][e] = __shfl_sync(0xffffffffu, scale_q, (2 * t4 + e) * 4);
                     const int hh = nt * 8 + 2 * t4 + e;
-                    slope[nt][e] = mod.alibi && hh < un.heads
-                                       ? p.alibi_slopes[un.head0 + hh] * kLog2e : 0.f;
+                    slope[nt][e] = mod.alibi && hh < heads
+                                       ? p.alibi_slopes[head0 + hh] * kLog2e : 0.f;
                     m[nt][e] = mv[nt][e] = -INFINITY;
                     l[nt][e] = 0.f;
                 }
@@ -800,7 +829,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
 
         if (h.w & kLast) {
             piece_flags |= h.w & kUnitEnd;
-            const bool whole = piece_flags == (kUnitBegin | kUnitEnd);
+            const bool whole = (piece_flags & ~kHeadsMask) == (kUnitBegin | kUnitEnd);
             // the last piece of the range stays in shared memory (the ring is
             // free: no tile follows), an earlier one goes to the workspace
             const bool end = hdr[slot + 1 == ST ? 0 : slot + 1].z < 0;
@@ -835,12 +864,16 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                     const float4 v = make_float4(o[nt][i][0] * fac[0], o[nt][i][1] * fac[1],
                                                  o[nt][i][2] * fac[0], o[nt][i][3] * fac[1]);
                     if (whole)
-                        write_frag<QT, F::kQ8>(out, p, un, D, nt, i, lane, v, inv[0], inv[1]);
+                        write_frag<QT, F::kQ8, D>(p.out, row, heads, nt, i, lane, v, inv[0], inv[1]);
                     else
                         dst[(nt * F::kTiles + i) * 32 + lane] = v;
                 }
             }
-            if (!whole && lane == 0) ids[entry] = make_int4(h.z, piece_flags, part, 0);
+            if (!whole && lane == 0) {
+                ids[entry] = make_int4(row, piece_flags, part, 0);
+                const Span sp = span_of(h.z, p);
+                points[entry] = make_int2(hdr_point[slot], (sp.len + TT - 1) / TT - sp.first / TT);
+            }
         }
         __syncwarp();
         if (++slot == ST) {
@@ -872,7 +905,8 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     const int4 mine = lane < 2 * W ? ids[lane] : make_int4(-1, 0, 0, 0);
     const uint32_t run = __match_any_sync(0xffffffffu, mine.x);  // entries of the same unit
     uint32_t there = __ballot_sync(0xffffffffu, mine.x >= 0);
-    int2 left = make_int2(-1, 0), right = make_int2(-1, 0);
+    // units that other CTAs share: [0] begins before this CTA, [1] ends after it
+    int shared_row[2] = {-1, -1}, owner[2] = {0, 0}, shares[2] = {0, 0}, shared_heads[2] = {0, 0};
     if (there) {
         // weights of the entries, a warp for each head
         if (mine.x >= 0)
@@ -891,49 +925,60 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
             const int e0 = __ffs(there) - 1;
             uint32_t k = __shfl_sync(0xffffffffu, run, e0);
             const int u = __shfl_sync(0xffffffffu, mine.x, e0);
-            const int flags = __reduce_or_sync(0xffffffffu, (k >> lane) & 1 ? mine.y : 0);
+            // the first entry says whether the unit begins here, the last
+            // whether it ends
+            const int flags = __shfl_sync(0xffffffffu, mine.y, e0) |
+                              __shfl_sync(0xffffffffu, mine.y, 31 - __clz(k));
+            const int n_heads = (flags & kHeadsMask) >> kHeadsShift;
             there &= ~k;
             const uint32_t entries = k;
-            const bool whole = flags == (kUnitBegin | kUnitEnd);
+            const bool whole = (flags & ~kHeadsMask) == (kUnitBegin | kUnitEnd);
             const int side = (flags & kUnitBegin) ? 1 : 0, at = 2 * blockIdx.x + side;
             if (!whole) {
-                if (side) right = make_int2(u, flags); else left = make_int2(u, flags);
+                // the CTAs of the unit's first and last tile
+                const int2 pt = points[e0];
+                const int first = cta_of(pt.x), n = cta_of(pt.x + pt.y - 1) - first + 1;
+#pragma unroll
+                for (int sd = 0; sd < 2; ++sd)
+                    if (sd == side) {
+                        shared_row[sd] = u;
+                        shared_heads[sd] = n_heads;
+                        owner[sd] = first;
+                        shares[sd] = n;
+                    }
             }
-            const Unit un_k = unit_of(u, p);
             for (int f0 = warp * 32; f0 < F::kFrags; f0 += THREADS) {
                 const int f = f0 + lane, nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles;
                 const int h0 = nt * 8 + 2 * (lane & 3);
                 float L0 = 0.f, L1 = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                // six entries' loads in flight, those past the last with weight 0
                 for (k = entries; k;) {
-                    // four entries' loads in flight
-                    float4 v[4], w[4];
+                    float4 v[6], w[6];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        v[j] = w[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (k) {
-                            const int e = __ffs(k) - 1;
-                            k &= k - 1;
-                            const int off = __shfl_sync(0xffffffffu, from, e);
-                            v[j] = off >= 0 ? reinterpret_cast<const float4*>(smem + off)[f]
-                                            : p.warp_partials[((long long)blockIdx.x * W + (e >> 1)) *
-                                                                  F::kFrags + f];
-                            w[j] = *reinterpret_cast<const float4*>(wl + e * G + h0);
-                        }
+                    for (int j = 0; j < 6; ++j) {
+                        const int e = k ? __ffs(k) - 1 : e0;
+                        const int off = __shfl_sync(0xffffffffu, from, e);
+                        v[j] = off >= 0 ? *reinterpret_cast<const float4*>(smem + off + 16 * f)
+                                        : p.warp_partials[((long long)blockIdx.x * W + (e >> 1)) *
+                                                              F::kFrags + f];
+                        w[j] = k ? *reinterpret_cast<const float4*>(wl + e * G + h0)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+                        k &= k - 1;
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        acc.x += w[j].x * v[j].x;
-                        acc.y += w[j].z * v[j].y;
-                        acc.z += w[j].x * v[j].z;
-                        acc.w += w[j].z * v[j].w;
+                    for (int j = 0; j < 6; ++j) {
+                        acc.x = fmaf(w[j].x, v[j].x, acc.x);
+                        acc.y = fmaf(w[j].z, v[j].y, acc.y);
+                        acc.z = fmaf(w[j].x, v[j].z, acc.z);
+                        acc.w = fmaf(w[j].z, v[j].w, acc.w);
                         L0 += w[j].y;
                         L1 += w[j].w;
                     }
                 }
                 if (whole) {
-                    write_frag<QT, F::kQ8>(out, p, un_k, D, nt, i, lane, acc, inverse(L0),
-                                           inverse(L1));
+                    write_frag<QT, F::kQ8, D>(p.out, u, n_heads, nt, i, lane, acc, inverse(L0),
+                                              inverse(L1));
                 } else {
                     p.cta_partials[(long long)at * F::kFrags + f] = acc;
                     if (i == 0 && lane < 4)
@@ -943,9 +988,61 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
             }
         }
     }
-    if (tid == 0 && !p.aligned) {
-        p.cta_ids[2 * blockIdx.x] = left;
-        p.cta_ids[2 * blockIdx.x + 1] = right;
+    // ---- join units across CTAs: the last CTA to publish its partial of a unit
+    // sums all of them, in range order whichever CTA it is. The counters are
+    // zero between calls.
+    if (shared_row[0] >= 0 || shared_row[1] >= 0) {
+        __syncthreads();
+        if (lane == 0 && warp < 2) {
+            const int c0 = warp ? owner[1] : owner[0], n = warp ? shares[1] : shares[0];
+            bool last = false;
+            if ((warp ? shared_row[1] : shared_row[0]) >= 0) {
+                __threadfence();
+                last = atomic_inc_acq_rel(p.counters + c0, n - 1) == (unsigned)n - 1;
+            }
+            last_cta[warp] = last;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int sd = 0; sd < 2; ++sd) {
+            if (!last_cta[sd]) continue;
+            const int c0 = sd ? owner[1] : owner[0], n = sd ? shares[1] : shares[0];
+            const int u = sd ? shared_row[1] : shared_row[0];
+            const int n_heads = sd ? shared_heads[1] : shared_heads[0];
+            for (int f = tid; f < F::kFrags; f += THREADS) {
+                const int nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles;
+                const int h0 = nt * 8 + 2 * (lane & 3);
+                float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k0 = 0; k0 < n; k0 += 4) {
+                    float4 v[4], w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        // past the last: the last again, with nothing in it
+                        const int k = min(k0 + j, n - 1), at = k == 0 ? 2 * c0 + 1 : 2 * (c0 + k);
+                        v[j] = __ldcg(p.cta_partials + (long long)at * F::kFrags + f);
+                        w[j] = __ldcg(reinterpret_cast<const float4*>(p.cta_ml + at * G + h0));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (k0 + j >= n) break;
+                        const float N0 = fmaxf(M0, w[j].x), N1 = fmaxf(M1, w[j].z);
+                        const float a0 = piece_weight(M0, N0), a1 = piece_weight(M1, N1);
+                        const float b0 = piece_weight(w[j].x, N0), b1 = piece_weight(w[j].z, N1);
+                        L0 = L0 * a0 + w[j].y * b0;
+                        L1 = L1 * a1 + w[j].w * b1;
+                        acc.x = acc.x * a0 + v[j].x * b0;
+                        acc.y = acc.y * a1 + v[j].y * b1;
+                        acc.z = acc.z * a0 + v[j].z * b0;
+                        acc.w = acc.w * a1 + v[j].w * b1;
+                        M0 = N0;
+                        M1 = N1;
+                    }
+                }
+                write_frag<QT, F::kQ8, D>(p.out, u, n_heads, nt, i, lane, acc, inverse(L0),
+                                          inverse(L1));
+            }
+        }
     }
     // ---- sequences with no token: zeros
     for (int s = blockIdx.x; s < p.num_seqs; s += gridDim.x) {
@@ -956,101 +1053,22 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     }
 }
 
-// Units that several CTAs share: CTA c takes the unit whose first partial is
-// c's right one; its others are the left partials of the CTAs after c, up to
-// the one that holds the unit's end. blockIdx.y takes a quarter of the
-// fragments; the threads split the partials of a fragment between them. What
-// the first 32 partials need is loaded before their number is known, so a
-// short join waits for memory once.
-constexpr int kJoinParts = 4;
-
-template <typename QT, bool Q8, int D, int NT>
-__global__ void __launch_bounds__(256) scored_join_kernel(const Params p, int ctas) {
-    constexpr int kTiles = D / 16, kFrags = NT * kTiles * 32, G = 8 * NT;
-    constexpr int P = kFrags / kJoinParts;  // fragments of this block
-    constexpr int LANES = 256 / P;          // threads per fragment
-    static_assert(P <= 256 && 256 % P == 0 && G % 8 == 0, "fragments split over the block");
-    __shared__ float sM[G], sL[G];
-    __shared__ float4 red[256];
-    const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int f = blockIdx.y * P + tid % P, part = tid / P;
-    auto slot = [&](int i) { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
-    grid_dependency_wait();
-    const int2 id = p.cta_ids[2 * c + 1];
-    const bool in = c + lane < ctas;
-    const int2 next = in && lane > 0 ? p.cta_ids[2 * (c + lane)] : make_int2(-1, 0);
-    float2 mine[G / 8];
-#pragma unroll
-    for (int i = 0; i < G / 8; ++i)
-        mine[i] = in ? p.cta_ml[slot(lane) * G + warp + 8 * i] : make_float2(-INFINITY, 0.f);
-    const float4 v0 = c + part < ctas ? p.cta_partials[(long long)slot(part) * kFrags + f]
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (id.x < 0) return;
-    // partials of the unit
-    uint32_t ends = __ballot_sync(0xffffffffu, next.x == id.x && (next.y & kUnitEnd));
-    int n = __ffs(ends);
-    for (int i0 = 32; n == 0 && c + i0 < ctas; i0 += 32) {
-        const int2 more = c + i0 + lane < ctas ? p.cta_ids[2 * (c + i0 + lane)] : make_int2(-1, 0);
-        ends = __ballot_sync(0xffffffffu, more.x == id.x && (more.y & kUnitEnd));
-        if (ends) n = i0 + __ffs(ends);
-    }
-    if (n == 0) return;  // a wait gave up: the status word says so
-#pragma unroll
-    for (int i = 0; i < G / 8; ++i) {
-        const int h = warp + 8 * i;
-        float M = lane < n ? mine[i].x : -INFINITY;
-        for (int k = lane + 32; k < n; k += 32) M = fmaxf(M, p.cta_ml[slot(k) * G + h].x);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        float L = lane < n ? piece_weight(mine[i].x, M) * mine[i].y : 0.f;
-        for (int k = lane + 32; k < n; k += 32) {
-            const float2 v = p.cta_ml[slot(k) * G + h];
-            L += piece_weight(v.x, M) * v.y;
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
-        if (lane == 0) {
-            sM[h] = M;
-            sL[h] = L;
-        }
-    }
-    __syncthreads();
-    const int nt = f / (kTiles * 32), fl = f & 31, h0 = nt * 8 + 2 * (fl & 3);
-    const float M0 = sM[h0], M1 = sM[h0 + 1];
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = part; i < n; i += LANES) {
-        const float4 v = i == part ? v0 : p.cta_partials[(long long)slot(i) * kFrags + f];
-        const float4 w = *reinterpret_cast<const float4*>(p.cta_ml + slot(i) * G + h0);
-        const float w0 = piece_weight(w.x, M0), w1 = piece_weight(w.z, M1);
-        acc.x += w0 * v.x;
-        acc.y += w1 * v.y;
-        acc.z += w0 * v.z;
-        acc.w += w1 * v.w;
-    }
-    red[tid] = acc;
-    __syncthreads();
-    if (part == 0) {
-        for (int i = 1; i < LANES; ++i) {
-            const float4 v = red[i * P + tid];
-            acc.x += v.x;
-            acc.y += v.y;
-            acc.z += v.z;
-            acc.w += v.w;
-        }
-        write_frag<QT, Q8>(reinterpret_cast<QT*>(p.out), p, unit_of(id.x, p), D, nt,
-                           (f >> 5) % kTiles, fl, acc, inverse(sL[h0]), inverse(sL[h0 + 1]));
-    }
-}
-
 template <typename QT, typename CT, int D, int NT>
 cudaError_t launch_fast(const Params& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
                         int ctas, bool overlap, cudaStream_t st) {
     using F = Cfg<QT, CT, D, NT>;
     auto kern = scored_attention_kernel<QT, CT, D, NT>;
-    cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+    // the attribute is the kernel's on one device: set once for each
+    static std::atomic<unsigned long long> set{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (!(set.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+        if (e != cudaSuccess) return e;
+        set.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1061,13 +1079,7 @@ cudaError_t launch_fast(const Params& p, const CUtensorMap& map_k, const CUtenso
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = overlap ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kern, map_k, map_v, p);
-    if (e != cudaSuccess || p.aligned) return e;
-    cfg.gridDim = dim3(ctas, kJoinParts);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, scored_join_kernel<QT, F::kQ8, D, NT>, p, ctas);
+    return cudaLaunchKernelEx(&cfg, kern, map_k, map_v, p);
 }
 
 template <typename QT, typename CT>
