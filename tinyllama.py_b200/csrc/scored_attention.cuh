@@ -489,14 +489,22 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     fetch_bid();
     grid_dependency_wait();
 
-    // the CTA whose ranges hold cost point x
-    auto cta_of = [&](int x) {
-        int c = total < W * gridDim.x
-                    ? x / W
-                    : min((int)(__fdividef((float)x, (float)total) * gridDim.x), (int)gridDim.x - 1);
-        while (c > 0 && start_of(c * W) > (unsigned)x) --c;
-        while (start_of((c + 1) * W) <= (unsigned)x) ++c;
-        return c;
+    // the CTAs (from this one down, from this one up) whose ranges hold cost
+    // points x0 <= x1 of a unit that this CTA has a part of; 32 CTAs a step
+    auto first_cta = [&](unsigned x0) {
+        for (int c = blockIdx.x;; c -= 32) {
+            const int mine = c - lane;
+            const uint32_t at = __ballot_sync(0xffffffffu, mine <= 0 || start_of(mine * W) <= x0);
+            if (at) return c - (__ffs(at) - 1);
+        }
+    };
+    auto final_cta = [&](unsigned x1) {
+        for (int c = blockIdx.x;; c += 32) {
+            const int mine = c + lane;
+            const uint32_t at = __ballot_sync(0xffffffffu, mine >= (int)gridDim.x - 1 ||
+                                                               start_of((mine + 1) * W) > x1);
+            if (at) return c + __ffs(at) - 1;
+        }
     };
 
     // ---- state of the piece in flight
@@ -921,6 +929,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
         // byte offset of the entry's partial in shared memory, -1: workspace
         const int from = (lane & 1) ? (lane >> 1) * F::kRingBytes
                          : mine.z < F::kParts ? F::kPartOff + mine.z * F::kPartBytes : -1;
+#pragma unroll 1
         while (there) {
             const int e0 = __ffs(there) - 1;
             uint32_t k = __shfl_sync(0xffffffffu, run, e0);
@@ -937,7 +946,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
             if (!whole) {
                 // the CTAs of the unit's first and last tile
                 const int2 pt = points[e0];
-                const int first = cta_of(pt.x), n = cta_of(pt.x + pt.y - 1) - first + 1;
+                const int first = first_cta(pt.x), n = final_cta(pt.x + pt.y - 1) - first + 1;
 #pragma unroll
                 for (int sd = 0; sd < 2; ++sd)
                     if (sd == side) {
@@ -947,34 +956,31 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                         shares[sd] = n;
                     }
             }
+#pragma unroll 1
             for (int f0 = warp * 32; f0 < F::kFrags; f0 += THREADS) {
                 const int f = f0 + lane, nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles;
                 const int h0 = nt * 8 + 2 * (lane & 3);
                 float L0 = 0.f, L1 = 0.f;
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                // six entries' loads in flight, those past the last with weight 0
-                for (k = entries; k;) {
-                    float4 v[6], w[6];
-#pragma unroll
-                    for (int j = 0; j < 6; ++j) {
-                        const int e = k ? __ffs(k) - 1 : e0;
-                        const int off = __shfl_sync(0xffffffffu, from, e);
-                        v[j] = off >= 0 ? *reinterpret_cast<const float4*>(smem + off + 16 * f)
-                                        : p.warp_partials[((long long)blockIdx.x * W + (e >> 1)) *
-                                                              F::kFrags + f];
-                        w[j] = k ? *reinterpret_cast<const float4*>(wl + e * G + h0)
-                                 : make_float4(0.f, 0.f, 0.f, 0.f);
-                        k &= k - 1;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 6; ++j) {
-                        acc.x = fmaf(w[j].x, v[j].x, acc.x);
-                        acc.y = fmaf(w[j].z, v[j].y, acc.y);
-                        acc.z = fmaf(w[j].x, v[j].z, acc.z);
-                        acc.w = fmaf(w[j].z, v[j].w, acc.w);
-                        L0 += w[j].y;
-                        L1 += w[j].w;
-                    }
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), v, w;
+                auto fetch = [&](int e) {
+                    const int off = __shfl_sync(0xffffffffu, from, e);
+                    v = off >= 0 ? *reinterpret_cast<const float4*>(smem + off + 16 * f)
+                                 : p.warp_partials[((long long)blockIdx.x * W + (e >> 1)) *
+                                                       F::kFrags + f];
+                    w = *reinterpret_cast<const float4*>(wl + e * G + h0);
+                };
+                fetch(e0);
+#pragma unroll 1
+                for (k = entries & (entries - 1);; k &= k - 1) {
+                    const float4 v0 = v, w0 = w;
+                    if (k) fetch(__ffs(k) - 1);
+                    acc.x = fmaf(w0.x, v0.x, acc.x);
+                    acc.y = fmaf(w0.z, v0.y, acc.y);
+                    acc.z = fmaf(w0.x, v0.z, acc.z);
+                    acc.w = fmaf(w0.z, v0.w, acc.w);
+                    L0 += w0.y;
+                    L1 += w0.w;
+                    if (!k) break;
                 }
                 if (whole) {
                     write_frag<QT, F::kQ8, D>(p.out, u, n_heads, nt, i, lane, acc, inverse(L0),
@@ -1009,34 +1015,48 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
             const int c0 = sd ? owner[1] : owner[0], n = sd ? shares[1] : shares[0];
             const int u = sd ? shared_row[1] : shared_row[0];
             const int n_heads = sd ? shared_heads[1] : shared_heads[0];
+#pragma unroll 1
             for (int f = tid; f < F::kFrags; f += THREADS) {
                 const int nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles;
                 const int h0 = nt * 8 + 2 * (lane & 3);
                 float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int k0 = 0; k0 < n; k0 += 4) {
-                    float4 v[4], w[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        // past the last: the last again, with nothing in it
-                        const int k = min(k0 + j, n - 1), at = k == 0 ? 2 * c0 + 1 : 2 * (c0 + k);
-                        v[j] = __ldcg(p.cta_partials + (long long)at * F::kFrags + f);
-                        w[j] = __ldcg(reinterpret_cast<const float4*>(p.cta_ml + at * G + h0));
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (k0 + j >= n) break;
-                        const float N0 = fmaxf(M0, w[j].x), N1 = fmaxf(M1, w[j].z);
-                        const float a0 = piece_weight(M0, N0), a1 = piece_weight(M1, N1);
-                        const float b0 = piece_weight(w[j].x, N0), b1 = piece_weight(w[j].z, N1);
-                        L0 = L0 * a0 + w[j].y * b0;
-                        L1 = L1 * a1 + w[j].w * b1;
-                        acc.x = acc.x * a0 + v[j].x * b0;
-                        acc.y = acc.y * a1 + v[j].y * b1;
-                        acc.z = acc.z * a0 + v[j].z * b0;
-                        acc.w = acc.w * a1 + v[j].w * b1;
-                        M0 = N0;
-                        M1 = N1;
+                float4 v, w;
+                auto fetch = [&](int k) {
+                    const int at = k == 0 ? 2 * c0 + 1 : 2 * (c0 + k);
+                    v = __ldcg(p.cta_partials + (long long)at * F::kFrags + f);
+                    w = __ldcg(reinterpret_cast<const float4*>(p.cta_ml + at * G + h0));
+                };
+                auto add = [&](const float4& x, const float4& y) {
+                    const float N0 = fmaxf(M0, y.x), N1 = fmaxf(M1, y.z);
+                    const float a0 = piece_weight(M0, N0), a1 = piece_weight(M1, N1);
+                    const float b0 = piece_weight(y.x, N0), b1 = piece_weight(y.z, N1);
+                    L0 = L0 * a0 + y.y * b0;
+                    L1 = L1 * a1 + y.w * b1;
+                    acc.x = acc.x * a0 + x.x * b0;
+                    acc.y = acc.y * a1 + x.y * b1;
+                    acc.z = acc.z * a0 + x.z * b0;
+                    acc.w = acc.w * a1 + x.w * b1;
+                    M0 = N0;
+                    M1 = N1;
+                };
+                // four partials' loads in flight
+                int k = 0;
+                while (k < n) {
+                    fetch(k);
+                    const float4 v0 = v, w0 = w;
+                    fetch(min(k + 1, n - 1));
+                    const float4 v1 = v, w1 = w;
+                    fetch(min(k + 2, n - 1));
+                    const float4 v2 = v, w2 = w;
+                    fetch(min(k + 3, n - 1));
+                    float4 x = v0, y = w0;
+#pragma unroll 1
+                    for (int j = 0;; ++j) {
+                        add(x, y);
+                        if (++k == n || j == 3) break;
+                        x = j == 0 ? v1 : j == 1 ? v2 : v;
+                        y = j == 0 ? w1 : j == 1 ? w2 : w;
                     }
                 }
                 write_frag<QT, F::kQ8, D>(p.out, u, n_heads, nt, i, lane, acc, inverse(L0),
