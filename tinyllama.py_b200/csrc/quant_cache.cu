@@ -10,62 +10,123 @@ namespace tlb {
 
 namespace {
 
-// Eight elements <-> registers, 16-byte accesses for half types, two for fp32.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-    constexpr int N = 8 * sizeof(T) / 16;
+// Eight elements, as read: 16 bytes of half types, 32 of fp32.
+template <typename T> struct Raw8 {
+    static constexpr int N = 8 * sizeof(T) / 16;
     uint4 u[N];
+    __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
-    const T* e = reinterpret_cast<const T*>(u);
+        for (int i = 0; i < N; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    // read once, by one SM
+    __device__ __forceinline__ void load_stream(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f(e[i]);
+        for (int i = 0; i < N; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        const T* e = reinterpret_cast<const T*>(u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f(e[i]);
+    }
+    __device__ __forceinline__ void set(const float (&f)[8]) {
+        if constexpr (sizeof(T) == 2) {
+            u[0] = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]),
+                              pack2<T>(f[6], f[7]));
+        } else {
+            T* e = reinterpret_cast<T*>(u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = f[i];
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
+    }
+    // fp32 bits of the largest magnitude, infinities and NaN above all numbers.
+    // The bits of a type's magnitudes are ordered, so half types compare in
+    // pairs of 16-bit integers.
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(T) == 2)
+                    m = __vmaxu2(m, w[k] & 0x7fff7fffu);
+                else
+                    m = max(m, w[k] & 0x7fffffffu);
+            }
+        }
+        return m;
+    }
+};
+// top() of a row from the maximum of its lanes' (combined with max_top).
+template <typename T> __device__ __forceinline__ uint32_t max_top(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 2)
+        return __vmaxu2(a, b);
+    else
+        return max(a, b);
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-    constexpr int N = 8 * sizeof(T) / 16;
-    uint4 u[N];
-    T* e = reinterpret_cast<T*>(u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f(f[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
+template <typename T> __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
+    if constexpr (sizeof(T) == 2) {
+        const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+        T e;
+        memcpy(&e, &h, 2);
+        return __float_as_uint(Elem<T>::to_f(e));
+    } else {
+        return m;
+    }
 }
 
-__device__ __forceinline__ uint32_t max_abs8(const float (&f)[8]) {
+__device__ __forceinline__ uint32_t max_finite8(const float (&f)[8]) {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, finite_abs_bits(f[i]));
     return m;
 }
 
-template <typename C>
-__device__ __forceinline__ void store_quantized8(C* dst, const float (&f)[8], float inv) {
+template <typename C, bool kBounded>
+__device__ __forceinline__ uint2 quantized8(const float (&f)[8], float inv) {
     uint2 u;
-    u.x = quantize4<C>(mul_keep(f[0], inv), mul_keep(f[1], inv), mul_keep(f[2], inv),
-                       mul_keep(f[3], inv));
-    u.y = quantize4<C>(mul_keep(f[4], inv), mul_keep(f[5], inv), mul_keep(f[6], inv),
-                       mul_keep(f[7], inv));
-    *reinterpret_cast<uint2*>(dst) = u;
+    u.x = quantize4<C, kBounded>(mul_keep(f[0], inv), mul_keep(f[1], inv), mul_keep(f[2], inv),
+                                 mul_keep(f[3], inv));
+    u.y = quantize4<C, kBounded>(mul_keep(f[4], inv), mul_keep(f[5], inv), mul_keep(f[6], inv),
+                                 mul_keep(f[7], inv));
+    return u;
 }
 template <typename C>
 __device__ __forceinline__ void store_quantized1(C* dst, float x, float inv) {
-    *reinterpret_cast<uint8_t*>(dst) = (uint8_t)quantize4<C>(mul_keep(x, inv), 0.f, 0.f, 0.f);
+    *reinterpret_cast<uint8_t*>(dst) =
+        (uint8_t)quantize4<C, false>(mul_keep(x, inv), 0.f, 0.f, 0.f);
 }
 
-// Maximum over the `lanes` (a power of two) lanes of a group, which `mask`
-// names.
-__device__ __forceinline__ uint32_t group_max(uint32_t v, int lanes, uint32_t mask) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(mask, v, o));
+// Over the LANES (a power of two) lanes of a group, which `mask` names.
+template <int LANES>
+__device__ __forceinline__ uint32_t group_max(uint32_t v, uint32_t mask) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(mask, v, o));
     return v;
 }
-__device__ __forceinline__ float group_sum(float v, int lanes, uint32_t mask) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+template <int LANES, typename T>
+__device__ __forceinline__ uint32_t group_top(uint32_t v, uint32_t mask) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max_top<T>(v, __shfl_xor_sync(mask, v, o));
+    return top_bits<T>(v);
+}
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v, uint32_t mask) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
     return v;
 }
-__device__ __forceinline__ uint32_t group_mask(int lanes) {
-    const uint32_t ones = lanes == 32 ? 0xffffffffu : (1u << lanes) - 1u;
-    return ones << ((threadIdx.x & 31) / lanes * lanes);
+template <int LANES> __device__ __forceinline__ uint32_t group_mask() {
+    constexpr uint32_t ones = LANES == 32 ? 0xffffffffu : (1u << (LANES & 31)) - 1u;
+    return ones << ((threadIdx.x & 31) / LANES * LANES);
 }
 
 __device__ __forceinline__ long long load_int(const void* p, bool wide, long long i) {
@@ -73,22 +134,37 @@ __device__ __forceinline__ long long load_int(const void* p, bool wide, long lon
                 : (long long)reinterpret_cast<const int32_t*>(p)[i];
 }
 
+// (quotient, remainder) by a positive 32-bit divisor; 32-bit division when the
+// dividend fits, a quarter of the instructions.
+__device__ __forceinline__ long long divide(long long x, int by, int& rest) {
+    if (x < (1ll << 32)) {
+        const unsigned q = (unsigned)x / (unsigned)by;
+        rest = (int)((unsigned)x - q * (unsigned)by);
+        return q;
+    }
+    const long long q = x / by;
+    rest = (int)(x - q * by);
+    return q;
+}
+
 // Row index of (slot's block, head 0, slot's offset) in a
 // [blocks, kv_heads, block_size] cache, or -1 to skip the token.
 __device__ __forceinline__ long long slot_row(long long slot, const QuantCacheParams& p) {
     if (slot < 0) return -1;
-    const long long blk = slot / p.block_size;
+    int off;
+    const long long blk = divide(slot, p.block_size, off);
     if (blk >= p.num_blocks) {
         flag_status(TLB_STATUS_BAD_SLOT);
         return -1;
     }
-    return blk * p.num_kv_heads * p.block_size + (slot - blk * p.block_size);
+    return blk * p.num_kv_heads * p.block_size + off;
 }
 
 // The row of token t at position pos through its block-table row.
 __device__ __forceinline__ long long table_row(long long t, long long pos,
                                                const QuantCacheParams& p) {
-    const long long logical = pos < 0 ? -1 : pos / p.block_size;
+    int off = 0;
+    const long long logical = pos < 0 ? -1 : divide(pos, p.block_size, off);
     if (logical < 0 || logical >= p.max_blocks) {
         flag_status(TLB_STATUS_BAD_SLOT);
         return -1;
@@ -99,25 +175,81 @@ __device__ __forceinline__ long long table_row(long long t, long long pos,
         flag_status(TLB_STATUS_BAD_SLOT);
         return -1;
     }
-    return blk * p.num_kv_heads * p.block_size + (pos - logical * p.block_size);
+    return blk * p.num_kv_heads * p.block_size + off;
 }
 
 // ------------------------------------------------------------- cache write
-// A row is read by `lanes` lanes, eight elements each (VEC), which keep it in
-// registers between the maximum and the store; rows of other widths or
-// alignments take a warp each, element by element, and read the row twice.
-template <typename T, typename C, bool VEC>
-__global__ void __launch_bounds__(256) quantize_write_kernel(const QuantCacheParams p, int lanes) {
-    const int per_block = 256 / lanes;
-    const int sub = threadIdx.x % lanes;
-    const uint32_t mask = group_mask(lanes);
+// HBM bound: 2 e D bytes in, D + 1 out for each row of e-byte values. A warp
+// takes rows of one token (its slot is looked up once): all keys, then all
+// values. A row is held by LANES lanes, eight elements each (16-byte loads,
+// 8-byte stores), between its one read and its one write; kSteps rows of a
+// group are in flight. Rows wider than 256, of a width that is no multiple of
+// eight, or unaligned take a warp each, element by element, and are read twice.
+// Eight-element lanes against sixteen, 16381 fp16 tokens of 8 heads of 128 to
+// int8: see the table of the design notes for the rate reached.
+constexpr int kSteps = 4;
+
+template <typename T, typename C, int LANES>
+__global__ void __launch_bounds__(256) quantize_write_kernel(const QuantCacheParams p, int parts) {
+    constexpr int GROUPS = 32 / LANES;
+    const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
+    const uint32_t mask = group_mask<LANES>();
+    const int D = p.head_size, rows = 2 * p.num_kv_heads;
+    const bool on = sub * 8 < D;
+    const long long items = p.num_tokens * parts;
+    const int warps = gridDim.x * 8;
+    for (long long it = blockIdx.x * 8 + threadIdx.x / 32; it < items; it += warps) {
+        int part;
+        const long long t = divide(it, parts, part);
+        const long long base = slot_row(load_int(p.slots, p.slots64, t), p);
+        if (base < 0) continue;
+        const T* key = reinterpret_cast<const T*>(p.key) + t * p.key_stride + sub * 8;
+        const T* value = reinterpret_cast<const T*>(p.value) + t * p.value_stride + sub * 8;
+        for (int r0 = part * GROUPS * kSteps + grp; r0 < rows; r0 += parts * GROUPS * kSteps) {
+            Raw8<T> raw[kSteps];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int r = r0 + i * GROUPS;
+                const bool is_value = r >= p.num_kv_heads;
+                const int h = is_value ? r - p.num_kv_heads : r;
+                raw[i].zero();
+                if (r < rows && on) raw[i].load_stream((is_value ? value : key) + h * D);
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const int r = r0 + i * GROUPS;
+                if (r >= rows) break;
+                const bool is_value = r >= p.num_kv_heads;
+                const int h = is_value ? r - p.num_kv_heads : r;
+                const long long row = base + (long long)h * p.block_size;
+                float f[8];
+                raw[i].get(f);
+                uint32_t top = group_top<LANES, T>(raw[i].top(), mask);
+                uint2 q;
+                if (top < 0x7f800000u) {
+                    q = quantized8<C, true>(f, inverse_scale(scale_byte<C>(top)));
+                } else {
+                    top = group_max<LANES>(max_finite8(f), mask);
+                    q = quantized8<C, false>(f, inverse_scale(scale_byte<C>(top)));
+                }
+                if (on)
+                    *reinterpret_cast<uint2*>(
+                        reinterpret_cast<uint8_t*>(is_value ? p.value_cache : p.key_cache) +
+                        row * D + sub * 8) = q;
+                if (sub == 0)
+                    (is_value ? p.value_scales : p.key_scales)[row] = (uint8_t)scale_byte<C>(top);
+            }
+        }
+    }
+}
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) quantize_write_any_kernel(const QuantCacheParams p) {
+    const int lane = threadIdx.x & 31, D = p.head_size;
     const long long rows = p.num_tokens * 2 * p.num_kv_heads;
-    const int D = p.head_size;
-    for (long long r = (long long)blockIdx.x * per_block + threadIdx.x / lanes; r < rows;
-         r += (long long)gridDim.x * per_block) {
-        const long long th = r / p.num_kv_heads;
-        const int h = (int)(r - th * p.num_kv_heads);
-        const long long t = th >> 1;
+    for (long long r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8) {
+        int h;
+        const long long th = divide(r, p.num_kv_heads, h), t = th >> 1;
         const bool is_value = th & 1;
         const long long base = slot_row(load_int(p.slots, p.slots64, t), p);
         if (base < 0) continue;
@@ -125,82 +257,101 @@ __global__ void __launch_bounds__(256) quantize_write_kernel(const QuantCachePar
         const T* src = reinterpret_cast<const T*>(is_value ? p.value : p.key) +
                        t * (is_value ? p.value_stride : p.key_stride) + (long long)h * D;
         C* dst = reinterpret_cast<C*>(is_value ? p.value_cache : p.key_cache) + row * D;
-        uint8_t* scale = (is_value ? p.value_scales : p.key_scales) + row;
-        if constexpr (VEC) {
-            const bool on = sub * 8 < D;
-            float f[8] = {};
-            if (on) load8(src + sub * 8, f);
-            const uint32_t byte = scale_byte<C>(group_max(max_abs8(f), lanes, mask));
-            if (on) store_quantized8(dst + sub * 8, f, inverse_scale(byte));
-            if (sub == 0) *scale = (uint8_t)byte;
-        } else {
-            uint32_t m = 0;
-            for (int i = sub; i < D; i += lanes) m = max(m, finite_abs_bits(Elem<T>::to_f(src[i])));
-            const uint32_t byte = scale_byte<C>(group_max(m, lanes, mask));
-            const float inv = inverse_scale(byte);
-            for (int i = sub; i < D; i += lanes)
-                store_quantized1(dst + i, Elem<T>::to_f(src[i]), inv);
-            if (sub == 0) *scale = (uint8_t)byte;
-        }
+        uint32_t m = 0;
+        for (int i = lane; i < D; i += 32) m = max(m, finite_abs_bits(Elem<T>::to_f(src[i])));
+        const uint32_t byte = scale_byte<C>(group_max<32>(m, 0xffffffffu));
+        const float inv = inverse_scale(byte);
+        for (int i = lane; i < D; i += 32) store_quantized1(dst + i, Elem<T>::to_f(src[i]), inv);
+        if (lane == 0) (is_value ? p.value_scales : p.key_scales)[row] = (uint8_t)byte;
     }
 }
 
 // -------------------------------------------------------------- read back
-// Flat over 16-value pieces of the listed blocks; the two caches' pieces of a
-// thread are in flight together. Pieces never straddle a row.
-template <typename T, typename C, int VEC>
+// HBM bound: D + 1 bytes in, e D out for each row. Flat over 16-value pieces of
+// the listed blocks (pieces never straddle a row); two pieces of both caches are
+// in flight for each thread. IX: index type of the piece arithmetic (32-bit
+// unsigned where it fits).
+template <typename T, typename C>
+__device__ __forceinline__ void widen16(T* out, uint4 u, float scale) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            f[j] = mul_keep(dequantize1<C>((w[2 * half + (j >> 2)] >> (8 * (j & 3))) & 0xff), scale);
+        Raw8<T> r;
+        r.set(f);
+        r.store(out + 8 * half);
+    }
+}
+
+template <typename T, typename C, typename IX>
 __global__ void __launch_bounds__(256) dequantize_blocks_kernel(const DequantParams p) {
+    constexpr int U = 2;
+    const unsigned row_pieces = p.head_size / 16;
+    const IX pieces = (IX)p.rows_per_block * row_pieces;  // of a block
+    const IX total = pieces * (IX)p.num_ids;
+    const IX step = (IX)gridDim.x * 256;
+    const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.key_cache);
+    const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.value_cache);
+    for (IX i0 = (IX)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += U * step) {
+        uint4 k[U], v[U];
+        uint32_t ks[U], vs[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const IX i = i0 + j * step;
+            k[j] = v[j] = make_uint4(0, 0, 0, 0);
+            ks[j] = vs[j] = 0;
+            if (i < total && i >= i0) {
+                const IX n = i / pieces;
+                const unsigned piece = (unsigned)(i - n * pieces);
+                const long long blk = load_int(p.ids, p.ids64, n);
+                if (blk >= p.num_blocks) flag_status(TLB_STATUS_BAD_BLOCK_ID);
+                if (blk >= 0 && blk < p.num_blocks) {
+                    const long long from = (blk * (long long)pieces + piece) * 16;
+                    const long long row = blk * p.rows_per_block + piece / row_pieces;
+                    k[j] = __ldcs(reinterpret_cast<const uint4*>(kc + from));
+                    v[j] = __ldcs(reinterpret_cast<const uint4*>(vc + from));
+                    ks[j] = p.key_scales[row];
+                    vs[j] = p.value_scales[row];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const IX i = i0 + j * step;
+            if (i < total && i >= i0) {
+                widen16<T, C>(reinterpret_cast<T*>(p.key_out) + (long long)i * 16, k[j],
+                              scale_value(ks[j]));
+                widen16<T, C>(reinterpret_cast<T*>(p.value_out) + (long long)i * 16, v[j],
+                              scale_value(vs[j]));
+            }
+        }
+    }
+}
+
+// Any row width and alignment, value by value.
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) dequantize_any_kernel(const DequantParams p) {
     const long long block_values = (long long)p.rows_per_block * p.head_size;
-    const long long pieces = block_values / VEC;
-    const long long total = pieces * p.num_ids;
+    const long long total = block_values * p.num_ids;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
          i += (long long)gridDim.x * 256) {
-        const long long n = i / pieces;
-        const long long at = (i - n * pieces) * VEC;  // value within the block
+        const long long n = i / block_values, at = i - n * block_values;
         const long long blk = load_int(p.ids, p.ids64, n);
-        T* ok = reinterpret_cast<T*>(p.key_out) + n * block_values + at;
-        T* ov = reinterpret_cast<T*>(p.value_out) + n * block_values + at;
-        const bool there = blk >= 0 && blk < p.num_blocks;
+        float k = 0.f, v = 0.f;
         if (blk >= p.num_blocks) flag_status(TLB_STATUS_BAD_BLOCK_ID);
-        const long long from = there ? blk * block_values + at : 0;
-        const long long row = there ? blk * p.rows_per_block + at / p.head_size : 0;
-        if constexpr (VEC == 16) {
-            uint4 uk = make_uint4(0, 0, 0, 0), uv = uk;
-            uint32_t bk = 0, bv = 0;
-            if (there) {
-                uk = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.key_cache) +
-                                                     from);
-                uv = *reinterpret_cast<const uint4*>(
-                    reinterpret_cast<const uint8_t*>(p.value_cache) + from);
-                bk = p.key_scales[row];
-                bv = p.value_scales[row];
-            }
-            const float sk = scale_value(bk), sv = scale_value(bv);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float f[8];
-                const uint32_t k0 = half ? uk.z : uk.x, k1 = half ? uk.w : uk.y;
-                const uint32_t v0 = half ? uv.z : uv.x, v1 = half ? uv.w : uv.y;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    f[j] = mul_keep(dequantize1<C>(((j < 4 ? k0 : k1) >> (8 * (j & 3))) & 0xff), sk);
-                store8(ok + 8 * half, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    f[j] = mul_keep(dequantize1<C>(((j < 4 ? v0 : v1) >> (8 * (j & 3))) & 0xff), sv);
-                store8(ov + 8 * half, f);
-            }
-        } else {
-            float fk = 0.f, fv = 0.f;
-            if (there) {
-                fk = mul_keep(dequantize1<C>(reinterpret_cast<const uint8_t*>(p.key_cache)[from]),
-                              scale_value(p.key_scales[row]));
-                fv = mul_keep(dequantize1<C>(reinterpret_cast<const uint8_t*>(p.value_cache)[from]),
-                              scale_value(p.value_scales[row]));
-            }
-            *ok = Elem<T>::from_f(fk);
-            *ov = Elem<T>::from_f(fv);
+        if (blk >= 0 && blk < p.num_blocks) {
+            const long long from = blk * block_values + at;
+            const long long row = blk * p.rows_per_block + at / p.head_size;
+            k = mul_keep(dequantize1<C>(reinterpret_cast<const uint8_t*>(p.key_cache)[from]),
+                         scale_value(p.key_scales[row]));
+            v = mul_keep(dequantize1<C>(reinterpret_cast<const uint8_t*>(p.value_cache)[from]),
+                         scale_value(p.value_scales[row]));
         }
+        reinterpret_cast<T*>(p.key_out)[i] = Elem<T>::from_f(k);
+        reinterpret_cast<T*>(p.value_out)[i] = Elem<T>::from_f(v);
     }
 }
 
@@ -213,117 +364,118 @@ __global__ void __launch_bounds__(256) dequantize_blocks_kernel(const DequantPar
 // rounded to the storage type, so the bytes are those of a separate
 // quantising write of this kernel's key.
 //
-// An item is one row kind (query, key, value) of one token. VEC: `lanes`
-// lanes hold a row, 16 values each: lane l < rot/16 the eight values at 8 l and
-// their partners at 8 l + rot/2 (so the rotation needs no exchange), the
-// others 16 values beyond rot. Otherwise a warp walks the row by element.
-template <typename T, typename C>
-__device__ __forceinline__ void store_row16(C* cache, uint8_t* scales, long long row, int D, int i0,
-                                            int i1, bool on, int sub, const float (&a)[8],
-                                            const float (&b)[8], int lanes, uint32_t mask) {
-    if constexpr (sizeof(C) == 1) {
-        const uint32_t m = on ? max(max_abs8(a), max_abs8(b)) : 0u;
-        const uint32_t byte = scale_byte<C>(group_max(m, lanes, mask));
-        const float inv = inverse_scale(byte);
-        if (on) {
-            store_quantized8(cache + row * D + i0, a, inv);
-            store_quantized8(cache + row * D + i1, b, inv);
-        }
-        if (sub == 0) scales[row] = (uint8_t)byte;
-    } else if (on) {
-        store8(cache + row * D + i0, a);
-        store8(cache + row * D + i1, b);
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ float rounded(float x) {
-    return Elem<T>::to_f(Elem<T>::from_f(x));
-}
-
+// HBM bound (every row read and written once). A warp takes rows of one token,
+// so that position, cos/sin row and slot are looked up once: query heads, key
+// heads, value heads. A row is held by LANES lanes, 16 values each: lane
+// l < rot/16 the eight values at 8 l and their partners at 8 l + rot/2 (so the
+// rotation needs no exchange), the others 16 values beyond rot. A group keeps
+// its weights while it stays with queries or with keys, and has two rows in
+// flight. Other widths and alignments: a warp for each row, by element.
 enum RowKind { kQuery = 0, kKey = 1, kValue = 2 };
 
-template <typename T, typename C, bool VEC>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QuantCacheParams p, int lanes) {
+struct NormRow {
+    RowKind kind;
+    int h;
+};
+__device__ __forceinline__ NormRow norm_row(int r, const QuantCacheParams& p) {
+    if (r < p.num_heads) return {kQuery, r};
+    r -= p.num_heads;
+    return r < p.num_kv_heads ? NormRow{kKey, r} : NormRow{kValue, r - p.num_kv_heads};
+}
+
+template <typename T, typename C, int LANES>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QuantCacheParams p, int parts) {
     grid_launch_dependents();
-    const int per_block = 256 / lanes;
-    const int sub = threadIdx.x % lanes;
-    const uint32_t mask = group_mask(lanes);
+    constexpr int GROUPS = 32 / LANES, U = 2;
+    const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
+    const uint32_t mask = group_mask<LANES>();
     const int D = p.head_size, rot = p.rot_dim, half = rot / 2;
     const bool with_cache = p.key_cache != nullptr;
-    const int per_token = p.num_heads + p.num_kv_heads * (with_cache ? 2 : 1);
-    const long long items = p.num_tokens * per_token;
-    for (long long it = (long long)blockIdx.x * per_block + threadIdx.x / lanes; it < items;
-         it += (long long)gridDim.x * per_block) {
-        const long long t = it / per_token;
-        int h = (int)(it - t * per_token);
-        RowKind kind = kQuery;
-        if (h >= p.num_heads) {
-            h -= p.num_heads;
-            kind = kKey;
-            if (h >= p.num_kv_heads) {
-                h -= p.num_kv_heads;
-                kind = kValue;
-            }
-        }
+    const int rows = p.num_heads + p.num_kv_heads * (with_cache ? 2 : 1);
+    const int pairs = rot / 16;  // lanes that rotate
+    const bool on = sub * 16 < D, turn = on && sub < pairs;
+    const int i0 = sub < pairs ? 8 * sub : rot + 16 * (sub - pairs);
+    const int i1 = sub < pairs ? i0 + half : i0 + 8;
+    const float inv_d = 1.f / (float)D;
+    const long long items = p.num_tokens * parts;
+    const int warps = gridDim.x * 8;
+    for (long long it = blockIdx.x * 8 + threadIdx.x / 32; it < items; it += warps) {
+        int part;
+        const long long t = divide(it, parts, part);
         const long long pos = load_int(p.positions, p.positions64, t);
-        const T* cs = nullptr;
-        if (pos >= 0 && pos < p.cache_rows)
-            cs = reinterpret_cast<const T*>(p.cos_sin) + pos * rot;
-        else if (kind != kValue)
-            flag_status(TLB_STATUS_BAD_POSITION);
-        long long row = -1;  // cache row of this item
-        if (with_cache && kind != kQuery) {
-            row = p.slots ? slot_row(load_int(p.slots, p.slots64, t), p) : table_row(t, pos, p);
-            if (row < 0) continue;
-            row += (long long)h * p.block_size;
-        }
-        const T* src;
-        T* dst = nullptr;
-        if (kind == kQuery) {
-            src = reinterpret_cast<const T*>(p.query) + t * p.query_stride + (long long)h * D;
-            dst = reinterpret_cast<T*>(p.out) + (t * p.num_heads + h) * D;
-        } else if (kind == kKey) {
-            src = reinterpret_cast<const T*>(p.key) + t * p.key_stride + (long long)h * D;
-            if (!with_cache) dst = reinterpret_cast<T*>(p.key_out) + (t * p.num_kv_heads + h) * D;
+        float c[8], s[8];
+        bool rotate = turn;
+        if (pos >= 0 && pos < p.cache_rows) {
+            if (turn) {
+                const T* cs = reinterpret_cast<const T*>(p.cos_sin) + pos * rot;
+                Raw8<T> r;
+                r.load(cs + i0);
+                r.get(c);
+                r.load(cs + half + i0);
+                r.get(s);
+            }
         } else {
-            src = reinterpret_cast<const T*>(p.value) + t * p.value_stride + (long long)h * D;
+            flag_status(TLB_STATUS_BAD_POSITION);
+            rotate = false;
         }
-        C* cache = reinterpret_cast<C*>(kind == kValue ? p.value_cache : p.key_cache);
-        uint8_t* scales = kind == kValue ? p.value_scales : p.key_scales;
-        const T* w = reinterpret_cast<const T*>(kind == kQuery ? p.query_weight : p.key_weight);
-        if constexpr (VEC) {
-            const int pairs = rot / 16;  // lanes that rotate
-            const bool on = sub * 16 < D, turn = sub < pairs;
-            const int i0 = turn ? 8 * sub : rot + 16 * (sub - pairs);
-            const int i1 = turn ? i0 + half : i0 + 8;
-            float a[8] = {}, b[8] = {}, wa[8], wb[8], c[8], s[8];
-            if (on && kind != kValue) {
-                load8(w + i0, wa);
-                load8(w + i1, wb);
-                if (turn && cs) {
-                    load8(cs + i0, c);
-                    load8(cs + half + i0, s);
+        long long base = -1;  // cache row of the token for head 0
+        if (with_cache)
+            base = p.slots ? slot_row(load_int(p.slots, p.slots64, t), p) : table_row(t, pos, p);
+        grid_dependency_wait();
+        const T* query = reinterpret_cast<const T*>(p.query) + t * p.query_stride;
+        const T* key = reinterpret_cast<const T*>(p.key) + t * p.key_stride;
+        const T* value = reinterpret_cast<const T*>(p.value) + t * p.value_stride;
+        Raw8<T> w0, w1;  // weights of the group's current kind
+        int have = -1;
+        for (int r0 = part * GROUPS * U + grp; r0 < rows; r0 += parts * GROUPS * U) {
+            Raw8<T> x0[U], x1[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int r = r0 + i * GROUPS;
+                x0[i].zero();
+                x1[i].zero();
+                if (r < rows && on) {
+                    const NormRow nr = norm_row(r, p);
+                    const T* src = (nr.kind == kQuery ? query : nr.kind == kKey ? key : value) +
+                                   nr.h * D;
+                    x0[i].load_stream(src + i0);
+                    x1[i].load_stream(src + i1);
                 }
             }
-            grid_dependency_wait();
-            if (on) {
-                load8(src + i0, a);
-                load8(src + i1, b);
-            }
-            if (kind != kValue) {
-                float ss = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ss += a[j] * a[j] + b[j] * b[j];
-                ss = group_sum(ss, lanes, mask);
-                const float inv = rsqrtf(ss / (float)D + p.eps);
-                if (on) {
+            for (int i = 0; i < U; ++i) {
+                const int r = r0 + i * GROUPS;
+                if (r >= rows) break;
+                const NormRow nr = norm_row(r, p);
+                if (nr.kind != kValue) {
+                    if (have != nr.kind) {
+                        have = nr.kind;
+                        const T* w = reinterpret_cast<const T*>(nr.kind == kQuery ? p.query_weight
+                                                                                  : p.key_weight);
+                        w0.zero();
+                        w1.zero();
+                        if (on) {
+                            w0.load(w + i0);
+                            w1.load(w + i1);
+                        }
+                    }
+                    float a[8], b[8], w[8];
+                    x0[i].get(a);
+                    x1[i].get(b);
+                    float sa = 0.f, sb = 0.f;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        a[j] = a[j] * inv * wa[j];
-                        b[j] = b[j] * inv * wb[j];
+                        sa = fmaf(a[j], a[j], sa);
+                        sb = fmaf(b[j], b[j], sb);
                     }
-                    if (turn && cs) {
+                    const float inv = rsqrtf(group_sum<LANES>(sa + sb, mask) * inv_d + p.eps);
+                    w0.get(w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) a[j] = a[j] * inv * w[j];
+                    w1.get(w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) b[j] = b[j] * inv * w[j];
+                    if (rotate) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             float x, y;
@@ -332,61 +484,132 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QuantCacheParam
                             b[j] = y;
                         }
                     }
+                    x0[i].set(a);
+                    x1[i].set(b);
                 }
-            }
-            if (dst) {
-                if (on) {
-                    store8(dst + i0, a);
-                    store8(dst + i1, b);
-                }
-            } else {
-                if constexpr (sizeof(C) == 1) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        a[j] = rounded<T>(a[j]);
-                        b[j] = rounded<T>(b[j]);
+                if (nr.kind == kQuery || !with_cache) {
+                    T* dst = nr.kind == kQuery
+                                 ? reinterpret_cast<T*>(p.out) + (t * p.num_heads + nr.h) * D
+                                 : reinterpret_cast<T*>(p.key_out) + (t * p.num_kv_heads + nr.h) * D;
+                    if (on) {
+                        x0[i].store(dst + i0);
+                        x1[i].store(dst + i1);
                     }
+                    continue;
                 }
-                store_row16<T, C>(cache, scales, row, D, i0, i1, on, sub, a, b, lanes, mask);
+                if (base < 0) continue;
+                const long long row = base + (long long)nr.h * p.block_size;
+                if constexpr (sizeof(C) == 1) {
+                    float a[8], b[8];
+                    x0[i].get(a);
+                    x1[i].get(b);
+                    uint32_t top =
+                        group_top<LANES, T>(max_top<T>(x0[i].top(), x1[i].top()), mask);
+                    uint2 q0, q1;
+                    if (top < 0x7f800000u) {
+                        const float qs = inverse_scale(scale_byte<C>(top));
+                        q0 = quantized8<C, true>(a, qs);
+                        q1 = quantized8<C, true>(b, qs);
+                    } else {
+                        top = group_max<LANES>(max(max_finite8(a), max_finite8(b)), mask);
+                        const float qs = inverse_scale(scale_byte<C>(top));
+                        q0 = quantized8<C, false>(a, qs);
+                        q1 = quantized8<C, false>(b, qs);
+                    }
+                    uint8_t* dst = reinterpret_cast<uint8_t*>(nr.kind == kValue ? p.value_cache
+                                                                                : p.key_cache) +
+                                   row * D;
+                    if (on) {
+                        *reinterpret_cast<uint2*>(dst + i0) = q0;
+                        *reinterpret_cast<uint2*>(dst + i1) = q1;
+                    }
+                    if (sub == 0)
+                        (nr.kind == kValue ? p.value_scales : p.key_scales)[row] =
+                            (uint8_t)scale_byte<C>(top);
+                } else if (on) {
+                    T* dst = reinterpret_cast<T*>(nr.kind == kValue ? p.value_cache : p.key_cache) +
+                             row * D;
+                    x0[i].store(dst + i0);
+                    x1[i].store(dst + i1);
+                }
             }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float rounded(float x) {
+    return Elem<T>::to_f(Elem<T>::from_f(x));
+}
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(const QuantCacheParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, D = p.head_size, rot = p.rot_dim, half = rot / 2;
+    const bool with_cache = p.key_cache != nullptr;
+    const int rows = p.num_heads + p.num_kv_heads * (with_cache ? 2 : 1);
+    const long long items = p.num_tokens * rows;
+    for (long long it = blockIdx.x * 8 + threadIdx.x / 32; it < items; it += gridDim.x * 8) {
+        int r;
+        const long long t = divide(it, rows, r);
+        const NormRow nr = norm_row(r, p);
+        const long long pos = load_int(p.positions, p.positions64, t);
+        const T* cs = nullptr;
+        if (pos >= 0 && pos < p.cache_rows)
+            cs = reinterpret_cast<const T*>(p.cos_sin) + pos * rot;
+        else
+            flag_status(TLB_STATUS_BAD_POSITION);
+        long long row = -1;  // cache row of this item
+        if (with_cache && nr.kind != kQuery) {
+            row = p.slots ? slot_row(load_int(p.slots, p.slots64, t), p) : table_row(t, pos, p);
+            if (row < 0) continue;
+            row += (long long)nr.h * p.block_size;
+        }
+        const T* src = nr.kind == kQuery ? reinterpret_cast<const T*>(p.query) + t * p.query_stride
+                       : nr.kind == kKey ? reinterpret_cast<const T*>(p.key) + t * p.key_stride
+                                         : reinterpret_cast<const T*>(p.value) + t * p.value_stride;
+        src += (long long)nr.h * D;
+        const T* w = reinterpret_cast<const T*>(nr.kind == kQuery ? p.query_weight : p.key_weight);
+        float inv = 0.f;
+        if (nr.kind != kValue) {
+            float ss = 0.f;
+            for (int i = lane; i < D; i += 32) {
+                const float x = Elem<T>::to_f(src[i]);
+                ss = fmaf(x, x, ss);
+            }
+            inv = rsqrtf(group_sum<32>(ss, 0xffffffffu) * (1.f / (float)D) + p.eps);
+        }
+        auto out = [&](int i) -> float {
+            float x = Elem<T>::to_f(src[i]);
+            if (nr.kind == kValue) return x;
+            x = x * inv * Elem<T>::to_f(w[i]);
+            if (i >= rot || !cs) return x;
+            const bool first = i < half;
+            const int j = first ? i + half : i - half, k = first ? i : j;
+            const float y = Elem<T>::to_f(src[j]) * inv * Elem<T>::to_f(w[j]);
+            float xo, yo;
+            rope_pair(first ? x : y, first ? y : x, Elem<T>::to_f(cs[k]),
+                      Elem<T>::to_f(cs[half + k]), xo, yo);
+            return first ? xo : yo;
+        };
+        if (nr.kind == kQuery || !with_cache) {
+            T* dst = nr.kind == kQuery
+                         ? reinterpret_cast<T*>(p.out) + (t * p.num_heads + nr.h) * D
+                         : reinterpret_cast<T*>(p.key_out) + (t * p.num_kv_heads + nr.h) * D;
+            for (int i = lane; i < D; i += 32) dst[i] = Elem<T>::from_f(out(i));
+            continue;
+        }
+        C* dst = reinterpret_cast<C*>(nr.kind == kValue ? p.value_cache : p.key_cache) + row * D;
+        if constexpr (sizeof(C) == 1) {
+            uint32_t m = 0;
+            for (int i = lane; i < D; i += 32) m = max(m, finite_abs_bits(rounded<T>(out(i))));
+            const uint32_t byte = scale_byte<C>(group_max<32>(m, 0xffffffffu));
+            const float qs = inverse_scale(byte);
+            for (int i = lane; i < D; i += 32) store_quantized1(dst + i, rounded<T>(out(i)), qs);
+            if (lane == 0) (nr.kind == kValue ? p.value_scales : p.key_scales)[row] = (uint8_t)byte;
         } else {
-            grid_dependency_wait();
-            float inv = 0.f;
-            if (kind != kValue) {
-                float ss = 0.f;
-                for (int i = sub; i < D; i += lanes) {
-                    const float x = Elem<T>::to_f(src[i]);
-                    ss += x * x;
-                }
-                inv = rsqrtf(group_sum(ss, lanes, mask) / (float)D + p.eps);
-            }
-            auto value = [&](int i) -> float {
-                float x = Elem<T>::to_f(src[i]);
-                if (kind == kValue) return x;
-                x = x * inv * Elem<T>::to_f(w[i]);
-                if (i >= rot || !cs) return x;
-                const bool first = i < half;
-                const int j = first ? i + half : i - half, k = first ? i : j;
-                const float y = Elem<T>::to_f(src[j]) * inv * Elem<T>::to_f(w[j]);
-                float xo, yo;
-                rope_pair(first ? x : y, first ? y : x, Elem<T>::to_f(cs[k]),
-                          Elem<T>::to_f(cs[half + k]), xo, yo);
-                return first ? xo : yo;
-            };
-            if (dst) {
-                for (int i = sub; i < D; i += lanes) dst[i] = Elem<T>::from_f(value(i));
-            } else if constexpr (sizeof(C) == 1) {
-                uint32_t m = 0;
-                for (int i = sub; i < D; i += lanes)
-                    m = max(m, finite_abs_bits(rounded<T>(value(i))));
-                const uint32_t byte = scale_byte<C>(group_max(m, lanes, mask));
-                const float qs = inverse_scale(byte);
-                for (int i = sub; i < D; i += lanes)
-                    store_quantized1(cache + row * D + i, rounded<T>(value(i)), qs);
-                if (sub == 0) scales[row] = (uint8_t)byte;
-            } else {
-                for (int i = sub; i < D; i += lanes) cache[row * D + i] = Elem<T>::from_f(value(i));
-            }
+            for (int i = lane; i < D; i += 32) dst[i] = Elem<T>::from_f(out(i));
         }
     }
 }
@@ -399,28 +622,39 @@ int sm_count() {
         return 148;
     return n;
 }
-// CTAs of 256 threads for `items` items of `lanes` lanes: all of them up to
-// eight CTAs per SM, which then stride.
-int grid_of(long long items, int lanes) {
-    const long long need = (items * lanes + 255) / 256, cap = (long long)sm_count() * 8;
+// CTAs of 256 threads that stride over `items` items of `per_cta` a CTA.
+int grid_of(long long items, int per_cta, int ctas_per_sm = 8) {
+    const long long need = (items + per_cta - 1) / per_cta, cap = (long long)sm_count() * ctas_per_sm;
     return (int)(need < cap ? (need > 0 ? need : 1) : cap);
 }
-// Lanes of a row of `units` units: the power of two that holds them.
-int lanes_for(int units) {
-    int n = 1;
-    while (n < units) n <<= 1;
-    return n;
+// Warps that share a token's `rows` rows, `step` rows each time: as many as keep
+// 16 warps an SM busy, one where there are tokens enough.
+int parts_of(long long tokens, int rows, int step) {
+    const int most = (rows + step - 1) / step;
+    const long long want = (16ll * sm_count() + tokens - 1) / tokens;
+    return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
+template <typename T, typename C, int LANES>
+void write_lanes(const QuantCacheParams& p, cudaStream_t st) {
+    const int parts = parts_of(p.num_tokens, 2 * p.num_kv_heads, 32 / LANES * kSteps);
+    quantize_write_kernel<T, C, LANES>
+        <<<grid_of(p.num_tokens * parts, 8), 256, 0, st>>>(p, parts);
+}
 template <typename T, typename C>
 cudaError_t write_tc(const QuantCacheParams& p, bool vec, cudaStream_t st) {
-    const long long rows = p.num_tokens * 2 * p.num_kv_heads;
-    if (vec && p.head_size <= 256) {
-        const int lanes = lanes_for(p.head_size / 8);
-        quantize_write_kernel<T, C, true><<<grid_of(rows, lanes), 256, 0, st>>>(p, lanes);
-    } else {
-        quantize_write_kernel<T, C, false><<<grid_of(rows, 32), 256, 0, st>>>(p, 32);
-    }
+    const int units = vec ? p.head_size / 8 : 33;
+    if (units <= 4)
+        write_lanes<T, C, 4>(p, st);
+    else if (units <= 8)
+        write_lanes<T, C, 8>(p, st);
+    else if (units <= 16)
+        write_lanes<T, C, 16>(p, st);
+    else if (units <= 32)
+        write_lanes<T, C, 32>(p, st);
+    else
+        quantize_write_any_kernel<T, C>
+            <<<grid_of(p.num_tokens * 2 * p.num_kv_heads, 8), 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 template <typename T>
@@ -431,10 +665,14 @@ cudaError_t write_t(int cache_dtype, const QuantCacheParams& p, bool vec, cudaSt
 template <typename T, typename C>
 cudaError_t dequant_tc(const DequantParams& p, bool vec, cudaStream_t st) {
     const long long values = p.num_ids * p.rows_per_block * p.head_size;
-    if (vec)
-        dequantize_blocks_kernel<T, C, 16><<<grid_of(values / 16, 1), 256, 0, st>>>(p);
+    // 32-bit piece numbers, with room for one step past the end
+    if (vec && values / 16 < (1ll << 31))
+        dequantize_blocks_kernel<T, C, unsigned><<<grid_of(values / 32, 256), 256, 0, st>>>(p);
+    else if (vec)
+        dequantize_blocks_kernel<T, C, unsigned long long>
+            <<<grid_of(values / 32, 256), 256, 0, st>>>(p);
     else
-        dequantize_blocks_kernel<T, C, 1><<<grid_of(values, 1), 256, 0, st>>>(p);
+        dequantize_any_kernel<T, C><<<grid_of(values, 256), 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 template <typename T>
@@ -443,14 +681,16 @@ cudaError_t dequant_t(int cache_dtype, const DequantParams& p, bool vec, cudaStr
                                    : dequant_tc<T, E4M3>(p, vec, st);
 }
 
+template <typename T, typename C, int LANES>
+cudaError_t norm_lanes(const QuantCacheParams& p, cudaLaunchConfig_t& cfg) {
+    const int rows = p.num_heads + p.num_kv_heads * (p.key_cache != nullptr ? 2 : 1);
+    const int parts = parts_of(p.num_tokens, rows, 32 / LANES * 2);
+    cfg.gridDim = dim3(grid_of(p.num_tokens * parts, 8));
+    return cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<T, C, LANES>, p, parts);
+}
 template <typename T, typename C>
 cudaError_t norm_tc(const QuantCacheParams& p, bool vec, cudaStream_t st) {
-    const long long rows =
-        p.num_tokens * (p.num_heads + p.num_kv_heads * (p.key_cache != nullptr ? 2 : 1));
-    vec = vec && p.head_size <= 512;
-    const int lanes = vec ? lanes_for(p.head_size / 16) : 32;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid_of(rows, lanes));
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -458,8 +698,15 @@ cudaError_t norm_tc(const QuantCacheParams& p, bool vec, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.overlap ? 1 : 0;
-    if (vec) return cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<T, C, true>, p, lanes);
-    return cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<T, C, false>, p, lanes);
+    const int units = vec ? p.head_size / 16 : 33;
+    if (units <= 4) return norm_lanes<T, C, 4>(p, cfg);
+    if (units <= 8) return norm_lanes<T, C, 8>(p, cfg);
+    if (units <= 16) return norm_lanes<T, C, 16>(p, cfg);
+    if (units <= 32) return norm_lanes<T, C, 32>(p, cfg);
+    const long long rows =
+        p.num_tokens * (p.num_heads + p.num_kv_heads * (p.key_cache != nullptr ? 2 : 1));
+    cfg.gridDim = dim3(grid_of(rows, 8));
+    return cudaLaunchKernelEx(&cfg, qk_norm_rope_any_kernel<T, C>, p);
 }
 template <typename T>
 cudaError_t norm_t(int cache_dtype, const QuantCacheParams& p, bool vec, cudaStream_t st) {
