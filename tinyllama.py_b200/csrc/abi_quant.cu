@@ -58,7 +58,7 @@ int cache_checks(const void* key_cache, const void* value_cache, int64_t num_tok
                 "cache sizes must be positive");
     TLB_REQUIRE(num_tokens < (1ll << 40) && num_kv_heads < (1 << 16) && head_size < (1 << 16) &&
                     block_size < (1 << 20) && num_blocks < (1ll << 31) &&
-                    num_kv_heads * block_size < (1ll << 31),
+                    num_kv_heads * block_size * head_size < (1ll << 31),
                 "sizes exceed the supported range");
     TLB_REQUIRE(key_cache && value_cache, "cache pointers must not be null");
     return TLB_OK;
@@ -102,8 +102,7 @@ int tlb_reshape_and_cache_quantized(const void* key, const void* value, void* ke
     p.num_kv_heads = (int)num_kv_heads;
     p.head_size = (int)head_size;
     p.block_size = (int)block_size;
-    // rows of the cache start at multiples of head_size bytes: 8-byte stores
-    const bool vec = head_size % 8 == 0 && vec_ok(dtype, {key, value, key_cache, value_cache},
+    const bool vec = head_size % 16 == 0 && vec_ok(dtype, {key, value, key_cache, value_cache},
                                                   {key_stride, value_stride});
     return cuda_result(tlb::launch_quantize_write(dtype, cache_dtype, p, vec,
                                                   reinterpret_cast<cudaStream_t>(stream)),
@@ -163,7 +162,7 @@ int tlb_qk_norm_rotary_embedding_neox(
     TLB_REQUIRE(num_tokens >= 0 && num_heads > 0 && num_kv_heads > 0 && head_size > 0,
                 "sizes must be positive");
     TLB_REQUIRE(num_tokens < (1ll << 40) && num_heads < (1 << 16) && num_kv_heads < (1 << 16) &&
-                    head_size < (1 << 16),
+                    head_size < (1 << 16) && (num_heads + num_kv_heads) * head_size < (1ll << 30),
                 "sizes exceed the supported range");
     TLB_REQUIRE(rot_dim > 0 && rot_dim % 2 == 0, "rotary dimension must be even and positive");
     TLB_REQUIRE(rot_dim <= head_size, "rotary dimension must not exceed head_size");

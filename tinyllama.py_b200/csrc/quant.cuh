@@ -68,23 +68,31 @@ __device__ __forceinline__ float inverse_scale(uint32_t byte) {
 // 2^E (E >= -126; byte 0, which the writes here never store, reads as 0).
 __device__ __forceinline__ float scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// Four scaled values -> four stored bytes (first in the low byte). kBounded: all
-// are finite (and so at most qmax), which spares int8 the conversion unit:
-// x + 1.5 * 2^23 is the nearest integer, to even, in the low bits.
+// Four values times 2^-E -> four stored bytes (first in the low byte). kBounded:
+// all are finite (and so at most qmax), which spares int8 the conversion unit:
+// x * 2^-E + 1.5 * 2^23, rounded once, is the nearest integer, to even, in the low
+// bits.
 template <typename C, bool kBounded>
-__device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d) {
-    if constexpr (sizeof(C) == 1 && Quant8<C>::kTopExponent == 8) {  // e4m3
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d, float inv) {
+    if constexpr (Quant8<C>::kTopExponent == 8) {  // e4m3
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(mul_keep(a, inv), mul_keep(b, inv)),
+                                                     __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(mul_keep(c, inv), mul_keep(d, inv)),
+                                                     __NV_SATFINITE, __NV_E4M3);
         return lo | (hi << 16);
     } else if constexpr (kBounded) {
-        auto one = [](float x) { return __float_as_uint(__fadd_rn(x, 12582912.f)); };
-        const uint32_t lo = __byte_perm(one(a), one(b), 0x0040), hi = __byte_perm(one(c), one(d), 0x0040);
+        auto one = [inv](float x) {
+            float y;  // subnormal x kept, as in mul_keep
+            asm("fma.rn.f32 %0, %1, %2, 0f4B400000;" : "=f"(y) : "f"(x), "f"(inv));
+            return __float_as_uint(y);
+        };
+        const uint32_t lo = __byte_perm(one(a), one(b), 0x0040);
+        const uint32_t hi = __byte_perm(one(c), one(d), 0x0040);
         return __byte_perm(lo, hi, 0x5410);
     } else {
-        auto one = [](float x) {
+        auto one = [inv](float x) {
             // NaN converts to 0, infinities to the integer bounds
-            return (uint32_t)min(max(__float2int_rn(x), -127), 127) & 0xffu;
+            return (uint32_t)min(max(__float2int_rn(mul_keep(x, inv)), -127), 127) & 0xffu;
         };
         return one(a) | (one(b) << 8) | (one(c) << 16) | (one(d) << 24);
     }

@@ -3,12 +3,40 @@
 //
 // All three are streaming kernels bounded by HBM; each row is held in the
 // registers of a few lanes between its one read and its one write.
+#include <type_traits>
+
 #include "kernels.h"
 #include "quant.cuh"
 
 namespace tlb {
 
 namespace {
+
+// Of two words of elements the larger magnitudes, NaN kept.
+template <typename T> __device__ __forceinline__ uint32_t max_top(uint32_t a, uint32_t b) {
+    uint32_t m;
+    if constexpr (std::is_same<T, __half>::value)
+        asm("{\n\t.reg .b32 x, y;\n\tabs.f16x2 x, %1;\n\tabs.f16x2 y, %2;\n\t"
+            "max.NaN.f16x2 %0, x, y;\n\t}" : "=r"(m) : "r"(a), "r"(b));
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm("{\n\t.reg .b32 x, y;\n\tabs.bf16x2 x, %1;\n\tabs.bf16x2 y, %2;\n\t"
+            "max.NaN.bf16x2 %0, x, y;\n\t}" : "=r"(m) : "r"(a), "r"(b));
+    else
+        m = max(a & 0x7fffffffu, b & 0x7fffffffu);
+    return m;
+}
+// fp32 bits of the largest magnitude of such a word: infinities and NaN come
+// above all numbers.
+template <typename T> __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
+    if constexpr (sizeof(T) == 2) {
+        const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+        T e;
+        memcpy(&e, &h, 2);
+        return __float_as_uint(Elem<T>::to_f(e)) & 0x7fffffffu;
+    } else {
+        return m;
+    }
+}
 
 // Eight elements, as read: 16 bytes of half types, 32 of fp32.
 template <typename T> struct Raw8 {
@@ -46,42 +74,19 @@ template <typename T> struct Raw8 {
 #pragma unroll
         for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
     }
-    // fp32 bits of the largest magnitude, infinities and NaN above all numbers.
-    // The bits of a type's magnitudes are ordered, so half types compare in
-    // pairs of 16-bit integers.
+    // The largest magnitude, for half types one of the even and one of the odd
+    // elements packed; NaN where there is one.
     __device__ __forceinline__ uint32_t top() const {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if constexpr (sizeof(T) == 2)
-                    m = __vmaxu2(m, w[k] & 0x7fff7fffu);
-                else
-                    m = max(m, w[k] & 0x7fffffffu);
-            }
+            for (int k = 0; k < 4; ++k) m = max_top<T>(m, w[k]);
         }
         return m;
     }
 };
-// top() of a row from the maximum of its lanes' (combined with max_top).
-template <typename T> __device__ __forceinline__ uint32_t max_top(uint32_t a, uint32_t b) {
-    if constexpr (sizeof(T) == 2)
-        return __vmaxu2(a, b);
-    else
-        return max(a, b);
-}
-template <typename T> __device__ __forceinline__ uint32_t top_bits(uint32_t m) {
-    if constexpr (sizeof(T) == 2) {
-        const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
-        T e;
-        memcpy(&e, &h, 2);
-        return __float_as_uint(Elem<T>::to_f(e));
-    } else {
-        return m;
-    }
-}
 
 __device__ __forceinline__ uint32_t max_finite8(const float (&f)[8]) {
     uint32_t m = 0;
@@ -93,16 +98,39 @@ __device__ __forceinline__ uint32_t max_finite8(const float (&f)[8]) {
 template <typename C, bool kBounded>
 __device__ __forceinline__ uint2 quantized8(const float (&f)[8], float inv) {
     uint2 u;
-    u.x = quantize4<C, kBounded>(mul_keep(f[0], inv), mul_keep(f[1], inv), mul_keep(f[2], inv),
-                                 mul_keep(f[3], inv));
-    u.y = quantize4<C, kBounded>(mul_keep(f[4], inv), mul_keep(f[5], inv), mul_keep(f[6], inv),
-                                 mul_keep(f[7], inv));
+    u.x = quantize4<C, kBounded>(f[0], f[1], f[2], f[3], inv);
+    u.y = quantize4<C, kBounded>(f[4], f[5], f[6], f[7], inv);
     return u;
 }
+
+// fp16 values scaled and converted in pairs. The product with 2^-E is exact where
+// it is a normal fp16 number; below 2^-14 it may be rounded, but then the
+// stored value is 0 either way (e4m3 rounds to 0 up to 2^-10, int8 up to 1/2).
+// int8: x * 2^-E + 1.5 * 2^10 is the nearest integer, to even, in the low bits.
+template <typename C>
+__device__ __forceinline__ uint2 quantized8_half(const uint4& u, __half2 inv) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 x = *reinterpret_cast<const __half2*>(&w[i]);
+        if constexpr (Quant8<C>::kTopExponent == 8) {  // e4m3
+            const __half2 y = __hmul2(x, inv);
+            q[i] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(y), __NV_SATFINITE, __NV_E4M3);
+        } else {
+            const __half2 y = __hfma2(x, inv, __float2half2_rn(1536.f));
+            q[i] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+    }
+    if constexpr (Quant8<C>::kTopExponent == 8)
+        return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+    else
+        return make_uint2(__byte_perm(q[0], q[1], 0x6420), __byte_perm(q[2], q[3], 0x6420));
+}
+
 template <typename C>
 __device__ __forceinline__ void store_quantized1(C* dst, float x, float inv) {
-    *reinterpret_cast<uint8_t*>(dst) =
-        (uint8_t)quantize4<C, false>(mul_keep(x, inv), 0.f, 0.f, 0.f);
+    *reinterpret_cast<uint8_t*>(dst) = (uint8_t)quantize4<C, false>(x, 0.f, 0.f, 0.f, inv);
 }
 
 // Over the LANES (a power of two) lanes of a group, which `mask` names.
@@ -123,6 +151,35 @@ __device__ __forceinline__ float group_sum(float v, uint32_t mask) {
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
     return v;
+}
+// A row's lane's two pieces quantised, and the row's scale byte, from the group's
+// maximum (group_top).
+template <typename T, typename C, int LANES>
+__device__ __forceinline__ uint32_t quantize_pieces(const Raw8<T>& x0, const Raw8<T>& x1,
+                                                    uint32_t top, uint32_t mask, uint2& q0,
+                                                    uint2& q1) {
+    const uint32_t byte = scale_byte<C>(top);
+    if constexpr (std::is_same<T, __half>::value) {
+        // finite rows whose 2^-E is an fp16 number (E >= -15)
+        if (top < 0x7f800000u && byte >= 112) {
+            const __half2 inv = __half2half2(__float2half_rn(inverse_scale(byte)));
+            q0 = quantized8_half<C>(x0.u[0], inv);
+            q1 = quantized8_half<C>(x1.u[0], inv);
+            return byte;
+        }
+    }
+    float a[8], b[8];
+    x0.get(a);
+    x1.get(b);
+    if (top < 0x7f800000u) {
+        q0 = quantized8<C, true>(a, inverse_scale(byte));
+        q1 = quantized8<C, true>(b, inverse_scale(byte));
+        return byte;
+    }
+    const uint32_t finite = scale_byte<C>(group_max<LANES>(max(max_finite8(a), max_finite8(b)), mask));
+    q0 = quantized8<C, false>(a, inverse_scale(finite));
+    q1 = quantized8<C, false>(b, inverse_scale(finite));
+    return finite;
 }
 template <int LANES> __device__ __forceinline__ uint32_t group_mask() {
     constexpr uint32_t ones = LANES == 32 ? 0xffffffffu : (1u << (LANES & 31)) - 1u;
@@ -178,68 +235,111 @@ __device__ __forceinline__ long long table_row(long long t, long long pos,
     return blk * p.num_kv_heads * p.block_size + off;
 }
 
+// A warp's place in its share of the work: rows [first, first + step) of token
+// t's `rows` rows, taken `step` at a time by each of the `parts` warps that share
+// a token; then the same of a later token.
+struct Place {
+    long long item, t;
+    int first;
+    bool valid;
+};
+__device__ __forceinline__ Place place_of(long long item, long long items, int parts, int step) {
+    Place c{item, 0, 0, item < items};
+    if (c.valid) {
+        int part;
+        c.t = divide(item, parts, part);
+        c.first = part * step;
+    }
+    return c;
+}
+__device__ __forceinline__ Place next_place(const Place& c, long long items, int parts, int step,
+                                            int rows) {
+    Place n = c;
+    n.first += parts * step;
+    if (n.first < rows) return n;
+    return place_of(c.item + (long long)gridDim.x * 8, items, parts, step);
+}
+
 // ------------------------------------------------------------- cache write
 // HBM bound: 2 e D bytes in, D + 1 out for each row of e-byte values. A warp
-// takes rows of one token (its slot is looked up once): all keys, then all
-// values. A row is held by LANES lanes, eight elements each (16-byte loads,
-// 8-byte stores), between its one read and its one write; kSteps rows of a
-// group are in flight. Rows wider than 256, of a width that is no multiple of
-// eight, or unaligned take a warp each, element by element, and are read twice.
-// Eight-element lanes against sixteen, 16381 fp16 tokens of 8 heads of 128 to
-// int8: see the table of the design notes for the rate reached.
-constexpr int kSteps = 4;
+// takes rows of one token: all keys, then all values. A row is held by LANES
+// lanes, 16 values each (two 16-byte loads, 8-byte stores) between its one read
+// and its one write; kRows rows of a group are read while kRows are quantised
+// and stored (rows in one buffer only: the loads waited half the time). Rows of
+// other widths and alignments take a warp each, element by element, and are
+// read twice.
+constexpr int kRows = 2;
 
 template <typename T, typename C, int LANES>
-__global__ void __launch_bounds__(256) quantize_write_kernel(const QuantCacheParams p, int parts) {
-    constexpr int GROUPS = 32 / LANES;
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quantize_write_kernel(const QuantCacheParams p, int parts) {
+    constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
     const uint32_t mask = group_mask<LANES>();
-    const int D = p.head_size, rows = 2 * p.num_kv_heads;
-    const bool on = sub * 8 < D;
+    const int D = p.head_size, kvh = p.num_kv_heads, rows = 2 * kvh;
+    const bool on = sub * 16 < D;
+    const int i0 = sub * 8, i1 = i0 + D / 2;
     const long long items = p.num_tokens * parts;
-    const int warps = gridDim.x * 8;
-    for (long long it = blockIdx.x * 8 + threadIdx.x / 32; it < items; it += warps) {
-        int part;
-        const long long t = divide(it, parts, part);
-        const long long base = slot_row(load_int(p.slots, p.slots64, t), p);
-        if (base < 0) continue;
-        const T* key = reinterpret_cast<const T*>(p.key) + t * p.key_stride + sub * 8;
-        const T* value = reinterpret_cast<const T*>(p.value) + t * p.value_stride + sub * 8;
-        for (int r0 = part * GROUPS * kSteps + grp; r0 < rows; r0 += parts * GROUPS * kSteps) {
-            Raw8<T> raw[kSteps];
+    const int head_stride = p.block_size * D;  // of a cache, in values
+
+    Raw8<T> a0[kRows], a1[kRows], b0[kRows], b1[kRows];
+    auto load = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
+        const T* key = reinterpret_cast<const T*>(p.key) + c.t * p.key_stride;
+        const T* value = reinterpret_cast<const T*>(p.value) + c.t * p.value_stride;
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int r = r0 + i * GROUPS;
-                const bool is_value = r >= p.num_kv_heads;
-                const int h = is_value ? r - p.num_kv_heads : r;
-                raw[i].zero();
-                if (r < rows && on) raw[i].load_stream((is_value ? value : key) + h * D);
-            }
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int r = r0 + i * GROUPS;
-                if (r >= rows) break;
-                const bool is_value = r >= p.num_kv_heads;
-                const int h = is_value ? r - p.num_kv_heads : r;
-                const long long row = base + (long long)h * p.block_size;
-                float f[8];
-                raw[i].get(f);
-                uint32_t top = group_top<LANES, T>(raw[i].top(), mask);
-                uint2 q;
-                if (top < 0x7f800000u) {
-                    q = quantized8<C, true>(f, inverse_scale(scale_byte<C>(top)));
-                } else {
-                    top = group_max<LANES>(max_finite8(f), mask);
-                    q = quantized8<C, false>(f, inverse_scale(scale_byte<C>(top)));
-                }
-                if (on)
-                    *reinterpret_cast<uint2*>(
-                        reinterpret_cast<uint8_t*>(is_value ? p.value_cache : p.key_cache) +
-                        row * D + sub * 8) = q;
-                if (sub == 0)
-                    (is_value ? p.value_scales : p.key_scales)[row] = (uint8_t)scale_byte<C>(top);
+        for (int i = 0; i < kRows; ++i) {
+            const int r = c.first + i * GROUPS + grp;
+            x0[i].zero();
+            x1[i].zero();
+            if (c.valid && r < rows && on) {
+                const T* src = r < kvh ? key + r * D : value + (r - kvh) * D;
+                x0[i].load_stream(src + i0);
+                x1[i].load_stream(src + i1);
             }
         }
+    };
+    long long known = -1;  // the token looked up last, and its rows of head 0
+    uint8_t *key_row = nullptr, *value_row = nullptr, *key_scale = nullptr, *value_scale = nullptr;
+    auto store = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
+        if (known != c.t) {
+            known = c.t;
+            const long long base = slot_row(load_int(p.slots, p.slots64, c.t), p);
+            key_row = nullptr;
+            if (base >= 0) {
+                key_row = reinterpret_cast<uint8_t*>(p.key_cache) + base * D;
+                value_row = reinterpret_cast<uint8_t*>(p.value_cache) + base * D;
+                key_scale = p.key_scales + base;
+                value_scale = p.value_scales + base;
+            }
+        }
+        if (key_row == nullptr) return;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int r = c.first + i * GROUPS + grp;
+            if (r >= rows) break;
+            const bool is_value = r >= kvh;
+            const int h = is_value ? r - kvh : r;
+            uint2 q0, q1;
+            const uint32_t byte = quantize_pieces<T, C, LANES>(
+                x0[i], x1[i], group_top<LANES, T>(max_top<T>(x0[i].top(), x1[i].top()), mask), mask,
+                q0, q1);
+            uint8_t* dst = (is_value ? value_row : key_row) + h * head_stride;
+            if (on) {
+                *reinterpret_cast<uint2*>(dst + i0) = q0;
+                *reinterpret_cast<uint2*>(dst + i1) = q1;
+            }
+            if (sub == 0) (is_value ? value_scale : key_scale)[h * p.block_size] = (uint8_t)byte;
+        }
+    };
+    Place c = place_of(blockIdx.x * 8 + threadIdx.x / 32, items, parts, STEP);
+    load(c, a0, a1);
+    while (c.valid) {
+        Place n = next_place(c, items, parts, STEP, rows);
+        load(n, b0, b1);
+        store(c, a0, a1);
+        if (!n.valid) break;
+        c = next_place(n, items, parts, STEP, rows);
+        load(c, a0, a1);
+        store(n, b0, b1);
     }
 }
 
@@ -369,8 +469,8 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const DequantParams
 // heads, value heads. A row is held by LANES lanes, 16 values each: lane
 // l < rot/16 the eight values at 8 l and their partners at 8 l + rot/2 (so the
 // rotation needs no exchange), the others 16 values beyond rot. A group keeps
-// its weights while it stays with queries or with keys, and has two rows in
-// flight. Other widths and alignments: a warp for each row, by element.
+// its weights while it stays with queries or with keys; kRows of its rows are
+// read while kRows are worked on. Other widths and alignments: a warp for each row, by element.
 enum RowKind { kQuery = 0, kKey = 1, kValue = 2 };
 
 struct NormRow {
@@ -383,157 +483,171 @@ __device__ __forceinline__ NormRow norm_row(int r, const QuantCacheParams& p) {
     return r < p.num_kv_heads ? NormRow{kKey, r} : NormRow{kValue, r - p.num_kv_heads};
 }
 
+// x' = x cos - y sin, y' = y cos + x sin, a rounding less than rope_pair has: what
+// comes in is an unrounded fp32 value, so there are no bits to agree with.
+__device__ __forceinline__ void turn_pair(float x, float y, float c, float s, float& xo, float& yo) {
+    xo = fmaf(x, c, -(y * s));
+    yo = fmaf(y, c, x * s);
+}
+
 template <typename T, typename C, int LANES>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QuantCacheParams p, int parts) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kernel(const QuantCacheParams p, int parts) {
     grid_launch_dependents();
-    constexpr int GROUPS = 32 / LANES, U = 2;
+    constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
     const uint32_t mask = group_mask<LANES>();
     const int D = p.head_size, rot = p.rot_dim, half = rot / 2;
+    const int H = p.num_heads, kvh = p.num_kv_heads;
     const bool with_cache = p.key_cache != nullptr;
-    const int rows = p.num_heads + p.num_kv_heads * (with_cache ? 2 : 1);
+    const int rows = H + kvh * (with_cache ? 2 : 1);
     const int pairs = rot / 16;  // lanes that rotate
     const bool on = sub * 16 < D, turn = on && sub < pairs;
     const int i0 = sub < pairs ? 8 * sub : rot + 16 * (sub - pairs);
     const int i1 = sub < pairs ? i0 + half : i0 + 8;
     const float inv_d = 1.f / (float)D;
     const long long items = p.num_tokens * parts;
-    const int warps = gridDim.x * 8;
-    for (long long it = blockIdx.x * 8 + threadIdx.x / 32; it < items; it += warps) {
-        int part;
-        const long long t = divide(it, parts, part);
-        const long long pos = load_int(p.positions, p.positions64, t);
-        float c[8], s[8];
-        bool rotate = turn;
-        if (pos >= 0 && pos < p.cache_rows) {
-            if (turn) {
-                const T* cs = reinterpret_cast<const T*>(p.cos_sin) + pos * rot;
-                Raw8<T> r;
-                r.load(cs + i0);
-                r.get(c);
-                r.load(cs + half + i0);
-                r.get(s);
+    const int head_stride = p.block_size * D;  // of a cache, in values
+
+    Raw8<T> a0[kRows], a1[kRows], b0[kRows], b1[kRows];
+    auto load = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
+        const T* query = reinterpret_cast<const T*>(p.query) + c.t * p.query_stride;
+        const T* key = reinterpret_cast<const T*>(p.key) + c.t * p.key_stride;
+        const T* value = reinterpret_cast<const T*>(p.value) + c.t * p.value_stride;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int r = c.first + i * GROUPS + grp;
+            x0[i].zero();
+            x1[i].zero();
+            if (c.valid && r < rows && on) {
+                const T* src = r < H         ? query + r * D
+                               : r < H + kvh ? key + (r - H) * D
+                                             : value + (r - H - kvh) * D;
+                x0[i].load_stream(src + i0);
+                x1[i].load_stream(src + i1);
             }
-        } else {
-            flag_status(TLB_STATUS_BAD_POSITION);
-            rotate = false;
         }
-        long long base = -1;  // cache row of the token for head 0
-        if (with_cache)
-            base = p.slots ? slot_row(load_int(p.slots, p.slots64, t), p) : table_row(t, pos, p);
-        grid_dependency_wait();
-        const T* query = reinterpret_cast<const T*>(p.query) + t * p.query_stride;
-        const T* key = reinterpret_cast<const T*>(p.key) + t * p.key_stride;
-        const T* value = reinterpret_cast<const T*>(p.value) + t * p.value_stride;
-        Raw8<T> w0, w1;  // weights of the group's current kind
-        int have = -1;
-        for (int r0 = part * GROUPS * U + grp; r0 < rows; r0 += parts * GROUPS * U) {
-            Raw8<T> x0[U], x1[U];
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int r = r0 + i * GROUPS;
-                x0[i].zero();
-                x1[i].zero();
-                if (r < rows && on) {
-                    const NormRow nr = norm_row(r, p);
-                    const T* src = (nr.kind == kQuery ? query : nr.kind == kKey ? key : value) +
-                                   nr.h * D;
-                    x0[i].load_stream(src + i0);
-                    x1[i].load_stream(src + i1);
+    };
+    long long known = -1;  // the token looked up last
+    long long base = -1;   // its first cache row
+    bool rotate = false;
+    float cs[8], sn[8];  // cos and sin of the lane's pairs
+    float w0[8], w1[8];  // weights of the kind of row the group had last
+    int have = -1;
+    auto process = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
+        if (known != c.t) {
+            known = c.t;
+            const long long pos = load_int(p.positions, p.positions64, c.t);
+            rotate = false;
+            if (pos >= 0 && pos < p.cache_rows) {
+                rotate = turn;
+                if (turn) {
+                    const T* table = reinterpret_cast<const T*>(p.cos_sin) + pos * rot;
+                    Raw8<T> u, v;
+                    u.load(table + i0);
+                    v.load(table + half + i0);
+                    u.get(cs);
+                    v.get(sn);
                 }
+            } else {
+                flag_status(TLB_STATUS_BAD_POSITION);
             }
+            if (with_cache)
+                base = p.slots ? slot_row(load_int(p.slots, p.slots64, c.t), p)
+                               : table_row(c.t, pos, p);
+        }
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int r = r0 + i * GROUPS;
-                if (r >= rows) break;
-                const NormRow nr = norm_row(r, p);
-                if (nr.kind != kValue) {
-                    if (have != nr.kind) {
-                        have = nr.kind;
-                        const T* w = reinterpret_cast<const T*>(nr.kind == kQuery ? p.query_weight
-                                                                                  : p.key_weight);
-                        w0.zero();
-                        w1.zero();
-                        if (on) {
-                            w0.load(w + i0);
-                            w1.load(w + i1);
-                        }
+        for (int i = 0; i < kRows; ++i) {
+            const int r = c.first + i * GROUPS + grp;
+            if (r >= rows) break;
+            const int kind = r < H ? kQuery : r < H + kvh ? kKey : kValue;
+            if (kind != kValue) {
+                if (have != kind) {
+                    have = kind;
+                    const T* w = reinterpret_cast<const T*>(kind == kQuery ? p.query_weight
+                                                                           : p.key_weight);
+                    Raw8<T> u, v;
+                    u.zero();
+                    v.zero();
+                    if (on) {
+                        u.load(w + i0);
+                        v.load(w + i1);
                     }
-                    float a[8], b[8], w[8];
-                    x0[i].get(a);
-                    x1[i].get(b);
-                    float sa = 0.f, sb = 0.f;
+                    u.get(w0);
+                    v.get(w1);
+                }
+                float a[8], b[8];
+                x0[i].get(a);
+                x1[i].get(b);
+                float sa = 0.f, sb = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sa = fmaf(a[j], a[j], sa);
+                    sb = fmaf(b[j], b[j], sb);
+                }
+                const float inv = rsqrtf(group_sum<LANES>(sa + sb, mask) * inv_d + p.eps);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    a[j] = a[j] * inv * w0[j];
+                    b[j] = b[j] * inv * w1[j];
+                }
+                if (rotate) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        sa = fmaf(a[j], a[j], sa);
-                        sb = fmaf(b[j], b[j], sb);
+                        float x, y;
+                        turn_pair(a[j], b[j], cs[j], sn[j], x, y);
+                        a[j] = x;
+                        b[j] = y;
                     }
-                    const float inv = rsqrtf(group_sum<LANES>(sa + sb, mask) * inv_d + p.eps);
-                    w0.get(w);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) a[j] = a[j] * inv * w[j];
-                    w1.get(w);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) b[j] = b[j] * inv * w[j];
-                    if (rotate) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            float x, y;
-                            rope_pair(a[j], b[j], c[j], s[j], x, y);
-                            a[j] = x;
-                            b[j] = y;
-                        }
-                    }
-                    x0[i].set(a);
-                    x1[i].set(b);
                 }
-                if (nr.kind == kQuery || !with_cache) {
-                    T* dst = nr.kind == kQuery
-                                 ? reinterpret_cast<T*>(p.out) + (t * p.num_heads + nr.h) * D
-                                 : reinterpret_cast<T*>(p.key_out) + (t * p.num_kv_heads + nr.h) * D;
-                    if (on) {
-                        x0[i].store(dst + i0);
-                        x1[i].store(dst + i1);
-                    }
-                    continue;
-                }
-                if (base < 0) continue;
-                const long long row = base + (long long)nr.h * p.block_size;
-                if constexpr (sizeof(C) == 1) {
-                    float a[8], b[8];
-                    x0[i].get(a);
-                    x1[i].get(b);
-                    uint32_t top =
-                        group_top<LANES, T>(max_top<T>(x0[i].top(), x1[i].top()), mask);
-                    uint2 q0, q1;
-                    if (top < 0x7f800000u) {
-                        const float qs = inverse_scale(scale_byte<C>(top));
-                        q0 = quantized8<C, true>(a, qs);
-                        q1 = quantized8<C, true>(b, qs);
-                    } else {
-                        top = group_max<LANES>(max(max_finite8(a), max_finite8(b)), mask);
-                        const float qs = inverse_scale(scale_byte<C>(top));
-                        q0 = quantized8<C, false>(a, qs);
-                        q1 = quantized8<C, false>(b, qs);
-                    }
-                    uint8_t* dst = reinterpret_cast<uint8_t*>(nr.kind == kValue ? p.value_cache
-                                                                                : p.key_cache) +
-                                   row * D;
-                    if (on) {
-                        *reinterpret_cast<uint2*>(dst + i0) = q0;
-                        *reinterpret_cast<uint2*>(dst + i1) = q1;
-                    }
-                    if (sub == 0)
-                        (nr.kind == kValue ? p.value_scales : p.key_scales)[row] =
-                            (uint8_t)scale_byte<C>(top);
-                } else if (on) {
-                    T* dst = reinterpret_cast<T*>(nr.kind == kValue ? p.value_cache : p.key_cache) +
-                             row * D;
+                x0[i].set(a);
+                x1[i].set(b);
+            }
+            if (kind == kQuery || !with_cache) {
+                T* dst = kind == kQuery
+                             ? reinterpret_cast<T*>(p.out) + c.t * (H * D) + r * D
+                             : reinterpret_cast<T*>(p.key_out) + c.t * (kvh * D) + (r - H) * D;
+                if (on) {
                     x0[i].store(dst + i0);
                     x1[i].store(dst + i1);
                 }
+                continue;
+            }
+            if (base < 0) continue;
+            const int h = kind == kKey ? r - H : r - H - kvh;
+            const long long at = base * D + (long long)h * head_stride;
+            if constexpr (sizeof(C) == 1) {
+                uint2 q0, q1;
+                const uint32_t byte = quantize_pieces<T, C, LANES>(
+                    x0[i], x1[i], group_top<LANES, T>(max_top<T>(x0[i].top(), x1[i].top()), mask),
+                    mask, q0, q1);
+                uint8_t* dst =
+                    reinterpret_cast<uint8_t*>(kind == kValue ? p.value_cache : p.key_cache) + at;
+                if (on) {
+                    *reinterpret_cast<uint2*>(dst + i0) = q0;
+                    *reinterpret_cast<uint2*>(dst + i1) = q1;
+                }
+                if (sub == 0)
+                    (kind == kValue ? p.value_scales : p.key_scales)[base + (long long)h *
+                                                                                p.block_size] =
+                        (uint8_t)byte;
+            } else if (on) {
+                T* dst = reinterpret_cast<T*>(kind == kValue ? p.value_cache : p.key_cache) + at;
+                x0[i].store(dst + i0);
+                x1[i].store(dst + i1);
             }
         }
+    };
+    grid_dependency_wait();
+    Place c = place_of(blockIdx.x * 8 + threadIdx.x / 32, items, parts, STEP);
+    load(c, a0, a1);
+    while (c.valid) {
+        Place n = next_place(c, items, parts, STEP, rows);
+        load(n, b0, b1);
+        process(c, a0, a1);
+        if (!n.valid) break;
+        c = next_place(n, items, parts, STEP, rows);
+        load(c, a0, a1);
+        process(n, b0, b1);
     }
 }
 
@@ -589,7 +703,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(const QuantCacheP
             const int j = first ? i + half : i - half, k = first ? i : j;
             const float y = Elem<T>::to_f(src[j]) * inv * Elem<T>::to_f(w[j]);
             float xo, yo;
-            rope_pair(first ? x : y, first ? y : x, Elem<T>::to_f(cs[k]),
+            turn_pair(first ? x : y, first ? y : x, Elem<T>::to_f(cs[k]),
                       Elem<T>::to_f(cs[half + k]), xo, yo);
             return first ? xo : yo;
         };
@@ -637,13 +751,13 @@ int parts_of(long long tokens, int rows, int step) {
 
 template <typename T, typename C, int LANES>
 void write_lanes(const QuantCacheParams& p, cudaStream_t st) {
-    const int parts = parts_of(p.num_tokens, 2 * p.num_kv_heads, 32 / LANES * kSteps);
+    const int parts = parts_of(p.num_tokens, 2 * p.num_kv_heads, 32 / LANES * kRows);
     quantize_write_kernel<T, C, LANES>
-        <<<grid_of(p.num_tokens * parts, 8), 256, 0, st>>>(p, parts);
+        <<<grid_of(p.num_tokens * parts, 8, 3), 256, 0, st>>>(p, parts);
 }
 template <typename T, typename C>
 cudaError_t write_tc(const QuantCacheParams& p, bool vec, cudaStream_t st) {
-    const int units = vec ? p.head_size / 8 : 33;
+    const int units = vec ? p.head_size / 16 : 33;
     if (units <= 4)
         write_lanes<T, C, 4>(p, st);
     else if (units <= 8)
@@ -684,8 +798,8 @@ cudaError_t dequant_t(int cache_dtype, const DequantParams& p, bool vec, cudaStr
 template <typename T, typename C, int LANES>
 cudaError_t norm_lanes(const QuantCacheParams& p, cudaLaunchConfig_t& cfg) {
     const int rows = p.num_heads + p.num_kv_heads * (p.key_cache != nullptr ? 2 : 1);
-    const int parts = parts_of(p.num_tokens, rows, 32 / LANES * 2);
-    cfg.gridDim = dim3(grid_of(p.num_tokens * parts, 8));
+    const int parts = parts_of(p.num_tokens, rows, 32 / LANES * kRows);
+    cfg.gridDim = dim3(grid_of(p.num_tokens * parts, 8, 2));
     return cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<T, C, LANES>, p, parts);
 }
 template <typename T, typename C>
