@@ -420,20 +420,38 @@ TLB_API int tlb_step_metadata(const int32_t* prompt_lens, const int32_t* prompt_
  * block_ids[n], [num_ids, num_kv_heads, block_size, head_size] of dtype, zeros
  * for ids < 0 or outside the cache (the latter flagged,
  * TLB_STATUS_BAD_BLOCK_ID).
+ *
+ * These and the two entry points below take their arguments as a struct of
+ * 64-bit fields (a binding packs it in one step); `args` is read during the call
+ * only. Its dtype fields hold tlb_dtype values.
  * ---------------------------------------------------------------------- */
-TLB_API int tlb_reshape_and_cache_quantized(const void* key, const void* value, void* key_cache,
-                        void* value_cache, void* key_scales, void* value_scales,
-                        const void* slots, int slot_dtype, int64_t num_tokens,
-                        int64_t num_kv_heads, int64_t head_size, int64_t num_blocks,
-                        int64_t block_size, int64_t key_stride, int64_t value_stride,
-                        int dtype, int cache_dtype, void* stream);
+typedef struct tlb_quantized_write_args {
+    const void* key;
+    const void* value;
+    void* key_cache;
+    void* value_cache;
+    void* key_scales;
+    void* value_scales;
+    const void* slots;
+    int64_t slot_dtype, num_tokens, num_kv_heads, head_size, num_blocks, block_size;
+    int64_t key_stride, value_stride, dtype, cache_dtype;
+} tlb_quantized_write_args;
 
-TLB_API int tlb_dequantize_blocks(void* key_out, void* value_out, const void* key_cache,
-                        const void* value_cache, const void* key_scales,
-                        const void* value_scales, const void* block_ids, int id_dtype,
-                        int64_t num_ids, int64_t num_kv_heads, int64_t head_size,
-                        int64_t num_blocks, int64_t block_size, int dtype,
-                        int cache_dtype, void* stream);
+TLB_API int tlb_reshape_and_cache_quantized(const tlb_quantized_write_args* args, void* stream);
+
+typedef struct tlb_dequantize_args {
+    void* key_out;
+    void* value_out;
+    const void* key_cache;
+    const void* value_cache;
+    const void* key_scales;
+    const void* value_scales;
+    const void* block_ids;
+    int64_t id_dtype, num_ids, num_kv_heads, head_size, num_blocks, block_size;
+    int64_t dtype, cache_dtype;
+} tlb_dequantize_args;
+
+TLB_API int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * RMS norm of each query and key head, the NeoX rotation, and the KV-cache
@@ -456,16 +474,29 @@ TLB_API int tlb_dequantize_blocks(void* key_out, void* value_out, const void* ke
  * TLB_STATUS_BAD_POSITION. flags: TLB_ROPE_OVERLAP_PREVIOUS as above (the
  * norm weights too must not be written by the kernel before).
  * ---------------------------------------------------------------------- */
-TLB_API int tlb_qk_norm_rotary_embedding_neox(
-    void* query_out, void* key_out, const void* positions, int pos_dtype,
-    const void* query, const void* key, const void* value, const void* query_weight,
-    const void* key_weight, float eps, void* key_cache, void* value_cache,
-    void* key_scales, void* value_scales, const void* slots, int slot_dtype,
-    const int32_t* block_tables, int64_t max_blocks_per_seq, int64_t num_tokens,
-    int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
-    const void* cos_sin_cache, int64_t cache_rows, int64_t rot_dim, int64_t num_blocks,
-    int64_t block_size, int64_t query_stride, int64_t key_stride, int64_t value_stride,
-    int dtype, int cache_dtype, unsigned flags, void* stream);
+typedef struct tlb_qk_norm_rope_args {
+    void* query_out;
+    void* key_out;
+    const void* positions;
+    const void* query;
+    const void* key;
+    const void* value;
+    const void* query_weight;
+    const void* key_weight;
+    void* key_cache;
+    void* value_cache;
+    void* key_scales;
+    void* value_scales;
+    const void* slots;
+    const int32_t* block_tables;
+    const void* cos_sin_cache;
+    int64_t pos_dtype, slot_dtype, max_blocks_per_seq, num_tokens, num_heads, num_kv_heads;
+    int64_t head_size, cache_rows, rot_dim, num_blocks, block_size;
+    int64_t query_stride, key_stride, value_stride, dtype, cache_dtype, flags;
+    double eps;
+} tlb_qk_norm_rope_args;
+
+TLB_API int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * Paged decode attention over 8-bit caches, and with capped, distance-biased
@@ -496,16 +527,23 @@ TLB_API int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t
                         int64_t head_dim, int64_t block_size, int dtype,
                         int cache_dtype, size_t* bytes_out, size_t* zeroed_out);
 
-TLB_API int tlb_paged_attention_scored(void* out, const void* query, const void* key_cache,
-                        const void* value_cache, const void* key_scales,
-                        const void* value_scales, const int32_t* block_tables,
-                        const int32_t* seq_lens, const float* alibi_slopes,
-                        int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
-                        int64_t head_dim, int64_t num_blocks, int64_t block_size,
-                        int64_t max_blocks_per_seq, int64_t query_stride, int64_t window,
-                        float scale, float softcap, int dtype, int cache_dtype,
-                        void* workspace, size_t workspace_bytes, unsigned flags,
-                        void* stream);
+typedef struct tlb_scored_attention_args {
+    void* out;
+    const void* query;
+    const void* key_cache;
+    const void* value_cache;
+    const void* key_scales;
+    const void* value_scales;
+    const int32_t* block_tables;
+    const int32_t* seq_lens;
+    const float* alibi_slopes;
+    void* workspace;
+    int64_t workspace_bytes, num_seqs, num_heads, num_kv_heads, head_dim, num_blocks;
+    int64_t block_size, max_blocks_per_seq, query_stride, window, dtype, cache_dtype, flags;
+    double scale, softcap;
+} tlb_scored_attention_args;
+
+TLB_API int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -3,6 +3,8 @@ operators, without a GPU: the C ABI refuses bad arguments before any CUDA call,
 and the op modules refuse CPU tensors and wrong shapes or types. The 64-bit
 oracle's quantiser against torch's own conversion."""
 
+import re
+
 import pytest
 import torch
 
@@ -10,53 +12,74 @@ from cscr import _lib
 from cscr import attention as A
 from cscr import cache as C
 from cscr import pos_encoding as PE
+from conftest import REPO
 from oracle import quant_oracle as Q
+
+HEADER = REPO / "include" / "tinyllama_b200.h"
 
 P = 1 << 12  # stands in for an aligned device pointer; nothing is dereferenced
 OK, BAD, WORKSPACE = 0, 1, 4
 F32, F16, BF16, I32, I64, E4M3, I8 = range(7)
 
 
+def call(lib, entry, *fields):
+    name, pack = entry
+    return getattr(lib, name)(pack(*fields), None)
+
+
+def test_struct_layouts_match_the_header():
+    """Every struct of the header has as many fields as its packing."""
+    text = HEADER.read_text()
+    for name, (entry, pack) in (("quantized_write", _lib.QUANTIZED_WRITE),
+                                ("dequantize", _lib.DEQUANTIZE),
+                                ("qk_norm_rope", _lib.QK_NORM_ROPE),
+                                ("scored_attention", _lib.SCORED_ATTENTION)):
+        body = re.search(r"struct tlb_%s_args \{(.*?)\}" % name, text, re.S).group(1)
+        fields = sum(len(line.split(",")) for line in body.split(";") if line.strip())
+        doubles = sum(len(line.split(",")) for line in body.split(";") if "double" in line)
+        assert len(pack(*[0] * (fields - doubles), *[0.0] * doubles)) == 8 * fields
+        assert getattr(_lib.load(), entry)(None, None) == BAD  # no struct at all
+
+
 def write(lib, key=P, slots=P, slot_dtype=I64, tokens=4, kvh=2, d=128, nb=10, bs=16, dtype=BF16,
           cache=E4M3, scales=P, kc=P):
-    return lib.tlb_reshape_and_cache_quantized(key, P, kc, P, scales, P, slots, slot_dtype, tokens,
-                                               kvh, d, nb, bs, kvh * d, kvh * d, dtype, cache, None)
+    return call(lib, _lib.QUANTIZED_WRITE, key, P, kc, P, scales, P, slots, slot_dtype, tokens, kvh,
+                d, nb, bs, kvh * d, kvh * d, dtype, cache)
 
 
 def test_write_refuses_before_any_cuda_call(built_lib):
     lib = _lib.load()
     for kw, msg in ((dict(dtype=I32), "dtype must be"), (dict(cache=BF16), "cache dtype"),
                     (dict(tokens=-1), "num_tokens"), (dict(kvh=0), "positive"),
-                    (dict(bs=0), "positive"), (dict(kc=None), "cache pointers"),
-                    (dict(slot_dtype=F32), "slot_mapping"), (dict(scales=None), "scale pointers"),
-                    (dict(key=None), "tensor pointers"), (dict(key=P + 1), "aligned")):
+                    (dict(bs=0), "positive"), (dict(kc=0), "cache pointers"),
+                    (dict(slot_dtype=F32), "slot_mapping"), (dict(scales=0), "scale pointers"),
+                    (dict(key=0), "tensor pointers"), (dict(key=P + 1), "aligned")):
         assert write(lib, **kw) == BAD and msg in _lib.last_error(), kw
     assert write(lib, tokens=0) == OK  # nothing to do, nothing launched
 
 
 def read(lib, out=P, ids=P, id_dtype=I32, n=4, kvh=2, d=128, nb=10, bs=16, dtype=BF16, cache=I8,
          scales=P):
-    return lib.tlb_dequantize_blocks(out, P, P, P, scales, P, ids, id_dtype, n, kvh, d, nb, bs,
-                                     dtype, cache, None)
+    return call(lib, _lib.DEQUANTIZE, out, P, P, P, scales, P, ids, id_dtype, n, kvh, d, nb, bs,
+                dtype, cache)
 
 
 def test_read_refuses_before_any_cuda_call(built_lib):
     lib = _lib.load()
     for kw, msg in ((dict(dtype=I8), "dtype must be"), (dict(cache=F16), "cache dtype"),
                     (dict(n=-1), "num_tokens"), (dict(d=0), "positive"),
-                    (dict(id_dtype=BF16), "block_ids"), (dict(scales=None), "scale pointers"),
-                    (dict(ids=None), "tensor pointers"), (dict(out=P + 1), "aligned")):
+                    (dict(id_dtype=BF16), "block_ids"), (dict(scales=0), "scale pointers"),
+                    (dict(ids=0), "tensor pointers"), (dict(out=P + 1), "aligned")):
         assert read(lib, **kw) == BAD and msg in _lib.last_error(), kw
     assert read(lib, n=0) == OK
 
 
-def norm(lib, q_out=P, k_out=None, value=P, eps=1e-6, kc=P, ks=P, slots=P, tables=None, maxb=0,
+def norm(lib, q_out=P, k_out=0, value=P, eps=1e-6, kc=P, ks=P, slots=P, tables=0, maxb=0,
          tokens=4, heads=16, kvh=2, d=128, rows=64, rot=128, nb=10, bs=16, dtype=BF16, cache=E4M3,
          flags=0, pos_dtype=I64, w=P):
-    return lib.tlb_qk_norm_rotary_embedding_neox(
-        q_out, k_out, P, pos_dtype, P, P, value, w, P, eps, kc, P if kc else None, ks, ks, slots,
-        I64, tables, maxb, tokens, heads, kvh, d, P, rows, rot, nb, bs, heads * d, kvh * d, kvh * d,
-        dtype, cache, flags, None)
+    return call(lib, _lib.QK_NORM_ROPE, q_out, k_out, P, P, P, value, w, P, kc, P if kc else 0, ks,
+                ks, slots, tables, P, pos_dtype, I64, maxb, tokens, heads, kvh, d, rows, rot, nb, bs,
+                heads * d, kvh * d, kvh * d, dtype, cache, flags, eps)
 
 
 def test_norm_refuses_before_any_cuda_call(built_lib):
@@ -66,18 +89,17 @@ def test_norm_refuses_before_any_cuda_call(built_lib):
                     (dict(rot=63), "even"), (dict(rot=130), "must not exceed"),
                     (dict(rows=0), "at least one row"), (dict(eps=-1.0), "eps"),
                     (dict(eps=float("nan")), "eps"), (dict(cache=F16), "query dtype"),
-                    (dict(ks=None), "8-bit caches need"), (dict(slots=None), "slots or block"),
-                    (dict(value=None), "must not be null"), (dict(w=P + 1), "aligned"),
-                    (dict(kc=None, k_out=None), "must not be null")):
+                    (dict(ks=0), "8-bit caches need"), (dict(slots=0), "slots or block"),
+                    (dict(value=0), "must not be null"), (dict(w=P + 1), "aligned"),
+                    (dict(kc=0, k_out=0), "must not be null")):
         assert norm(lib, **kw) == BAD and msg in _lib.last_error(), kw
     assert norm(lib, tokens=0) == OK
 
 
 def attend(lib, q=P, seqs=4, heads=16, kvh=2, d=128, nb=10, bs=16, maxb=4, stride=2048, window=0,
-           cap=0.0, dtype=BF16, cache=E4M3, scales=P, flags=0, ws=None, nbytes=0):
-    return lib.tlb_paged_attention_scored(P, q, P, P, scales, scales, P, P, None, seqs, heads, kvh,
-                                          d, nb, bs, maxb, stride, window, 0.1, cap, dtype, cache,
-                                          ws, nbytes, flags, None)
+           cap=0.0, dtype=BF16, cache=E4M3, scales=P, flags=0, ws=0, nbytes=0):
+    return call(lib, _lib.SCORED_ATTENTION, P, q, P, P, scales, scales, P, P, 0, ws, nbytes, seqs,
+                heads, kvh, d, nb, bs, maxb, stride, window, dtype, cache, flags, 0.1, cap)
 
 
 def test_attention_refuses_before_any_cuda_call(built_lib):
@@ -87,8 +109,8 @@ def test_attention_refuses_before_any_cuda_call(built_lib):
                     (dict(heads=15), "divisible"), (dict(d=2048), "1024"),
                     (dict(nb=0), "positive"), (dict(window=-1), "window"),
                     (dict(cap=-1.0), "softcap"), (dict(cap=float("inf")), "softcap"),
-                    (dict(cap=float("nan")), "softcap"), (dict(q=None), "must not be null"),
-                    (dict(scales=None), "8-bit caches need"), (dict(q=P + 1), "aligned"),
+                    (dict(cap=float("nan")), "softcap"), (dict(q=0), "must not be null"),
+                    (dict(scales=0), "8-bit caches need"), (dict(q=P + 1), "aligned"),
                     (dict(maxb=1 << 30, bs=16), "supported range")):
         assert attend(lib, **kw) == BAD and msg in _lib.last_error(), kw
 

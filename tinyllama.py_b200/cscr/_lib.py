@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -67,19 +68,12 @@ _PROTOS = {
     "tlb_decode_metadata": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp],
     "tlb_step_metadata": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
                           _vp],
-    "tlb_reshape_and_cache_quantized": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64,
-                                        _i64, _i64, _i64, _i64, _i32, _i32, _vp],
-    "tlb_dequantize_blocks": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64,
-                              _i64, _i32, _i32, _vp],
-    "tlb_qk_norm_rotary_embedding_neox": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _vp,
-                                          _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64,
-                                          _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-                                          _i32, _i32, ctypes.c_uint, _vp],
+    "tlb_reshape_and_cache_quantized": [ctypes.c_char_p, _vp],
+    "tlb_dequantize_blocks": [ctypes.c_char_p, _vp],
+    "tlb_qk_norm_rotary_embedding_neox": [ctypes.c_char_p, _vp],
     "tlb_paged_attention_scored_workspace_size": [_i64, _i64, _i64, _i64, _i32, _i32,
                                                   ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
-    "tlb_paged_attention_scored": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
-                                   _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _i32, _i32, _vp,
-                                   _sz, ctypes.c_uint, _vp],
+    "tlb_paged_attention_scored": [ctypes.c_char_p, _vp],
 }
 _RESTYPES = {"tlb_last_error": ctypes.c_char_p, "tlb_version": ctypes.c_char_p}
 
@@ -141,15 +135,24 @@ def stream_of(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
-def launch(name: str, index: int, *args) -> None:
-    """Call entry point `name` with `args` and the current stream of device
+# Layouts of the argument structs (64-bit fields in the header's order): packing
+# one takes 0.3 us, converting its fields one by one 2 us.
+QUANTIZED_WRITE = ("tlb_reshape_and_cache_quantized", struct.Struct("=17q").pack)
+DEQUANTIZE = ("tlb_dequantize_blocks", struct.Struct("=15q").pack)
+QK_NORM_ROPE = ("tlb_qk_norm_rotary_embedding_neox", struct.Struct("=32qd").pack)
+SCORED_ATTENTION = ("tlb_paged_attention_scored", struct.Struct("=23q2d").pack)
+
+
+def launch(entry, index: int, *args) -> None:
+    """Call one of the struct entry points above with the current stream of device
     `index`, with that device current; raises the library's message on failure."""
+    name, pack = entry
     fn = getattr(_lib or load(), name)
     if _get_device() == index:
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(pack(*args), _raw_stream(index))
     else:
         with device_guard(torch.device("cuda", index)):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(pack(*args), _raw_stream(index))
     if rc or DEBUG:
         check(rc)
 

@@ -294,6 +294,7 @@ def paged_prefill_attention(query: torch.Tensor, key_cache: torch.Tensor,
 
 
 _CACHE8_TYPES = (torch.float8_e4m3fn, torch.int8)
+_capturing = torch.cuda.is_current_stream_capturing
 _scored_ws_sizes: dict[tuple, tuple[int, int]] = {}
 # (device index, stream handle) -> scratch whose counter prefix is zero between calls
 _scored_workspaces: dict[tuple[int, int], torch.Tensor] = {}
@@ -317,7 +318,7 @@ def _scored_workspace(query: torch.Tensor, index: int, nbytes: int, zeroed: int)
     """Scratch of a call: the stream's own, or while the stream is captured one
     of the graph's (zeroed in the graph), so that graphs replayed together share
     none."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         ws = query.new_empty(nbytes, dtype=torch.uint8)
         ws[:zeroed].zero_()
         return ws
@@ -402,16 +403,15 @@ def _paged_attention_scored(query, key_cache, value_cache, key_scales, value_sca
         return out
     nbytes, zeroed = _scored_workspace_bytes(shape[1], num_kv_heads, head_dim, block_size, dtype,
                                              cache_dtype, index)
-    ws = _scored_workspace(query, index, nbytes, zeroed).data_ptr() if nbytes else None
-    _lib.launch("tlb_paged_attention_scored", index, out.data_ptr(), query.data_ptr(),
+    ws = _scored_workspace(query, index, nbytes, zeroed).data_ptr() if nbytes else 0
+    _lib.launch(_lib.SCORED_ATTENTION, index, out.data_ptr(), query.data_ptr(),
                 key_cache.data_ptr(), value_cache.data_ptr(),
-                None if key_scales is None else key_scales.data_ptr(),
-                None if value_scales is None else value_scales.data_ptr(),
-                block_tables.data_ptr(), seq_lens.data_ptr(),
-                None if alibi_slopes is None else alibi_slopes.data_ptr(), shape[0], shape[1],
-                num_kv_heads, head_dim, num_blocks, block_size, tshape[1], strides[0], window,
-                scale, softcap, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype], ws, nbytes,
-                1 if overlap_prologue else 0)
+                0 if key_scales is None else key_scales.data_ptr(),
+                0 if value_scales is None else value_scales.data_ptr(), block_tables.data_ptr(),
+                seq_lens.data_ptr(), 0 if alibi_slopes is None else alibi_slopes.data_ptr(), ws,
+                nbytes, shape[0], shape[1], num_kv_heads, head_dim, num_blocks, block_size,
+                tshape[1], strides[0], window, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype],
+                1 if overlap_prologue else 0, scale, softcap)
     return out
 
 

@@ -288,7 +288,7 @@ def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cach
     v_stride = token_stride(value, T, kvh, head_size, "value")
     if T == 0 or kvh * head_size == 0:
         return
-    _lib.launch("tlb_reshape_and_cache_quantized", index, key.data_ptr(), value.data_ptr(),
+    _lib.launch(_lib.QUANTIZED_WRITE, index, key.data_ptr(), value.data_ptr(),
                 key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
                 value_scales.data_ptr(), slot_mapping.data_ptr(), DTYPE_CODE[slot_dtype], T, kvh,
                 head_size, num_blocks, block_size, k_stride, v_stride, DTYPE_CODE[dtype],
@@ -332,7 +332,7 @@ def dequantize_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor,
         return k, v
     if num_blocks == 0:
         return k.zero_(), v.zero_()
-    _lib.launch("tlb_dequantize_blocks", index, k.data_ptr(), v.data_ptr(), key_cache.data_ptr(),
+    _lib.launch(_lib.DEQUANTIZE, index, k.data_ptr(), v.data_ptr(), key_cache.data_ptr(),
                 value_cache.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
                 block_ids.data_ptr(), DTYPE_CODE[block_ids.dtype], n, kvh, head_size, num_blocks,
                 block_size, DTYPE_CODE[dtype], DTYPE_CODE[key_cache.dtype])

@@ -149,42 +149,62 @@ _FLOAT_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def _check_qk_norm(positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache):
-    """Checks shared by the two entry points below: (device index, tokens, query
-    stride, key stride, table shape)."""
-    index, dtype = query.get_device(), query.dtype
-    torch_check(index >= 0, "query must be a CUDA tensor")
-    torch_check(key.get_device() == index and positions.get_device() == index
-                and cos_sin_cache.get_device() == index and query_weight.get_device() == index
-                and key_weight.get_device() == index,
+    """The checks of ``_qk_norm_shapes`` one by one, for their messages."""
+    torch_check(query.is_cuda, "query must be a CUDA tensor")
+    dev, dtype = query.device, query.dtype
+    torch_check(key.device == dev and positions.device == dev and cos_sin_cache.device == dev
+                and query_weight.device == dev and key_weight.device == dev,
                 "all tensors must be on the same CUDA device")
     torch_check(dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
     torch_check(key.dtype == dtype and cos_sin_cache.dtype == dtype
                 and query_weight.dtype == dtype and key_weight.dtype == dtype,
                 "query, key, cos_sin_cache and the weights must share a dtype")
-    pshape = positions.shape
-    torch_check(len(pshape) == 1 and positions.dtype in _INDEX_TYPES and positions.is_contiguous(),
+    torch_check(positions.dim() == 1 and positions.dtype in _INDEX_TYPES
+                and positions.is_contiguous(),
                 "positions must be a contiguous [num_tokens] int32 or int64 tensor")
     torch_check(head_size > 0, "head_size must be positive")
-    strides = []
     for x in (query, key):
-        shape, stride = x.shape, x.stride()
-        if not (len(shape) == 2 and shape[0] == pshape[0] and shape[1] > 0
-                and shape[1] % head_size == 0 and stride[1] == 1):
-            raise RuntimeError("query and key must be [num_tokens, heads * head_size] with unit "
-                               "inner stride")
-        strides.append(stride[0])
-    wshape = (head_size,)
-    torch_check(query_weight.shape == wshape and key_weight.shape == wshape
+        torch_check(x.dim() == 2 and x.size(0) == positions.size(0) and x.size(1) > 0
+                    and x.size(1) % head_size == 0 and x.stride(1) == 1,
+                    "query and key must be [num_tokens, heads * head_size] with unit inner stride")
+    torch_check(query_weight.shape == (head_size,) and key_weight.shape == (head_size,)
                 and query_weight.is_contiguous() and key_weight.is_contiguous(),
                 "query_weight and key_weight must be contiguous [head_size] tensors")
-    tshape = cos_sin_cache.shape
-    torch_check(len(tshape) == 2 and tshape[0] > 0 and cos_sin_cache.is_contiguous(),
+    torch_check(cos_sin_cache.dim() == 2 and cos_sin_cache.size(0) > 0
+                and cos_sin_cache.is_contiguous(),
                 "cos_sin_cache must be a contiguous [rows, rotary_dim] tensor")
-    rot_dim = tshape[1]
+    rot_dim = cos_sin_cache.size(1)
     torch_check(rot_dim > 0 and rot_dim % 2 == 0, "rotary dimension must be even and positive")
     torch_check(rot_dim <= head_size, "rotary dimension must not exceed head_size")
     torch_check(eps >= 0, "eps must not be negative")
-    return index, pshape[0], strides[0], strides[1], tshape
+    raise RuntimeError("qk_norm_rotary_embedding_neox: unsupported arguments")
+
+
+def _qk_norm_shapes(positions, query, key, query_weight, key_weight, eps, head_size,
+                    cos_sin_cache):
+    """Checks shared by the two entry points below, as one expression (a call's
+    host time counts in a decode step): (device index, tokens, query stride, key
+    stride, query width, key width, table rows, rotary dimension)."""
+    index, dtype = query.get_device(), query.dtype
+    (qs, ks), (qshape, kshape, tshape) = (query.stride(), key.stride()), (
+        query.shape, key.shape, cos_sin_cache.shape)
+    wshape = (head_size,)
+    if not (index >= 0 and len(qshape) == 2 and len(kshape) == 2 and len(tshape) == 2
+            and dtype in _FLOAT_TYPES and key.dtype == dtype and cos_sin_cache.dtype == dtype
+            and query_weight.dtype == dtype and key_weight.dtype == dtype and head_size > 0
+            and positions.shape == qshape[:1] and positions.dtype in _INDEX_TYPES
+            and kshape[0] == qshape[0] and qs[1] == 1 and ks[1] == 1 and qshape[1] > 0
+            and kshape[1] > 0 and qshape[1] % head_size == 0 and kshape[1] % head_size == 0
+            and query_weight.shape == wshape and key_weight.shape == wshape and tshape[0] > 0
+            and 0 < tshape[1] <= head_size and tshape[1] % 2 == 0 and eps >= 0
+            and positions.is_contiguous() and query_weight.is_contiguous()
+            and key_weight.is_contiguous() and cos_sin_cache.is_contiguous()
+            and key.get_device() == index and positions.get_device() == index
+            and cos_sin_cache.get_device() == index and query_weight.get_device() == index
+            and key_weight.get_device() == index):
+        _check_qk_norm(positions, query, key, query_weight, key_weight, eps, head_size,
+                       cos_sin_cache)
+    return index, qshape[0], qs[0], ks[0], qshape[1], kshape[1], tshape[0], tshape[1]
 
 
 def qk_norm_rotary_embedding_neox(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
@@ -199,19 +219,19 @@ def qk_norm_rotary_embedding_neox(positions: torch.Tensor, query: torch.Tensor, 
     head_size], rows possibly strided (parts of a fused projection); weights
     [head_size]. Returns new dense (query, key); the inputs are left as they are.
     """
-    index, num_tokens, q_stride, k_stride, (rows, rot_dim) = _check_qk_norm(
+    index, num_tokens, q_stride, k_stride, q_width, k_width, rows, rot_dim = _qk_norm_shapes(
         positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache)
     q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
     if num_tokens == 0:
         return q_out, k_out
     code = DTYPE_CODE[query.dtype]
-    _lib.launch("tlb_qk_norm_rotary_embedding_neox", index, q_out.data_ptr(), k_out.data_ptr(),
-                positions.data_ptr(), DTYPE_CODE[positions.dtype], query.data_ptr(),
-                key.data_ptr(), None, query_weight.data_ptr(), key_weight.data_ptr(), eps, None,
-                None, None, None, None, 4, None, 0, num_tokens, query.size(1) // head_size,
-                key.size(1) // head_size, head_size, cos_sin_cache.data_ptr(), rows, rot_dim, 0, 0,
-                q_stride, k_stride, 0, code, code, 0)
+    _lib.launch(_lib.QK_NORM_ROPE, index, q_out.data_ptr(), k_out.data_ptr(),
+                positions.data_ptr(), query.data_ptr(), key.data_ptr(), 0,
+                query_weight.data_ptr(), key_weight.data_ptr(), 0, 0, 0, 0, 0, 0,
+                cos_sin_cache.data_ptr(), DTYPE_CODE[positions.dtype], 4, 0, num_tokens,
+                q_width // head_size, k_width // head_size, head_size, rows, rot_dim, 0, 0,
+                q_stride, k_stride, 0, code, code, 0, eps)
     return q_out, k_out
 
 
@@ -234,11 +254,11 @@ def qk_norm_rotary_embedding_neox_with_cache(
     the query dtype. Destinations and ``overlap_previous`` as in
     ``rotary_embedding_neox_with_cache``; the slots of one call must differ.
     """
-    index, num_tokens, q_stride, k_stride, (rows, rot_dim) = _check_qk_norm(
+    index, num_tokens, q_stride, k_stride, q_width, k_width, rows, rot_dim = _qk_norm_shapes(
         positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache)
     dtype, cache_dtype, cshape = query.dtype, key_cache.dtype, key_cache.shape
-    kvh = key.size(1) // head_size
-    ks_ptr = vs_ptr = None
+    kvh = k_width // head_size
+    ks_ptr = vs_ptr = 0
     if cache_dtype in _CACHE8_TYPES:
         torch_check(key_scales is not None and value_scales is not None,
                     "8-bit caches need key_scales and value_scales")
@@ -259,32 +279,30 @@ def qk_norm_rotary_embedding_neox_with_cache(
                     "all tensors must be on the same CUDA device")
     torch_check(cache_index == index and value.get_device() == index,
                 "all tensors must be on the same CUDA device")
-    torch_check(cshape[1] == kvh and cshape[3] == head_size,
-                "cache heads / head_size must match key")
-    torch_check(value.dtype == dtype, "value must have the query dtype")
+    torch_check(cshape[1] == kvh and cshape[3] == head_size and value.dtype == dtype,
+                "cache heads / head_size must match key, and value must have the query dtype")
     v_stride = token_stride(value, num_tokens, kvh, head_size, "value")
     if slot_mapping is not None:
         torch_check(slot_mapping.get_device() == index and slot_mapping.shape == (num_tokens,)
                     and slot_mapping.dtype in _INDEX_TYPES and slot_mapping.is_contiguous(),
                     "slot_mapping must be a contiguous [num_tokens] int32/int64 CUDA tensor")
         slots, slot_code, tables, width = (slot_mapping.data_ptr(),
-                                           DTYPE_CODE[slot_mapping.dtype], None, 0)
+                                           DTYPE_CODE[slot_mapping.dtype], 0, 0)
     else:
         torch_check(block_tables is not None, "either slot_mapping or block_tables is required")
         torch_check(block_tables.get_device() == index and block_tables.dim() == 2
                     and block_tables.dtype == torch.int32 and block_tables.is_contiguous()
                     and block_tables.size(0) >= num_tokens and block_tables.size(1) > 0,
                     "block_tables must be a contiguous int32 CUDA tensor with a row per token")
-        slots, slot_code, tables, width = None, 4, block_tables.data_ptr(), block_tables.size(1)
+        slots, slot_code, tables, width = 0, 4, block_tables.data_ptr(), block_tables.size(1)
     q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if num_tokens == 0:
         return q_out
-    _lib.launch("tlb_qk_norm_rotary_embedding_neox", index, q_out.data_ptr(), None,
-                positions.data_ptr(), DTYPE_CODE[positions.dtype], query.data_ptr(),
-                key.data_ptr(), value.data_ptr(), query_weight.data_ptr(), key_weight.data_ptr(),
-                eps, key_cache.data_ptr(), value_cache.data_ptr(), ks_ptr, vs_ptr, slots,
-                slot_code, tables, width, num_tokens, query.size(1) // head_size, kvh, head_size,
-                cos_sin_cache.data_ptr(), rows, rot_dim, cshape[0], cshape[2], q_stride, k_stride,
-                v_stride, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype],
-                1 if overlap_previous else 0)
+    _lib.launch(_lib.QK_NORM_ROPE, index, q_out.data_ptr(), 0, positions.data_ptr(),
+                query.data_ptr(), key.data_ptr(), value.data_ptr(), query_weight.data_ptr(),
+                key_weight.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), ks_ptr,
+                vs_ptr, slots, tables, cos_sin_cache.data_ptr(), DTYPE_CODE[positions.dtype],
+                slot_code, width, num_tokens, q_width // head_size, kvh, head_size, rows,
+                rot_dim, cshape[0], cshape[2], q_stride, k_stride, v_stride, DTYPE_CODE[dtype],
+                DTYPE_CODE[cache_dtype], 1 if overlap_previous else 0, eps)
     return q_out

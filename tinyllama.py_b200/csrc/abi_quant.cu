@@ -39,6 +39,13 @@ bool is_8bit(int dtype) { return dtype == TLB_FLOAT8_E4M3 || dtype == TLB_INT8; 
 bool is_index(int dtype) { return dtype == TLB_INT32 || dtype == TLB_INT64; }
 int elem_bytes(int dtype) { return dtype == TLB_FLOAT32 ? 4 : is_8bit(dtype) ? 1 : 2; }
 
+// log2 of a power of two, -1 for other numbers.
+int shift_of(int64_t x) {
+    for (int i = 0; i < 24; ++i)
+        if (x == (1ll << i)) return i;
+    return -1;
+}
+
 // 16-byte accesses: every listed pointer aligned, every stride a multiple of
 // 16 bytes.
 bool vec_ok(int dtype, std::initializer_list<const void*> ptrs,
@@ -68,12 +75,25 @@ int cache_checks(const void* key_cache, const void* value_cache, int64_t num_tok
 
 extern "C" {
 
-int tlb_reshape_and_cache_quantized(const void* key, const void* value, void* key_cache,
-                                    void* value_cache, void* key_scales, void* value_scales,
-                                    const void* slots, int slot_dtype, int64_t num_tokens,
-                                    int64_t num_kv_heads, int64_t head_size, int64_t num_blocks,
-                                    int64_t block_size, int64_t key_stride, int64_t value_stride,
-                                    int dtype, int cache_dtype, void* stream) {
+int tlb_reshape_and_cache_quantized(const tlb_quantized_write_args* args, void* stream) {
+    TLB_REQUIRE(args != nullptr, "args must not be null");
+    const void* key = args->key;
+    const void* value = args->value;
+    void* key_cache = args->key_cache;
+    void* value_cache = args->value_cache;
+    void* key_scales = args->key_scales;
+    void* value_scales = args->value_scales;
+    const void* slots = args->slots;
+    const int64_t num_tokens = args->num_tokens;
+    const int64_t num_kv_heads = args->num_kv_heads;
+    const int64_t head_size = args->head_size;
+    const int64_t num_blocks = args->num_blocks;
+    const int64_t block_size = args->block_size;
+    const int64_t key_stride = args->key_stride;
+    const int64_t value_stride = args->value_stride;
+    const int slot_dtype = (int)args->slot_dtype;
+    const int dtype = (int)args->dtype;
+    const int cache_dtype = (int)args->cache_dtype;
     TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
     TLB_REQUIRE(is_8bit(cache_dtype), "cache dtype must be float8_e4m3 or int8");
     if (int rc = cache_checks(key_cache, value_cache, num_tokens, num_kv_heads, head_size,
@@ -102,6 +122,7 @@ int tlb_reshape_and_cache_quantized(const void* key, const void* value, void* ke
     p.num_kv_heads = (int)num_kv_heads;
     p.head_size = (int)head_size;
     p.block_size = (int)block_size;
+    p.block_shift = shift_of(block_size);
     const bool vec = head_size % 16 == 0 && vec_ok(dtype, {key, value, key_cache, value_cache},
                                                   {key_stride, value_stride});
     return cuda_result(tlb::launch_quantize_write(dtype, cache_dtype, p, vec,
@@ -109,12 +130,23 @@ int tlb_reshape_and_cache_quantized(const void* key, const void* value, void* ke
                        "reshape_and_cache_quantized");
 }
 
-int tlb_dequantize_blocks(void* key_out, void* value_out, const void* key_cache,
-                          const void* value_cache, const void* key_scales,
-                          const void* value_scales, const void* block_ids, int id_dtype,
-                          int64_t num_ids, int64_t num_kv_heads, int64_t head_size,
-                          int64_t num_blocks, int64_t block_size, int dtype, int cache_dtype,
-                          void* stream) {
+int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream) {
+    TLB_REQUIRE(args != nullptr, "args must not be null");
+    void* key_out = args->key_out;
+    void* value_out = args->value_out;
+    const void* key_cache = args->key_cache;
+    const void* value_cache = args->value_cache;
+    const void* key_scales = args->key_scales;
+    const void* value_scales = args->value_scales;
+    const void* block_ids = args->block_ids;
+    const int64_t num_ids = args->num_ids;
+    const int64_t num_kv_heads = args->num_kv_heads;
+    const int64_t head_size = args->head_size;
+    const int64_t num_blocks = args->num_blocks;
+    const int64_t block_size = args->block_size;
+    const int id_dtype = (int)args->id_dtype;
+    const int dtype = (int)args->dtype;
+    const int cache_dtype = (int)args->cache_dtype;
     TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
     TLB_REQUIRE(is_8bit(cache_dtype), "cache dtype must be float8_e4m3 or int8");
     if (int rc = cache_checks(key_cache, value_cache, num_ids, num_kv_heads, head_size, num_blocks,
@@ -147,18 +179,44 @@ int tlb_dequantize_blocks(void* key_out, void* value_out, const void* key_cache,
                        "dequantize_blocks");
 }
 
-int tlb_qk_norm_rotary_embedding_neox(
-    void* query_out, void* key_out, const void* positions, int pos_dtype, const void* query,
-    const void* key, const void* value, const void* query_weight, const void* key_weight,
-    float eps, void* key_cache, void* value_cache, void* key_scales, void* value_scales,
-    const void* slots, int slot_dtype, const int32_t* block_tables, int64_t max_blocks_per_seq,
-    int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_size,
-    const void* cos_sin_cache, int64_t cache_rows, int64_t rot_dim, int64_t num_blocks,
-    int64_t block_size, int64_t query_stride, int64_t key_stride, int64_t value_stride, int dtype,
-    int cache_dtype, unsigned flags, void* stream) {
+int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args, void* stream) {
+    TLB_REQUIRE(args != nullptr, "args must not be null");
+    void* query_out = args->query_out;
+    void* key_out = args->key_out;
+    const void* positions = args->positions;
+    const void* query = args->query;
+    const void* key = args->key;
+    const void* value = args->value;
+    const void* query_weight = args->query_weight;
+    const void* key_weight = args->key_weight;
+    void* key_cache = args->key_cache;
+    void* value_cache = args->value_cache;
+    void* key_scales = args->key_scales;
+    void* value_scales = args->value_scales;
+    const void* slots = args->slots;
+    const int32_t* block_tables = args->block_tables;
+    const void* cos_sin_cache = args->cos_sin_cache;
+    const int64_t max_blocks_per_seq = args->max_blocks_per_seq;
+    const int64_t num_tokens = args->num_tokens;
+    const int64_t num_heads = args->num_heads;
+    const int64_t num_kv_heads = args->num_kv_heads;
+    const int64_t head_size = args->head_size;
+    const int64_t cache_rows = args->cache_rows;
+    const int64_t rot_dim = args->rot_dim;
+    const int64_t num_blocks = args->num_blocks;
+    const int64_t block_size = args->block_size;
+    const int64_t query_stride = args->query_stride;
+    const int64_t key_stride = args->key_stride;
+    const int64_t value_stride = args->value_stride;
+    const int64_t flags = args->flags;
+    const int pos_dtype = (int)args->pos_dtype;
+    const int slot_dtype = (int)args->slot_dtype;
+    const int dtype = (int)args->dtype;
+    const int cache_dtype = (int)args->cache_dtype;
+    const float eps = (float)args->eps;
     TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
     TLB_REQUIRE(is_index(pos_dtype), "positions must be int32 or int64");
-    TLB_REQUIRE((flags & ~TLB_ROPE_OVERLAP_PREVIOUS) == 0, "unknown flags");
+    TLB_REQUIRE((flags & ~(int64_t)TLB_ROPE_OVERLAP_PREVIOUS) == 0, "unknown flags");
     TLB_REQUIRE(num_tokens >= 0 && num_heads > 0 && num_kv_heads > 0 && head_size > 0,
                 "sizes must be positive");
     TLB_REQUIRE(num_tokens < (1ll << 40) && num_heads < (1 << 16) && num_kv_heads < (1 << 16) &&
@@ -223,6 +281,7 @@ int tlb_qk_norm_rotary_embedding_neox(
     p.head_size = (int)head_size;
     p.rot_dim = (int)rot_dim;
     p.block_size = with_cache ? (int)block_size : 1;
+    p.block_shift = shift_of(p.block_size);
     p.eps = eps;
     p.overlap = (flags & TLB_ROPE_OVERLAP_PREVIOUS) != 0;
     const bool vec = head_size % 16 == 0 && rot_dim % 16 == 0 &&
@@ -292,20 +351,36 @@ int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t num_kv_
     return TLB_OK;
 }
 
-int tlb_paged_attention_scored(void* out, const void* query, const void* key_cache,
-                               const void* value_cache, const void* key_scales,
-                               const void* value_scales, const int32_t* block_tables,
-                               const int32_t* seq_lens, const float* alibi_slopes,
-                               int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
-                               int64_t head_dim, int64_t num_blocks, int64_t block_size,
-                               int64_t max_blocks_per_seq, int64_t query_stride, int64_t window,
-                               float scale, float softcap, int dtype, int cache_dtype,
-                               void* workspace, size_t workspace_bytes, unsigned flags,
-                               void* stream) {
+int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stream) {
+    TLB_REQUIRE(args != nullptr, "args must not be null");
+    void* out = args->out;
+    const void* query = args->query;
+    const void* key_cache = args->key_cache;
+    const void* value_cache = args->value_cache;
+    const void* key_scales = args->key_scales;
+    const void* value_scales = args->value_scales;
+    const int32_t* block_tables = args->block_tables;
+    const int32_t* seq_lens = args->seq_lens;
+    const float* alibi_slopes = args->alibi_slopes;
+    void* workspace = args->workspace;
+    const int64_t num_seqs = args->num_seqs;
+    const int64_t num_heads = args->num_heads;
+    const int64_t num_kv_heads = args->num_kv_heads;
+    const int64_t head_dim = args->head_dim;
+    const int64_t num_blocks = args->num_blocks;
+    const int64_t block_size = args->block_size;
+    const int64_t max_blocks_per_seq = args->max_blocks_per_seq;
+    const int64_t query_stride = args->query_stride;
+    const int64_t window = args->window;
+    const int64_t flags = args->flags;
+    const int dtype = (int)args->dtype;
+    const int cache_dtype = (int)args->cache_dtype;
+    const float scale = (float)args->scale;
+    const float softcap = (float)args->softcap;
     TLB_REQUIRE(is_float(dtype), "dtype must be float16, bfloat16 or float32");
     TLB_REQUIRE(cache_dtype == dtype || is_8bit(cache_dtype),
                 "the caches must have the query dtype, or be float8_e4m3 or int8");
-    TLB_REQUIRE((flags & ~TLB_ATTN_OVERLAP_PROLOGUE) == 0, "unknown flags");
+    TLB_REQUIRE((flags & ~(int64_t)TLB_ATTN_OVERLAP_PROLOGUE) == 0, "unknown flags");
     TLB_REQUIRE(num_seqs > 0, "query must contain at least one sequence");
     TLB_REQUIRE(num_heads > 0 && num_kv_heads > 0 && head_dim > 0 && num_blocks > 0 &&
                     block_size > 0 && max_blocks_per_seq > 0,
@@ -326,6 +401,7 @@ int tlb_paged_attention_scored(void* out, const void* query, const void* key_cac
     TLB_REQUIRE(aligned(query, e) && aligned(out, e) && aligned(key_cache, ce) &&
                     aligned(value_cache, ce),
                 "tensor pointers must be aligned to the element size");
+    const size_t workspace_bytes = args->workspace_bytes > 0 ? (size_t)args->workspace_bytes : 0;
     namespace sc = tlb::scored;
     sc::Params p{};
     p.out = out;
@@ -348,9 +424,7 @@ int tlb_paged_attention_scored(void* out, const void* query, const void* key_cac
     p.units_per_seq = p.num_kv_heads * p.head_chunks;
     p.head_dim = (int)head_dim;
     p.block_size = (int)block_size;
-    p.block_shift = -1;
-    for (int i = 0; i < 24; ++i)
-        if (block_size == (1ll << i)) p.block_shift = i;
+    p.block_shift = shift_of(block_size);
     p.max_blocks = (int)max_blocks_per_seq;
     p.max_tokens = (int)(max_blocks_per_seq * block_size);
     p.window = window < p.max_tokens ? (int)window : 0;

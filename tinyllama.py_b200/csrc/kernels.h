@@ -213,6 +213,7 @@ struct QuantCacheParams {
     int head_size;
     int rot_dim;
     int block_size;
+    int block_shift;           // log2(block_size), -1 when it is no power of two
     float eps;
     bool positions64, slots64;
     bool overlap;              // launched with programmatic stream serialization

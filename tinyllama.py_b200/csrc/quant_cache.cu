@@ -209,7 +209,13 @@ __device__ __forceinline__ long long divide(long long x, int by, int& rest) {
 __device__ __forceinline__ long long slot_row(long long slot, const QuantCacheParams& p) {
     if (slot < 0) return -1;
     int off;
-    const long long blk = divide(slot, p.block_size, off);
+    long long blk;
+    if (p.block_shift >= 0) {
+        blk = slot >> p.block_shift;
+        off = (int)(slot & (p.block_size - 1));
+    } else {
+        blk = divide(slot, p.block_size, off);
+    }
     if (blk >= p.num_blocks) {
         flag_status(TLB_STATUS_BAD_SLOT);
         return -1;
@@ -245,7 +251,9 @@ struct Place {
 };
 __device__ __forceinline__ Place place_of(long long item, long long items, int parts, int step) {
     Place c{item, 0, 0, item < items};
-    if (c.valid) {
+    if (parts == 1) {
+        c.t = item;
+    } else if (c.valid) {
         int part;
         c.t = divide(item, parts, part);
         c.first = part * step;
