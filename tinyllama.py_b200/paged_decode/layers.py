@@ -17,6 +17,10 @@ dtype instead of on every call (:148-150).
 position of every token is ``seq_lens - 1``; with full-width rotary
 (``rotary_dim == head_size``) the whole step then runs as ONE launch
 (``cscr.attention.paged_attention_with_rope``).
+
+``PagedAttentionWithQKNorm`` (not in the reference) is the same layer for models
+that normalise each query and key head, cap their scores or limit them to a
+window, over caches of the model dtype or of 8 bits.
 """
 
 from __future__ import annotations
@@ -120,3 +124,88 @@ class PagedAttentionWithRoPE(PagedAttention):
         return _C.paged_attention(query=query, key_cache=key_cache, value_cache=value_cache,
                                   block_tables=tables, seq_lens=seq_lens, scale=self.scale,
                                   overlap_prologue=fused)
+
+
+class PagedAttentionWithQKNorm(PagedAttentionWithRoPE):
+    """``PagedAttentionWithRoPE`` with an RMS norm of each query and key head,
+    optionally capped scores (``softcap``) and a window, over 16-bit caches or
+    8-bit ones with their row scales (``paged_decode.pool.
+    allocate_quantized_kv_cache``).
+
+    A decode step is two launches: norm, rotation and cache write, then
+    attention. ``prompt`` serves prompt chunks; over 8-bit caches it reads the
+    chunks' blocks back and runs the 16-bit prefill kernel on them.
+    """
+
+    def __init__(self, num_heads: int, head_size: int, scale: float, rotary_dim: int,
+                 max_position: int = 8192, base: int = 10000, eps: float = 1e-6,
+                 softcap: float = 0.0, window: int = 0):
+        super().__init__(num_heads, head_size, scale, rotary_dim, max_position, base)
+        self.eps, self.softcap, self.window = eps, softcap, window
+        self.q_norm = nn.Parameter(torch.ones(head_size), requires_grad=False)
+        self.k_norm = nn.Parameter(torch.ones(head_size), requires_grad=False)
+
+    def _norm_rope_write(self, positions, query, key, value, key_cache, value_cache, slots, tables,
+                         key_scales, value_scales):
+        num_tokens, num_heads, head_size = query.shape
+        if head_size != self.head_size:
+            raise ValueError("query head_dim must match head_size")
+        dtype = query.dtype
+        out = _PE.qk_norm_rotary_embedding_neox_with_cache(
+            positions, query.reshape(num_tokens, -1), key.reshape(num_tokens, -1), value,
+            self.q_norm.to(dtype), self.k_norm.to(dtype), self.eps, key_cache, value_cache, slots,
+            head_size, self._table(query.device, dtype), block_tables=tables,
+            key_scales=key_scales, value_scales=value_scales)
+        return out.view(num_tokens, num_heads, head_size)
+
+    def forward(self, positions: torch.Tensor | None, query: torch.Tensor, key: torch.Tensor,
+                value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                key_scales: torch.Tensor | None = None,
+                value_scales: torch.Tensor | None = None) -> torch.Tensor:
+        """A decode step: query [S, H, D], key and value [S, KVH, D], one token per
+        sequence, at ``positions`` or (None) at ``seq_lens - 1`` -> [S, H, D]."""
+        if query.dim() != 3 or query.size(0) != block_tables.size(0):
+            raise NotImplementedError(
+                "PagedAttentionWithQKNorm.forward is a decode step: there must be one token per "
+                "sequence")
+        tables = block_tables.to(torch.int32).contiguous()
+        if positions is None:
+            positions = seq_lens.to(torch.int64) - 1
+        query = self._norm_rope_write(positions, query, key, value, key_cache, value_cache, None,
+                                      tables, key_scales, value_scales)
+        # The kernel just launched writes neither the tables nor seq_lens, so
+        # attention may overlap its prologue.
+        if key_scales is not None:
+            return _C.paged_attention_quantized(
+                query, key_cache, value_cache, key_scales, value_scales, tables, seq_lens,
+                self.scale, softcap=self.softcap, window=self.window, overlap_prologue=True)
+        if self.softcap or self.window:
+            return _C.paged_attention_biased(query, key_cache, value_cache, tables, seq_lens,
+                                             self.scale, softcap=self.softcap, window=self.window,
+                                             overlap_prologue=True)
+        return _C.paged_attention(query, key_cache, value_cache, tables, seq_lens, self.scale,
+                                  overlap_prologue=True)
+
+    def prompt(self, positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
+               value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+               slot_mapping: torch.Tensor, block_tables: torch.Tensor, query_start: torch.Tensor,
+               context_lens: torch.Tensor, max_query_len: int | None = None,
+               key_scales: torch.Tensor | None = None,
+               value_scales: torch.Tensor | None = None) -> torch.Tensor:
+        """Prompt chunks (packed tokens [T, ...]), as ``cscr.attention.
+        paged_prefill_attention`` takes them; the new rows go to ``slot_mapping``."""
+        if self.softcap or self.window:
+            raise NotImplementedError("prompt chunks have plain scores: no softcap, no window")
+        query = self._norm_rope_write(positions, query, key, value, key_cache, value_cache,
+                                      slot_mapping, None, key_scales, value_scales)
+        tables = block_tables.to(torch.int32).contiguous()
+        if key_scales is not None:
+            # the chunks' blocks in the query dtype: entry j of chunk c is block
+            # c * max_blocks + j of what is read back (holes stay holes)
+            key_cache, value_cache = _Cache.dequantize_blocks(
+                key_cache, value_cache, key_scales, value_scales, tables.view(-1), query.dtype)
+            places = torch.arange(tables.numel(), dtype=torch.int32, device=tables.device)
+            tables = torch.where(tables < 0, tables, places.view_as(tables))
+        return _C.paged_prefill_attention(query, key_cache, value_cache, tables, query_start,
+                                          context_lens, self.scale, max_query_len)

@@ -60,3 +60,37 @@ def allocate_kv_cache(num_layers: int, num_blocks: int, num_kv_heads: int, head_
     shape = (num_blocks, num_kv_heads, block_size, head_size)
     return [(torch.empty(shape, dtype=dtype, device=device),
              torch.empty(shape, dtype=dtype, device=device)) for _ in range(num_layers)]
+
+
+QuantizedKVCache = tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
+
+
+def quantized_block_bytes(num_layers: int, num_kv_heads: int, head_size: int,
+                          block_size: int) -> int:
+    """Bytes one block number of 8-bit caches costs across all layers: K and V,
+    a byte for each value and one for each row's scale."""
+    return num_layers * 2 * block_size * num_kv_heads * (head_size + 1)
+
+
+def allocate_quantized_kv_cache(num_layers: int, num_blocks: int, num_kv_heads: int,
+                                head_size: int, block_size: int,
+                                dtype: torch.dtype = torch.float8_e4m3fn,
+                                device: torch.device | str = "cuda") -> list[QuantizedKVCache]:
+    """One ``(key_cache, value_cache, key_scales, value_scales)`` per layer:
+    caches ``[num_blocks, num_kv_heads, block_size, head_size]`` of
+    float8_e4m3fn or int8, scales ``[num_blocks, num_kv_heads, block_size]`` of
+    float8_e8m0fnu, uninitialised. ``cscr.cache.copy_blocks`` moves blocks of
+    both: pass the scales as further caches."""
+    if num_blocks <= 0:
+        raise ValueError(
+            "No KV cache blocks allocated. Profile the available memory before creating "
+            "the cache.")
+    if dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise ValueError("8-bit caches are float8_e4m3fn or int8")
+    rows = (num_blocks, num_kv_heads, block_size)
+    shape = (*rows, head_size)
+    return [(torch.empty(shape, dtype=dtype, device=device),
+             torch.empty(shape, dtype=dtype, device=device),
+             torch.empty(rows, dtype=torch.float8_e8m0fnu, device=device),
+             torch.empty(rows, dtype=torch.float8_e8m0fnu, device=device))
+            for _ in range(num_layers)]
