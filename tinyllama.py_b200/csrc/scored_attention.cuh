@@ -1003,7 +1003,8 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
             const int c0 = warp ? owner[1] : owner[0], n = warp ? shares[1] : shares[0];
             bool last = false;
             if ((warp ? shared_row[1] : shared_row[0]) >= 0) {
-                __threadfence();
+                // releases what the barrier has made this thread see: all the
+                // CTA's stores of its partial
                 last = atomic_inc_acq_rel(p.counters + c0, n - 1) == (unsigned)n - 1;
             }
             last_cta[warp] = last;
