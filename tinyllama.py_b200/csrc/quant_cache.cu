@@ -244,28 +244,34 @@ __device__ __forceinline__ long long table_row(long long t, long long pos,
 // A warp's place in its share of the work: rows [first, first + step) of token
 // t's `rows` rows, taken `step` at a time by each of the `parts` warps that share
 // a token; then the same of a later token.
+// The token's position and slot are loaded when the place is taken, a step
+// before they are used.
 struct Place {
-    long long item, t;
+    long long item, t, pos, slot;
     int first;
     bool valid;
 };
-__device__ __forceinline__ Place place_of(long long item, long long items, int parts, int step) {
-    Place c{item, 0, 0, item < items};
-    if (parts == 1) {
+__device__ __forceinline__ Place place_of(long long item, long long items, int parts, int step,
+                                          const QuantCacheParams& p) {
+    Place c{item, 0, 0, -1, 0, item < items};
+    if (c.valid) {
         c.t = item;
-    } else if (c.valid) {
-        int part;
-        c.t = divide(item, parts, part);
-        c.first = part * step;
+        if (parts != 1) {
+            int part;
+            c.t = divide(item, parts, part);
+            c.first = part * step;
+        }
+        if (p.positions) c.pos = load_int(p.positions, p.positions64, c.t);
+        if (p.slots) c.slot = load_int(p.slots, p.slots64, c.t);
     }
     return c;
 }
 __device__ __forceinline__ Place next_place(const Place& c, long long items, int parts, int step,
-                                            int rows) {
+                                            int rows, const QuantCacheParams& p) {
     Place n = c;
     n.first += parts * step;
     if (n.first < rows) return n;
-    return place_of(c.item + (long long)gridDim.x * 8, items, parts, step);
+    return place_of(c.item + (long long)gridDim.x * 8, items, parts, step, p);
 }
 
 // ------------------------------------------------------------- cache write
@@ -310,7 +316,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quantize_write_ke
     auto store = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
         if (known != c.t) {
             known = c.t;
-            const long long base = slot_row(load_int(p.slots, p.slots64, c.t), p);
+            const long long base = slot_row(c.slot, p);
             key_row = nullptr;
             if (base >= 0) {
                 key_row = reinterpret_cast<uint8_t*>(p.key_cache) + base * D;
@@ -338,14 +344,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quantize_write_ke
             if (sub == 0) (is_value ? value_scale : key_scale)[h * p.block_size] = (uint8_t)byte;
         }
     };
-    Place c = place_of(blockIdx.x * 8 + threadIdx.x / 32, items, parts, STEP);
+    Place c = place_of(blockIdx.x * 8 + threadIdx.x / 32, items, parts, STEP, p);
     load(c, a0, a1);
     while (c.valid) {
-        Place n = next_place(c, items, parts, STEP, rows);
+        Place n = next_place(c, items, parts, STEP, rows, p);
         load(n, b0, b1);
         store(c, a0, a1);
         if (!n.valid) break;
-        c = next_place(n, items, parts, STEP, rows);
+        c = next_place(n, items, parts, STEP, rows, p);
         load(c, a0, a1);
         store(n, b0, b1);
     }
@@ -544,7 +550,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kern
     auto process = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
         if (known != c.t) {
             known = c.t;
-            const long long pos = load_int(p.positions, p.positions64, c.t);
+            const long long pos = c.pos;
             rotate = false;
             if (pos >= 0 && pos < p.cache_rows) {
                 rotate = turn;
@@ -560,8 +566,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kern
                 flag_status(TLB_STATUS_BAD_POSITION);
             }
             if (with_cache)
-                base = p.slots ? slot_row(load_int(p.slots, p.slots64, c.t), p)
-                               : table_row(c.t, pos, p);
+                base = p.slots ? slot_row(c.slot, p) : table_row(c.t, pos, p);
         }
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
@@ -646,14 +651,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kern
         }
     };
     grid_dependency_wait();
-    Place c = place_of(blockIdx.x * 8 + threadIdx.x / 32, items, parts, STEP);
+    Place c = place_of(blockIdx.x * 8 + threadIdx.x / 32, items, parts, STEP, p);
     load(c, a0, a1);
     while (c.valid) {
-        Place n = next_place(c, items, parts, STEP, rows);
+        Place n = next_place(c, items, parts, STEP, rows, p);
         load(n, b0, b1);
         process(c, a0, a1);
         if (!n.valid) break;
-        c = next_place(n, items, parts, STEP, rows);
+        c = next_place(n, items, parts, STEP, rows, p);
         load(c, a0, a1);
         process(n, b0, b1);
     }
