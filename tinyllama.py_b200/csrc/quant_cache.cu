@@ -74,6 +74,10 @@ template <typename T> struct Raw8 {
 #pragma unroll
         for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
     }
+    __device__ __forceinline__ void store_stream(T* p) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, u[i]);
+    }
     // The largest magnitude, for half types one of the even and one of the odd
     // elements packed; NaN where there is one.
     __device__ __forceinline__ uint32_t top() const {
@@ -275,18 +279,20 @@ __device__ __forceinline__ Place next_place(const Place& c, long long items, int
 }
 
 // ------------------------------------------------------------- cache write
-// HBM bound: 2 e D bytes in, D + 1 out for each row of e-byte values. A warp
-// takes rows of one token: all keys, then all values. A row is held by LANES
-// lanes, 16 values each (two 16-byte loads, 8-byte stores) between its one read
-// and its one write; kRows rows of a group are read while kRows are quantised
-// and stored (rows in one buffer only: the loads waited half the time). Rows of
-// other widths and alignments take a warp each, element by element, and are
-// read twice.
-constexpr int kRows = 2;
+// HBM bound: e D bytes in, D + 1 out for each row of e-byte values. A warp takes
+// rows of one token: all keys, then all values. A row is held by LANES lanes, 16
+// values each (two 16-byte loads, 8-byte stores) between its one read and its one
+// write; kWriteRows rows of a group are read while kWriteRows are quantised and
+// stored. 16381 fp16 tokens of 8 heads of 128 to int8 (101 MB): 19.7 us with 4
+// rows and 16 warps an SM, 21.3 us with 2, 23.5 us with 1 row and 24 warps. Of
+// 24 us, 3 went into the scales' single bytes and 5.5 into the rows' stores.
+// Rows of other widths and alignments take a warp each, element by element, and
+// are read twice.
+constexpr int kWriteRows = 4;
 
 template <typename T, typename C, int LANES>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quantize_write_kernel(const QuantCacheParams p, int parts) {
-    constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kRows;
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) quantize_write_kernel(const QuantCacheParams p, int parts) {
+    constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kWriteRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
     const uint32_t mask = group_mask<LANES>();
     const int D = p.head_size, kvh = p.num_kv_heads, rows = 2 * kvh;
@@ -295,12 +301,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quantize_write_ke
     const long long items = p.num_tokens * parts;
     const int head_stride = p.block_size * D;  // of a cache, in values
 
-    Raw8<T> a0[kRows], a1[kRows], b0[kRows], b1[kRows];
-    auto load = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
+    Raw8<T> a0[kWriteRows], a1[kWriteRows], b0[kWriteRows], b1[kWriteRows];
+    auto load = [&](const Place& c, Raw8<T> (&x0)[kWriteRows], Raw8<T> (&x1)[kWriteRows]) {
         const T* key = reinterpret_cast<const T*>(p.key) + c.t * p.key_stride;
         const T* value = reinterpret_cast<const T*>(p.value) + c.t * p.value_stride;
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
+        for (int i = 0; i < kWriteRows; ++i) {
             const int r = c.first + i * GROUPS + grp;
             x0[i].zero();
             x1[i].zero();
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quantize_write_ke
     };
     long long known = -1;  // the token looked up last, and its rows of head 0
     uint8_t *key_row = nullptr, *value_row = nullptr, *key_scale = nullptr, *value_scale = nullptr;
-    auto store = [&](const Place& c, Raw8<T> (&x0)[kRows], Raw8<T> (&x1)[kRows]) {
+    auto store = [&](const Place& c, Raw8<T> (&x0)[kWriteRows], Raw8<T> (&x1)[kWriteRows]) {
         if (known != c.t) {
             known = c.t;
             const long long base = slot_row(c.slot, p);
@@ -327,7 +333,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 1) quantize_write_ke
         }
         if (key_row == nullptr) return;
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
+        for (int i = 0; i < kWriteRows; ++i) {
             const int r = c.first + i * GROUPS + grp;
             if (r >= rows) break;
             const bool is_value = r >= kvh;
@@ -382,9 +388,11 @@ __global__ void __launch_bounds__(256) quantize_write_any_kernel(const QuantCach
 
 // -------------------------------------------------------------- read back
 // HBM bound: D + 1 bytes in, e D out for each row. Flat over 16-value pieces of
-// the listed blocks (pieces never straddle a row); two pieces of both caches are
-// in flight for each thread. IX: index type of the piece arithmetic (32-bit
-// unsigned where it fits).
+// the listed blocks (pieces never straddle a row), a piece of each cache for a
+// thread and step. The values go past the caches (streaming stores): 9000 blocks
+// of 2 x 16 rows of 128 (222 MB) take 38.7 us, with plain stores and two pieces
+// in flight 42.5. IX: index type of the piece arithmetic (32-bit unsigned where
+// it fits).
 template <typename T, typename C>
 __device__ __forceinline__ void widen16(T* out, uint4 u, float scale) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -396,52 +404,34 @@ __device__ __forceinline__ void widen16(T* out, uint4 u, float scale) {
             f[j] = mul_keep(dequantize1<C>((w[2 * half + (j >> 2)] >> (8 * (j & 3))) & 0xff), scale);
         Raw8<T> r;
         r.set(f);
-        r.store(out + 8 * half);
+        r.store_stream(out + 8 * half);
     }
 }
 
 template <typename T, typename C, typename IX>
 __global__ void __launch_bounds__(256) dequantize_blocks_kernel(const DequantParams p) {
-    constexpr int U = 2;
     const unsigned row_pieces = p.head_size / 16;
     const IX pieces = (IX)p.rows_per_block * row_pieces;  // of a block
     const IX total = pieces * (IX)p.num_ids;
-    const IX step = (IX)gridDim.x * 256;
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.key_cache);
     const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.value_cache);
-    for (IX i0 = (IX)blockIdx.x * 256 + threadIdx.x; i0 < total; i0 += U * step) {
-        uint4 k[U], v[U];
-        uint32_t ks[U], vs[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const IX i = i0 + j * step;
-            k[j] = v[j] = make_uint4(0, 0, 0, 0);
-            ks[j] = vs[j] = 0;
-            if (i < total && i >= i0) {
-                const IX n = i / pieces;
-                const unsigned piece = (unsigned)(i - n * pieces);
-                const long long blk = load_int(p.ids, p.ids64, n);
-                if (blk >= p.num_blocks) flag_status(TLB_STATUS_BAD_BLOCK_ID);
-                if (blk >= 0 && blk < p.num_blocks) {
-                    const long long from = (blk * (long long)pieces + piece) * 16;
-                    const long long row = blk * p.rows_per_block + piece / row_pieces;
-                    k[j] = __ldcs(reinterpret_cast<const uint4*>(kc + from));
-                    v[j] = __ldcs(reinterpret_cast<const uint4*>(vc + from));
-                    ks[j] = p.key_scales[row];
-                    vs[j] = p.value_scales[row];
-                }
-            }
+    for (IX i = (IX)blockIdx.x * 256 + threadIdx.x; i < total; i += (IX)gridDim.x * 256) {
+        const IX n = i / pieces;
+        const unsigned piece = (unsigned)(i - n * pieces);
+        const long long blk = load_int(p.ids, p.ids64, n);
+        uint4 k = make_uint4(0, 0, 0, 0), v = k;
+        uint32_t ks = 0, vs = 0;
+        if (blk >= p.num_blocks) flag_status(TLB_STATUS_BAD_BLOCK_ID);
+        if (blk >= 0 && blk < p.num_blocks) {
+            const long long from = (blk * (long long)pieces + piece) * 16;
+            const long long row = blk * p.rows_per_block + piece / row_pieces;
+            k = __ldcs(reinterpret_cast<const uint4*>(kc + from));
+            v = __ldcs(reinterpret_cast<const uint4*>(vc + from));
+            ks = p.key_scales[row];
+            vs = p.value_scales[row];
         }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const IX i = i0 + j * step;
-            if (i < total && i >= i0) {
-                widen16<T, C>(reinterpret_cast<T*>(p.key_out) + (long long)i * 16, k[j],
-                              scale_value(ks[j]));
-                widen16<T, C>(reinterpret_cast<T*>(p.value_out) + (long long)i * 16, v[j],
-                              scale_value(vs[j]));
-            }
-        }
+        widen16<T, C>(reinterpret_cast<T*>(p.key_out) + (long long)i * 16, k, scale_value(ks));
+        widen16<T, C>(reinterpret_cast<T*>(p.value_out) + (long long)i * 16, v, scale_value(vs));
     }
 }
 
@@ -485,6 +475,8 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const DequantParams
 // rotation needs no exchange), the others 16 values beyond rot. A group keeps
 // its weights while it stays with queries or with keys; kRows of its rows are
 // read while kRows are worked on. Other widths and alignments: a warp for each row, by element.
+constexpr int kRows = 2;
+
 enum RowKind { kQuery = 0, kKey = 1, kValue = 2 };
 
 struct NormRow {
@@ -764,9 +756,9 @@ int parts_of(long long tokens, int rows, int step) {
 
 template <typename T, typename C, int LANES>
 void write_lanes(const QuantCacheParams& p, cudaStream_t st) {
-    const int parts = parts_of(p.num_tokens, 2 * p.num_kv_heads, 32 / LANES * kRows);
+    const int parts = parts_of(p.num_tokens, 2 * p.num_kv_heads, 32 / LANES * kWriteRows);
     quantize_write_kernel<T, C, LANES>
-        <<<grid_of(p.num_tokens * parts, 8, 3), 256, 0, st>>>(p, parts);
+        <<<grid_of(p.num_tokens * parts, 8, 2), 256, 0, st>>>(p, parts);
 }
 template <typename T, typename C>
 cudaError_t write_tc(const QuantCacheParams& p, bool vec, cudaStream_t st) {
@@ -792,12 +784,12 @@ cudaError_t write_t(int cache_dtype, const QuantCacheParams& p, bool vec, cudaSt
 template <typename T, typename C>
 cudaError_t dequant_tc(const DequantParams& p, bool vec, cudaStream_t st) {
     const long long values = p.num_ids * p.rows_per_block * p.head_size;
-    // 32-bit piece numbers, with room for one step past the end
+    // 32-bit piece numbers, with room for a step past the end
     if (vec && values / 16 < (1ll << 31))
-        dequantize_blocks_kernel<T, C, unsigned><<<grid_of(values / 32, 256), 256, 0, st>>>(p);
+        dequantize_blocks_kernel<T, C, unsigned><<<grid_of(values / 16, 256), 256, 0, st>>>(p);
     else if (vec)
         dequantize_blocks_kernel<T, C, unsigned long long>
-            <<<grid_of(values / 32, 256), 256, 0, st>>>(p);
+            <<<grid_of(values / 16, 256), 256, 0, st>>>(p);
     else
         dequantize_any_kernel<T, C><<<grid_of(values, 256), 256, 0, st>>>(p);
     return cudaGetLastError();
