@@ -428,6 +428,7 @@ int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stre
     p.max_blocks = (int)max_blocks_per_seq;
     p.max_tokens = (int)(max_blocks_per_seq * block_size);
     p.window = window < p.max_tokens ? (int)window : 0;
+    p.overlap = (flags & TLB_ATTN_OVERLAP_PROLOGUE) != 0;
     p.scale = scale;
     p.cap_log2 = softcap * 1.4426950408889634f;
     p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
@@ -466,7 +467,6 @@ int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stre
     p.warp_partials = reinterpret_cast<float4*>(ws + w.warp_partials);
     p.cta_partials = reinterpret_cast<float4*>(ws + w.cta_partials);
     p.cta_ml = reinterpret_cast<float2*>(ws + w.cta_ml);
-    const bool overlap = (flags & TLB_ATTN_OVERLAP_PROLOGUE) != 0;
     p.box_shift = sc::box_shift_of(p.block_size, tt);
     p.wait_limit = tlb::attention_wait_limit();
     CUtensorMap tk, tv;
@@ -476,7 +476,7 @@ int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stre
     auto launch = cache_dtype == TLB_FLOAT8_E4M3 ? sc::launch_e4m3
                   : cache_dtype == TLB_INT8      ? sc::launch_int8
                                                  : sc::launch_16bit;
-    const cudaError_t err = launch(dtype, p, tk, tv, ctas, overlap, st);
+    const cudaError_t err = launch(dtype, p, tk, tv, ctas, st);
     return cuda_result(err, "paged attention");
 }
 

@@ -216,7 +216,7 @@ struct QuantCacheParams {
     int block_shift;           // log2(block_size), -1 when it is no power of two
     float eps;
     bool positions64, slots64;
-    bool overlap;              // launched with programmatic stream serialization
+    bool overlap;              // the kernel before writes no positions, slots, tables, weights
 };
 struct DequantParams {
     void* key_out;
@@ -285,6 +285,7 @@ struct Params {
     int max_blocks;
     int max_tokens;               // max_blocks * block_size
     int window;                   // tokens the query sees, 0: all
+    bool overlap;                 // the kernel before writes neither lengths nor tables
     unsigned long long inv_warps; // ceil(2^64 / warps of the grid)
     bool aligned;                 // a CTA takes one whole unit
     int box_shift;                // log2 of the cache rows a TMA box holds
@@ -313,11 +314,11 @@ int ctas_for(long long units, long long unit_tiles, int group, int sms);
 int box_shift_of(int block_size, int tile);
 
 cudaError_t launch_e4m3(int dtype, const Params& p, const CUtensorMap& map_k,
-                        const CUtensorMap& map_v, int ctas, bool overlap, cudaStream_t stream);
+                        const CUtensorMap& map_v, int ctas, cudaStream_t stream);
 cudaError_t launch_int8(int dtype, const Params& p, const CUtensorMap& map_k,
-                        const CUtensorMap& map_v, int ctas, bool overlap, cudaStream_t stream);
+                        const CUtensorMap& map_v, int ctas, cudaStream_t stream);
 cudaError_t launch_16bit(int dtype, const Params& p, const CUtensorMap& map_k,
-                         const CUtensorMap& map_v, int ctas, bool overlap, cudaStream_t stream);
+                         const CUtensorMap& map_v, int ctas, cudaStream_t stream);
 // Any shape and type, one CTA per (sequence, query head).
 cudaError_t launch_generic(int dtype, int cache_dtype, const Params& p, cudaStream_t stream);
 

@@ -19,6 +19,29 @@
 
 namespace tlb {
 
+template <typename T> struct Same {
+    using type = T;
+};
+// Launches that may begin while the kernel before them on the stream ends
+// (programmatic stream serialization). Their kernels wait for it
+// (grid_dependency_wait) before they touch memory, or before they touch what
+// an `overlap` flag does not except; what is saved is the launch itself.
+template <typename... Args>
+cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t smem,
+                         cudaStream_t stream, typename Same<Args>::type... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Storage tag of an e4m3 cache (one byte per value, as int8_t is for int8).
 struct E4M3 {
     uint8_t bits;

@@ -292,6 +292,8 @@ constexpr int kWriteRows = 4;
 
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) quantize_write_kernel(const QuantCacheParams p, int parts) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kWriteRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
     const uint32_t mask = group_mask<LANES>();
@@ -365,6 +367,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) quantize_write_ke
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) quantize_write_any_kernel(const QuantCacheParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int lane = threadIdx.x & 31, D = p.head_size;
     const long long rows = p.num_tokens * 2 * p.num_kv_heads;
     for (long long r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8) {
@@ -410,6 +414,8 @@ __device__ __forceinline__ void widen16(T* out, uint4 u, float scale) {
 
 template <typename T, typename C, typename IX>
 __global__ void __launch_bounds__(256) dequantize_blocks_kernel(const DequantParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     const unsigned row_pieces = p.head_size / 16;
     const IX pieces = (IX)p.rows_per_block * row_pieces;  // of a block
     const IX total = pieces * (IX)p.num_ids;
@@ -438,6 +444,8 @@ __global__ void __launch_bounds__(256) dequantize_blocks_kernel(const DequantPar
 // Any row width and alignment, value by value.
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) dequantize_any_kernel(const DequantParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     const long long block_values = (long long)p.rows_per_block * p.head_size;
     const long long total = block_values * p.num_ids;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
@@ -499,6 +507,7 @@ __device__ __forceinline__ void turn_pair(float x, float y, float c, float s, fl
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kernel(const QuantCacheParams p, int parts) {
     grid_launch_dependents();
+    if (!p.overlap) grid_dependency_wait();
     constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
     const uint32_t mask = group_mask<LANES>();
@@ -755,26 +764,20 @@ int parts_of(long long tokens, int rows, int step) {
 }
 
 template <typename T, typename C, int LANES>
-void write_lanes(const QuantCacheParams& p, cudaStream_t st) {
+cudaError_t write_lanes(const QuantCacheParams& p, cudaStream_t st) {
     const int parts = parts_of(p.num_tokens, 2 * p.num_kv_heads, 32 / LANES * kWriteRows);
-    quantize_write_kernel<T, C, LANES>
-        <<<grid_of(p.num_tokens * parts, 8, 2), 256, 0, st>>>(p, parts);
+    return launch_early(quantize_write_kernel<T, C, LANES>, grid_of(p.num_tokens * parts, 8, 2), 256,
+                        0, st, p, parts);
 }
 template <typename T, typename C>
 cudaError_t write_tc(const QuantCacheParams& p, bool vec, cudaStream_t st) {
     const int units = vec ? p.head_size / 16 : 33;
-    if (units <= 4)
-        write_lanes<T, C, 4>(p, st);
-    else if (units <= 8)
-        write_lanes<T, C, 8>(p, st);
-    else if (units <= 16)
-        write_lanes<T, C, 16>(p, st);
-    else if (units <= 32)
-        write_lanes<T, C, 32>(p, st);
-    else
-        quantize_write_any_kernel<T, C>
-            <<<grid_of(p.num_tokens * 2 * p.num_kv_heads, 8), 256, 0, st>>>(p);
-    return cudaGetLastError();
+    if (units <= 4) return write_lanes<T, C, 4>(p, st);
+    if (units <= 8) return write_lanes<T, C, 8>(p, st);
+    if (units <= 16) return write_lanes<T, C, 16>(p, st);
+    if (units <= 32) return write_lanes<T, C, 32>(p, st);
+    return launch_early(quantize_write_any_kernel<T, C>,
+                        grid_of(p.num_tokens * 2 * p.num_kv_heads, 8), 256, 0, st, p);
 }
 template <typename T>
 cudaError_t write_t(int cache_dtype, const QuantCacheParams& p, bool vec, cudaStream_t st) {
@@ -786,13 +789,12 @@ cudaError_t dequant_tc(const DequantParams& p, bool vec, cudaStream_t st) {
     const long long values = p.num_ids * p.rows_per_block * p.head_size;
     // 32-bit piece numbers, with room for a step past the end
     if (vec && values / 16 < (1ll << 31))
-        dequantize_blocks_kernel<T, C, unsigned><<<grid_of(values / 16, 256), 256, 0, st>>>(p);
-    else if (vec)
-        dequantize_blocks_kernel<T, C, unsigned long long>
-            <<<grid_of(values / 16, 256), 256, 0, st>>>(p);
-    else
-        dequantize_any_kernel<T, C><<<grid_of(values, 256), 256, 0, st>>>(p);
-    return cudaGetLastError();
+        return launch_early(dequantize_blocks_kernel<T, C, unsigned>, grid_of(values / 16, 256), 256,
+                            0, st, p);
+    if (vec)
+        return launch_early(dequantize_blocks_kernel<T, C, unsigned long long>,
+                            grid_of(values / 16, 256), 256, 0, st, p);
+    return launch_early(dequantize_any_kernel<T, C>, grid_of(values, 256), 256, 0, st, p);
 }
 template <typename T>
 cudaError_t dequant_t(int cache_dtype, const DequantParams& p, bool vec, cudaStream_t st) {
@@ -801,31 +803,20 @@ cudaError_t dequant_t(int cache_dtype, const DequantParams& p, bool vec, cudaStr
 }
 
 template <typename T, typename C, int LANES>
-cudaError_t norm_lanes(const QuantCacheParams& p, cudaLaunchConfig_t& cfg) {
-    const int rows = p.num_heads + p.num_kv_heads * (p.key_cache != nullptr ? 2 : 1);
+cudaError_t norm_lanes(const QuantCacheParams& p, int rows, cudaStream_t st) {
     const int parts = parts_of(p.num_tokens, rows, 32 / LANES * kRows);
-    cfg.gridDim = dim3(grid_of(p.num_tokens * parts, 8, 2));
-    return cudaLaunchKernelEx(&cfg, qk_norm_rope_kernel<T, C, LANES>, p, parts);
+    return launch_early(qk_norm_rope_kernel<T, C, LANES>, grid_of(p.num_tokens * parts, 8, 2), 256, 0,
+                        st, p, parts);
 }
 template <typename T, typename C>
 cudaError_t norm_tc(const QuantCacheParams& p, bool vec, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.overlap ? 1 : 0;
+    const int rows = p.num_heads + p.num_kv_heads * (p.key_cache != nullptr ? 2 : 1);
     const int units = vec ? p.head_size / 16 : 33;
-    if (units <= 4) return norm_lanes<T, C, 4>(p, cfg);
-    if (units <= 8) return norm_lanes<T, C, 8>(p, cfg);
-    if (units <= 16) return norm_lanes<T, C, 16>(p, cfg);
-    if (units <= 32) return norm_lanes<T, C, 32>(p, cfg);
-    const long long rows =
-        p.num_tokens * (p.num_heads + p.num_kv_heads * (p.key_cache != nullptr ? 2 : 1));
-    cfg.gridDim = dim3(grid_of(rows, 8));
-    return cudaLaunchKernelEx(&cfg, qk_norm_rope_any_kernel<T, C>, p);
+    if (units <= 4) return norm_lanes<T, C, 4>(p, rows, st);
+    if (units <= 8) return norm_lanes<T, C, 8>(p, rows, st);
+    if (units <= 16) return norm_lanes<T, C, 16>(p, rows, st);
+    if (units <= 32) return norm_lanes<T, C, 32>(p, rows, st);
+    return launch_early(qk_norm_rope_any_kernel<T, C>, grid_of(p.num_tokens * rows, 8), 256, 0, st, p);
 }
 template <typename T>
 cudaError_t norm_t(int cache_dtype, const QuantCacheParams& p, bool vec, cudaStream_t st) {

@@ -106,11 +106,8 @@ template <typename QT, typename CT>
 cudaError_t generic_tc(const Params& p, cudaStream_t st) {
     const dim3 grid(p.num_seqs, p.num_heads);
     const size_t smem = (size_t)kWarps * p.head_dim * sizeof(float);
-    if (p.head_dim <= 128)
-        generic_kernel<QT, CT, 4><<<grid, kThreads, smem, st>>>(p);
-    else
-        generic_kernel<QT, CT, 32><<<grid, kThreads, smem, st>>>(p);
-    return cudaGetLastError();
+    return p.head_dim <= 128 ? launch_early(generic_kernel<QT, CT, 4>, grid, kThreads, smem, st, p)
+                             : launch_early(generic_kernel<QT, CT, 32>, grid, kThreads, smem, st, p);
 }
 template <typename QT>
 cudaError_t generic_t(int cache_dtype, const Params& p, cudaStream_t st) {

@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     const uint32_t ring = smem_u32(smem) + warp * F::kRingBytes;
 
     grid_launch_dependents();
+    if (!p.overlap) grid_dependency_wait();
     // ---- cost line: thread i holds the sequences [i * per, (i + 1) * per)
     auto cost_of = [&](int s) {
         const Span sp = span_of(s, p);
@@ -1076,7 +1077,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
 
 template <typename QT, typename CT, int D, int NT>
 cudaError_t launch_fast(const Params& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
-                        int ctas, bool overlap, cudaStream_t st) {
+                        int ctas, cudaStream_t st) {
     using F = Cfg<QT, CT, D, NT>;
     auto kern = scored_attention_kernel<QT, CT, D, NT>;
     // the attribute is the kernel's on one device: set once for each
@@ -1090,27 +1091,17 @@ cudaError_t launch_fast(const Params& p, const CUtensorMap& map_k, const CUtenso
         if (e != cudaSuccess) return e;
         set.fetch_or(bit, std::memory_order_relaxed);
     }
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(F::kThreads);
-    cfg.dynamicSmemBytes = F::kSmem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = overlap ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, map_k, map_v, p);
+    return launch_early(kern, ctas, F::kThreads, F::kSmem, st, map_k, map_v, p);
 }
 
 template <typename QT, typename CT>
 cudaError_t launch_fast_shape(const Params& p, const CUtensorMap& map_k, const CUtensorMap& map_v,
-                              int ctas, bool overlap, cudaStream_t st) {
+                              int ctas, cudaStream_t st) {
     if (p.head_dim == 128)
-        return p.unit_heads <= 8 ? launch_fast<QT, CT, 128, 1>(p, map_k, map_v, ctas, overlap, st)
-                                 : launch_fast<QT, CT, 128, 2>(p, map_k, map_v, ctas, overlap, st);
-    return p.unit_heads <= 8 ? launch_fast<QT, CT, 64, 1>(p, map_k, map_v, ctas, overlap, st)
-                             : launch_fast<QT, CT, 64, 2>(p, map_k, map_v, ctas, overlap, st);
+        return p.unit_heads <= 8 ? launch_fast<QT, CT, 128, 1>(p, map_k, map_v, ctas, st)
+                                 : launch_fast<QT, CT, 128, 2>(p, map_k, map_v, ctas, st);
+    return p.unit_heads <= 8 ? launch_fast<QT, CT, 64, 1>(p, map_k, map_v, ctas, st)
+                             : launch_fast<QT, CT, 64, 2>(p, map_k, map_v, ctas, st);
 }
 
 }  // namespace scored
