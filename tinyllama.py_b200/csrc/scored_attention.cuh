@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     int* wsum = pre + THREADS;                                     // [W] cost of a warp's threads
     __shared__ int parts_used;
     __shared__ bool last_cta[2];
+    __shared__ int4 shared_unit[2];
     const uint32_t bars = smem_u32(smem + F::kBarOff) + warp * ST * 8;
     const uint32_t ring = smem_u32(smem) + warp * F::kRingBytes;
 
@@ -913,9 +914,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     // the last of its range (odd e).
     const int4 mine = lane < 2 * W ? ids[lane] : make_int4(-1, 0, 0, 0);
     const uint32_t run = __match_any_sync(0xffffffffu, mine.x);  // entries of the same unit
-    uint32_t there = __ballot_sync(0xffffffffu, mine.x >= 0);
-    // units that other CTAs share: [0] begins before this CTA, [1] ends after it
-    int shared_row[2] = {-1, -1}, owner[2] = {0, 0}, shares[2] = {0, 0}, shared_heads[2] = {0, 0};
+    const uint32_t there = __ballot_sync(0xffffffffu, mine.x >= 0);
     if (there) {
         // weights of the entries, a warp for each head
         if (mine.x >= 0)
@@ -926,97 +925,101 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                 wl[lane * G + h] = make_float2(w, w * v.y);
                 ml[lane * G + h].x = M;
             }
+        if (warp >= W - 2) {
+            // units that other CTAs share, one for each of these warps: [0] begins
+            // before this CTA, [1] ends after it. (output row or -1, heads, CTA of
+            // the unit's first tile, CTAs that hold a part)
+            const int side = warp - (W - 2);
+            const int e1 = side ? 31 - __clz(there) : __ffs(there) - 1;
+            const uint32_t k = __shfl_sync(0xffffffffu, run, e1);
+            const int e0 = __ffs(k) - 1;
+            const int begin = __shfl_sync(0xffffffffu, mine.y, e0);
+            const int end = __shfl_sync(0xffffffffu, mine.y, 31 - __clz(k));
+            int4 unit = make_int4(-1, (begin & kHeadsMask) >> kHeadsShift, 0, 0);
+            if (side ? (begin & kUnitBegin) && !(end & kUnitEnd) : !(begin & kUnitBegin)) {
+                const int2 pt = points[e0];
+                unit.x = __shfl_sync(0xffffffffu, mine.x, e0);
+                unit.z = first_cta(pt.x);
+                unit.w = final_cta(pt.x + pt.y - 1) - unit.z + 1;
+            }
+            if (lane == 0) shared_unit[side] = unit;
+        }
         __syncthreads();
         // byte offset of the entry's partial in shared memory, -1: workspace
         const int from = (lane & 1) ? (lane >> 1) * F::kRingBytes
                          : mine.z < F::kParts ? F::kPartOff + mine.z * F::kPartBytes : -1;
+        // a warp for each 32 fragments of each unit
+        constexpr int FG = F::kFrags / 32;
 #pragma unroll 1
-        while (there) {
-            const int e0 = __ffs(there) - 1;
-            uint32_t k = __shfl_sync(0xffffffffu, run, e0);
-            const int u = __shfl_sync(0xffffffffu, mine.x, e0);
+        for (int task = warp;; task += W) {
+            int e0 = 0;
+            uint32_t rest = there, entries = 0;
+            for (int i = task / FG;; --i) {
+                if (!rest) break;
+                e0 = __ffs(rest) - 1;
+                entries = __shfl_sync(0xffffffffu, run, e0);
+                if (i == 0) break;
+                rest &= ~entries;
+            }
+            if (!rest) break;
             // the first entry says whether the unit begins here, the last
             // whether it ends
             const int flags = __shfl_sync(0xffffffffu, mine.y, e0) |
-                              __shfl_sync(0xffffffffu, mine.y, 31 - __clz(k));
-            const int n_heads = (flags & kHeadsMask) >> kHeadsShift;
-            there &= ~k;
-            const uint32_t entries = k;
-            const bool whole = (flags & ~kHeadsMask) == (kUnitBegin | kUnitEnd);
-            const int side = (flags & kUnitBegin) ? 1 : 0, at = 2 * blockIdx.x + side;
-            if (!whole) {
-                // the CTAs of the unit's first and last tile
-                const int2 pt = points[e0];
-                const int first = first_cta(pt.x), n = final_cta(pt.x + pt.y - 1) - first + 1;
-#pragma unroll
-                for (int sd = 0; sd < 2; ++sd)
-                    if (sd == side) {
-                        shared_row[sd] = u;
-                        shared_heads[sd] = n_heads;
-                        owner[sd] = first;
-                        shares[sd] = n;
-                    }
+                              __shfl_sync(0xffffffffu, mine.y, 31 - __clz(entries));
+            const int u = __shfl_sync(0xffffffffu, mine.x, e0);
+            const int f = task % FG * 32 + lane, nt = f / (F::kTiles * 32);
+            const int i = (f >> 5) % F::kTiles, h0 = nt * 8 + 2 * (lane & 3);
+            float L0 = 0.f, L1 = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), v, w;
+            auto fetch = [&](int e) {
+                const int off = __shfl_sync(0xffffffffu, from, e);
+                v = off >= 0 ? *reinterpret_cast<const float4*>(smem + off + 16 * f)
+                             : p.warp_partials[((long long)blockIdx.x * W + (e >> 1)) * F::kFrags + f];
+                w = *reinterpret_cast<const float4*>(wl + e * G + h0);
+            };
+            fetch(e0);
+#pragma unroll 1
+            for (uint32_t k = entries & (entries - 1);; k &= k - 1) {
+                const float4 v0 = v, w0 = w;
+                if (k) fetch(__ffs(k) - 1);
+                acc.x = fmaf(w0.x, v0.x, acc.x);
+                acc.y = fmaf(w0.z, v0.y, acc.y);
+                acc.z = fmaf(w0.x, v0.z, acc.z);
+                acc.w = fmaf(w0.z, v0.w, acc.w);
+                L0 += w0.y;
+                L1 += w0.w;
+                if (!k) break;
             }
-#pragma unroll 1
-            for (int f0 = warp * 32; f0 < F::kFrags; f0 += THREADS) {
-                const int f = f0 + lane, nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles;
-                const int h0 = nt * 8 + 2 * (lane & 3);
-                float L0 = 0.f, L1 = 0.f;
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), v, w;
-                auto fetch = [&](int e) {
-                    const int off = __shfl_sync(0xffffffffu, from, e);
-                    v = off >= 0 ? *reinterpret_cast<const float4*>(smem + off + 16 * f)
-                                 : p.warp_partials[((long long)blockIdx.x * W + (e >> 1)) *
-                                                       F::kFrags + f];
-                    w = *reinterpret_cast<const float4*>(wl + e * G + h0);
-                };
-                fetch(e0);
-#pragma unroll 1
-                for (k = entries & (entries - 1);; k &= k - 1) {
-                    const float4 v0 = v, w0 = w;
-                    if (k) fetch(__ffs(k) - 1);
-                    acc.x = fmaf(w0.x, v0.x, acc.x);
-                    acc.y = fmaf(w0.z, v0.y, acc.y);
-                    acc.z = fmaf(w0.x, v0.z, acc.z);
-                    acc.w = fmaf(w0.z, v0.w, acc.w);
-                    L0 += w0.y;
-                    L1 += w0.w;
-                    if (!k) break;
-                }
-                if (whole) {
-                    write_frag<QT, F::kQ8, D>(p.out, u, n_heads, nt, i, lane, acc, inverse(L0),
-                                              inverse(L1));
-                } else {
-                    p.cta_partials[(long long)at * F::kFrags + f] = acc;
-                    if (i == 0 && lane < 4)
-                        *reinterpret_cast<float4*>(p.cta_ml + at * G + h0) =
-                            make_float4(ml[e0 * G + h0].x, L0, ml[e0 * G + h0 + 1].x, L1);
-                }
+            if ((flags & ~kHeadsMask) == (kUnitBegin | kUnitEnd)) {
+                write_frag<QT, F::kQ8, D>(p.out, u, (flags & kHeadsMask) >> kHeadsShift, nt, i, lane,
+                                          acc, inverse(L0), inverse(L1));
+            } else {
+                const int at = 2 * blockIdx.x + ((flags & kUnitBegin) ? 1 : 0);
+                p.cta_partials[(long long)at * F::kFrags + f] = acc;
+                if (i == 0 && lane < 4)
+                    *reinterpret_cast<float4*>(p.cta_ml + at * G + h0) =
+                        make_float4(ml[e0 * G + h0].x, L0, ml[e0 * G + h0 + 1].x, L1);
             }
         }
     }
     // ---- join units across CTAs: the last CTA to publish its partial of a unit
     // sums all of them, in range order whichever CTA it is. The counters are
     // zero between calls.
-    if (shared_row[0] >= 0 || shared_row[1] >= 0) {
+    if (there && (shared_unit[0].x >= 0 || shared_unit[1].x >= 0)) {
         __syncthreads();
         if (lane == 0 && warp < 2) {
-            const int c0 = warp ? owner[1] : owner[0], n = warp ? shares[1] : shares[0];
-            bool last = false;
-            if ((warp ? shared_row[1] : shared_row[0]) >= 0) {
-                // releases what the barrier has made this thread see: all the
-                // CTA's stores of its partial
-                last = atomic_inc_acq_rel(p.counters + c0, n - 1) == (unsigned)n - 1;
-            }
-            last_cta[warp] = last;
+            const int4 unit = shared_unit[warp];
+            // releases what the barrier has made this thread see: all the CTA's
+            // stores of its partial
+            last_cta[warp] = unit.x >= 0 && atomic_inc_acq_rel(p.counters + unit.z, unit.w - 1) ==
+                                                (unsigned)unit.w - 1;
         }
         __syncthreads();
 #pragma unroll 1
         for (int sd = 0; sd < 2; ++sd) {
             if (!last_cta[sd]) continue;
-            const int c0 = sd ? owner[1] : owner[0], n = sd ? shares[1] : shares[0];
-            const int u = sd ? shared_row[1] : shared_row[0];
-            const int n_heads = sd ? shared_heads[1] : shared_heads[0];
+            const int4 unit = shared_unit[sd];
+            const int c0 = unit.z, n = unit.w;
 #pragma unroll 1
             for (int f = tid; f < F::kFrags; f += THREADS) {
                 const int nt = f / (F::kTiles * 32), i = (f >> 5) % F::kTiles;
@@ -1061,7 +1064,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                         y = j == 0 ? w1 : j == 1 ? w2 : w;
                     }
                 }
-                write_frag<QT, F::kQ8, D>(p.out, u, n_heads, nt, i, lane, acc, inverse(L0),
+                write_frag<QT, F::kQ8, D>(p.out, unit.x, unit.y, nt, i, lane, acc, inverse(L0),
                                           inverse(L1));
             }
         }
