@@ -114,6 +114,14 @@ def test_score_modifiers(mods, dtype, kind):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("kind", [E4M3, F16], ids=short)
+@pytest.mark.parametrize("cap", [1e-30, 1e-3, 1e4, 1e30])
+def test_caps_far_from_the_scores(cap, kind):
+    """A tiny cap makes all scores alike, a huge one leaves them as they are."""
+    c = Case([300, 40], 8, 2, 64, 16, F16, kind, seed=18)
+    c.check(c.run(softcap=cap), softcap=cap)
+
+
 @pytest.mark.parametrize("dtype,kind", [(BF16, E4M3), (F16, INT8), (BF16, BF16), (F32, INT8)],
                          ids=short)
 @pytest.mark.parametrize("h,kvh,d,bs", [(6, 2, 80, 16), (4, 1, 96, 16), (2, 2, 37, 8),

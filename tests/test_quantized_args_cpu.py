@@ -109,6 +109,7 @@ def test_attention_refuses_before_any_cuda_call(built_lib):
                     (dict(heads=15), "divisible"), (dict(d=2048), "1024"),
                     (dict(nb=0), "positive"), (dict(window=-1), "window"),
                     (dict(cap=-1.0), "softcap"), (dict(cap=float("inf")), "softcap"),
+                    (dict(cap=1e-31), "softcap"), (dict(cap=2e30), "softcap"),
                     (dict(cap=float("nan")), "softcap"), (dict(q=0), "must not be null"),
                     (dict(scales=0), "8-bit caches need"), (dict(q=P + 1), "aligned"),
                     (dict(maxb=1 << 30, bs=16), "supported range")):

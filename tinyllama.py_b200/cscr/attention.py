@@ -317,8 +317,9 @@ def _scored_workspace_bytes(*key) -> tuple[int, int]:
 def _scored_workspace(query: torch.Tensor, index: int, nbytes: int, zeroed: int) -> torch.Tensor:
     """Scratch of a call: the stream's own, or while the stream is captured one
     of the graph's (zeroed in the graph), so that graphs replayed together share
-    none."""
-    if _capturing():
+    none. (Whether another device's stream is captured is not asked: a call on it
+    from this one gets a new one too.)"""
+    if _capturing() or _lib.current_device() != index:
         ws = query.new_empty(nbytes, dtype=torch.uint8)
         ws[:zeroed].zero_()
         return ws
@@ -360,7 +361,8 @@ def _check_scored(query, key_cache, value_cache, block_tables, seq_lens, softcap
     torch_check(query.dtype in _FLOAT_TYPES, "dtype must be float16, bfloat16 or float32")
     torch_check(value_cache.dtype == key_cache.dtype,
                 "key_cache and value_cache must share the same dtype")
-    torch_check(0 <= softcap < float("inf"), "softcap must be finite and not negative")
+    torch_check(softcap == 0 or 1e-30 <= softcap <= 1e30,
+                "softcap must be 0 or between 1e-30 and 1e30")
     torch_check(window >= 0, "window must not be negative")
     torch_check(alibi_slopes is None
                 or (alibi_slopes.device == dev and alibi_slopes.dtype == torch.float32
@@ -389,7 +391,8 @@ def _paged_attention_scored(query, key_cache, value_cache, key_scales, value_sca
             and value_cache.is_contiguous() and block_tables.is_contiguous()
             and seq_lens.is_contiguous() and key_cache.get_device() == index
             and value_cache.get_device() == index and block_tables.get_device() == index
-            and seq_lens.get_device() == index and 0 <= softcap < float("inf") and window >= 0
+            and seq_lens.get_device() == index and (softcap == 0 or 1e-30 <= softcap <= 1e30)
+            and window >= 0
             and (alibi_slopes is None
                  or (alibi_slopes.get_device() == index and alibi_slopes.dtype == torch.float32
                      and alibi_slopes.shape == shape[1:2] and alibi_slopes.is_contiguous()))):

@@ -392,7 +392,9 @@ int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stre
                     max_blocks_per_seq * block_size < (1ll << 31) - 64 && num_blocks < (1ll << 31),
                 "sizes exceed the supported range");
     TLB_REQUIRE(window >= 0, "window must not be negative");
-    TLB_REQUIRE(softcap >= 0.f && softcap <= 3.0e38f, "softcap must be finite and not negative");
+    // beyond these its reciprocal or its product with a score leaves fp32
+    TLB_REQUIRE(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f),
+                "softcap must be 0 or between 1e-30 and 1e30");
     TLB_REQUIRE(out && query && key_cache && value_cache && block_tables && seq_lens,
                 "tensor pointers must not be null");
     TLB_REQUIRE(!is_8bit(cache_dtype) || (key_scales && value_scales),
