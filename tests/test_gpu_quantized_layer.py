@@ -207,3 +207,47 @@ def test_pool_sizes():
         pool.allocate_quantized_kv_cache(1, 5, KVH, D, BS, torch.float16)
     with pytest.raises(ValueError, match="No KV cache blocks"):
         pool.allocate_quantized_kv_cache(1, 0, KVH, D, BS)
+
+
+def test_calls_without_the_fast_module_are_the_same(monkeypatch):
+    """Every op with its Python argument handling alone, and through cscr._fast."""
+    from cscr import attention as A
+
+    g = torch.Generator(device="cuda").manual_seed(6)
+    dtype = torch.bfloat16
+    m = layer(dtype)
+    q, k, v = tokens(g, 40, dtype)
+    pos = torch.arange(40, device="cuda")
+    tables = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    lens = torch.tensor([40, 23], dtype=torch.int32, device="cuda")
+    slots = torch.randperm(128, generator=g, device="cuda")[:40]
+    table = m._table(q.device, dtype)
+
+    def everything():
+        out = []
+        for kind in KINDS:
+            kv = caches(kind, dtype, 8)
+            for c in kv:
+                if c is not None:
+                    c.view(torch.uint8).fill_(0)
+            out.append(PE.qk_norm_rotary_embedding_neox_with_cache(
+                pos, q.view(40, -1), k.view(40, -1), v, m.q_norm, m.k_norm, 1e-6, kv[0], kv[1],
+                slots, D, table, key_scales=kv[2], value_scales=kv[3]))
+            if kind is not None:
+                C.reshape_and_cache_quantized(v, k, *kv, slots.flip(0))
+                out += C.dequantize_blocks(*kv, tables.view(-1), torch.float16)
+                out.append(A.paged_attention_quantized(q[:2], *kv, tables, lens, 0.1, window=9))
+            else:
+                out.append(A.paged_attention_biased(q[:2], kv[0], kv[1], tables, lens, 0.1,
+                                                    softcap=4.0))
+            out += [c.view(torch.uint8) for c in kv if c is not None]
+        out += PE.qk_norm_rotary_embedding_neox(pos, q.view(40, -1), k.view(40, -1), m.q_norm,
+                                                m.k_norm, 1e-6, D, table)
+        return out
+
+    assert _lib.fast is not None
+    everything()  # scratch of the stream
+    quick = everything()
+    monkeypatch.setattr(_lib, "fast", None)
+    for a, b in zip(quick, everything(), strict=True):
+        assert torch.equal(a, b)

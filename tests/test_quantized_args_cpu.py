@@ -164,3 +164,26 @@ def test_oracle_quantiser_on_unbounded_rows():
     assert q.float()[0, :3].tolist() == [0.25, 448.0, -448.0] and bool(q.float()[0, 3].isnan())
     q, s = Q.quantize(x, torch.int8)
     assert q[0].tolist() == [0, 127, -127, 0, -112] and s.view(torch.uint8).tolist() == [131]
+
+
+def test_fast_calls_leave_everything_unusual_to_the_ops(built_lib):
+    """cscr._fast answers None, and raises nothing, for what is not an ordinary
+    call on the current device: other objects, other counts, CPU tensors."""
+    fast = _lib.fast
+    assert fast is not None
+    _lib.load()
+    x, i = torch.zeros(2, 2, 64), torch.zeros(2, dtype=torch.int32)
+    c8 = torch.zeros(2, 2, 8, 64, dtype=torch.int8)
+    sc = torch.zeros(2, 2, 8, dtype=torch.float8_e8m0fnu)
+    for args in ((), (None,) * 12, ("a",) * 12, (x,) * 12,
+                 (x, c8, c8, sc, sc, i.view(2, 1), i, 0.1, 0.0, None, 0, False)):
+        assert fast.attention(*args) is None
+    for args in ((), (1,) * 7, (x, x, c8, c8, sc, sc, i)):
+        assert fast.write(*args) is None
+    for args in ((), ({},) * 6, (c8, c8, sc, sc, i, torch.float16), (c8, c8, sc, sc, i, "x")):
+        assert fast.read(*args) is None
+    w = torch.ones(64)
+    for args in ((), (None,) * 16,
+                 (i, x.view(2, -1), x.view(2, -1), None, w, w, 1e-6, None, None, None, 64,
+                  torch.zeros(4, 64), None, None, None, False)):
+        assert fast.norm(*args) is None

@@ -6,6 +6,9 @@ linked into one shared library next to the ``cscr`` package, where the op
 modules load it. The library lives in-tree, so a copy of the repository
 carries it as built.
 
+``csrc/fast_calls.cpp`` (host code on torch's C++ headers) becomes the module
+``cscr._fast`` beside it.
+
 Usage: ``python tinyllama.py_b200/build.py [--force] [--verbose]``.
 """
 
@@ -17,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -24,6 +28,8 @@ CSRC = PKG_ROOT / "csrc"
 INCLUDE = PKG_ROOT.parent / "include"
 BUILD_DIR = PKG_ROOT.parent / "_build"
 LIB_PATH = PKG_ROOT / "cscr" / "libtinyllama_b200.so"
+FAST_SRC = CSRC / "fast_calls.cpp"
+FAST_PATH = PKG_ROOT / "cscr" / f"_fast{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -56,10 +62,35 @@ def _deps() -> list[Path]:
 
 
 def up_to_date() -> bool:
-    if not LIB_PATH.exists():
+    if not LIB_PATH.exists() or not _fast_up_to_date():
         return False
     built = LIB_PATH.stat().st_mtime
     return all(p.stat().st_mtime <= built for p in _deps())
+
+
+def _fast_up_to_date() -> bool:
+    deps = [FAST_SRC, *INCLUDE.glob("*.h")]
+    return FAST_PATH.exists() and all(p.stat().st_mtime <= FAST_PATH.stat().st_mtime for p in deps)
+
+
+def _build_fast() -> None:
+    """Compile cscr._fast against the running interpreter and its torch."""
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(nvcc()).resolve().parent.parent
+    lib = Path(torch.__file__).resolve().parent / "lib"
+    tmp = FAST_PATH.with_suffix(".tmp")
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-isystem{p}" for p in cpp_extension.include_paths()),
+           f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{cuda / 'include'}",
+           f"-I{INCLUDE}", str(FAST_SRC), "-o", str(tmp), f"-L{lib}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compiling {FAST_SRC.name} failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, FAST_PATH)
 
 
 def _compile(src: Path, verbose: bool) -> Path:
@@ -81,9 +112,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB_PATH
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     srcs = sources()
-    workers = min(len(srcs), os.cpu_count() or 4)
+    workers = min(len(srcs) + 1, os.cpu_count() or 4)
     with cf.ThreadPoolExecutor(max_workers=workers) as ex:
+        fast = None if _fast_up_to_date() and not force else ex.submit(_build_fast)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        if fast is not None:
+            fast.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objs), "-cudart", "static"]
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -18,6 +18,10 @@ import torch
 LIB_NAME = "libtinyllama_b200.so"
 LIB_PATH = Path(__file__).resolve().with_name(LIB_NAME)
 
+# With TLB_DEBUG=1 every op synchronises and raises on a non-zero device
+# status word (bounds problems the kernels skipped instead of faulting).
+DEBUG = os.environ.get("TLB_DEBUG", "0") not in ("", "0")
+
 TLB_OK = 0
 TLB_ERR_UNSUPPORTED = 2
 DTYPE_CODE = {
@@ -101,6 +105,10 @@ def load():
                 fn.argtypes = args
                 fn.restype = _RESTYPES.get(name, ctypes.c_int)
             _lib = lib
+            if fast is not None:
+                fast.bind(*(ctypes.cast(getattr(lib, entry[0]), ctypes.c_void_p).value
+                            for entry in (SCORED_ATTENTION, QUANTIZED_WRITE, DEQUANTIZE,
+                                          QK_NORM_ROPE)))
     return _lib
 
 
@@ -140,6 +148,17 @@ QUANTIZED_WRITE = ("tlb_reshape_and_cache_quantized", struct.Struct("=17q").pack
 DEQUANTIZE = ("tlb_dequantize_blocks", struct.Struct("=15q").pack)
 QK_NORM_ROPE = ("tlb_qk_norm_rotary_embedding_neox", struct.Struct("=32qd").pack)
 SCORED_ATTENTION = ("tlb_paged_attention_scored", struct.Struct("=23q2d").pack)
+
+
+# The ordinary calls without their Python argument handling (csrc/fast_calls.cpp):
+# its functions answer None for what the Python code has to look at. Not used in
+# debug mode; unbound, and so answering None, until the library is loaded.
+try:
+    if DEBUG:
+        raise ImportError
+    from . import _fast as fast
+except ImportError:
+    fast = None
 
 
 def launch(entry, index: int, *args) -> None:
@@ -194,11 +213,6 @@ def set_wait_limit(tries: int) -> None:
 
 
 WAIT_LIMIT_DEFAULT = 1 << 22
-
-# With TLB_DEBUG=1 every op synchronises and raises on a non-zero device
-# status word (bounds problems the kernels skipped instead of faulting).
-DEBUG = os.environ.get("TLB_DEBUG", "0") not in ("", "0")
-
 
 def device_status(clear: bool = True, raise_on_error: bool = False) -> int:
     """Read (and clear) the current device's status word; see STATUS_BITS."""

@@ -55,6 +55,8 @@ def invalidate_workspaces(device_index: int) -> None:
             ws.clean = 0
     for key in [k for k in _scored_workspaces if k[0] == device_index]:
         del _scored_workspaces[key]
+    if _lib.fast is not None:
+        _lib.fast.scratch(device_index, 0, 0, 0)
 
 
 def workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -326,7 +328,9 @@ def _scored_workspace(query: torch.Tensor, index: int, nbytes: int, zeroed: int)
     key = (index, _lib.stream_of(query.device))
     ws = _scored_workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _scored_workspaces[key] = query.new_zeros(max(nbytes, 1 << 23), dtype=torch.uint8)
+        ws = _scored_workspaces[key] = query.new_zeros(max(nbytes, 1 << 24), dtype=torch.uint8)
+        if _lib.fast is not None:
+            _lib.fast.scratch(*key, ws.data_ptr(), ws.numel())
     return ws
 
 
@@ -435,6 +439,12 @@ def paged_attention_quantized(query: torch.Tensor, key_cache: torch.Tensor,
     ``softcap``, ``alibi_slopes`` and ``window`` as in ``paged_attention_biased``,
     ``overlap_prologue`` as in ``paged_attention``.
     """
+    if _lib.fast is not None:
+        out = _lib.fast.attention(query, key_cache, value_cache, key_scales, value_scales,
+                                  block_tables, seq_lens, scale, softcap, alibi_slopes, window,
+                                  overlap_prologue)
+        if out is not None:
+            return out
     torch_check(key_cache.dtype in _CACHE8_TYPES,
                 "key_cache must be float8_e4m3fn or int8")
     rows, index = key_cache.shape[:3], query.get_device()
@@ -465,6 +475,11 @@ def paged_attention_biased(query: torch.Tensor, key_cache: torch.Tensor,
     ``window > 0`` (their blocks alone are read). A sequence with no token
     to see yields zeros.
     """
+    if _lib.fast is not None:
+        out = _lib.fast.attention(query, key_cache, value_cache, None, None, block_tables,
+                                  seq_lens, scale, softcap, alibi_slopes, window, overlap_prologue)
+        if out is not None:
+            return out
     torch_check(key_cache.dtype == query.dtype,
                 "query, key_cache and value_cache must share the same dtype")
     return _paged_attention_scored(query, key_cache, value_cache, None, None, block_tables,

@@ -272,6 +272,9 @@ def reshape_and_cache_quantized(key: torch.Tensor, value: torch.Tensor, key_cach
     slot = block * block_size + offset; negative slots are skipped. The other
     slots of a call must differ.
     """
+    if _lib.fast is not None and _lib.fast.write(key, value, key_cache, value_cache, key_scales,
+                                                 value_scales, slot_mapping):
+        return
     index = check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
     torch_check(key.get_device() == index and value.get_device() == index
                 and slot_mapping.get_device() == index,
@@ -309,6 +312,10 @@ def dequantize_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor,
     ``s * max_blocks + j``, which ``paged_prefill_attention`` and
     ``paged_attention`` read. ``out``: two tensors to fill instead of new ones.
     """
+    if out is None and _lib.fast is not None:
+        both = _lib.fast.read(key_cache, value_cache, key_scales, value_scales, block_ids, dtype)
+        if both is not None:
+            return both
     index = check_quantized_caches(key_cache, value_cache, key_scales, value_scales)
     torch_check(block_ids.get_device() == index, "all tensors must be on the same CUDA device")
     torch_check(block_ids.dim() == 1 and block_ids.dtype in _INDEX_TYPES

@@ -219,6 +219,11 @@ def qk_norm_rotary_embedding_neox(positions: torch.Tensor, query: torch.Tensor, 
     head_size], rows possibly strided (parts of a fused projection); weights
     [head_size]. Returns new dense (query, key); the inputs are left as they are.
     """
+    if _lib.fast is not None:
+        both = _lib.fast.norm(positions, query, key, None, query_weight, key_weight, eps, None,
+                              None, None, head_size, cos_sin_cache, None, None, None, False)
+        if both is not None:
+            return both
     index, num_tokens, q_stride, k_stride, q_width, k_width, rows, rot_dim = _qk_norm_shapes(
         positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache)
     q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
@@ -254,6 +259,12 @@ def qk_norm_rotary_embedding_neox_with_cache(
     the query dtype. Destinations and ``overlap_previous`` as in
     ``rotary_embedding_neox_with_cache``; the slots of one call must differ.
     """
+    if _lib.fast is not None:
+        out = _lib.fast.norm(positions, query, key, value, query_weight, key_weight, eps,
+                             key_cache, value_cache, slot_mapping, head_size, cos_sin_cache,
+                             block_tables, key_scales, value_scales, overlap_previous)
+        if out is not None:
+            return out
     index, num_tokens, q_stride, k_stride, q_width, k_width, rows, rot_dim = _qk_norm_shapes(
         positions, query, key, query_weight, key_weight, eps, head_size, cos_sin_cache)
     dtype, cache_dtype, cshape = query.dtype, key_cache.dtype, key_cache.shape
