@@ -125,9 +125,10 @@ bool fast_supported(int dtype, int cache_dtype, int head_dim, int block_size) {
 }
 
 // Units of 16 heads read a kv head's rows once for all of them, units of 8 run
-// more warps with less to hold: 64 bf16 queries' groups of 16 over e4m3 rows of
-// 128 take 30.8 us as one unit and 30.9 us as two (fp16 over int8: 32.9 and 35.3),
-// groups of 24 take 43.0 us as 16 + 8 and 39.0 us as 8 + 8 + 8.
+// more warps with less to hold. 128 sequences of 500-3000 tokens, one kv head of
+// 128, bf16 over e4m3: groups of 16 take 30.8 us as one unit and 30.9 us as two
+// (fp16 over int8: 32.9 and 35.3), groups of 24 take 43.0 us as 16 + 8 and 39.0 us
+// as 8 + 8 + 8.
 int unit_heads_of(int group) {
     const int rest = group % 16;
     return group <= 8 ? group : rest > 0 && rest <= 8 ? 8 : group < 16 ? group : 16;
