@@ -472,7 +472,9 @@ TLB_API int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream)
  *     tlb_reshape_and_cache_quantized stores for the rounded key.
  * Positions outside the table leave the normed row unrotated and set
  * TLB_STATUS_BAD_POSITION. flags: TLB_ROPE_OVERLAP_PREVIOUS as above (the
- * norm weights too must not be written by the kernel before).
+ * norm weights too must not be written by the kernel before; if that is a
+ * tlb_paged_attention or tlb_paged_attention_with_rope launch that itself
+ * overlaps, nor by the one before it, which may still be running).
  * ---------------------------------------------------------------------- */
 typedef struct tlb_qk_norm_rope_args {
     void* query_out;
@@ -521,7 +523,9 @@ TLB_API int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args,
  * starts and are zero again when it ends, the rest may hold anything: calls on
  * one stream can share a buffer, calls that overlap in time need separate
  * ones. The zeroed size depends on the device alone. After TLB_STATUS_WAIT_TIMEOUT
- * the caller zeroes it again. flags: TLB_ATTN_OVERLAP_PROLOGUE as above.
+ * the caller zeroes it again. flags: TLB_ATTN_OVERLAP_PROLOGUE as above (after
+ * a launch of tlb_paged_attention(_with_rope) that itself overlaps, the kernel before
+ * that one must not write block_tables or seq_lens either).
  * ---------------------------------------------------------------------- */
 TLB_API int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t num_kv_heads,
                         int64_t head_dim, int64_t block_size, int dtype,

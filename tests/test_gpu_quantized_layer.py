@@ -145,6 +145,46 @@ def test_prompt_chunks_then_decode(kind):
         layer(dtype, softcap=5.0).prompt(pos, q, k, v, kv[0], kv[1], slots, tables, start, ctx)
 
 
+@pytest.mark.parametrize("kind", [k for k in KINDS if k is not None], ids=short)
+def test_lengths_and_tables_written_just_before_a_step(kind):
+    """The attention of a step reads lengths and tables while the norm kernel before
+    it runs; kernels that write them ahead of that one are complete by then. Steps
+    queued without a pause, each after in-place changes of both, equal those with a
+    synchronisation after every launch."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    m = layer(torch.bfloat16)
+    n, width, blocks = 5, 12, 64
+    kv = caches(kind, torch.bfloat16, blocks)
+    _, k0, v0 = tokens(g, blocks * BS, torch.bfloat16)
+    C.reshape_and_cache_quantized(k0, v0, *kv, torch.arange(blocks * BS, device="cuda"))
+    plans = [(torch.randint(1, width * BS, (n,), generator=g, device="cuda").to(torch.int32),
+              torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)[:n * width]
+              .view(n, width), tokens(g, n, torch.bfloat16)) for _ in range(40)]
+    torch.cuda.synchronize()
+
+    def steps(pause):
+        cache = [c.clone() for c in kv]
+        lens = torch.ones(n, dtype=torch.int32, device="cuda")
+        tables = torch.zeros(n, width, dtype=torch.int32, device="cuda")
+        pos = torch.zeros(n, dtype=torch.int64, device="cuda")
+        outs = []
+        for new_lens, new_tables, (q, k, v) in plans:
+            pos.copy_(new_lens - 1)
+            tables.copy_(new_tables)
+            lens.copy_(new_lens)
+            if pause:
+                torch.cuda.synchronize()
+            outs.append(m(pos, q, k, v, cache[0], cache[1], tables, lens, cache[2], cache[3]))
+            if pause:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+
+    for a, b in zip(steps(False), steps(True)):
+        assert torch.equal(a, b)
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("kind", KINDS, ids=short)
 def test_a_captured_step_replays(kind):
     """A decode step in a graph, replayed over growing contexts, equals the eager

@@ -26,6 +26,9 @@ template <typename T> struct Same {
 // (programmatic stream serialization). Their kernels wait for it
 // (grid_dependency_wait) before they touch memory, or before they touch what
 // an `overlap` flag does not except; what is saved is the launch itself.
+// They let the next launch begin (grid_launch_dependents) only after that wait:
+// what an `overlap` flag of the next kernel excepts may have been written by
+// the kernel before this one, which is then complete.
 template <typename... Args>
 cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t smem,
                          cudaStream_t stream, typename Same<Args>::type... args) {

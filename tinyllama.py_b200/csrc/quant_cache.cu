@@ -292,8 +292,8 @@ constexpr int kWriteRows = 4;
 
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) quantize_write_kernel(const QuantCacheParams p, int parts) {
-    grid_launch_dependents();
     grid_dependency_wait();
+    grid_launch_dependents();
     constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kWriteRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
     const uint32_t mask = group_mask<LANES>();
@@ -367,8 +367,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) quantize_write_ke
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) quantize_write_any_kernel(const QuantCacheParams p) {
-    grid_launch_dependents();
     grid_dependency_wait();
+    grid_launch_dependents();
     const int lane = threadIdx.x & 31, D = p.head_size;
     const long long rows = p.num_tokens * 2 * p.num_kv_heads;
     for (long long r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8) {
@@ -414,8 +414,8 @@ __device__ __forceinline__ void widen16(T* out, uint4 u, float scale) {
 
 template <typename T, typename C, typename IX>
 __global__ void __launch_bounds__(256) dequantize_blocks_kernel(const DequantParams p) {
-    grid_launch_dependents();
     grid_dependency_wait();
+    grid_launch_dependents();
     const unsigned row_pieces = p.head_size / 16;
     const IX pieces = (IX)p.rows_per_block * row_pieces;  // of a block
     const IX total = pieces * (IX)p.num_ids;
@@ -444,8 +444,8 @@ __global__ void __launch_bounds__(256) dequantize_blocks_kernel(const DequantPar
 // Any row width and alignment, value by value.
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) dequantize_any_kernel(const DequantParams p) {
-    grid_launch_dependents();
     grid_dependency_wait();
+    grid_launch_dependents();
     const long long block_values = (long long)p.rows_per_block * p.head_size;
     const long long total = block_values * p.num_ids;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
@@ -511,7 +511,6 @@ __device__ __forceinline__ void turn_pair(float x, float y, float c, float s, fl
 
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kernel(const QuantCacheParams p, int parts) {
-    grid_launch_dependents();
     if (!p.overlap) grid_dependency_wait();
     constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
@@ -657,6 +656,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kern
         }
     };
     grid_dependency_wait();
+    grid_launch_dependents();
     Place c = place_of(blockIdx.x * 8 + threadIdx.x / 32, items, parts, STEP, p);
     load(c, a0, a1);
     while (c.valid) {
@@ -677,8 +677,8 @@ __device__ __forceinline__ float rounded(float x) {
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(const QuantCacheParams p) {
-    grid_launch_dependents();
     grid_dependency_wait();
+    grid_launch_dependents();
     const int lane = threadIdx.x & 31, D = p.head_size, rot = p.rot_dim, half = rot / 2;
     const bool with_cache = p.key_cache != nullptr;
     const int rows = p.num_heads + p.num_kv_heads * (with_cache ? 2 : 1);

@@ -16,13 +16,13 @@ constexpr int kWarps = 8, kThreads = 256;
 // kernel (scored_attention.cuh).
 template <typename QT, typename CT, int NPL>
 __global__ void __launch_bounds__(kThreads) generic_kernel(const Params p) {
-    grid_launch_dependents();
     extern __shared__ float gsm[];
     __shared__ float m_s[kWarps], l_s[kWarps];
     const int D = p.head_dim, s = blockIdx.x, h = blockIdx.y;
     const int kvh = h / p.group;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_dependency_wait();
+    grid_launch_dependents();
     const Span sp = span_of(s, p);
     if (p.seq_lens[s] > p.max_tokens && tid == 0) flag_status(TLB_STATUS_SEQ_TOO_LONG);
     const QT* query = reinterpret_cast<const QT*>(p.query) + (long long)s * p.query_stride +

@@ -273,7 +273,6 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
     const uint32_t bars = smem_u32(smem + F::kBarOff) + warp * ST * 8;
     const uint32_t ring = smem_u32(smem) + warp * F::kRingBytes;
 
-    grid_launch_dependents();
     if (!p.overlap) grid_dependency_wait();
     // ---- cost line: thread i holds the sequences [i * per, (i + 1) * per)
     auto cost_of = [&](int s) {
@@ -495,6 +494,7 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
 
     fetch_bid();
     grid_dependency_wait();
+    grid_launch_dependents();
 
     // the CTAs (from this one down, from this one up) whose ranges hold cost
     // points x0 <= x1 of a unit that this CTA has a part of; 32 CTAs a step
