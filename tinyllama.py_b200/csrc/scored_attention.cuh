@@ -38,8 +38,8 @@
 //    publish its partial sums them all. The order of every sum is fixed, so
 //    results are the same bits on every run.
 // Measured, one B200, calls back to back: 256 sequences of 7000-8192 tokens, 14 + 2
-// heads of 64, bf16 over e4m3 (508 MB), 88 us (5.8 TB/s). 64 sequences of 128-4096
-// tokens, 16 + 2 heads of 128, bf16 over e4m3 (71.6 MB), 22.7 us: the rows stream
+// heads of 64, bf16 over e4m3 (508 MB), 86 us (5.9 TB/s). 64 sequences of 128-4096
+// tokens, 16 + 2 heads of 128, bf16 over e4m3 (71.6 MB), 22.5 us: the rows stream
 // until 15 us, the joins take the rest. An L2 policy of evict_normal for the rows
 // cost 4 % of the latter. Without the scale bytes' copies the former, at 133 us
 // then, took 128 us; without its arithmetic 92 us.
