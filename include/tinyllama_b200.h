@@ -99,6 +99,8 @@ TLB_API int tlb_attention_set_wait_limit(uint32_t tries);
  *   out, query   : [num_seqs, num_heads, head_dim]            dtype
  *   key_cache    : [num_blocks, num_kv_heads, block_size, head_dim]  dtype
  *   value_cache  : same shape as key_cache                     dtype
+ *                  (the tensor-core kernel wants query and caches 16-byte, out
+ *                  8-byte aligned; others go to the kernel for any shape)
  *   block_tables : [num_seqs, max_blocks_per_seq] int32 (entries < 0 skipped)
  *   seq_lens     : [num_seqs] int32
  *   dtype        : TLB_FLOAT32, TLB_FLOAT16 or TLB_BFLOAT16
@@ -514,7 +516,8 @@ TLB_API int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args,
  * max_blocks_per_seq * block_size tokens (TLB_STATUS_SEQ_TOO_LONG).
  *
  *   query        : [num_seqs, num_heads, head_dim], rows query_stride apart
- *   out          : dense
+ *   out          : dense, aligned to its elements (off 4 bytes, the kernel for any
+ *                  shape serves the call)
  *   alibi_slopes : [num_heads] float or NULL
  *   cache_dtype  : dtype, or TLB_FLOAT8_E4M3 / TLB_INT8 with scales
  * `workspace`: device scratch of the size that the _workspace_size call gives

@@ -1,0 +1,46 @@
+"""Calls that the documentation of the operators allows and that only a C caller,
+or an unusual one, makes: what they are served by or refused with, without a
+GPU."""
+
+import pytest
+import torch
+
+from cscr import _lib
+
+P = 1 << 12  # stands in for an aligned device pointer; nothing is dereferenced
+CUDA_ERROR = 3
+F32, F16, BF16, I32, I64, E4M3, I8 = range(7)
+
+# The kernel that serves a call shows in the first CUDA call, which fails where
+# there is no device: the tensor-core kernels ask for it, the others are launched.
+no_device = pytest.mark.skipif(torch.cuda.is_available(), reason="would launch on made-up pointers")
+
+
+def scored(out=P, dtype=BF16, cache=E4M3, d=128):
+    name, pack = _lib.SCORED_ATTENTION
+    fields = (out, P, P, P, P, P, P, P, 0, 0, 0, 4, 16, 2, d, 10, 16, 4, 2048, 0, dtype, cache, 0,
+              0.1, 0.0)
+    return getattr(_lib.load(), name)(pack(*fields), None)
+
+
+@no_device
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("cache", [E4M3, I8, None])
+def test_scored_attention_stores_pairs_only_where_they_are_aligned(built_lib, cache, dtype):
+    cache = dtype if cache is None else cache
+    for out, tensor_cores in ((P, True), (P + 4, True), (P + 2, False), (P + 6, False)):
+        assert scored(out, dtype, cache) == CUDA_ERROR
+        assert ("device query" in _lib.last_error()) == tensor_cores, out
+
+
+@no_device
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_paged_attention_stores_four_only_where_they_are_aligned(built_lib, dtype):
+    lib = _lib.load()
+    for out, tensor_cores in ((P, True), (P + 8, True), (P + 2, False), (P + 4, False)):
+        assert lib.tlb_paged_attention(out, P, P, P, P, P, 4, 16, 2, 128, 10, 16, 4, 0.1, dtype,
+                                       None, 0, 0, None) == CUDA_ERROR
+        assert ("cudaGetDevice" in _lib.last_error()) == tensor_cores, out
+        rc = lib.tlb_paged_attention_with_rope(out, P, P, P, P, P, P, P, P, 64, 4, 16, 2, 128, 10,
+                                               16, 4, 256, 256, 0.1, dtype, None, 0, 0, None)
+        assert rc == (CUDA_ERROR if tensor_cores else _lib.TLB_ERR_UNSUPPORTED), out

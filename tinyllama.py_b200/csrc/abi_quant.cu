@@ -436,15 +436,16 @@ int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stre
     p.inv_cap = softcap > 0.f ? 1.f / softcap : 0.f;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // The tensor-core kernel copies rows by TMA, whose coordinates are 32-bit
-    // and whose base is 16-byte aligned, and scales four bytes at a time, and
-    // numbers the tiles of a call (with their charges) in 31 bits.
+    // and whose base is 16-byte aligned, and scales four bytes at a time, stores
+    // pairs of outputs, and numbers the tiles of a call (with their charges) in
+    // 31 bits.
     const int tt = sc::tile_tokens((int)head_dim * ce);
     const long long seen = p.window > 0 ? (long long)p.window + tt : p.max_tokens;
     const long long tiles = (seen + tt - 1) / tt * p.units_per_seq * num_seqs;
     const bool fast =
         sc::fast_supported(dtype, cache_dtype, (int)head_dim, (int)block_size) &&
-        aligned(query, 16) && query_stride % 8 == 0 && aligned(key_cache, 16) &&
-        aligned(value_cache, 16) && aligned(key_scales, 4) && aligned(value_scales, 4) &&
+        aligned(out, 4) && aligned(query, 16) && query_stride % 8 == 0 &&
+        aligned(key_cache, 16) && aligned(value_cache, 16) && aligned(key_scales, 4) && aligned(value_scales, 4) &&
         num_blocks * num_kv_heads < (1ll << 31) / block_size && tiles < (1ll << 30);
     if (!fast)
         return cuda_result(sc::launch_generic(dtype, cache_dtype, p, st), "paged attention");
