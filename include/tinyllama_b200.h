@@ -130,7 +130,11 @@ TLB_API int tlb_paged_attention_workspace_zeroed_bytes(int64_t num_seqs,
  * nor seq_lens (nor reads the output buffer): the attention kernel may then
  * start while that kernel finishes and read this metadata early
  * (programmatic dependent launch); query and cache are still read only after
- * it completes. Leave unset when the predecessor is unknown. */
+ * it completes. Leave unset when the predecessor is unknown. Kernels further
+ * back do not matter, here and for the flags below, with one exception: if the
+ * predecessor was launched with TLB_ROPE_OVERLAP_PREVIOUS (which lets the next
+ * kernel begin at once), the kernel before it counts as a predecessor too, and
+ * must not write what this one reads early. */
 #define TLB_ATTN_OVERLAP_PROLOGUE 0x1u
 
 TLB_API int tlb_paged_attention(void* out, const void* query, const void* key_cache,
@@ -315,7 +319,9 @@ TLB_API int tlb_write_kv_cache(const void* key, const void* value, void* key_cac
  * kernel completes this one reads only positions, slots, block_tables and
  * cos_sin_cache and writes nothing. Set it only when the preceding kernel
  * does not write those four arrays (a QKV projection or an attention
- * launch do not); leave it unset when the predecessor is unknown.
+ * launch do not); leave it unset when the predecessor is unknown. A launch with
+ * TLB_ATTN_OVERLAP_PROLOGUE or this flag right after it may begin while both
+ * kernels before it run: neither may write what that launch reads early.
  * ---------------------------------------------------------------------- */
 #define TLB_ROPE_OVERLAP_PREVIOUS 0x1u
 
@@ -474,9 +480,7 @@ TLB_API int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream)
  *     tlb_reshape_and_cache_quantized stores for the rounded key.
  * Positions outside the table leave the normed row unrotated and set
  * TLB_STATUS_BAD_POSITION. flags: TLB_ROPE_OVERLAP_PREVIOUS as above (the
- * norm weights too must not be written by the kernel before; if that is a
- * tlb_paged_attention or tlb_paged_attention_with_rope launch that itself
- * overlaps, nor by the one before it, which may still be running).
+ * norm weights too must not be written by the kernel before).
  * ---------------------------------------------------------------------- */
 typedef struct tlb_qk_norm_rope_args {
     void* query_out;
@@ -526,9 +530,7 @@ TLB_API int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args,
  * starts and are zero again when it ends, the rest may hold anything: calls on
  * one stream can share a buffer, calls that overlap in time need separate
  * ones. The zeroed size depends on the device alone. After TLB_STATUS_WAIT_TIMEOUT
- * the caller zeroes it again. flags: TLB_ATTN_OVERLAP_PROLOGUE as above (after
- * a launch of tlb_paged_attention(_with_rope) that itself overlaps, the kernel before
- * that one must not write block_tables or seq_lens either).
+ * the caller zeroes it again. flags: TLB_ATTN_OVERLAP_PROLOGUE as above.
  * ---------------------------------------------------------------------- */
 TLB_API int tlb_paged_attention_scored_workspace_size(int64_t num_heads, int64_t num_kv_heads,
                         int64_t head_dim, int64_t block_size, int dtype,

@@ -6,6 +6,7 @@ import torch
 
 from cscr import _lib
 from cscr import attention as A
+from cscr import pos_encoding as PE
 from cscr._lib import DTYPE_CODE
 from oracle import quant_oracle as Q
 from test_gpu_scored_attention import Case
@@ -51,3 +52,56 @@ def test_outputs_off_by_an_element_through_the_c_abi(dtype, kind):
         ref = Q.attention(c.q, c.k, c.v, None, None, c.tables, c.lens, c.scale)
         Q.assert_within(out, ref[0], Q.attention_bound(*ref, dtype, kind))
     assert bool((buf[0] == 7) & (buf[-1] == 7))
+
+
+@pytest.mark.parametrize("before", ["rope", "attention"])
+def test_early_reads_see_what_two_launches_back_wrote(before):
+    """Lengths and tables written right before a launch (an attention that itself
+    overlaps its predecessor, or a rotation, which must not), then an attention
+    that reads them early: steps queued without a pause equal those with a
+    synchronisation after every launch."""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    h, kvh, d, bs, n, width, blocks = 16, 2, 128, 16, 24, 40, 1200
+    c = Case([500] * n, h, kvh, d, bs, BF16, BF16, seed=23)
+    k, v = (torch.randn(blocks, kvh, bs, d, generator=g, device="cuda").to(BF16) for _ in "kv")
+    table = torch.rand(1024, d, generator=g, device="cuda").to(BF16)
+    key = torch.randn(n, kvh * d, generator=g, device="cuda").to(BF16)
+    value = torch.randn(n, kvh, d, generator=g, device="cuda").to(BF16)
+    pos = torch.arange(n, device="cuda")
+    slots = torch.full((n,), -1, device="cuda")  # nothing is written: the caches stay
+    own_lens, own_tables = c.lens, c.tables[:, :-1].clamp(max=blocks - 1).contiguous()
+    plans = [(torch.randint(0, width * bs, (n,), generator=g, device="cuda").to(torch.int32),
+              torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)[:n * width]
+              .view(n, width)) for _ in range(40)]
+    long = torch.randn(8192, 8192, generator=g, device="cuda")
+    torch.cuda.synchronize()
+
+    def steps(pause):
+        for _ in range(0 if pause else 8):  # the steps queue up behind these
+            long @ long
+        lens = torch.ones(n, dtype=torch.int32, device="cuda")
+        tables = torch.zeros(n, width, dtype=torch.int32, device="cuda")
+        outs = []
+        for new_lens, new_tables in plans:
+            tables.copy_(new_tables)
+            lens.copy_(new_lens)
+            if pause:
+                torch.cuda.synchronize()
+            if before == "rope":
+                PE.rotary_embedding_neox_with_cache(pos, c.q.view(n, -1), key, value, k, v,
+                                                    slots, d, table)
+            else:
+                A.paged_attention(c.q, k, v, own_tables, own_lens, c.scale, overlap_prologue=True)
+            if pause:
+                torch.cuda.synchronize()
+            outs.append(A.paged_attention_biased(c.q, k, v, tables, lens, c.scale, softcap=20.0,
+                                                 overlap_prologue=True))
+            outs.append(A.paged_attention(c.q, k, v, tables, lens, c.scale, overlap_prologue=True))
+            if pause:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+
+    for a, b in zip(steps(False), steps(True), strict=True):
+        assert torch.equal(a, b)
+    assert _lib.device_status() == 0

@@ -102,7 +102,9 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     ``overlap_prologue`` (keyword only, not in the reference API) lets the
     kernel start while the kernel launched just before it on this stream is
     finishing; set it only when that kernel writes neither block_tables nor
-    seq_lens — e.g. right after ``rotary_embedding_neox_with_cache``.
+    seq_lens — e.g. right after ``rotary_embedding_neox_with_cache``. After a
+    ``rotary_embedding_neox_with_cache`` with ``overlap_previous=True`` the
+    kernel before that one must not write them either: it may still be running.
     """
     torch_check(query.is_cuda, "query must be a CUDA tensor")
     torch_check(key_cache.is_cuda, "key_cache must be a CUDA tensor")
@@ -182,8 +184,8 @@ def paged_attention_with_rope(query: torch.Tensor, key: torch.Tensor, value: tor
 
     ``overlap_prologue`` has the contract of ``paged_attention``'s: set it
     only when the kernel launched just before on this stream writes neither
-    block_tables nor seq_lens (query, key, value and the caches are read only
-    after that kernel has finished).
+    block_tables, seq_lens nor cos_sin_cache (query, key, value and the caches
+    are read only after that kernel has finished).
     """
     torch_check(query.is_cuda and key.is_cuda and value.is_cuda and cos_sin_cache.is_cuda,
                 "query, key, value and cos_sin_cache must be CUDA tensors")

@@ -97,7 +97,9 @@ def rotary_embedding_neox_with_cache(postions: torch.Tensor, query: torch.Tensor
     starts while the kernel before it on the stream finishes; until then it
     reads only positions, slots, block tables and the cos/sin table. Use it
     only when that kernel writes none of those (an attention launch or a QKV
-    projection).
+    projection). The next launch on the stream, if it overlaps too, may then
+    begin while both run: neither may write what that one reads early (for an
+    attention with overlap_prologue block_tables and seq_lens).
     """
     out = torch.empty_like(query)
     num_tokens, rot_dim = _check_rope(postions, query, key, head_size, cos_sin_cache, out)

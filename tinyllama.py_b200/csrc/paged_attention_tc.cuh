@@ -310,11 +310,6 @@ __global__ void __launch_bounds__((CW + 2) * 32, (NT == 1 && CW == 4) ? 2 : 1)
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_v);
     }
-    // The next kernel on the stream, if launched programmatically, may start
-    // its own prologue once SMs free up; it waits for this grid to finish
-    // before it writes or reads anything this kernel produces.
-    grid_launch_dependents();
-
     // ---- pass 1: context lengths -> shared memory, exclusive prefix of
     // cost per sequence (per kv head), total. Thread t owns sequences [t*per, t*per+per):
     // one batch of independent loads, one block scan.
@@ -767,6 +762,12 @@ __global__ void __launch_bounds__((CW + 2) * 32, (NT == 1 && CW == 4) ? 2 : 1)
         // Everything above reads only metadata; the query and the cache may
         // still be written by the kernel launched just before this one.
         grid_dependency_wait();
+        // The next kernel on the stream, if launched programmatically, may start
+        // its own prologue once SMs free up; it waits for this grid to finish
+        // before it writes or reads anything this kernel produces. Not before
+        // the wait: what it reads early may have been written by the kernel
+        // before this one.
+        grid_launch_dependents();
         while (nf < 2) prefetch(nf++);
         bool ok = true;
         for (int k = 0;; ++k) {
