@@ -105,3 +105,20 @@ def test_early_reads_see_what_two_launches_back_wrote(before):
     for a, b in zip(steps(False), steps(True), strict=True):
         assert torch.equal(a, b)
     assert _lib.device_status() == 0
+
+
+def test_quantised_attention_refuses_caches_without_scales():
+    """Also on a stream whose scratch is there, where cscr._fast takes the calls."""
+    c = Case([40, 7], 8, 2, 64, 16, F16, F16, seed=24)
+    c.run()
+    args = (c.tables, c.lens, c.scale)
+    fast = _lib.fast.attention(c.q, c.k, c.v, None, None, *args, 0.0, None, 0, False)
+    assert fast is not None and torch.equal(fast, c.run())
+    for ks, vs in ((None, None), (None, c.lens)):
+        with pytest.raises(RuntimeError, match="float8_e4m3fn or int8"):
+            A.paged_attention_quantized(c.q, c.k, c.v, ks, vs, *args)
+    assert _lib.fast.attention(c.q, c.k, c.v, None, c.lens, *args, 0.0, None, 0, False) is None
+    c = Case([40, 7], 8, 2, 64, 16, F16, INT8, seed=24)
+    for ks, vs in ((None, None), (c.ks, None), (None, c.vs)):
+        with pytest.raises(RuntimeError, match="float8_e8m0fnu"):
+            A.paged_attention_quantized(c.q, c.k, c.v, ks, vs, *args)

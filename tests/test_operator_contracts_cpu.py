@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from cscr import _lib
+from cscr import attention as A
 
 P = 1 << 12  # stands in for an aligned device pointer; nothing is dereferenced
 CUDA_ERROR = 3
@@ -44,3 +45,20 @@ def test_paged_attention_stores_four_only_where_they_are_aligned(built_lib, dtyp
         rc = lib.tlb_paged_attention_with_rope(out, P, P, P, P, P, P, P, P, 64, 4, 16, 2, 128, 10,
                                                16, 4, 256, 256, 0.1, dtype, None, 0, 0, None)
         assert rc == (CUDA_ERROR if tensor_cores else _lib.TLB_ERR_UNSUPPORTED), out
+
+
+class AnswersAll:
+    """Stands for cscr._fast on a warm stream: it has an answer to every call."""
+
+    def __getattr__(self, name):
+        return lambda *args: "answered"
+
+
+def test_quantised_attention_needs_scales_on_a_warm_stream_too(monkeypatch):
+    monkeypatch.setattr(_lib, "fast", AnswersAll())
+    x, c8 = torch.zeros(3, 2, 64), torch.zeros(2, 2, 8, 64, dtype=torch.int8)
+    tables, lens = torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="float8_e4m3fn or int8"):
+        A.paged_attention_quantized(x, x[None], x[None], None, None, tables, lens, 0.1)
+    with pytest.raises(RuntimeError, match="float8_e8m0fnu"):
+        A.paged_attention_quantized(x, c8, c8, None, None, tables, lens, 0.1)

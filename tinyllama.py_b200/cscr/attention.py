@@ -441,7 +441,8 @@ def paged_attention_quantized(query: torch.Tensor, key_cache: torch.Tensor,
     ``softcap``, ``alibi_slopes`` and ``window`` as in ``paged_attention_biased``,
     ``overlap_prologue`` as in ``paged_attention``.
     """
-    if _lib.fast is not None:
+    # without scales the short way would take the call for paged_attention_biased
+    if _lib.fast is not None and key_scales is not None:
         out = _lib.fast.attention(query, key_cache, value_cache, key_scales, value_scales,
                                   block_tables, seq_lens, scale, softcap, alibi_slopes, window,
                                   overlap_prologue)
@@ -451,8 +452,8 @@ def paged_attention_quantized(query: torch.Tensor, key_cache: torch.Tensor,
                 "key_cache must be float8_e4m3fn or int8")
     rows, index = key_cache.shape[:3], query.get_device()
     for s in (key_scales, value_scales):
-        if not (s.dtype == torch.float8_e8m0fnu and s.shape == rows and s.is_contiguous()
-                and s.get_device() == index):
+        if not (s is not None and s.dtype == torch.float8_e8m0fnu and s.shape == rows
+                and s.is_contiguous() and s.get_device() == index):
             raise RuntimeError("key_scales and value_scales must be contiguous float8_e8m0fnu "
                                "tensors [num_blocks, num_kv_heads, block_size] on the query's "
                                "device")

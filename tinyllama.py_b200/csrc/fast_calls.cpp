@@ -148,7 +148,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         sl->scalar_type() != ScalarType::Int)
         return later();
     if (ks != nullptr ? !quantized_caches(at, kc, vc, ks, vs)
-                      : a[3] != Py_None || kc->scalar_type() != q->scalar_type())
+                      : a[3] != Py_None || a[4] != Py_None || kc->scalar_type() != q->scalar_type())
         return later();
     if (slopes != nullptr ? !at.has(slopes) || slopes->scalar_type() != ScalarType::Float ||
                                 slopes->dim() != 1 || slopes->size(0) != H
