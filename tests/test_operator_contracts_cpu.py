@@ -7,6 +7,7 @@ import torch
 
 from cscr import _lib
 from cscr import attention as A
+from cscr import pos_encoding as PE
 
 P = 1 << 12  # stands in for an aligned device pointer; nothing is dereferenced
 CUDA_ERROR = 3
@@ -62,3 +63,15 @@ def test_quantised_attention_needs_scales_on_a_warm_stream_too(monkeypatch):
         A.paged_attention_quantized(x, x[None], x[None], None, None, tables, lens, 0.1)
     with pytest.raises(RuntimeError, match="float8_e8m0fnu"):
         A.paged_attention_quantized(x, c8, c8, None, None, tables, lens, 0.1)
+
+
+@pytest.mark.parametrize("missing", ["value", "key_cache", "value_cache"])
+def test_norm_with_cache_needs_its_caches_on_a_warm_stream_too(monkeypatch, missing):
+    monkeypatch.setattr(_lib, "fast", AnswersAll())
+    x, w, i = torch.zeros(3, 64), torch.ones(64), torch.zeros(3, dtype=torch.int64)
+    kw = dict(value=x, key_cache=x.view(3, 1, 1, 64), value_cache=x.view(3, 1, 1, 64))
+    kw[missing] = None
+    with pytest.raises(RuntimeError, match="must be given"):
+        PE.qk_norm_rotary_embedding_neox_with_cache(i, x, x, query_weight=w, key_weight=w, eps=1e-6,
+                                                    slot_mapping=i, head_size=64, cos_sin_cache=x,
+                                                    **kw)

@@ -261,6 +261,9 @@ def qk_norm_rotary_embedding_neox_with_cache(
     the query dtype. Destinations and ``overlap_previous`` as in
     ``rotary_embedding_neox_with_cache``; the slots of one call must differ.
     """
+    if key_cache is None or value_cache is None or value is None:
+        raise RuntimeError("key_cache, value_cache and value must be given "
+                           "(qk_norm_rotary_embedding_neox writes no cache)")
     if _lib.fast is not None:
         out = _lib.fast.norm(positions, query, key, value, query_weight, key_weight, eps,
                              key_cache, value_cache, slot_mapping, head_size, cos_sin_cache,
