@@ -122,3 +122,26 @@ def test_quantised_attention_refuses_caches_without_scales():
     for ks, vs in ((None, None), (c.ks, None), (None, c.vs)):
         with pytest.raises(RuntimeError, match="float8_e8m0fnu"):
             A.paged_attention_quantized(c.q, c.k, c.v, ks, vs, *args)
+
+
+class NoTruth:
+    def __bool__(self):
+        raise ArithmeticError("neither")
+
+
+def test_flags_without_a_truth_value():
+    """What a flag's __bool__ raises reaches the caller, and nothing is launched."""
+    c = Case([40, 7], 8, 2, 64, 16, F16, INT8, seed=25)
+    want = c.run()
+    with pytest.raises(ArithmeticError, match="neither"):
+        c.run(overlap_prologue=NoTruth())
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        c.run(overlap_prologue=torch.zeros(2))
+    x = c.q.view(2, -1)[:, :128].contiguous()
+    w, pos = torch.ones(64, dtype=F16, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    args = (w, w, 1e-6, c.k, c.v, pos, 64, x.view(4, 64))
+    before = c.k.clone()
+    with pytest.raises(ArithmeticError, match="neither"):
+        PE.qk_norm_rotary_embedding_neox_with_cache(pos, x, x, x, *args, key_scales=c.ks,
+                                                    value_scales=c.vs, overlap_previous=NoTruth())
+    assert torch.equal(c.k, before) and torch.equal(c.run(), want)

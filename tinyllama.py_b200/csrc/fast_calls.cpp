@@ -118,6 +118,13 @@ bool whole(PyObject* o, int64_t* x) {
     return true;
 }
 
+bool truth(PyObject* o, bool* x) {
+    const int t = PyObject_IsTrue(o);
+    *x = t > 0;
+    if (t < 0) PyErr_Clear();
+    return t >= 0;
+}
+
 PyObject* later() { Py_RETURN_NONE; }
 
 Tensor dense(const Tensor& like, at::IntArrayRef sizes, ScalarType type) {
@@ -133,7 +140,9 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                  *vs = tensor(a[4]), *bt = tensor(a[5]), *sl = tensor(a[6]), *slopes = tensor(a[9]);
     double scale, softcap;
     int64_t window;
-    if (q == nullptr || !number(a[7], &scale) || !number(a[8], &softcap) || !whole(a[10], &window))
+    bool overlap;
+    if (q == nullptr || !number(a[7], &scale) || !number(a[8], &softcap) ||
+        !whole(a[10], &window) || !truth(a[11], &overlap))
         return later();
     const Place at(*q);
     if (!at.ok() || !at.has(kc) || !at.has(vc) || !at.has(bt) || !at.has(sl)) return later();
@@ -184,7 +193,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.window = window;
     p.dtype = code_of(q->scalar_type());
     p.cache_dtype = code_of(kc->scalar_type());
-    p.flags = PyObject_IsTrue(a[11]) ? TLB_ATTN_OVERLAP_PROLOGUE : 0;
+    p.flags = overlap ? TLB_ATTN_OVERLAP_PROLOGUE : 0;
     p.scale = scale;
     p.softcap = softcap;
     if (g_attention(&p, at.stream) != TLB_OK) return later();
@@ -281,7 +290,9 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                  *ks = tensor(a[13]), *vs = tensor(a[14]);
     double eps;
     int64_t D;
-    if (q == nullptr || k == nullptr || !number(a[6], &eps) || !whole(a[10], &D) || D <= 0)
+    bool overlap;
+    if (q == nullptr || k == nullptr || !number(a[6], &eps) || !whole(a[10], &D) || D <= 0 ||
+        !truth(a[15], &overlap))
         return later();
     const Place at(*q);
     if (!at.ok() || !at.has(pos) || !at.has(wq) || !at.has(wk) || !at.has(table) || !k->is_cuda() ||
@@ -359,7 +370,7 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.query_stride = q->stride(0);
     p.key_stride = k->stride(0);
     p.dtype = code_of(type);
-    p.flags = PyObject_IsTrue(a[15]) ? TLB_ROPE_OVERLAP_PREVIOUS : 0;
+    p.flags = overlap ? TLB_ROPE_OVERLAP_PREVIOUS : 0;
     p.eps = eps;
     if (g_norm(&p, at.stream) != TLB_OK) return later();
     PyObject* po = THPVariable_Wrap(std::move(q_out));
