@@ -2,6 +2,8 @@
 or an unusual one, makes: what they are served by or refused with, without a
 GPU."""
 
+import weakref
+
 import pytest
 import torch
 
@@ -75,3 +77,43 @@ def test_norm_with_cache_needs_its_caches_on_a_warm_stream_too(monkeypatch, miss
         PE.qk_norm_rotary_embedding_neox_with_cache(i, x, x, query_weight=w, key_weight=w, eps=1e-6,
                                                     slot_mapping=i, head_size=64, cos_sin_cache=x,
                                                     **kw)
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that passes the ops' device checks; nothing is launched on it."""
+
+    def get_device(self):
+        return 0
+
+
+def test_scratch_lives_until_the_launch(monkeypatch):
+    """Each call's scratch, the stream's or one of its own, is still held when the
+    launch gets its address."""
+    made, launched = [], []
+
+    def workspace(query, index, nbytes, zeroed):
+        ws = torch.zeros(nbytes, dtype=torch.uint8)
+        made.append((weakref.ref(ws), ws.data_ptr()))
+        return ws
+
+    def launch(entry, index, *args):
+        ref, address = made[-1]
+        launched.append(ref() is not None and address in args)
+
+    monkeypatch.setattr(_lib, "fast", None)
+    monkeypatch.setattr(_lib, "launch", launch)
+    monkeypatch.setattr(A, "_scored_workspace", workspace)
+    monkeypatch.setattr(A, "_scored_workspace_bytes", lambda *key: (256, 64))
+
+    def on(x):
+        return x.as_subclass(OnDevice)
+
+    q, c = on(torch.zeros(3, 2, 64, dtype=torch.bfloat16)), on(
+        torch.zeros(2, 2, 8, 64, dtype=torch.bfloat16))
+    tables = on(torch.zeros(3, 1, dtype=torch.int32))
+    lens = on(torch.ones(3, dtype=torch.int32))
+    A.paged_attention_biased(q, c, c, tables, lens, 0.1)
+    c8 = on(torch.zeros(2, 2, 8, 64, dtype=torch.int8))
+    sc = on(torch.zeros(2, 2, 8, dtype=torch.float8_e8m0fnu))
+    A.paged_attention_quantized(q, c8, c8, sc, sc, tables, lens, 0.1)
+    assert launched == [True, True]

@@ -412,15 +412,18 @@ def _paged_attention_scored(query, key_cache, value_cache, key_scales, value_sca
         return out
     nbytes, zeroed = _scored_workspace_bytes(shape[1], num_kv_heads, head_dim, block_size, dtype,
                                              cache_dtype, index)
-    ws = _scored_workspace(query, index, nbytes, zeroed).data_ptr() if nbytes else 0
+    # held until the launch: freed before, its memory could go to another thread's
+    # tensor whose work is queued first
+    ws = _scored_workspace(query, index, nbytes, zeroed) if nbytes else None
     _lib.launch(_lib.SCORED_ATTENTION, index, out.data_ptr(), query.data_ptr(),
                 key_cache.data_ptr(), value_cache.data_ptr(),
                 0 if key_scales is None else key_scales.data_ptr(),
                 0 if value_scales is None else value_scales.data_ptr(), block_tables.data_ptr(),
-                seq_lens.data_ptr(), 0 if alibi_slopes is None else alibi_slopes.data_ptr(), ws,
-                nbytes, shape[0], shape[1], num_kv_heads, head_dim, num_blocks, block_size,
-                tshape[1], strides[0], window, DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype],
-                1 if overlap_prologue else 0, scale, softcap)
+                seq_lens.data_ptr(), 0 if alibi_slopes is None else alibi_slopes.data_ptr(),
+                0 if ws is None else ws.data_ptr(), nbytes, shape[0], shape[1], num_kv_heads,
+                head_dim, num_blocks, block_size, tshape[1], strides[0], window,
+                DTYPE_CODE[dtype], DTYPE_CODE[cache_dtype], 1 if overlap_prologue else 0, scale,
+                softcap)
     return out
 
 
