@@ -6,9 +6,12 @@ import torch
 
 from cscr import _lib
 from cscr import attention as A
+from cscr import cache as C
 from cscr import pos_encoding as PE
 from cscr._lib import DTYPE_CODE
 from oracle import quant_oracle as Q
+from paged_decode import pool
+from paged_decode.layers import PagedAttentionWithQKNorm
 from test_gpu_scored_attention import Case
 
 pytestmark = pytest.mark.gpu
@@ -145,3 +148,47 @@ def test_flags_without_a_truth_value():
         PE.qk_norm_rotary_embedding_neox_with_cache(pos, x, x, x, *args, key_scales=c.ks,
                                                     value_scales=c.vs, overlap_previous=NoTruth())
     assert torch.equal(c.k, before) and torch.equal(c.run(), want)
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8], ids=short)
+def test_prompts_over_8_bit_caches_look_up_what_16_bit_ones_do(kind):
+    """Stale ids past a context are not looked up; a hole and an id outside the pool
+    inside one are skipped, the latter flagged: as over caches of the query dtype
+    that hold the same rows."""
+    h, kvh, d, bs, blocks = 8, 2, 64, 16, 30
+    g = torch.Generator(device="cuda").manual_seed(26)
+    m = PagedAttentionWithQKNorm(h, d, d ** -0.5, d, max_position=1024).cuda()
+    kv = pool.allocate_quantized_kv_cache(1, blocks, kvh, d, bs, kind)[0]
+    rows = torch.randn(2, blocks * bs, kvh, d, generator=g, device="cuda").to(BF16)
+    C.reshape_and_cache_quantized(rows[0], rows[1], *kv, torch.arange(blocks * bs, device="cuda"))
+    ctx = torch.tensor([100, 64, 33], dtype=torch.int32, device="cuda")
+    part = [20, 64, 33]
+    start = torch.tensor([0, 20, 84, 117], dtype=torch.int32, device="cuda")
+    good = torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)[:24].view(3, 8)
+    seq = torch.repeat_interleave(torch.arange(3), torch.tensor(part)).cuda()
+    pos = torch.cat([torch.arange(n - p, n) for n, p in zip(ctx.tolist(), part)]).cuda()
+    slots = good[seq, pos // bs].long() * bs + pos % bs
+    q = torch.randn(117, h, d, generator=g, device="cuda").to(BF16)
+    k, v = torch.randn(2, 117, kvh, d, generator=g, device="cuda").to(BF16)
+
+    def run(tables):
+        out = m.prompt(pos, q, k, v, kv[0], kv[1], slots, tables, start, ctx, 64, kv[2], kv[3])
+        status = _lib.device_status()
+        dense = [Q.dequantize(c, s).to(BF16) for c, s in ((kv[0], kv[2]), (kv[1], kv[3]))]
+        q_rot, _ = PE.qk_norm_rotary_embedding_neox(pos, q.view(117, -1), k.view(117, -1),
+                                                    m.q_norm.to(BF16), m.k_norm.to(BF16), m.eps, d,
+                                                    m._table(q.device, BF16))
+        want = A.paged_prefill_attention(q_rot.view(117, h, d), *dense, tables, start, ctx, m.scale,
+                                         64)
+        assert _lib.device_status() == status
+        assert torch.isfinite(out).all() and torch.equal(out, want)
+        return status
+
+    stale = good.clone()
+    for c, n in enumerate(ctx.tolist()):
+        stale[c, -(-n // bs):] = torch.tensor([blocks, 0, -1, 1 << 30], dtype=torch.int32,
+                                              device="cuda").repeat(2)[:8 + -n // bs]
+    assert run(stale) == 0
+    stale[0, 2] = blocks + 3
+    stale[1, 1] = -1
+    assert run(stale) == 0x1

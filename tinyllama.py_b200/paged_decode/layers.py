@@ -194,7 +194,9 @@ class PagedAttentionWithQKNorm(PagedAttentionWithRoPE):
                key_scales: torch.Tensor | None = None,
                value_scales: torch.Tensor | None = None) -> torch.Tensor:
         """Prompt chunks (packed tokens [T, ...]), as ``cscr.attention.
-        paged_prefill_attention`` takes them; the new rows go to ``slot_mapping``."""
+        paged_prefill_attention`` takes them; the new rows go to ``slot_mapping``.
+        Over 8-bit caches every entry of ``block_tables`` costs a block of each
+        cache in the query dtype: pass no more columns than the contexts need."""
         if self.softcap or self.window:
             raise NotImplementedError("prompt chunks have plain scores: no softcap, no window")
         query = self._norm_rope_write(positions, query, key, value, key_cache, value_cache,
@@ -202,10 +204,15 @@ class PagedAttentionWithQKNorm(PagedAttentionWithRoPE):
         tables = block_tables.to(torch.int32).contiguous()
         if key_scales is not None:
             # the chunks' blocks in the query dtype: entry j of chunk c is block
-            # c * max_blocks + j of what is read back (holes stay holes)
+            # c * max_blocks + j of what is read back. Entries past a context may
+            # be stale and are not looked up; holes, and ids outside the pool
+            # (which the read flags), are holes of the new table too.
+            num_blocks, _, block_size, _ = key_cache.shape
+            starts = torch.arange(0, tables.size(1) * block_size, block_size, device=tables.device)
+            tables = torch.where(starts < context_lens[:, None], tables, -1)
             key_cache, value_cache = _Cache.dequantize_blocks(
                 key_cache, value_cache, key_scales, value_scales, tables.view(-1), query.dtype)
             places = torch.arange(tables.numel(), dtype=torch.int32, device=tables.device)
-            tables = torch.where(tables < 0, tables, places.view_as(tables))
+            tables = torch.where((tables >= 0) & (tables < num_blocks), places.view_as(tables), -1)
         return _C.paged_prefill_attention(query, key_cache, value_cache, tables, query_start,
                                           context_lens, self.scale, max_query_len)
