@@ -409,8 +409,9 @@ TLB_API int tlb_step_metadata(const int32_t* prompt_lens, const int32_t* prompt_
  *                              TLB_FLOAT8_E4M3 or TLB_INT8
  *   key_scales, value_scales : [num_blocks, num_kv_heads, block_size] bytes, one
  *                              per row: byte b stands for the scale 2^(b - 127)
- *                              (1 .. 254; 0 reads as a scale of 0, 255 is not
- *                              a scale)
+ *                              (1 .. 254). 0 and 255 are no scales: the write
+ *                              stores neither, and what a row under one reads
+ *                              as is not defined
  *
  * A row x is stored as round_to_nearest_even(x_i / 2^E), 2^E the smallest power
  * of two with max|x| <= 448 * 2^E (e4m3) or 127 * 2^E (int8), E in [-126, 127].
