@@ -192,3 +192,17 @@ def test_prompts_over_8_bit_caches_look_up_what_16_bit_ones_do(kind):
     stale[0, 2] = blocks + 3
     stale[1, 1] = -1
     assert run(stale) == 0x1
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8], ids=short)
+@pytest.mark.parametrize("power", [-100, 100, 126])
+def test_queries_near_the_ends_of_bf16(kind, power):
+    """Queries some 2^power, keys and scale that bring the scores back."""
+    c = Case([100, 33], 8, 2, 64, 16, BF16, kind, seed=28)
+    c.q = (c.q.clamp(-3.9, 3.9).double() * 2.0 ** power).to(BF16)
+    back = 110 if power > 0 else -100
+    c.ks = (c.ks.view(torch.uint8) - back).view(torch.float8_e8m0fnu)
+    c.scale *= 2.0 ** (back - power)
+    assert bool(torch.isfinite(c.q).all()) and int(c.ks.view(torch.uint8)[c.tables[0, 0]].min()) > 0
+    c.check(c.run())
+    c.check(c.run(softcap=3.0), softcap=3.0)

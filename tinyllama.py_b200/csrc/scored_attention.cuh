@@ -565,8 +565,9 @@ __global__ void __launch_bounds__(Cfg<QT, CT, D, NT>::kThreads, 1)
                     }
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    // 2^n that brings the head's largest element into [2^14, 2^15)
-                    const int n = min(max(14 - ((int)(top >> 23) - 127), -110), 110);
+                    // 2^n that brings the head's largest element into [2^14, 2^15):
+                    // n >= 14 - 127; at most 110, so that 2^-n leaves room for the scale
+                    const int n = min(14 - ((int)(top >> 23) - 127), 110);
                     const float up = __uint_as_float((uint32_t)(n + 127) << 23);
                     scale_q *= __uint_as_float((uint32_t)(127 - n) << 23);
 #pragma unroll
