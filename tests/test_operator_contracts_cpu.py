@@ -2,6 +2,8 @@
 or an unusual one, makes: what they are served by or refused with, without a
 GPU."""
 
+import sys
+import types
 import weakref
 
 import pytest
@@ -117,3 +119,22 @@ def test_scratch_lives_until_the_launch(monkeypatch):
     sc = on(torch.zeros(2, 2, 8, dtype=torch.float8_e8m0fnu))
     A.paged_attention_quantized(q, c8, c8, sc, sc, tables, lens, 0.1)
     assert launched == [True, True]
+
+
+def test_a_module_of_another_torch_is_neither_used_nor_taken_as_built(built_lib, monkeypatch,
+                                                                      tmp_path):
+    import build as B
+    import cscr
+
+    assert _lib._load_fast() is _lib.fast and _lib.fast is not None and B._fast_up_to_date()
+    for version in ("1.0.0", None):
+        other = types.ModuleType("cscr._fast")
+        if version is not None:
+            other.torch_version = version
+        monkeypatch.setitem(sys.modules, "cscr._fast", other)
+        monkeypatch.setattr(cscr, "_fast", other)
+        assert _lib._load_fast() is None
+    module = tmp_path / "_fast.so"
+    module.write_bytes(b"built against 1.0.0\0")
+    monkeypatch.setattr(B, "FAST_PATH", module)
+    assert not B._fast_up_to_date()

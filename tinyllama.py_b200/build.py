@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -68,9 +69,17 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= built for p in _deps())
 
 
+def _torch_version() -> str:
+    return importlib.metadata.version("torch")
+
+
 def _fast_up_to_date() -> bool:
     deps = [FAST_SRC, *INCLUDE.glob("*.h")]
-    return FAST_PATH.exists() and all(p.stat().st_mtime <= FAST_PATH.stat().st_mtime for p in deps)
+    if not FAST_PATH.exists() or any(
+            p.stat().st_mtime > FAST_PATH.stat().st_mtime for p in deps):
+        return False
+    # the module names the torch it was compiled against (its torch_version)
+    return _torch_version().encode() + b"\0" in FAST_PATH.read_bytes()
 
 
 def _build_fast() -> None:
@@ -85,7 +94,7 @@ def _build_fast() -> None:
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-isystem{p}" for p in cpp_extension.include_paths()),
            f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{cuda / 'include'}",
-           f"-I{INCLUDE}", str(FAST_SRC), "-o", str(tmp), f"-L{lib}", "-ltorch_python", "-ltorch",
+           f"-I{INCLUDE}", f'-DTLB_TORCH_VERSION="{_torch_version()}"', str(FAST_SRC), "-o", str(tmp), f"-L{lib}", "-ltorch_python", "-ltorch",
            "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

@@ -150,15 +150,23 @@ QK_NORM_ROPE = ("tlb_qk_norm_rotary_embedding_neox", struct.Struct("=32qd").pack
 SCORED_ATTENTION = ("tlb_paged_attention_scored", struct.Struct("=23q2d").pack)
 
 
-# The ordinary calls without their Python argument handling (csrc/fast_calls.cpp):
-# its functions answer None for what the Python code has to look at. Not used in
-# debug mode; unbound, and so answering None, until the library is loaded.
-try:
+def _load_fast():
+    """The ordinary calls without their Python argument handling
+    (csrc/fast_calls.cpp): functions that answer None for what the Python code
+    has to look at; unbound, and so answering None, until the library is loaded.
+    None in debug mode and where the module was built against another torch,
+    whose tensors it would misread."""
     if DEBUG:
-        raise ImportError
-    from . import _fast as fast
-except ImportError:
-    fast = None
+        return None
+    try:
+        from . import _fast
+    except ImportError:
+        return None
+    same = getattr(_fast, "torch_version", None) == str(torch.__version__)
+    return _fast if same else None
+
+
+fast = _load_fast()
 
 
 def launch(entry, index: int, *args) -> None:

@@ -424,4 +424,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fast(void) { return PyModule_Create(&module); }
+// torch_version: the torch whose headers (and so tensor layout) this was built with
+PyMODINIT_FUNC PyInit__fast(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", TLB_TORCH_VERSION) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}
