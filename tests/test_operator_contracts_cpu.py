@@ -138,3 +138,19 @@ def test_a_module_of_another_torch_is_neither_used_nor_taken_as_built(built_lib,
     module.write_bytes(b"built against 1.0.0\0")
     monkeypatch.setattr(B, "FAST_PATH", module)
     assert not B._fast_up_to_date()
+
+
+def test_a_module_that_does_not_compile_leaves_the_build_whole(built_lib, monkeypatch, tmp_path,
+                                                               capsys):
+    import build as B
+
+    module = tmp_path / "_fast.so"
+    module.write_bytes(b"an older one")
+    source = tmp_path / "fast_calls.cpp"
+    source.write_text("#error does not compile\n")
+    monkeypatch.setattr(B, "FAST_PATH", module)
+    monkeypatch.setattr(B, "FAST_SRC", source)
+    before = B.LIB_PATH.stat().st_mtime
+    assert B.build() == B.LIB_PATH and B.LIB_PATH.stat().st_mtime == before
+    assert "does not compile" in capsys.readouterr().err
+    assert not module.exists()

@@ -63,7 +63,11 @@ def _deps() -> list[Path]:
 
 
 def up_to_date() -> bool:
-    if not LIB_PATH.exists() or not _fast_up_to_date():
+    return _lib_up_to_date() and _fast_up_to_date()
+
+
+def _lib_up_to_date() -> bool:
+    if not LIB_PATH.exists():
         return False
     built = LIB_PATH.stat().st_mtime
     return all(p.stat().st_mtime <= built for p in _deps())
@@ -83,7 +87,17 @@ def _fast_up_to_date() -> bool:
 
 
 def _build_fast() -> None:
-    """Compile cscr._fast against the running interpreter and its torch."""
+    """Compile cscr._fast against the running interpreter and its torch. The ops run
+    without it: a failure is a warning, and leaves no older module behind."""
+    try:
+        _compile_fast()
+    except Exception as exc:  # noqa: BLE001 - whatever kept it from being built
+        FAST_PATH.unlink(missing_ok=True)
+        print(f"warning: cscr._fast is not built, calls take longer on the host: {exc}",
+              file=sys.stderr)
+
+
+def _compile_fast() -> None:
     import torch
     from torch.utils import cpp_extension
 
@@ -117,16 +131,17 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the kernels and link the shared library; returns its path."""
-    if not force and up_to_date():
-        return LIB_PATH
+    stale = force or not _lib_up_to_date()
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
-    srcs = sources()
+    srcs = sources() if stale else []
     workers = min(len(srcs) + 1, os.cpu_count() or 4)
     with cf.ThreadPoolExecutor(max_workers=workers) as ex:
-        fast = None if _fast_up_to_date() and not force else ex.submit(_build_fast)
+        fast = ex.submit(_build_fast) if force or not _fast_up_to_date() else None
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
         if fast is not None:
             fast.result()
+    if not stale:
+        return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-o", str(tmp), *map(str, objs), "-cudart", "static"]
     res = subprocess.run(cmd, capture_output=True, text=True)
