@@ -480,8 +480,8 @@ TLB_API int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream)
  *     type with scales: then the rows stored are those that
  *     tlb_reshape_and_cache_quantized stores for the rounded key.
  * Positions outside the table leave the normed row unrotated and set
- * TLB_STATUS_BAD_POSITION. flags: TLB_ROPE_OVERLAP_PREVIOUS as above (the
- * norm weights too must not be written by the kernel before).
+ * TLB_STATUS_BAD_POSITION. flags: TLB_ROPE_OVERLAP_PREVIOUS is accepted and
+ * changes nothing: the kernel reads nothing before the one before it ends.
  * ---------------------------------------------------------------------- */
 typedef struct tlb_qk_norm_rope_args {
     void* query_out;

@@ -206,3 +206,50 @@ def test_queries_near_the_ends_of_bf16(kind, power):
     assert bool(torch.isfinite(c.q).all()) and int(c.ks.view(torch.uint8)[c.tables[0, 0]].min()) > 0
     c.check(c.run())
     c.check(c.run(softcap=3.0), softcap=3.0)
+
+
+@pytest.mark.parametrize("kind", [E4M3, None], ids=short)
+def test_norm_reads_nothing_before_the_kernel_before_it_ends(kind):
+    """overlap_previous asks nothing of the caller here: positions, slots, tables,
+    weights, angles and rows written right before each of a queue of calls."""
+    g = torch.Generator(device="cuda").manual_seed(29)
+    h, kvh, d, bs, n, blocks = 8, 2, 128, 16, 48, 64
+    long = torch.randn(8192, 8192, generator=g, device="cuda")
+
+    def new():
+        slots = torch.randperm(blocks * bs, generator=g, device="cuda")[:n]
+        return (torch.randint(0, 512, (n,), generator=g, device="cuda"), slots,
+                *(torch.randn(*s, generator=g, device="cuda").to(BF16)
+                  for s in ((n, h * d), (n, kvh * d), (n, kvh * d), (d,), (d,), (512, d))))
+
+    plans = [new() for _ in range(30)]
+
+    def steps(pause):
+        caches = (pool.allocate_kv_cache(1, blocks, kvh, d, bs, BF16)[0] if kind is None
+                  else pool.allocate_quantized_kv_cache(1, blocks, kvh, d, bs, kind)[0])
+        for c in caches:
+            c.view(torch.uint8).zero_()
+        scales = dict(zip(("key_scales", "value_scales"), caches[2:]))
+        now = [torch.zeros_like(x) for x in plans[0]]
+        outs = []
+        for _ in range(0 if pause else 8):  # the steps queue up behind these
+            long @ long
+        for plan in plans:
+            for i, x in enumerate(now):
+                # each of them is once the last one written
+                j = (i + len(outs)) % len(now)
+                now[j].copy_(plan[j])
+            if pause:
+                torch.cuda.synchronize()
+            pos, slots, q, k, v, wq, wk, table = now
+            outs.append(PE.qk_norm_rotary_embedding_neox_with_cache(
+                pos, q, k, v, wq, wk, 1e-6, *caches[:2], slots, d, table, overlap_previous=True,
+                **scales))
+            if pause:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs + [c.view(torch.uint8) for c in caches]
+
+    for a, b in zip(steps(False), steps(True), strict=True):
+        assert torch.equal(a, b)
+    assert _lib.device_status() == 0

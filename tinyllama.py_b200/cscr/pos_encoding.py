@@ -258,8 +258,9 @@ def qk_norm_rotary_embedding_neox_with_cache(
     are float8_e4m3fn or int8 with ``key_scales`` and ``value_scales``
     (float8_e8m0fnu): then the stored rows are those that
     ``cscr.cache.reshape_and_cache_quantized`` stores for the key as rounded to
-    the query dtype. Destinations and ``overlap_previous`` as in
-    ``rotary_embedding_neox_with_cache``; the slots of one call must differ.
+    the query dtype. Destinations as in ``rotary_embedding_neox_with_cache``; the
+    slots of one call must differ. ``overlap_previous`` is accepted and changes
+    nothing: the kernel reads nothing before the one before it has ended.
     """
     if key_cache is None or value_cache is None or value is None:
         raise RuntimeError("key_cache, value_cache and value must be given "

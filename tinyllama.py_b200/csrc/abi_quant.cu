@@ -283,7 +283,6 @@ int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args, void* s
     p.block_size = with_cache ? (int)block_size : 1;
     p.block_shift = shift_of(p.block_size);
     p.eps = eps;
-    p.overlap = (flags & TLB_ROPE_OVERLAP_PREVIOUS) != 0;
     const bool vec = head_size % 16 == 0 && rot_dim % 16 == 0 &&
                      vec_ok(dtype,
                             {query_out, key_out, query, key, value, query_weight, key_weight,

@@ -216,7 +216,6 @@ struct QuantCacheParams {
     int block_shift;           // log2(block_size), -1 when it is no power of two
     float eps;
     bool positions64, slots64;
-    bool overlap;              // the kernel before writes no positions, slots, tables, weights
 };
 struct DequantParams {
     void* key_out;

@@ -24,11 +24,11 @@ template <typename T> struct Same {
 };
 // Launches that may begin while the kernel before them on the stream ends
 // (programmatic stream serialization). Their kernels wait for it
-// (grid_dependency_wait) before they touch memory, or before they touch what
-// an `overlap` flag does not except; what is saved is the launch itself.
-// They let the next launch begin (grid_launch_dependents) only after that wait:
-// what an `overlap` flag of the next kernel excepts may have been written by
-// the kernel before this one, which is then complete.
+// (grid_dependency_wait) before they touch memory, the decode kernel with its
+// `overlap` flag before it touches anything but lengths and tables; what is saved
+// is the launch itself. They let the next launch begin (grid_launch_dependents)
+// only after that wait: what the next kernel reads early may have been written
+// by the kernel before this one, which is then complete.
 template <typename... Args>
 cudaError_t launch_early(void (*kernel)(Args...), dim3 grid, int threads, size_t smem,
                          cudaStream_t stream, typename Same<Args>::type... args) {

@@ -511,7 +511,6 @@ __device__ __forceinline__ void turn_pair(float x, float y, float c, float s, fl
 
 template <typename T, typename C, int LANES>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) qk_norm_rope_kernel(const QuantCacheParams p, int parts) {
-    if (!p.overlap) grid_dependency_wait();
     constexpr int GROUPS = 32 / LANES, STEP = GROUPS * kRows;
     const int lane = threadIdx.x & 31, grp = lane / LANES, sub = lane % LANES;
     const uint32_t mask = group_mask<LANES>();
