@@ -154,3 +154,44 @@ def test_a_module_that_does_not_compile_leaves_the_build_whole(built_lib, monkey
     assert B.build() == B.LIB_PATH and B.LIB_PATH.stat().st_mtime == before
     assert "does not compile" in capsys.readouterr().err
     assert not module.exists()
+
+
+BAD = 1
+
+
+def call(entry, *fields):
+    name, pack = entry
+    return getattr(_lib.load(), name)(pack(*fields), None)
+
+
+def refused(rc):
+    return rc == BAD and "aligned to the element size" in _lib.last_error()
+
+
+@no_device
+def test_pointers_off_their_elements_are_refused(built_lib):
+    """Index arrays, tables, lengths and caches of 16-bit values: off their elements
+    they are refused before any CUDA call, on them they are not."""
+    for dtype, step in ((I32, 4), (I64, 8)):
+        for off in (0, 1, 2, 4, 8):
+            bad = off % step != 0
+            at = P + off
+            assert refused(call(_lib.QUANTIZED_WRITE, P, P, P, P, P, P, at, dtype, 4, 2, 128, 10,
+                                16, 256, 256, BF16, E4M3)) == bad
+            assert refused(call(_lib.DEQUANTIZE, P, P, P, P, P, P, at, dtype, 4, 2, 128, 10, 16,
+                                BF16, I8)) == bad
+            for pos, slots in ((at, P), (P, at)):
+                assert refused(call(_lib.QK_NORM_ROPE, P, 0, pos, P, P, P, P, P, P, P, P, P, slots,
+                                    0, P, dtype, dtype, 0, 4, 16, 2, 128, 64, 128, 10, 16, 2048,
+                                    256, 256, BF16, E4M3, 0, 1e-6)) == bad
+    for off in (0, 1, 2, 4):
+        for kc, vc, tables in ((P + off, P, P), (P, P + off, P), (P, P, P + off)):
+            rc = call(_lib.QK_NORM_ROPE, P, 0, P, P, P, P, P, P, kc, vc, 0, 0, 0, tables, P, I64, I64,
+                      4, 4, 16, 2, 128, 64, 128, 10, 16, 2048, 256, 256, BF16, BF16, 0, 1e-6)
+            assert refused(rc) == (off % (4 if tables != P else 2) != 0)
+        for i in range(3):
+            arrays = [P, P, P]
+            arrays[i] += off
+            rc = call(_lib.SCORED_ATTENTION, P, P, P, P, P, P, *arrays, 0, 0, 4, 16, 2, 128, 10, 16,
+                      4, 2048, 0, BF16, E4M3, 0, 0.1, 0.0)
+            assert refused(rc) == (off % 4 != 0)

@@ -37,6 +37,7 @@ bool is_float(int dtype) {
 }
 bool is_8bit(int dtype) { return dtype == TLB_FLOAT8_E4M3 || dtype == TLB_INT8; }
 bool is_index(int dtype) { return dtype == TLB_INT32 || dtype == TLB_INT64; }
+int index_bytes(int dtype) { return dtype == TLB_INT64 ? 8 : 4; }
 int elem_bytes(int dtype) { return dtype == TLB_FLOAT32 ? 4 : is_8bit(dtype) ? 1 : 2; }
 
 // log2 of a power of two, -1 for other numbers.
@@ -104,7 +105,7 @@ int tlb_reshape_and_cache_quantized(const tlb_quantized_write_args* args, void* 
     if (num_tokens == 0) return TLB_OK;
     TLB_REQUIRE(key && value && slots, "tensor pointers must not be null");
     const int e = elem_bytes(dtype);
-    TLB_REQUIRE(aligned(key, e) && aligned(value, e),
+    TLB_REQUIRE(aligned(key, e) && aligned(value, e) && aligned(slots, index_bytes(slot_dtype)),
                 "tensor pointers must be aligned to the element size");
     tlb::QuantCacheParams p{};
     p.key = key;
@@ -157,7 +158,8 @@ int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream) {
     if (num_ids == 0) return TLB_OK;
     TLB_REQUIRE(key_out && value_out && block_ids, "tensor pointers must not be null");
     const int e = elem_bytes(dtype);
-    TLB_REQUIRE(aligned(key_out, e) && aligned(value_out, e),
+    TLB_REQUIRE(aligned(key_out, e) && aligned(value_out, e) &&
+                    aligned(block_ids, index_bytes(id_dtype)),
                 "tensor pointers must be aligned to the element size");
     tlb::DequantParams p{};
     p.key_out = key_out;
@@ -251,6 +253,12 @@ int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args, void* s
     for (const void* q : {(const void*)query_out, (const void*)key_out, query, key, value,
                           query_weight, key_weight, cos_sin_cache})
         TLB_REQUIRE(aligned(q, e), "tensor pointers must be aligned to the element size");
+    TLB_REQUIRE(aligned(positions, index_bytes(pos_dtype)) && aligned(block_tables, 4) &&
+                    (!with_cache || !slots || aligned(slots, index_bytes(slot_dtype))),
+                "tensor pointers must be aligned to the element size");
+    if (with_cache && !is_8bit(cache_dtype))
+        TLB_REQUIRE(aligned(key_cache, e) && aligned(value_cache, e),
+                    "tensor pointers must be aligned to the element size");
     tlb::QuantCacheParams p{};
     p.out = query_out;
     p.key_out = key_out;
@@ -400,7 +408,8 @@ int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stre
                 "8-bit caches need key_scales and value_scales");
     const int e = elem_bytes(dtype), ce = elem_bytes(cache_dtype);
     TLB_REQUIRE(aligned(query, e) && aligned(out, e) && aligned(key_cache, ce) &&
-                    aligned(value_cache, ce),
+                    aligned(value_cache, ce) && aligned(block_tables, 4) && aligned(seq_lens, 4) &&
+                    aligned(alibi_slopes, 4),
                 "tensor pointers must be aligned to the element size");
     const size_t workspace_bytes = args->workspace_bytes > 0 ? (size_t)args->workspace_bytes : 0;
     namespace sc = tlb::scored;
