@@ -253,3 +253,53 @@ def test_norm_reads_nothing_before_the_kernel_before_it_ends(kind):
     for a, b in zip(steps(False), steps(True), strict=True):
         assert torch.equal(a, b)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", [E4M3, INT8, BF16], ids=short)
+def test_the_short_way_takes_the_ordinary_calls(kind, monkeypatch):
+    """Each cscr._fast function answers an ordinary call itself, with what the op's
+    Python code answers."""
+    fast, h, kvh, d, bs, n = _lib.fast, 8, 2, 64, 16, 20
+    c = Case([70, 33], h, kvh, d, bs, BF16, kind, seed=30)
+    c.run()  # the stream's scratch
+    g = torch.Generator(device="cuda").manual_seed(31)
+    q, k, v = (torch.randn(n, heads * d, generator=g, device="cuda").to(BF16)
+               for heads in (h, kvh, kvh))
+    w, table = (torch.randn(*s, generator=g, device="cuda").to(BF16) for s in ((d,), (64, d)))
+    pos, slots = torch.arange(n, device="cuda"), torch.arange(n, device="cuda").flip(0)
+    ids = torch.arange(3, dtype=torch.int32, device="cuda")
+    eight = kind != BF16
+    new = lambda: [None if x is None else x.clone() for x in (c.k, c.v, c.ks, c.vs)]
+
+    def calls(direct):
+        out = []
+        if direct:
+            out.append(fast.attention(c.q, c.k, c.v, c.ks, c.vs, c.tables, c.lens, c.scale, 0.0,
+                                      None, 9, False))
+        else:
+            out.append(c.run(window=9))
+        kv = new()
+        if direct:
+            out.append(fast.norm(pos, q, k, v, w, w, 1e-6, kv[0], kv[1], slots, d, table, None,
+                                 kv[2], kv[3], False))
+            out += fast.norm(pos, q, k, None, w, w, 1e-6, None, None, None, d, table, None, None,
+                             None, False)
+        else:
+            out.append(PE.qk_norm_rotary_embedding_neox_with_cache(
+                pos, q, k, v, w, w, 1e-6, kv[0], kv[1], slots, d, table, key_scales=kv[2],
+                value_scales=kv[3]))
+            out += PE.qk_norm_rotary_embedding_neox(pos, q, k, w, w, 1e-6, d, table)
+        if eight:
+            if direct:
+                assert fast.write(v, k, *kv, pos) is True
+                out += fast.read(*kv, ids, F16)
+            else:
+                C.reshape_and_cache_quantized(v, k, *kv, pos)
+                out += C.dequantize_blocks(*kv, ids, F16)
+        return out + [x.view(torch.uint8) for x in kv if x is not None]
+
+    short_way = calls(True)
+    assert all(x is not None for x in short_way)
+    monkeypatch.setattr(_lib, "fast", None)
+    for a, b in zip(short_way, calls(False), strict=True):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
