@@ -12,6 +12,7 @@ import torch
 from cscr import _lib
 from cscr import attention as A
 from cscr import pos_encoding as PE
+from paged_decode.layers import PagedAttentionWithQKNorm
 
 P = 1 << 12  # stands in for an aligned device pointer; nothing is dereferenced
 CUDA_ERROR = 3
@@ -195,3 +196,13 @@ def test_pointers_off_their_elements_are_refused(built_lib):
             rc = call(_lib.SCORED_ATTENTION, P, P, P, P, P, P, *arrays, 0, 0, 4, 16, 2, 128, 10, 16,
                       4, 2048, 0, BF16, E4M3, 0, 0.1, 0.0)
             assert refused(rc) == (off % 4 != 0)
+
+
+def test_a_prompt_of_no_tokens():
+    m = PagedAttentionWithQKNorm(4, 64, 0.125, 64)
+    x, none = torch.zeros(0, 4, 64), torch.zeros(0, dtype=torch.int32)
+    kv = torch.zeros(0, 2, 64)
+    cache = torch.zeros(3, 2, 16, 64)
+    out = m.prompt(none, x, kv, kv, cache, cache, none, none.view(0, 1),
+                   torch.zeros(1, dtype=torch.int32), none)
+    assert out.shape == x.shape and out.dtype == x.dtype

@@ -199,6 +199,8 @@ class PagedAttentionWithQKNorm(PagedAttentionWithRoPE):
         cache in the query dtype: pass no more columns than the contexts need."""
         if self.softcap or self.window:
             raise NotImplementedError("prompt chunks have plain scores: no softcap, no window")
+        if query.size(0) == 0:  # a step without prompt tokens
+            return torch.empty_like(query)
         query = self._norm_rope_write(positions, query, key, value, key_cache, value_cache,
                                       slot_mapping, None, key_scales, value_scales)
         tables = block_tables.to(torch.int32).contiguous()
