@@ -463,6 +463,20 @@ typedef struct tlb_dequantize_args {
 TLB_API int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The block ids that prompt chunks over 8-bit caches read back, and the table by
+ * which tlb_paged_prefill_attention finds them afterwards: entry j of chunk c is
+ * block c * max_blocks + j of what tlb_dequantize_blocks reads for ids_out.
+ *   block_tables, ids_out, tables_out : [num_chunks, max_blocks] int32
+ *   context_lens : [num_chunks] int32
+ * Entries past a context are not looked up: they may be stale. Their id is 0,
+ * their place a hole. Holes stay holes; ids outside the pool (num_blocks) are
+ * kept for the read, which flags them, and are holes of the new table.
+ * ---------------------------------------------------------------------- */
+TLB_API int tlb_read_back_tables(const int32_t* block_tables, const int32_t* context_lens,
+                        int64_t num_chunks, int64_t max_blocks, int64_t block_size,
+                        int64_t num_blocks, int32_t* ids_out, int32_t* tables_out, void* stream);
+
+/* ------------------------------------------------------------------------
  * RMS norm of each query and key head, the NeoX rotation, and the KV-cache
  * write, in one pass (no reference counterpart; the rotation and the write are
  * those of tlb_rotary_embedding_neox and its _with_cache form).

@@ -10,6 +10,7 @@ from cscr import cache as C
 from cscr import pos_encoding as PE
 from cscr._lib import DTYPE_CODE
 from oracle import quant_oracle as Q
+from paged_decode import metadata as M
 from paged_decode import pool
 from paged_decode.layers import PagedAttentionWithQKNorm
 from test_gpu_scored_attention import Case
@@ -303,3 +304,22 @@ def test_the_short_way_takes_the_ordinary_calls(kind, monkeypatch):
     monkeypatch.setattr(_lib, "fast", None)
     for a, b in zip(short_way, calls(False), strict=True):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("chunks,width,bs", [(1, 1, 16), (3, 7, 5), (700, 513, 16)])
+def test_read_back_tables(chunks, width, bs):
+    g = torch.Generator(device="cuda").manual_seed(32)
+    nb = 90
+    tables = torch.randint(-3, nb + 3, (chunks, width), generator=g, device="cuda").int()
+    lens = torch.randint(-2, width * bs + 9, (chunks,), generator=g, device="cuda").int()
+    ids, places = M.read_back_tables(tables, lens, bs, nb)
+    at = torch.arange(chunks * width, device="cuda").view(chunks, width)
+    seen = at % width * bs < lens[:, None]
+    assert torch.equal(ids, torch.where(seen, tables, 0))
+    assert torch.equal(places, torch.where(seen & (tables >= 0) & (tables < nb), at, -1).int())
+    with pytest.raises(RuntimeError, match="int32"):
+        M.read_back_tables(tables.long(), lens, bs, nb)
+    with pytest.raises(RuntimeError, match="one row"):
+        M.read_back_tables(tables, lens.new_zeros(chunks + 1), bs, nb)
+    none, holes = M.read_back_tables(tables[:0], lens[:0], bs, nb)
+    assert none.shape == holes.shape == (0, width)

@@ -206,3 +206,22 @@ def test_a_prompt_of_no_tokens():
     out = m.prompt(none, x, kv, kv, cache, cache, none, none.view(0, 1),
                    torch.zeros(1, dtype=torch.int32), none)
     assert out.shape == x.shape and out.dtype == x.dtype
+
+
+def test_read_back_tables_refuses_before_any_cuda_call(built_lib):
+    lib = _lib.load()
+
+    def tables(bt=P, lens=P, chunks=3, width=8, bs=16, nb=30, ids=P, out=P):
+        return lib.tlb_read_back_tables(bt, lens, chunks, width, bs, nb, ids, out, None)
+
+    for kw, msg in ((dict(chunks=-1), "negative"), (dict(width=-1), "negative"),
+                    (dict(bs=0), "positive"), (dict(nb=0), "positive"),
+                    (dict(chunks=1 << 20, width=1 << 12), "supported range"),
+                    (dict(bt=0), "must not be null"), (dict(out=0), "must not be null"),
+                    (dict(lens=P + 2), "aligned"), (dict(ids=P + 1), "aligned")):
+        assert tables(**kw) == BAD and msg in _lib.last_error(), kw
+    assert tables(chunks=0) == 0 and tables(width=0) == 0
+    from paged_decode import metadata as M
+    x = torch.zeros(3, 8, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        M.read_back_tables(x, x[:, 0].contiguous(), 16, 30)

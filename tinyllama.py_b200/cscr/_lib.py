@@ -74,6 +74,7 @@ _PROTOS = {
                           _vp],
     "tlb_reshape_and_cache_quantized": [ctypes.c_char_p, _vp],
     "tlb_dequantize_blocks": [ctypes.c_char_p, _vp],
+    "tlb_read_back_tables": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
     "tlb_qk_norm_rotary_embedding_neox": [ctypes.c_char_p, _vp],
     "tlb_paged_attention_scored_workspace_size": [_i64, _i64, _i64, _i64, _i32, _i32,
                                                   ctypes.POINTER(_sz), ctypes.POINTER(_sz)],

@@ -181,6 +181,27 @@ int tlb_dequantize_blocks(const tlb_dequantize_args* args, void* stream) {
                        "dequantize_blocks");
 }
 
+int tlb_read_back_tables(const int32_t* block_tables, const int32_t* context_lens,
+                         int64_t num_chunks, int64_t max_blocks, int64_t block_size,
+                         int64_t num_blocks, int32_t* ids_out, int32_t* tables_out, void* stream) {
+    TLB_REQUIRE(num_chunks >= 0 && max_blocks >= 0, "counts must not be negative");
+    TLB_REQUIRE(block_size > 0 && num_blocks > 0, "cache sizes must be positive");
+    TLB_REQUIRE(num_chunks < (1ll << 31) && max_blocks < (1ll << 31) && block_size < (1ll << 31) &&
+                    num_chunks * max_blocks < (1ll << 31) - 1024 && num_blocks < (1ll << 31),
+                "sizes exceed the supported range");
+    if (num_chunks * max_blocks == 0) return TLB_OK;
+    TLB_REQUIRE(block_tables && context_lens && ids_out && tables_out,
+                "tensor pointers must not be null");
+    for (const void* q : {(const void*)block_tables, (const void*)context_lens,
+                          (const void*)ids_out, (const void*)tables_out})
+        TLB_REQUIRE(aligned(q, 4), "tensor pointers must be aligned to the element size");
+    return cuda_result(
+        tlb::launch_read_back_tables(block_tables, context_lens, (int)num_chunks, (int)max_blocks,
+                                     (int)block_size, num_blocks, ids_out, tables_out,
+                                     reinterpret_cast<cudaStream_t>(stream)),
+        "read_back_tables");
+}
+
 int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args, void* stream) {
     TLB_REQUIRE(args != nullptr, "args must not be null");
     void* query_out = args->query_out;

@@ -171,6 +171,12 @@ cudaError_t launch_step_metadata(const int32_t* prompt_lens, const int32_t* prom
                                  long long num_padded, int64_t* positions, int64_t* slots,
                                  cudaStream_t stream);
 
+// Ids to read back and the table over what is read (step_metadata.cu).
+cudaError_t launch_read_back_tables(const int32_t* tables, const int32_t* context_lens,
+                                    int num_chunks, int max_blocks, int block_size,
+                                    long long num_blocks, int32_t* ids, int32_t* places,
+                                    cudaStream_t stream);
+
 // Causal paged attention of prompt chunks (prefill_attention.cu).
 cudaError_t launch_prefill_attention(int dtype, int head_dim, void* out, const void* query,
                                      const void* key_cache, const void* value_cache,

@@ -92,7 +92,37 @@ __global__ void __launch_bounds__(kMetaThreads)
     }
 }
 
+// Id 0 for entries that are not looked up: the read back then loads a block that
+// is in L2 for each of them instead of storing zeros at once, which is faster
+// (8 chunks of 512 tokens, 512 columns: a prompt step of 66 against 80 us).
+__global__ void read_back_tables_kernel(const int32_t* __restrict__ tables,
+                                        const int32_t* __restrict__ context_lens, int total,
+                                        int max_blocks, int block_size, long long num_blocks,
+                                        int32_t* __restrict__ ids, int32_t* __restrict__ places) {
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+         i += (long long)gridDim.x * blockDim.x) {
+        const int c = (int)i / max_blocks, j = (int)i - c * max_blocks;
+        const bool seen = (long long)j * block_size < context_lens[c];
+        const int32_t id = seen ? tables[i] : 0;
+        ids[i] = id;
+        places[i] = seen && id >= 0 && id < num_blocks ? (int32_t)i : -1;
+    }
+}
+
 }  // namespace
+
+cudaError_t launch_read_back_tables(const int32_t* tables, const int32_t* context_lens,
+                                    int num_chunks, int max_blocks, int block_size,
+                                    long long num_blocks, int32_t* ids, int32_t* places,
+                                    cudaStream_t stream) {
+    const int total = num_chunks * max_blocks;
+    if (total <= 0) return cudaSuccess;
+    int blocks = (total + kMetaThreads - 1) / kMetaThreads;
+    if (blocks > 4 * 148) blocks = 4 * 148;
+    read_back_tables_kernel<<<blocks, kMetaThreads, 0, stream>>>(
+        tables, context_lens, total, max_blocks, block_size, num_blocks, ids, places);
+    return cudaGetLastError();
+}
 
 cudaError_t launch_step_metadata(const int32_t* prompt_lens, const int32_t* prompt_tables,
                                  int num_prompts, int prompt_max_blocks,

@@ -32,6 +32,8 @@ from cscr import attention as _C
 from cscr import cache as _Cache
 from cscr import pos_encoding as _PE
 
+from . import metadata
+
 
 class PagedAttention(nn.Module):
     def __init__(self, num_heads: int, head_size: int, scale: float):
@@ -205,16 +207,10 @@ class PagedAttentionWithQKNorm(PagedAttentionWithRoPE):
                                       slot_mapping, None, key_scales, value_scales)
         tables = block_tables.to(torch.int32).contiguous()
         if key_scales is not None:
-            # the chunks' blocks in the query dtype: entry j of chunk c is block
-            # c * max_blocks + j of what is read back. Entries past a context may
-            # be stale and are not looked up; holes, and ids outside the pool
-            # (which the read flags), are holes of the new table too.
-            num_blocks, _, block_size, _ = key_cache.shape
-            starts = torch.arange(0, tables.size(1) * block_size, block_size, device=tables.device)
-            tables = torch.where(starts < context_lens[:, None], tables, -1)
+            # the chunks' blocks in the query dtype, and the table that finds them
+            ids, tables = metadata.read_back_tables(tables, context_lens.contiguous(),
+                                                    key_cache.size(2), key_cache.size(0))
             key_cache, value_cache = _Cache.dequantize_blocks(
-                key_cache, value_cache, key_scales, value_scales, tables.view(-1), query.dtype)
-            places = torch.arange(tables.numel(), dtype=torch.int32, device=tables.device)
-            tables = torch.where((tables >= 0) & (tables < num_blocks), places.view_as(tables), -1)
+                key_cache, value_cache, key_scales, value_scales, ids.view(-1), query.dtype)
         return _C.paged_prefill_attention(query, key_cache, value_cache, tables, query_start,
                                           context_lens, self.scale, max_query_len)

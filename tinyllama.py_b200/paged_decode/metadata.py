@@ -85,6 +85,29 @@ def decode_metadata_from_tensors(context_lens: torch.Tensor, block_tables: torch
     return positions, slots
 
 
+def read_back_tables(block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int,
+                     num_blocks: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(ids, tables) for prompt chunks over 8-bit caches: the block ids to read back
+    (``cscr.cache.dequantize_blocks(..., ids.view(-1), ...)``) and the block tables
+    over what is read, both [num_chunks, max_blocks] int32. Entries past a context
+    are not looked up; holes and ids outside the pool are holes."""
+    _lib.torch_check(context_lens.is_cuda and block_tables.device == context_lens.device,
+                     "context_lens and block_tables must be tensors of one CUDA device")
+    _lib.torch_check(context_lens.dtype == torch.int32 and block_tables.dtype == torch.int32,
+                     "context_lens and block_tables must be int32")
+    _lib.torch_check(block_tables.dim() == 2 and context_lens.dim() == 1
+                     and block_tables.size(0) == context_lens.size(0)
+                     and block_tables.is_contiguous() and context_lens.is_contiguous(),
+                     "one row of contiguous block_tables for each of context_lens")
+    ids, tables = both = block_tables.new_empty((2, *block_tables.shape))
+    dev = both.device
+    with _lib.device_guard(dev):
+        _lib.check(_lib.load().tlb_read_back_tables(
+            block_tables.data_ptr(), context_lens.data_ptr(), *block_tables.shape, block_size,
+            num_blocks, ids.data_ptr(), tables.data_ptr(), _lib.stream_of(dev)))
+    return ids, tables
+
+
 @dataclass
 class StepMetadata:
     positions: torch.Tensor      # [padded] int64 (0 past num_tokens)
