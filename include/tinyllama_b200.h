@@ -428,7 +428,8 @@ TLB_API int tlb_step_metadata(const int32_t* prompt_lens, const int32_t* prompt_
  * tlb_dequantize_blocks reads blocks back: out[n] = the values of block
  * block_ids[n], [num_ids, num_kv_heads, block_size, head_size] of dtype, zeros
  * for ids < 0 or outside the cache (the latter flagged,
- * TLB_STATUS_BAD_BLOCK_ID).
+ * TLB_STATUS_BAD_BLOCK_ID). Values are rounded to dtype: in fp16 those stored
+ * for 63488 (e4m3) or 65024 (int8) and more may be infinite.
  *
  * These and the two entry points below take their arguments as a struct of
  * 64-bit fields (a binding packs it in one step); `args` is read during the call

@@ -304,7 +304,9 @@ def dequantize_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor,
                       out: tuple[torch.Tensor, torch.Tensor] | None = None
                       ) -> tuple[torch.Tensor, torch.Tensor]:
     """The values of blocks of 8-bit caches: (key blocks, value blocks), each
-    [N, KVH, block_size, D] of ``dtype`` (float16, bfloat16 or float32).
+    [N, KVH, block_size, D] of ``dtype`` (float16, bfloat16 or float32), rounded to
+    it: in float16 values stored for 63488 (float8_e4m3fn) or 65024 (int8) and more
+    may be infinite.
 
     block_ids [N] int32 or int64; a negative id (a hole of a block table) yields
     a block of zeros. A whole table can be passed as ``block_tables.view(-1)``:

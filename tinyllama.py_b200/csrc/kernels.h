@@ -281,7 +281,7 @@ struct Params {
     int num_heads;
     int num_kv_heads;
     int group;                    // query heads per kv head
-    int unit_heads;               // query heads of a unit: min(group, 16)
+    int unit_heads;               // query heads of a unit, 16 at most (unit_heads_of)
     int head_chunks;              // units per kv head
     int units_per_seq;
     int head_dim;

@@ -135,14 +135,4 @@ template <> __device__ __forceinline__ float dequantize1<int8_t>(uint32_t byte) 
     return (float)(int)(int8_t)byte;
 }
 
-// Two stored bytes (low half word) -> packed fp16 pair: exact for both types
-// (e4m3 has 4 significant bits, exponents 2^-9 .. 2^8; |int8| <= 128).
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t pair) {
-    uint32_t d;
-    asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}"
-        : "=r"(d)
-        : "r"(pair));
-    return d;
-}
-
 }  // namespace tlb
