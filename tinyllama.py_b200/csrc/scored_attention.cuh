@@ -15,8 +15,9 @@
 //    kUnitCost tiles for starting a unit, form one line, cut evenly over all
 //    warps of the grid (one CTA per SM; 12 warps for units of up to 8 heads, 8
 //    for 16). Each warp streams its contiguous part through a ring of its own
-//    (TMA boxes of a block's rows, scale bytes by cp.async) and never waits for another warp, so units of any mix of lengths keep every SM
-//    busy and a short sequence costs one warp one tile.
+//    (TMA boxes of a block's rows, scale bytes by cp.async) and never waits for
+//    another warp, so units of any mix of lengths keep every SM busy and a short
+//    sequence costs one warp one tile.
 //  * S^T = K Q^T and O^T += V^T P^T with mma.m16n8k16: the tokens (then the
 //    dims) fill m = 16 and the query heads of the kv head n = 8, so a group of
 //    8 wastes nothing; 8-bit values become fp16 in registers, exactly. bf16
@@ -37,10 +38,10 @@
 //    theirs in shared memory, CTAs through the workspace: the last CTA to
 //    publish its partial sums them all. The order of every sum is fixed, so
 //    results are the same bits on every run.
-// Measured, one B200, calls back to back: 256 sequences of 7000-8192 tokens, 14 + 2
-// heads of 64, bf16 over e4m3 (508 MB), 86 us (5.9 TB/s). 64 sequences of 128-4096
-// tokens, 16 + 2 heads of 128, bf16 over e4m3 (71.6 MB), 22.5 us: the rows stream
-// until 15 us, the joins take the rest. An L2 policy of evict_normal for the rows
+// Measured: 256 sequences of 7000-8192 tokens, 14 + 2 heads of 64, bf16 over e4m3
+// (508 MB), 90 to 97 us by box (5.6 to 5.2 TB/s; 86 us back to back on three
+// inputs). 64 sequences of 128-4096 tokens, 16 + 2 heads of 128, bf16 over e4m3
+// (71.6 MB), 22.2 us: the rows stream until 15 us, the joins take the rest. An L2 policy of evict_normal for the rows
 // cost 4 % of the latter. Without the scale bytes' copies the former, at 133 us
 // then, took 128 us; without its arithmetic 92 us.
 #pragma once
