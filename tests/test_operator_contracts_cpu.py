@@ -225,3 +225,29 @@ def test_read_back_tables_refuses_before_any_cuda_call(built_lib):
     x = torch.zeros(3, 8, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="CUDA device"):
         M.read_back_tables(x, x[:, 0].contiguous(), 16, 30)
+
+
+def test_cscr_fast_never_holds_the_address_of_freed_scratch(monkeypatch):
+    """A stream's scratch that grows or is forgotten: cscr._fast hears of it while the
+    old tensor is still held (it may take another thread's call in between)."""
+    held = []
+
+    class Fast:
+        @staticmethod
+        def scratch(device, stream, address, nbytes):
+            held.append([ref() is not None for ref in old])
+
+    monkeypatch.setattr(_lib, "fast", Fast)
+    monkeypatch.setattr(_lib, "current_device", lambda: 0)
+    monkeypatch.setattr(_lib, "stream_of", lambda device: 7)
+    monkeypatch.setattr(A, "_capturing", lambda: False)
+    monkeypatch.setattr(A, "_scored_workspaces", {})
+    old = []
+    for nbytes in (1 << 24, 1 << 25):
+        ws = A._scored_workspace(torch.zeros(1), 0, nbytes, 64)
+        assert A._scored_workspaces[(0, 7)] is ws
+        old = [weakref.ref(ws)]
+        del ws
+    A.invalidate_workspaces(0)
+    assert held == [[], [True], [True]]
+    assert old[0]() is None and not A._scored_workspaces

@@ -53,10 +53,10 @@ def invalidate_workspaces(device_index: int) -> None:
     for (dev, _stream), ws in _workspaces.items():
         if dev == device_index:
             ws.clean = 0
+    if _lib.fast is not None:  # before they go, as in _scored_workspace
+        _lib.fast.scratch(device_index, 0, 0, 0)
     for key in [k for k in _scored_workspaces if k[0] == device_index]:
         del _scored_workspaces[key]
-    if _lib.fast is not None:
-        _lib.fast.scratch(device_index, 0, 0, 0)
 
 
 def workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -330,9 +330,11 @@ def _scored_workspace(query: torch.Tensor, index: int, nbytes: int, zeroed: int)
     key = (index, _lib.stream_of(query.device))
     ws = _scored_workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _scored_workspaces[key] = query.new_zeros(max(nbytes, 1 << 24), dtype=torch.uint8)
+        ws = query.new_zeros(max(nbytes, 1 << 24), dtype=torch.uint8)
+        # before the old one goes: another thread's short call may be next to use it
         if _lib.fast is not None:
             _lib.fast.scratch(*key, ws.data_ptr(), ws.numel())
+        _scored_workspaces[key] = ws
     return ws
 
 
