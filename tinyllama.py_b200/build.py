@@ -16,7 +16,6 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
-import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -74,7 +73,9 @@ def _lib_up_to_date() -> bool:
 
 
 def _torch_version() -> str:
-    return importlib.metadata.version("torch")
+    import torch
+
+    return str(torch.__version__)
 
 
 def _fast_up_to_date() -> bool:
@@ -108,8 +109,9 @@ def _compile_fast() -> None:
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-isystem{p}" for p in cpp_extension.include_paths()),
            f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{cuda / 'include'}",
-           f"-I{INCLUDE}", f'-DTLB_TORCH_VERSION="{_torch_version()}"', str(FAST_SRC), "-o", str(tmp), f"-L{lib}", "-ltorch_python", "-ltorch",
-           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+           f"-I{INCLUDE}", f'-DTLB_TORCH_VERSION="{_torch_version()}"', str(FAST_SRC), "-o",
+           str(tmp), f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"compiling {FAST_SRC.name} failed:\n{res.stdout}\n{res.stderr}")

@@ -369,8 +369,8 @@ int plan_attention(const void* out, const void* query, const void* key_cache,
     pl->rows = (uint64_t)num_blocks * num_kv_heads * block_size;
     // the tensor-core kernel stores four outputs at once
     pl->tc = tlb::attn::tc_supported(dtype, (int)head_dim, pl->group, (int)block_size) &&
-             aligned(out, 8) && aligned(query, 16) && aligned(key_cache, 16) && aligned(value_cache, 16) &&
-             pl->rows < (1ull << 31);
+             aligned(out, 8) && aligned(query, 16) && aligned(key_cache, 16) &&
+             aligned(value_cache, 16) && pl->rows < (1ull << 31);
     pl->ws = WsLayout{};
     if (!pl->tc) return TLB_OK;
     int dev;

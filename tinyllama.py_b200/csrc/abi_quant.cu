@@ -274,12 +274,12 @@ int tlb_qk_norm_rotary_embedding_neox(const tlb_qk_norm_rope_args* args, void* s
     for (const void* q : {(const void*)query_out, (const void*)key_out, query, key, value,
                           query_weight, key_weight, cos_sin_cache})
         TLB_REQUIRE(aligned(q, e), "tensor pointers must be aligned to the element size");
-    TLB_REQUIRE(aligned(positions, index_bytes(pos_dtype)) && aligned(block_tables, 4) &&
-                    (!with_cache || !slots || aligned(slots, index_bytes(slot_dtype))),
+    const int ce = elem_bytes(cache_dtype);
+    TLB_REQUIRE(aligned(positions, index_bytes(pos_dtype)) &&
+                    (!with_cache || (aligned(key_cache, ce) && aligned(value_cache, ce) &&
+                                     (slots ? aligned(slots, index_bytes(slot_dtype))
+                                            : aligned(block_tables, 4)))),
                 "tensor pointers must be aligned to the element size");
-    if (with_cache && !is_8bit(cache_dtype))
-        TLB_REQUIRE(aligned(key_cache, e) && aligned(value_cache, e),
-                    "tensor pointers must be aligned to the element size");
     tlb::QuantCacheParams p{};
     p.out = query_out;
     p.key_out = key_out;
@@ -474,7 +474,8 @@ int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stre
     const bool fast =
         sc::fast_supported(dtype, cache_dtype, (int)head_dim, (int)block_size) &&
         aligned(out, 4) && aligned(query, 16) && query_stride % 8 == 0 &&
-        aligned(key_cache, 16) && aligned(value_cache, 16) && aligned(key_scales, 4) && aligned(value_scales, 4) &&
+        aligned(key_cache, 16) && aligned(value_cache, 16) && aligned(key_scales, 4) &&
+        aligned(value_scales, 4) &&
         num_blocks * num_kv_heads < (1ll << 31) / block_size && tiles < (1ll << 30);
     if (!fast)
         return cuda_result(sc::launch_generic(dtype, cache_dtype, p, st), "paged attention");

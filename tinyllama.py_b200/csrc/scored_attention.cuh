@@ -41,9 +41,10 @@
 // Measured: 256 sequences of 7000-8192 tokens, 14 + 2 heads of 64, bf16 over e4m3
 // (508 MB), 90 to 97 us by box (5.6 to 5.2 TB/s; 86 us back to back on three
 // inputs). 64 sequences of 128-4096 tokens, 16 + 2 heads of 128, bf16 over e4m3
-// (71.6 MB), 22.2 us: the rows stream until 15 us, the joins take the rest. An L2 policy of evict_normal for the rows
-// cost 4 % of the latter. Without the scale bytes' copies the former, at 133 us
-// then, took 128 us; without its arithmetic 92 us.
+// (71.6 MB), 22.2 us: the rows stream until 15 us, the joins take the rest. An L2
+// policy of evict_normal for the rows cost 4 % of the latter. Without the scale
+// bytes' copies the former, at 133 us then, took 128 us; without its arithmetic
+// 92 us.
 #pragma once
 
 #include <atomic>
