@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(256) dequantize_any_kernel(const DequantParams
 // its weights while it stays with queries or with keys; kRows of its rows are
 // read while kRows are worked on, with the next token's position and slot: 16383
 // fp16 tokens of 32 + 8 heads of 128, half of each rotated (338 MB), take 61.8 us
-// (62.7 and 64.6 on two other boxes; on the first, 66.6 without the next position
+// (62.7 and 64.6 on two other B200s; on the first, 66.6 without the next position
 // and slot, 79 one buffer of rows). Four neighbouring tokens for the four groups
 // of a warp, which would make the kind of row uniform, took 71.4 us. Other widths
 // and alignments: a warp for each row, by element.

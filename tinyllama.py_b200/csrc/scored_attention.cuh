@@ -39,7 +39,7 @@
 //    publish its partial sums them all. The order of every sum is fixed, so
 //    results are the same bits on every run.
 // Measured: 256 sequences of 7000-8192 tokens, 14 + 2 heads of 64, bf16 over e4m3
-// (508 MB), 90 to 97 us by box (5.6 to 5.2 TB/s; 86 us back to back on three
+// (508 MB), 90 to 97 us on three B200s (5.6 to 5.2 TB/s; 86 us back to back on three
 // inputs). 64 sequences of 128-4096 tokens, 16 + 2 heads of 128, bf16 over e4m3
 // (71.6 MB), 22.2 us: the rows stream until 15 us, the joins take the rest. An L2
 // policy of evict_normal for the rows cost 4 % of the latter. Without the scale
