@@ -570,6 +570,78 @@ typedef struct tlb_scored_attention_args {
 
 TLB_API int tlb_paged_attention_scored(const tlb_scored_attention_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Rows in 8 bits for tlb_matmul_quantized (no reference counterpart).
+ *
+ * A row of `width` values is stored as float8_e4m3fn values and a scale byte 2^E
+ * (biased exponent, E8M0) for each 128 of them; the last group of a row may be
+ * shorter. E is the smallest with max|x| <= 448 * 2^E over the group's finite
+ * values, E in [-126, 127]; the values are x / 2^E rounded to nearest even,
+ * infinities saturated, NaN kept: the rows of the 8-bit caches, by groups of 128.
+ *
+ * op:
+ *   TLB_ROWS_PLAIN        : the rows of x [num_rows, width]
+ *   TLB_ROWS_SILU_AND_MUL : x [num_rows, 2 * width] holds gate and up:
+ *                           gate / (1 + exp(-gate)) * up
+ *   TLB_ROWS_RMS_NORM     : h = x, or x + residual rounded to dtype and written to
+ *                           residual_out (which may be residual or x itself) when
+ *                           residual is not NULL; h * rsqrt(mean(h^2) + eps) * weight
+ * in fp32 with no rounding before the one to 8 bits.
+ *   out : [num_rows, width] dense;  scales : [num_rows, ceil(width / 128)] dense
+ *   x, residual, residual_out : rows their strides (in elements) apart
+ *   weight : [width] of dtype
+ * ---------------------------------------------------------------------- */
+#define TLB_ROWS_PLAIN 0
+#define TLB_ROWS_SILU_AND_MUL 1
+#define TLB_ROWS_RMS_NORM 2
+
+typedef struct tlb_quantize_rows_args {
+    void* out;
+    void* scales;
+    void* residual_out;
+    const void* x;
+    const void* residual;
+    const void* weight;
+    int64_t op, num_rows, width, x_stride, residual_stride, residual_out_stride, dtype;
+    double eps;
+} tlb_quantize_rows_args;
+
+TLB_API int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Product of 8-bit rows with 8-bit weights (no reference counterpart):
+ *   out[t, n] = sum_k x[t, k] 2^xs[t, k/128] * w[n, k] 2^ws[n/128, k/128] + bias[n]
+ * with fp32 sums and one rounding to out_dtype (float16, bfloat16 or float32).
+ *   x             : [num_tokens, width] float8_e4m3fn, rows x_stride apart
+ *   x_scales      : [num_tokens, ceil(width / 128)] scale bytes, rows
+ *                   x_scales_stride apart
+ *   weight        : [features, width] float8_e4m3fn, rows weight_stride apart
+ *   weight_scales : [ceil(features / 128), ceil(width / 128)] scale bytes, rows
+ *                   weight_scales_stride apart
+ *   bias          : [features] of out_dtype, or NULL
+ *   out           : rows out_stride apart
+ * A scale byte b stands for 2^(b - 127), 255 for NaN. The exponents of a product's
+ * two scales may add up to -120 .. 110; results past fp32 are infinite or 0.
+ * The tensor-core kernel wants x and weight on 16-byte boundaries with strides that
+ * are multiples of 16; others go to a kernel for any alignment.
+ * flags: TLB_PRODUCT_OVERLAP_PROLOGUE: the kernel before this one on the stream
+ * writes neither weight nor weight_scales, which may then be read while it ends.
+ * ---------------------------------------------------------------------- */
+#define TLB_PRODUCT_OVERLAP_PROLOGUE 0x1u
+
+typedef struct tlb_matmul_quantized_args {
+    void* out;
+    const void* x;
+    const void* x_scales;
+    const void* weight;
+    const void* weight_scales;
+    const void* bias;
+    int64_t num_tokens, width, features, x_stride, x_scales_stride, weight_stride;
+    int64_t weight_scales_stride, out_stride, out_dtype, flags;
+} tlb_matmul_quantized_args;
+
+TLB_API int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

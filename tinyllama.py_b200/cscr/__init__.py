@@ -7,6 +7,8 @@ backed by libtinyllama_b200.so, so ``from cscr import attention as _C`` in
 src/model_executor/layers/attention.py:4-5 and ``from cscr import cache`` in
 src/core/cache_engine.py:7 resolve here unchanged. Importing the package does
 not load the CUDA library; the first op call does.
+
+``cscr.linear`` (not in the reference) has the projections in 8 bits.
 """
 
-__all__ = ["attention", "cache", "pos_encoding"]
+__all__ = ["attention", "cache", "linear", "pos_encoding"]

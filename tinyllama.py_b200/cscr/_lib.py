@@ -79,6 +79,8 @@ _PROTOS = {
     "tlb_paged_attention_scored_workspace_size": [_i64, _i64, _i64, _i64, _i32, _i32,
                                                   ctypes.POINTER(_sz), ctypes.POINTER(_sz)],
     "tlb_paged_attention_scored": [ctypes.c_char_p, _vp],
+    "tlb_quantize_rows": [ctypes.c_char_p, _vp],
+    "tlb_matmul_quantized": [ctypes.c_char_p, _vp],
 }
 _RESTYPES = {"tlb_last_error": ctypes.c_char_p, "tlb_version": ctypes.c_char_p}
 
@@ -149,6 +151,8 @@ QUANTIZED_WRITE = ("tlb_reshape_and_cache_quantized", struct.Struct("=17q").pack
 DEQUANTIZE = ("tlb_dequantize_blocks", struct.Struct("=15q").pack)
 QK_NORM_ROPE = ("tlb_qk_norm_rotary_embedding_neox", struct.Struct("=32qd").pack)
 SCORED_ATTENTION = ("tlb_paged_attention_scored", struct.Struct("=23q2d").pack)
+QUANTIZE_ROWS = ("tlb_quantize_rows", struct.Struct("=13qd").pack)
+MATMUL_QUANTIZED = ("tlb_matmul_quantized", struct.Struct("=16q").pack)
 
 
 def _load_fast():

@@ -1,0 +1,134 @@
+// C ABI of the 8-bit rows and their product: argument checks, path choice and
+// launches (contract in tinyllama_b200.h).
+#include <cstdarg>
+#include <cstdio>
+#include <initializer_list>
+
+#include <cudaTypedefs.h>
+
+#include "kernels.h"
+#include "tinyllama_b200.h"
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    tlb::set_last_error(buf);
+    return code;
+}
+int cuda_result(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return TLB_OK;
+    return fail(TLB_ERR_CUDA, "launching %s: %s (%s)", what, cudaGetErrorString(e),
+                cudaGetErrorName(e));
+}
+
+#define TLB_REQUIRE(cond, ...)                                           \
+    do {                                                                 \
+        if (!(cond)) return fail(TLB_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
+    } while (0)
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+bool is_float(int64_t dtype) {
+    return dtype == TLB_FLOAT32 || dtype == TLB_FLOAT16 || dtype == TLB_BFLOAT16;
+}
+int elem_bytes(int64_t dtype) { return dtype == TLB_FLOAT32 ? 4 : 2; }
+
+int sm_count(int* sms) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+    return cuda_result(e, "a device query");
+}
+
+constexpr int64_t kGroup = 128;
+
+}  // namespace
+
+extern "C" {
+
+int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream) {
+    TLB_REQUIRE(args != nullptr, "args must not be null");
+    const tlb_quantize_rows_args& a = *args;
+    TLB_REQUIRE(a.op == TLB_ROWS_PLAIN || a.op == TLB_ROWS_SILU_AND_MUL ||
+                    a.op == TLB_ROWS_RMS_NORM,
+                "unknown op");
+    TLB_REQUIRE(is_float(a.dtype), "dtype must be float16, bfloat16 or float32");
+    TLB_REQUIRE(a.num_rows >= 0, "num_rows must not be negative");
+    TLB_REQUIRE(a.width > 0, "width must be positive");
+    TLB_REQUIRE(a.num_rows < (1ll << 40) && a.width < (1ll << 30), "sizes exceed the supported range");
+    const bool norm = a.op == TLB_ROWS_RMS_NORM;
+    TLB_REQUIRE(norm || (!a.residual && !a.weight), "residual and weight belong to the norm");
+    TLB_REQUIRE(!norm || a.eps >= 0, "eps must not be negative");
+    if (a.num_rows == 0) return TLB_OK;
+    TLB_REQUIRE(a.out && a.scales && a.x && (!norm || a.weight) && (!a.residual || a.residual_out),
+                "tensor pointers must not be null");
+    const int e = elem_bytes(a.dtype);
+    bool vec = a.width % kGroup == 0 && aligned(a.out, 8);
+    for (const void* p : {a.x, a.residual, a.weight, (const void*)(a.residual ? a.residual_out : nullptr)}) {
+        TLB_REQUIRE(!p || aligned(p, e), "tensor pointers must be aligned to the element size");
+        vec = vec && (!p || aligned(p, 16));
+    }
+    vec = vec && a.x_stride * e % 16 == 0 &&
+          (!a.residual || (a.residual_stride * e % 16 == 0 && a.residual_out_stride * e % 16 == 0));
+    tlb::RowQuantParams p{};
+    p.out = a.out;
+    p.scales = static_cast<uint8_t*>(a.scales);
+    p.residual_out = a.residual_out;
+    p.x = a.x;
+    p.residual = a.residual;
+    p.weight = a.weight;
+    p.num_rows = a.num_rows;
+    p.x_stride = a.x_stride;
+    p.residual_stride = a.residual_stride;
+    p.residual_out_stride = a.residual_out_stride;
+    p.width = (int)a.width;
+    p.op = (int)a.op;
+    p.eps = (float)a.eps;
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    return cuda_result(tlb::launch_quantize_rows((int)a.dtype, p, sms, vec,
+                                                 reinterpret_cast<cudaStream_t>(stream)),
+                       "quantize_rows");
+}
+
+int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
+    TLB_REQUIRE(args != nullptr, "args must not be null");
+    const tlb_matmul_quantized_args& a = *args;
+    TLB_REQUIRE(is_float(a.out_dtype), "out dtype must be float16, bfloat16 or float32");
+    TLB_REQUIRE(a.num_tokens >= 0 && a.features >= 0, "num_tokens and features must not be negative");
+    TLB_REQUIRE(a.width > 0, "width must be positive");
+    TLB_REQUIRE(a.num_tokens < (1ll << 31) - 1024 && a.features < (1ll << 31) - 1024 &&
+                    a.width < (1ll << 30),
+                "sizes exceed the supported range");
+    TLB_REQUIRE((a.flags & ~(int64_t)TLB_PRODUCT_OVERLAP_PROLOGUE) == 0, "unknown flags");
+    if (a.num_tokens == 0 || a.features == 0) return TLB_OK;
+    TLB_REQUIRE(a.out && a.x && a.x_scales && a.weight && a.weight_scales,
+                "tensor pointers must not be null");
+    const int e = elem_bytes(a.out_dtype);
+    TLB_REQUIRE(aligned(a.out, e) && (!a.bias || aligned(a.bias, e)),
+                "tensor pointers must be aligned to the element size");
+    tlb::ProductParams p{};
+    p.out = a.out;
+    p.x = static_cast<const uint8_t*>(a.x);
+    p.x_scales = static_cast<const uint8_t*>(a.x_scales);
+    p.weight = static_cast<const uint8_t*>(a.weight);
+    p.weight_scales = static_cast<const uint8_t*>(a.weight_scales);
+    p.bias = a.bias;
+    p.num_tokens = a.num_tokens;
+    p.features = a.features;
+    p.x_stride = a.x_stride;
+    p.x_scales_stride = a.x_scales_stride;
+    p.weight_stride = a.weight_stride;
+    p.weight_scales_stride = a.weight_scales_stride;
+    p.out_stride = a.out_stride;
+    p.width = (int)a.width;
+    return cuda_result(
+        tlb::launch_product_any((int)a.out_dtype, p, reinterpret_cast<cudaStream_t>(stream)),
+        "matmul_quantized");
+}
+
+}  // extern "C"

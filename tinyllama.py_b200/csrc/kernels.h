@@ -329,6 +329,38 @@ cudaError_t launch_generic(int dtype, int cache_dtype, const Params& p, cudaStre
 
 }  // namespace scored
 
+// ------------------------------------------- 8-bit rows and their product
+struct RowQuantParams {
+    void* out;                 // [rows, width] e4m3
+    uint8_t* scales;           // [rows, ceil(width / 128)] exponent bytes
+    void* residual_out;
+    const void* x;
+    const void* residual;      // null: none
+    const void* weight;        // [width] (norm)
+    long long num_rows;
+    long long x_stride, residual_stride, residual_out_stride;
+    int width;
+    int op;                    // TLB_ROWS_*
+    float eps;
+};
+// `vec`: pointers, strides and the width allow 16-byte accesses and whole groups.
+cudaError_t launch_quantize_rows(int dtype, const RowQuantParams& p, int sms, bool vec,
+                                 cudaStream_t stream);
+
+struct ProductParams {
+    void* out;                 // [tokens, features], rows out_stride apart
+    const uint8_t* x;          // [tokens, width] e4m3
+    const uint8_t* x_scales;   // [tokens, groups] exponent bytes
+    const uint8_t* weight;     // [features, width] e4m3
+    const uint8_t* weight_scales;  // [ceil(features / 128), groups]
+    const void* bias;          // [features] of the output type, or null
+    long long num_tokens, features;
+    long long x_stride, x_scales_stride, weight_stride, weight_scales_stride, out_stride;
+    int width;
+};
+// Any shape and alignment, on the CUDA cores.
+cudaError_t launch_product_any(int out_dtype, const ProductParams& p, cudaStream_t stream);
+
 // ------------------------------------------------------------ block copies
 constexpr int kCopyMaxCaches = 128;
 constexpr int kCopyMaxPairs = 1024;

@@ -1,0 +1,286 @@
+// Rows in 8 bits for the block-scaled product: plain rows, the gated activation
+// silu(gate) * up, and the RMS norm with the residual's addition.
+//
+// A row of K values is held as K e4m3 values and a power-of-two scale for each
+// 128 of them (the last group of a row may be shorter): the format of the 8-bit
+// cache rows, with groups in the place of heads. All three stream their input
+// once and are bounded by HBM; what they compute stays in the registers of the
+// lanes that read it until it is quantised.
+//
+// A lane holds eight neighbouring values, so a group is 16 lanes and its largest
+// magnitude takes four shuffles; a warp reads 512 bytes of a 16-bit row and
+// stores 256 in one access each.
+#include "kernels.h"
+#include "quant_rows.cuh"
+
+namespace tlb {
+
+namespace {
+
+constexpr int kGroup = 128;
+constexpr int kLanes = kGroup / 8;
+
+// Sum that keeps subnormal operands and results (the build flushes them
+// elsewhere): the residual of bf16 or fp32 may hold values below 2^-126.
+__device__ __forceinline__ float add_keep(float a, float b) {
+    float d;
+    asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// silu(g) * u. exp(-|g|) never overflows; values below 2^-126 may come out as 0.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+    const float e = __expf(-fabsf(g));
+    return __fdividef(g < 0.f ? g * e : g, 1.f + e) * u;
+}
+
+// Eight fp32 values of a lane -> their 8 stored bytes, and the scale byte of the
+// 16 lanes' group.
+__device__ __forceinline__ uint2 quantize_group(const float (&f)[8], uint32_t mask,
+                                                uint32_t& byte) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    top = group_max<kLanes>(top, mask);
+    if (top < 0x7f800000u) {
+        byte = scale_byte<E4M3>(top);
+    } else {  // infinities or NaN in the group: the scale comes from the others
+        byte = scale_byte<E4M3>(group_max<kLanes>(max_finite8(f), mask));
+    }
+    return quantized8<E4M3, false>(f, inverse_scale(byte));
+}
+
+// ------------------------------------------------- plain rows, gated activation
+// Flat over the eight-value pieces of all rows (K a multiple of 128, so a group
+// is half a warp wherever it lies), kSteps pieces of a lane in flight.
+template <typename T, bool kSilu, int kSteps>
+__global__ void __launch_bounds__(256) quantize_pieces_kernel(const RowQuantParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const unsigned row_pieces = p.width / 8;
+    const long long pieces = p.num_rows * row_pieces;
+    const uint32_t mask = group_mask<kLanes>();
+    const long long step = (long long)gridDim.x * 256 * kSteps;
+    for (long long base = (long long)blockIdx.x * 256 * kSteps + threadIdx.x;
+         base - threadIdx.x < pieces; base += step) {
+        Raw8<T> x[kSteps], u[kSilu ? kSteps : 1];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const long long i = base + s * 256;
+            x[s].zero();
+            if constexpr (kSilu) u[s].zero();
+            if (i < pieces) {
+                int rest;
+                const long long r = divide(i, (int)row_pieces, rest);
+                const T* src = reinterpret_cast<const T*>(p.x) + r * p.x_stride + (long long)rest * 8;
+                x[s].load_stream(src);
+                if constexpr (kSilu) u[s].load_stream(src + p.width);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const long long i = base + s * 256;
+            float f[8];
+            x[s].get(f);
+            if constexpr (kSilu) {
+                float v[8];
+                u[s].get(v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = silu_mul(f[j], v[j]);
+            }
+            uint32_t byte;
+            const uint2 q = quantize_group(f, mask, byte);
+            if (i < pieces) {
+                reinterpret_cast<uint2*>(p.out)[i] = q;
+                if ((threadIdx.x & (kLanes - 1)) == 0) p.scales[i / kLanes] = (uint8_t)byte;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------- RMS norm
+// A row is held by `warps` warps of a CTA, kPieces pieces a lane, between its one
+// read and its writes; the warps' sums of squares meet in shared memory.
+template <typename T, bool kResidual, int kPieces>
+__global__ void rms_norm_kernel(const RowQuantParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    __shared__ float sums[32];
+    const int threads = blockDim.x, tid = threadIdx.x;
+    const int row_pieces = p.width / 8;
+    const uint32_t mask = group_mask<kLanes>();
+    const long long r = blockIdx.x;
+    Raw8<T> x[kPieces];
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) {
+        const int i = tid + s * threads;
+        x[s].zero();
+        if (i < row_pieces) x[s].load_stream(reinterpret_cast<const T*>(p.x) + r * p.x_stride + i * 8);
+    }
+    if constexpr (kResidual) {
+        Raw8<T> y[kPieces];
+#pragma unroll
+        for (int s = 0; s < kPieces; ++s) {
+            const int i = tid + s * threads;
+            y[s].zero();
+            if (i < row_pieces)
+                y[s].load_stream(reinterpret_cast<const T*>(p.residual) + r * p.residual_stride + i * 8);
+        }
+#pragma unroll
+        for (int s = 0; s < kPieces; ++s) {
+            const int i = tid + s * threads;
+            float a[8], b[8];
+            x[s].get(a);
+            y[s].get(b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] = add_keep(a[j], b[j]);
+            x[s].set(a);  // the norm is that of the residual as stored
+            if (i < row_pieces)
+                x[s].store(reinterpret_cast<T*>(p.residual_out) + r * p.residual_out_stride + i * 8);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) {
+        float a[8];
+        x[s].get(a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(a[j], a[j], sum);
+    }
+    sum = group_sum<32>(sum, 0xffffffffu);
+    if (threads > 32) {
+        if ((tid & 31) == 0) sums[tid >> 5] = sum;
+        __syncthreads();
+        sum = group_sum<32>((tid & 31) < threads / 32 ? sums[tid & 31] : 0.f, 0xffffffffu);
+    }
+    const float inv = rsqrtf(sum / (float)p.width + p.eps);
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) {
+        const int i = tid + s * threads;
+        float a[8], w[8];
+        Raw8<T> wt;
+        wt.zero();
+        if (i < row_pieces) wt.load(reinterpret_cast<const T*>(p.weight) + i * 8);
+        x[s].get(a);
+        wt.get(w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = a[j] * inv * w[j];
+        uint32_t byte;
+        const uint2 q = quantize_group(a, mask, byte);
+        if (i < row_pieces) {
+            reinterpret_cast<uint2*>(p.out)[r * row_pieces + i] = q;
+            if ((tid & (kLanes - 1)) == 0)
+                p.scales[r * (row_pieces / kLanes) + i / kLanes] = (uint8_t)byte;
+        }
+    }
+}
+
+// ------------------------------------------------------- any width, any alignment
+// A CTA a row, a warp a group, element by element; rows are read twice (three
+// times by the norm).
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantParams p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    __shared__ float sums[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.width;
+    const int groups = (K + kGroup - 1) / kGroup;
+    for (long long r = blockIdx.x; r < p.num_rows; r += gridDim.x) {
+        const T* x = reinterpret_cast<const T*>(p.x) + r * p.x_stride;
+        const T* w = reinterpret_cast<const T*>(p.weight);
+        float inv = 1.f;
+        if (p.op == TLB_ROWS_RMS_NORM) {
+            const T* res = reinterpret_cast<const T*>(p.residual);
+            T* h = nullptr;
+            if (res) {
+                res += r * p.residual_stride;
+                h = reinterpret_cast<T*>(p.residual_out) + r * p.residual_out_stride;
+            }
+            float sum = 0.f;
+            // element i is the same thread's here and below, so that it reads back
+            // what it stored
+            for (int g = warp; g < groups; g += 8)
+                for (int i = g * kGroup + lane; i < min(K, (g + 1) * kGroup); i += 32) {
+                    float v = Elem<T>::to_f(x[i]);
+                    if (h) {
+                        h[i] = Elem<T>::from_f(add_keep(v, Elem<T>::to_f(res[i])));
+                        v = Elem<T>::to_f(h[i]);
+                    }
+                    sum = fmaf(v, v, sum);
+                }
+            sum = group_sum<32>(sum, 0xffffffffu);
+            if (lane == 0) sums[warp] = sum;
+            __syncthreads();
+            sum = group_sum<32>(lane < 8 ? sums[lane] : 0.f, 0xffffffffu);
+            __syncthreads();  // before the next row's sums
+            inv = rsqrtf(sum / (float)K + p.eps);
+            if (h) x = h;
+        }
+        for (int g = warp; g < groups; g += 8) {
+            float f[4];
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = g * kGroup + lane + 32 * j;
+                f[j] = 0.f;
+                if (i < K) {
+                    f[j] = Elem<T>::to_f(x[i]);
+                    if (p.op == TLB_ROWS_RMS_NORM) f[j] = f[j] * inv * Elem<T>::to_f(w[i]);
+                    if (p.op == TLB_ROWS_SILU_AND_MUL) f[j] = silu_mul(f[j], Elem<T>::to_f(x[K + i]));
+                }
+                m = max(m, finite_abs_bits(f[j]));
+            }
+            const uint32_t byte = scale_byte<E4M3>(group_max<32>(m, 0xffffffffu));
+            const float scale = inverse_scale(byte);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = g * kGroup + lane + 32 * j;
+                if (i < K) store_quantized1(reinterpret_cast<E4M3*>(p.out) + r * K + i, f[j], scale);
+            }
+            if (lane == 0) p.scales[r * groups + g] = (uint8_t)byte;
+        }
+    }
+}
+
+template <typename T, bool kResidual>
+cudaError_t launch_norm(const RowQuantParams& p, cudaStream_t st) {
+    const int pieces = p.width / 8;
+    const dim3 grid((unsigned)p.num_rows);
+    auto threads = [&](int each) { return ((pieces + each - 1) / each + 31) / 32 * 32; };
+    if (pieces <= 256)
+        return launch_early(rms_norm_kernel<T, kResidual, 1>, grid, threads(1), 0, st, p);
+    if (pieces <= 1024)
+        return launch_early(rms_norm_kernel<T, kResidual, 2>, grid, threads(2), 0, st, p);
+    return launch_early(rms_norm_kernel<T, kResidual, 4>, grid, threads(4), 0, st, p);
+}
+
+template <typename T>
+cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) {
+    // rows of the norm that a CTA holds in registers: 4 pieces of up to 512 threads
+    const bool held = p.op != TLB_ROWS_RMS_NORM || (p.width <= 16384 && p.num_rows < (1ll << 31));
+    if (!vec || !held) {
+        const long long rows = p.num_rows < 8ll * sms ? p.num_rows : 8ll * sms;
+        return launch_early(quantize_rows_any_kernel<T>, dim3((unsigned)rows), 256, 0, st, p);
+    }
+    if (p.op == TLB_ROWS_RMS_NORM)
+        return p.residual ? launch_norm<T, true>(p, st) : launch_norm<T, false>(p, st);
+    constexpr int kSteps = sizeof(T) == 2 ? 2 : 1;
+    const long long pieces = p.num_rows * (p.width / 8);
+    const long long want = (pieces + 256 * kSteps - 1) / (256 * kSteps), cap = 8ll * sms;
+    const dim3 grid((unsigned)(want < cap ? want : cap));
+    if (p.op == TLB_ROWS_SILU_AND_MUL)
+        return launch_early(quantize_pieces_kernel<T, true, kSteps>, grid, 256, 0, st, p);
+    return launch_early(quantize_pieces_kernel<T, false, kSteps>, grid, 256, 0, st, p);
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_rows(int dtype, const RowQuantParams& p, int sms, bool vec,
+                                 cudaStream_t st) {
+    switch (dtype) {
+        case TLB_FLOAT16: return launch<__half>(p, sms, vec, st);
+        case TLB_BFLOAT16: return launch<__nv_bfloat16>(p, sms, vec, st);
+        default: return launch<float>(p, sms, vec, st);
+    }
+}
+
+}  // namespace tlb
