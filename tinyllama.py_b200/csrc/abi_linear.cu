@@ -46,6 +46,24 @@ int sm_count(int* sms) {
 
 constexpr int64_t kGroup = 128;
 
+// Rows of bytes as a 2-D tensor {width, rows}, read in boxes of {128, box_rows} with
+// the 128-byte swizzle, zeros past the ends. Encoded for each call (under a
+// microsecond): nothing is kept by address.
+int rows_map(const void* base, int64_t rows, int64_t width, int64_t stride, int box_rows,
+             CUtensorMap* out) {
+    auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tlb::tensor_map_encoder());
+    if (fn == nullptr) return fail(TLB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)stride};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    cuuint32_t steps[2] = {1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides,
+                    box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(TLB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return TLB_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -126,9 +144,28 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
     p.weight_scales_stride = a.weight_scales_stride;
     p.out_stride = a.out_stride;
     p.width = (int)a.width;
+    const auto st = reinterpret_cast<cudaStream_t>(stream);
+    // A row's stride only counts where there is a second row.
+    const int64_t x_stride = a.num_tokens > 1 ? a.x_stride : (a.width + 15) / 16 * 16;
+    const int64_t w_stride = a.features > 1 ? a.weight_stride : (a.width + 15) / 16 * 16;
+    const bool tiled = aligned(a.x, 16) && aligned(a.weight, 16) && x_stride % 16 == 0 &&
+                       w_stride % 16 == 0 && x_stride >= a.width && w_stride >= a.width;
+    if (tiled) {
+        int sms = 0;
+        if (int rc = sm_count(&sms)) return rc;
+        const tlb::ProductPlan plan = tlb::plan_product(a.num_tokens, a.features, a.width, sms);
+        CUtensorMap map_w, map_x;
+        if (int rc = rows_map(a.weight, a.features, a.width, w_stride, 128, &map_w)) return rc;
+        if (int rc = rows_map(a.x, a.num_tokens, a.width, x_stride, plan.tile_tokens, &map_x))
+            return rc;
+        return cuda_result(
+            tlb::launch_product((int)a.out_dtype, p, plan, map_w, map_x,
+                                (a.flags & TLB_PRODUCT_OVERLAP_PROLOGUE) != 0,
+                                tlb::attention_wait_limit(), st),
+            "matmul_quantized");
+    }
     return cuda_result(
-        tlb::launch_product_any((int)a.out_dtype, p, reinterpret_cast<cudaStream_t>(stream)),
-        "matmul_quantized");
+        tlb::launch_product_any((int)a.out_dtype, p, st), "matmul_quantized");
 }
 
 }  // extern "C"

@@ -358,6 +358,20 @@ struct ProductParams {
     long long x_stride, x_scales_stride, weight_stride, weight_scales_stride, out_stride;
     int width;
 };
+// How the tensor-core kernel takes a product (plan_product).
+struct ProductPlan {
+    int tile_tokens;           // tokens of a tile, a multiple of 16, 224 at most
+    int split;                 // CTAs (a cluster) that share a tile's width
+    int stages;
+    int ctas;
+    size_t smem;
+};
+ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, int sms);
+// `map_w`, `map_x`: boxes of {128 bytes, 128 rows} and {128 bytes, tile_tokens rows},
+// 128-byte swizzle. overlap: see TLB_PRODUCT_OVERLAP_PROLOGUE.
+cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
+                           const CUtensorMap& map_w, const CUtensorMap& map_x, bool overlap,
+                           unsigned wait_limit, cudaStream_t stream);
 // Any shape and alignment, on the CUDA cores.
 cudaError_t launch_product_any(int out_dtype, const ProductParams& p, cudaStream_t stream);
 

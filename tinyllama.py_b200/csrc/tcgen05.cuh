@@ -61,6 +61,29 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
         "r"(0u), "r"(0u));
 }
 
+// Instruction descriptor of kind::mxf8f6f4 with e4m3 operands, both K-major, and
+// E8M0 scales: the scale bytes `sf` (0 .. 3) of the 32-bit columns are used.
+__host__ __device__ constexpr uint32_t idesc_mxf8(int m, int n, int sf) {
+    return ((uint32_t)sf << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) |
+           ((uint32_t)(m >> 7) << 27) | ((uint32_t)sf << 29);
+}
+
+// D[tmem] (+)= (A[smem] * scales of A's rows) * (B[smem] * scales of B's rows): 32
+// values of K an instruction, one scale for each row and instruction; issued by
+// one thread. The scale of row r is a byte of tensor-memory column r / 32 of the
+// scales' address, lane r % 32, the same in each of the four groups of 32 lanes.
+__device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                         uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
+                                         bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, "
+        "[%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales),
+        "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+
 // The mbarrier at `bar` gets one arrival once every tcgen05 operation this
 // thread issued before has completed.
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -103,6 +126,23 @@ __device__ __forceinline__ void ld32(uint32_t taddr, float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Stores 4 / 8 consecutive 32-bit columns of this thread's lane (st_wait completes
+// them).
+__device__ __forceinline__ void st4(uint32_t taddr, uint32_t v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%1,%1,%1};" ::"r"(taddr), "r"(v)
+                 : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(
+                     taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // Stores 32 consecutive 32-bit columns of this thread's lane, then waits.
