@@ -46,24 +46,25 @@ int sm_count(int* sms) {
 
 constexpr int64_t kGroup = 128;
 
-// Rows of bytes as a 2-D tensor {width, rows}, read in boxes of {128, box_rows} with
-// the 128-byte swizzle, zeros past the ends. Encoded for each call (under a
-// microsecond): nothing is kept by address.
-int rows_map(const void* base, int64_t rows, int64_t width, int64_t stride, int box_rows,
-             CUtensorMap* out) {
+// Rows of bytes or 16-bit elements as a 2-D tensor {width, rows}, read or written in
+// boxes of {box_width, box_rows}, swizzled by rows of a box, zeros past the ends.
+// Encoded for each call (under a microsecond): nothing is kept by address.
+int rows_map(const void* base, int64_t rows, int64_t width, int64_t stride_bytes, int bytes,
+             int box_width, int box_rows, CUtensorMap* out) {
     auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tlb::tensor_map_encoder());
     if (fn == nullptr) return fail(TLB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)stride};
-    cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    cuuint64_t strides[1] = {(cuuint64_t)stride_bytes};
+    cuuint32_t box[2] = {(cuuint32_t)box_width, (cuuint32_t)box_rows};
     cuuint32_t steps[2] = {1, 1};
-    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides,
-                    box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    CUresult r = fn(out, bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                    2, const_cast<void*>(base), dims, strides, box, steps,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    box_width * bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(TLB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return TLB_OK;
 }
-
 }  // namespace
 
 extern "C" {
@@ -153,13 +154,21 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
     if (tiled) {
         int sms = 0;
         if (int rc = sm_count(&sms)) return rc;
-        const tlb::ProductPlan plan = tlb::plan_product(a.num_tokens, a.features, a.width, sms);
-        CUtensorMap map_w, map_x;
-        if (int rc = rows_map(a.weight, a.features, a.width, w_stride, 128, &map_w)) return rc;
-        if (int rc = rows_map(a.x, a.num_tokens, a.width, x_stride, plan.tile_tokens, &map_x))
+        const int64_t out_stride = a.num_tokens > 1 ? a.out_stride : (a.features + 7) / 8 * 8;
+        const bool wide_stores = e == 2 && aligned(a.out, 16) && out_stride % 8 == 0 &&
+                                 out_stride >= a.features;
+        const tlb::ProductPlan plan =
+            tlb::plan_product(a.num_tokens, a.features, a.width, wide_stores, sms);
+        CUtensorMap map_w, map_x, map_out{};
+        if (int rc = rows_map(a.weight, a.features, a.width, w_stride, 1, 128, 128, &map_w)) return rc;
+        if (int rc = rows_map(a.x, a.num_tokens, a.width, x_stride, 1, 128,
+                              plan.pair ? plan.tile_tokens / 2 : plan.tile_tokens, &map_x))
             return rc;
+        if (plan.pieces)
+            if (int rc = rows_map(a.out, a.num_tokens, a.features, out_stride * 2, 2, 32, 16, &map_out))
+                return rc;
         return cuda_result(
-            tlb::launch_product((int)a.out_dtype, p, plan, map_w, map_x,
+            tlb::launch_product((int)a.out_dtype, p, plan, map_w, map_x, map_out,
                                 (a.flags & TLB_PRODUCT_OVERLAP_PROLOGUE) != 0,
                                 tlb::attention_wait_limit(), st),
             "matmul_quantized");

@@ -362,16 +362,22 @@ struct ProductParams {
 struct ProductPlan {
     int tile_tokens;           // tokens of a tile, a multiple of 16, 224 at most
     int split;                 // CTAs (a cluster) that share a tile's width
+    bool pair;                 // two CTAs take 256 features as one
+    int chunks;                // of 128 values of the width a stage
+    bool pieces;               // 16-bit results leave by TMA stores
     int stages;
     int ctas;
     size_t smem;
 };
-ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, int sms);
-// `map_w`, `map_x`: boxes of {128 bytes, 128 rows} and {128 bytes, tile_tokens rows},
-// 128-byte swizzle. overlap: see TLB_PRODUCT_OVERLAP_PROLOGUE.
+// wide_stores: results in 16 bits whose rows allow stores of 16 bytes.
+ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool wide_stores,
+                         int sms);
+// `map_w`, `map_x`: boxes of {128 bytes, 128 rows} and {128 bytes, tile_tokens rows (half
+// of them for a pair)}, 128-byte swizzle. overlap: see TLB_PRODUCT_OVERLAP_PROLOGUE.
 cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
-                           const CUtensorMap& map_w, const CUtensorMap& map_x, bool overlap,
-                           unsigned wait_limit, cudaStream_t stream);
+                           const CUtensorMap& map_w, const CUtensorMap& map_x,
+                           const CUtensorMap& map_out, bool overlap, unsigned wait_limit,
+                           cudaStream_t stream);
 // Any shape and alignment, on the CUDA cores.
 cudaError_t launch_product_any(int out_dtype, const ProductParams& p, cudaStream_t stream);
 

@@ -6,18 +6,20 @@
 // row's 128 four times. The sums stay in tensor memory in fp32 from the first
 // value of K to the last.
 //
-// The weights are the M side (128 features, so a weight block of 128 x 128 has one
-// scale for all lanes of a tile), the tokens the N side, of any multiple of 16:
+// The weights are the M side (128 features a CTA, so a weight block of 128 x 128 has
+// one scale for all lanes of a tile), the tokens the N side, of any multiple of 16:
 // the number of tokens is what varies from call to call, and a tile of few tokens
-// costs few bytes and few cycles. For few tokens a cluster of 2, 4 or 8 CTAs shares a
-// tile's width, and the CTAs send one another their part of the sums over
-// distributed shared memory.
+// costs few bytes and few cycles. For few tokens a cluster of 2 or 4 CTAs shares a
+// tile's width, and each joins the sums of some of its tokens, reading the others'
+// over distributed shared memory. For many tokens two CTAs of a pair take 256
+// features as one, each fetching half of the tokens' rows.
 //
-// Warps of a CTA: 0-3 load the scales and write them to tensor memory (each the
-// 32 lanes it can reach), 4-7 read the sums and write the results, 8 issues the TMA
-// copies (128 bytes of K a stage), 9 the tensor instructions. The accumulator is
-// double buffered: a tile is written out while the next one is summed.
+// Warps of a CTA: 0-3 bring the scales to tensor memory (each the 32 lanes it can
+// reach), 4-7 read the sums and write the results, 8 issues the TMA copies (one or
+// two chunks of 128 of K a stage), 9 the tensor instructions. The accumulator is double buffered: a tile
+// is written out while the next one is summed.
 #include <atomic>
+#include <type_traits>
 
 #include "kernels.h"
 #include "quant.cuh"
@@ -27,13 +29,13 @@ namespace tlb {
 
 namespace {
 
-constexpr int kFeatures = 128;             // of a tile (M)
-constexpr int kDepth = 128;                // bytes of K of a stage
+constexpr int kFeatures = 128;             // of a CTA's tile (M)
+constexpr int kChunk = 128;                // bytes of K of a shared-memory row
 constexpr int kMaxTokens = 224;            // of a tile (N): two accumulators and the scales
-constexpr int kWeightBytes = kFeatures * kDepth;
+constexpr int kWeightBytes = kFeatures * kChunk;  // of a chunk
 constexpr int kThreads = 320;
 constexpr int kMaxStages = 12;
-constexpr int kScaleSets = 4;              // sets of scales in tensor memory, 4 stages each
+constexpr int kScaleSets = 4;              // sets of scales in tensor memory, a word each
 constexpr int kSetColumns = 12;            // 4 of the weights, 8 of the tokens
 constexpr int kScaleColumn = 512 - kScaleSets * kSetColumns;
 constexpr int kColumns = 512;
@@ -44,21 +46,29 @@ constexpr int kBarFull = 0, kBarEmpty = kMaxStages, kBarScales = 2 * kMaxStages,
               kBarSumsFree = kBarSums + 2, kBarParts = kBarSumsFree + 2,
               kBarPartsFree = kBarParts + 1, kBarDrain = kBarPartsFree + 1,
               kNumBars = kBarDrain + 1;
-constexpr int kTail = 512;                 // bytes after the stages: barriers, tmem address, flag
-static_assert(kNumBars * 8 + 16 <= kTail, "barriers");
-constexpr int kMaxSplit = 8;
+// behind the barriers: the tensor-memory address, the number of stages issued
+constexpr int kSlot = kNumBars * 8, kIssued = kSlot + 4;
+constexpr int kTail = 512;                 // bytes of all of it, after the stages
+static_assert(kIssued + 4 <= kTail, "barriers");
+// CTAs that share a tile. Eight were slower everywhere (64 x 8192 -> 2048: 17.7 us, 10.4
+// with four): fewer than 16 clusters of that many large CTAs run at once.
+constexpr int kMaxSplit = 4;
 
 struct Work {
     ProductParams p;
     int tile_tokens;
-    int blocks;              // of 128 bytes of K
+    int depths;              // stages of a tile's whole width
+    int groups;              // scales of a row
     int stages;
     int split;
     int tiles_n, tiles_t;
     int band;                // token tiles whose weights' tiles follow one another
     unsigned wait_limit;
     bool overlap;
-    bool x_words, w_words;   // rows of scales allow 4-byte loads
+    bool words;              // rows of scales allow 4-byte loads, and are whole words
+    int parts_bytes;         // of shared memory for the results
+    bool aligned;            // results allow stores of four features
+    bool pieces;             // 16-bit results of one CTA a tile, eight features a store
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -76,8 +86,13 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void store_cluster(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ float4 load_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -97,17 +112,14 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, uint
     return false;
 }
 
-// The scale bytes of groups 4 w .. 4 w + 3 of a row, those past the last group 127.
-__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int w, int groups, bool words) {
-    if (words && 4 * w + 4 <= groups) return *reinterpret_cast<const uint32_t*>(row + 4 * w);
-    uint32_t v = 0x7f7f7f7fu;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (4 * w + i < groups) {
-            const uint32_t b = row[4 * w + i];
-            v = (v & ~(0xffu << (8 * i))) | (b << (8 * i));
-        }
-    return v;
+// A tile load into this CTA that completes at a barrier of either CTA of its pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int32_t x,
+                                              int32_t y, uint32_t bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        ".cta_group::2.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+        : "memory");
 }
 
 // Tile `i` of the order in which a band of token tiles goes through all features.
@@ -118,23 +130,310 @@ __device__ __forceinline__ void tile_at(const Work& w, int i, int& tn, int& tt) 
     tt = b * w.band + rest % height;
 }
 
+// Whether `ok` holds in every thread of four warps. They meet at barriers, so they go
+// on or give up together.
+template <int kBarrier>
+__device__ __forceinline__ bool all_agree(bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(ok ? 1u : 0u), "n"(kBarrier)
+        : "memory");
+    return all != 0;
+}
+
+// The scale bytes of groups 4 word .. 4 word + 3 of a row (past the last group: its
+// byte again, which no instruction reads).
+template <bool kWords>
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int word, int groups) {
+    if constexpr (kWords) return reinterpret_cast<const uint32_t*>(row)[word];
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v |= (uint32_t)row[min(4 * word + i, groups - 1)] << (8 * i);
+    return v;
+}
+
+// The scales' way to tensor memory (four warps). A tile's scales are read kWordsAtOnce
+// words (of four groups) of every row at a time, each word once, and kept in shared
+// memory, while the words before them go to tensor memory: four columns of the tile's
+// weight scale, the same in all lanes, and a column for each 32 tokens. Each warp
+// writes the 32 lanes it can reach. False: a wait gave up.
+constexpr int kWordsAtOnce = 4;
+constexpr int kRowsAtOnce = 128 / kWordsAtOnce;
+constexpr int kScalePitch = kWordsAtOnce + 1;  // words: rows in different banks
+constexpr int kScaleRows = kMaxTokens + 1;     // the weights' behind the tokens'
+constexpr int kScaleBytes = 2 * kScaleRows * kScalePitch * 4;
+
+template <bool kPair, bool kWords>
+__device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uint32_t tmem, uint32_t tail, int tid,
+                            int unit, int units, int tiles, int word_first, int word_end,
+                            int rank) {
+    const ProductParams& p = w.p;
+    const int warp = tid >> 5, lane = tid & 31;
+    const long long last_block = (p.features - 1) / kFeatures;
+    constexpr int kItems = kMaxTokens * kWordsAtOnce / 128;
+    uint32_t x[kItems], ws = 0;
+    int tile = unit, word = word_first;  // of the next read
+    auto read = [&]() {
+        if (tile >= tiles) return;
+        int tn, tt;
+        tile_at(w, tile, tn, tt);
+        const int at = min(word + (tid & (kWordsAtOnce - 1)), word_end - 1);
+        const long long last = p.num_tokens - 1;
+        long long t = (long long)tt * w.tile_tokens + tid / kWordsAtOnce;
+#pragma unroll
+        for (int m = 0; m < kItems; ++m, t += kRowsAtOnce)
+            if (kRowsAtOnce * m < w.tile_tokens)
+                x[m] = scale_word<kWords>(p.x_scales + min(t, last) * p.x_scales_stride, at, w.groups);
+        if (tid < kWordsAtOnce) {
+            const long long block = kPair ? min(2ll * tn + rank, last_block) : tn;
+            ws = scale_word<kWords>(p.weight_scales + block * p.weight_scales_stride, at, w.groups);
+        }
+        word += kWordsAtOnce;
+        if (word >= word_end) {
+            word = word_first;
+            tile += units;
+        }
+    };
+    read();
+    int set = 0, half = 0;
+    uint32_t parity = 1;  // of the wait for a free set: the first round's holds
+    const uint32_t lanes = (uint32_t)warp << 21;  // 32 warp, in the address's upper half
+    for (int i = unit; i < tiles; i += units)
+        for (int first = word_first; first < word_end; first += kWordsAtOnce, half ^= 1) {
+            uint32_t* buf = reinterpret_cast<uint32_t*>(buffers) + half * (kScaleRows * kScalePitch);
+#pragma unroll
+            for (int m = 0; m < kItems; ++m)
+                if (kRowsAtOnce * m < w.tile_tokens)
+                    buf[(tid / kWordsAtOnce + kRowsAtOnce * m) * kScalePitch + (tid & (kWordsAtOnce - 1))] = x[m];
+            if (tid < kWordsAtOnce) buf[kMaxTokens * kScalePitch + tid] = ws;
+            named_bar_sync(2, 128);  // the other half's readers are past it too
+            read();
+            const int count = min(kWordsAtOnce, word_end - first);
+            for (int k = 0; k < count; ++k) {
+                // a CTA's warps give up together: they meet at the barrier above
+                if (!all_agree<2>(mbar_wait_bounded(tail + 8u * (kBarScalesFree + set), parity,
+                                                    w.wait_limit)))
+                    return false;
+                tc5::fence_after_sync();
+                uint32_t v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[j] = buf[min(32 * j + lane, kMaxTokens - 1) * kScalePitch + k];
+                const uint32_t to = tmem + lanes + kScaleColumn + set * kSetColumns;
+                tc5::st4(to, buf[kMaxTokens * kScalePitch + k]);
+                tc5::st8(to + 4, v);
+                tc5::st_wait();
+                tc5::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    const uint32_t full = tail + 8u * (kBarScales + set);
+                    if constexpr (kPair) arrive_cluster(map_rank(full, 0));
+                    else mbar_arrive(full);
+                }
+                if (++set == kScaleSets) {
+                    set = 0;
+                    parity ^= 1;
+                }
+            }
+        }
+    return true;
+}
+
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, uint32_t from) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(x), "r"(y), "r"(from)
+        : "memory");
+}
+
+// A tile's results in 16 bits, a warp's 32 features and 32 tokens at a time: the sums
+// leave tensor memory in the layout of matrix fragments, are rounded in pairs of
+// tokens and turned round by stmatrix, so that a token's 32 features lie side by side
+// in shared memory (the 64-byte swizzle: unit u of 16 bytes at u ^ token / 2 % 4, free
+// of bank conflicts); a TMA store takes them from there, past the tensor's ends as
+// well. Each warp has two buffers of its own, so the warps do not wait for one another;
+// the next sums are read under the stores. (Written by the lanes, 32 tokens took 640
+// cycles, more than the instructions of a tile 896 wide.)
 template <typename T>
+__device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* map, uint32_t sums,
+                                             uint32_t stage, long long n0, long long t0, int here,
+                                             int quarter, int lane) {
+    if constexpr (sizeof(T) == 2) {
+        const ProductParams& p = w.p;
+        n0 += quarter * 32;
+        if (n0 >= p.features) return;
+        float bias[4] = {};
+        if (p.bias)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const long long n = n0 + 8 * i + (lane >> 2);
+                if (n < p.features) bias[i] = Elem<T>::to_f(reinterpret_cast<const T*>(p.bias)[n]);
+            }
+        const uint32_t buf = stage + quarter * 4096;  // two of 2 KB
+        // token 8 g + lane % 8, unit lane / 8
+        const uint32_t put = buf + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
+        uint32_t a[16], c[16];
+        tc5::ld_rows16(sums, a);
+        tc5::ld_rows16(sums + (16u << 16), c);
+#pragma unroll 1
+        for (int j = 0; j < here; j += 32) {
+            const uint32_t half = (j & 32) << 6;
+            tc5::ld_wait();
+            uint32_t m[16];
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t* v = (i < 2 ? a : c) + 4 * g + 2 * (i & 1);
+                    m[4 * g + i] = pack2<T>(__uint_as_float(v[0]) + bias[i],
+                                            __uint_as_float(v[1]) + bias[i]);
+                }
+            if (j + 32 < here) {
+                tc5::ld_rows16(sums + j + 32, a);
+                tc5::ld_rows16(sums + j + 32 + (16u << 16), c);
+            }
+            // the store before the last one has read this buffer
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            __syncwarp();
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                asm volatile(
+                    "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                        put + half + 512 * g),
+                    "r"(m[4 * g]), "r"(m[4 * g + 1]), "r"(m[4 * g + 2]), "r"(m[4 * g + 3])
+                    : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                store_box(map, (int)n0, (int)t0 + j, buf + half);
+                // of 16 tokens: a tile may end there
+                if (j + 16 < w.tile_tokens) store_box(map, (int)n0, (int)t0 + j + 16, buf + half + 1024);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        }
+    }
+}
+
+// A tile's results by way of fp32 sums in shared memory: of a cluster's CTAs, each
+// joins its share of the tile's tokens, reading its part of the sums from every CTA
+// (in the order of their ranks, so results do not depend on which is first). Also
+// for one CTA where the results are fp32 or not aligned for store_pieces. False: a
+// wait gave up.
+template <typename T>
+__device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8_t* stage,
+                                             uint32_t parts, uint32_t bar, uint32_t parity,
+                                             long long n0, long long t0, int here, int quarter,
+                                             int lane, int rank) {
+    const ProductParams& p = w.p;
+    const int split = w.split, f0 = lane * 4;
+    const int wide = (int)min(4ll, p.features - n0 - f0);  // features of this lane
+    float bias[4] = {};
+    if (p.bias)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < wide) bias[k] = Elem<T>::to_f(reinterpret_cast<const T*>(p.bias)[n0 + f0 + k]);
+    T* out = reinterpret_cast<T*>(p.out) + t0 * p.out_stride + n0 + f0;
+    // tokens at a time: all of a cluster's tile, else 32 in either of two buffers
+    const int rows = split > 1 ? w.tile_tokens : 32;
+    for (int j0 = 0; j0 < here; j0 += rows) {
+        const int count = min(rows, here - j0);
+        const uint32_t offset = split > 1 ? 0u : (uint32_t)(j0 & 32) * (kFeatures * 4);
+        float* column = reinterpret_cast<float*>(stage + offset) + quarter * 32 + lane;
+        for (int j = 0; j < count; j += 32) {
+            float v[32];
+            tc5::ld32(sums + j0 + j, v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+                if (j + k < rows) column[(j + k) * kFeatures] = v[k];
+        }
+        int first = 0, mine = count;
+        if (split > 1) {
+            const int share = (count + split - 1) / split;
+            first = rank * share;
+            mine = max(0, min(share, count - first));
+            __syncwarp();
+            if (lane < split) arrive_cluster(map_rank(bar, lane));
+            if (!all_agree<1>(wait_cluster(bar, parity, w.wait_limit))) return false;
+        } else {
+            named_bar_sync(1, 128);
+        }
+        const uint32_t from = parts + offset + f0 * 4;
+        for (int r0 = quarter; r0 < mine; r0 += 8) {  // two rows of all CTAs in flight
+            float4 v[2], x[kMaxSplit][2];
+#pragma unroll
+            for (int c = 0; c < kMaxSplit; ++c) {
+                if (c >= split) break;
+                const uint32_t at = split > 1 ? map_rank(from, c) : from;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    x[c][k] = load_cluster(at + (first + min(r0 + 4 * k, mine - 1)) * (kFeatures * 4));
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                v[k] = x[0][k];
+#pragma unroll
+                for (int c = 1; c < kMaxSplit; ++c) {
+                    if (c >= split) break;
+                    v[k].x += x[c][k].x;
+                    v[k].y += x[c][k].y;
+                    v[k].z += x[c][k].z;
+                    v[k].w += x[c][k].w;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int row = r0 + 4 * k;
+                if (row >= mine) break;
+                T* to = out + (j0 + first + row) * p.out_stride;
+                const float y[4] = {v[k].x + bias[0], v[k].y + bias[1], v[k].z + bias[2],
+                                    v[k].w + bias[3]};
+                if (wide == 4 && w.aligned) {
+                    if constexpr (sizeof(T) == 2)
+                        *reinterpret_cast<uint2*>(to) =
+                            make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+                    else
+                        *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < wide) to[e] = Elem<T>::from_f(y[e]);
+                }
+            }
+        }
+    }
+    return true;
+}
+
+// kChunks: of 128 values of K a stage. Two halve the waits and commits of the one thread
+// that issues the tensor instructions, which a tile of few tokens is bounded by; one
+// gives a wide tile's stages finer steps (2048 x 4096 -> 4096: 32.5 us with one, 36.3
+// with two; 64 x 2048 -> 16384: 10.4 and 9.1).
+template <typename T, bool kPair, int kChunks>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_w,
-                   const __grid_constant__ CUtensorMap map_x, const Work w) {
+                   const __grid_constant__ CUtensorMap map_x,
+                   const __grid_constant__ CUtensorMap map_out, const Work w) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
     const uint32_t base = smem_u32(smem);
+    constexpr int kDepth = kChunks * kChunk;  // of a stage
+    constexpr int kPerWord = 512 / kDepth;    // stages of a word of scales
     const ProductParams& p = w.p;
-    const uint32_t stage_bytes = kWeightBytes + w.tile_tokens * kDepth;
+    const int x_rows = kPair ? w.tile_tokens / 2 : w.tile_tokens;  // of this CTA's stages
+    const uint32_t x_bytes = x_rows * kChunk;                      // of a chunk
+    const uint32_t stage_bytes = kChunks * (kWeightBytes + x_bytes);
     const uint32_t tail = base + w.stages * stage_bytes, parts = tail + kTail;
     uint8_t* tail_ptr = smem + w.stages * stage_bytes;
     auto bar = [tail](int i) { return tail + 8u * i; };
-    const uint32_t slot = tail + kNumBars * 8;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = w.split;
-    const uint32_t rank = split > 1 ? cluster_rank() : 0;
+    // CTAs of a cluster: of a pair, or sharing a tile's width
+    const int split = kPair ? 1 : w.split, cluster = kPair ? 2 : split;
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0;
 
     if (tid == 0) {
         for (int i = 0; i < w.stages; ++i) {
@@ -142,34 +441,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(bar(kBarEmpty + i), 1);
         }
         for (int i = 0; i < kScaleSets; ++i) {
-            mbar_init(bar(kBarScales + i), 4);
+            mbar_init(bar(kBarScales + i), kPair ? 8 : 4);
             mbar_init(bar(kBarScalesFree + i), 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(kBarSums + i), 1);
-            mbar_init(bar(kBarSumsFree + i), 4);
+            mbar_init(bar(kBarSumsFree + i), kPair ? 8 : 4);
         }
         mbar_init(bar(kBarParts), 4 * split);
         mbar_init(bar(kBarPartsFree), 4 * split);
         mbar_init(bar(kBarDrain), 1);
         fence_mbar_init();
     }
-    if (warp == 9) tc5::alloc(slot, kColumns);
+    if (warp == 9) {
+        if constexpr (kPair) tc5::alloc_pair(tail + kSlot, kColumns);
+        else tc5::alloc(tail + kSlot, kColumns);
+    }
     if (tid == 256) {
         prefetch_tensormap(&map_w);
         prefetch_tensormap(&map_x);
     }
     tc5::fence_before_sync();
     __syncthreads();
-    if (split > 1) cluster_sync();  // all barriers of the cluster are set up
+    if (cluster > 1) cluster_sync();  // all barriers of the cluster are set up
     tc5::fence_after_sync();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tail_ptr + kNumBars * 8);
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tail_ptr + kSlot);
 
     // this CTA's tiles, and its part of their width
-    const int tiles = w.tiles_n * w.tiles_t, units = gridDim.x / split, unit = blockIdx.x / split;
-    const int k_first = (int)((long long)w.blocks * rank / split);
-    const int k_last = (int)((long long)w.blocks * (rank + 1) / split);
+    const int tiles = w.tiles_n * w.tiles_t, units = gridDim.x / cluster, unit = blockIdx.x / cluster;
+    const int d_first = (int)((long long)w.depths * (split > 1 ? rank : 0) / split);
+    const int d_last = (int)((long long)w.depths * (split > 1 ? rank + 1 : 1) / split);
+    const int word_first = d_first / kPerWord, word_end = (d_last - 1) / kPerWord + 1;
     const uint32_t limit = w.wait_limit;
+    auto wait = [limit](uint32_t b, uint32_t parity) {
+        if constexpr (kPair) return wait_cluster(b, parity, limit);
+        else return mbar_wait_bounded(b, parity, limit);
+    };
     bool ok = true;
 
     if (warp == 8) {
@@ -179,100 +486,141 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t once = l2_policy_evict_first();
             // weights that only this tile's tokens want pass through the L2
             const uint64_t w_policy = w.tiles_t > 1 ? keep : once;
-            int n = 0;  // stages issued
-            bool waited = false;
-            int ahead = 0;  // stages whose weights were issued before the wait
-            if (w.overlap) {
-                int i = unit, kb = k_first;
-                for (; ahead < w.stages && i < tiles; ++ahead) {
-                    if (kb == k_last) {
-                        kb = k_first;
-                        i += units;
-                        if (i >= tiles) break;
-                    }
-                    int tn, tt;
-                    tile_at(w, i, tn, tt);
-                    mbar_arrive_expect_tx(bar(kBarFull + ahead), stage_bytes);
-                    tma_load_2d(base + ahead * stage_bytes, &map_w, kb * kDepth, tn * kFeatures,
-                                bar(kBarFull + ahead), w_policy);
-                    ++kb;
-                }
-            }
-            for (int i = unit; i < tiles && ok; i += units) {
+            const uint32_t full0 = kPair && rank == 1 ? map_rank(bar(kBarFull), 0) : bar(kBarFull);
+            auto load = [](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t b,
+                           uint64_t policy) {
+                if constexpr (kPair) tma_load_pair(dst, map, x, y, b, policy);
+                else tma_load_2d(dst, map, x, y, b, policy);
+            };
+            // the stage's bytes are expected (a pair's by its even CTA; a copy may complete
+            // before that), and its weights fetched
+            auto load_weights = [&](uint32_t at, uint32_t full, int k, int y) {
+                const bool both = kChunks == 2 && k + kChunk < p.width;
+                if (!kPair || rank == 0)
+                    mbar_arrive_expect_tx(full, (kPair ? 2 : 1) * (both ? stage_bytes : stage_bytes / kChunks));
+                load(at, &map_w, k, y, full, w_policy);
+                if (both) load(at + kWeightBytes, &map_w, k + kChunk, y, full, w_policy);
+            };
+            auto load_tokens = [&](uint32_t at, uint32_t full, int k, int y) {
+                load(at + kChunks * kWeightBytes, &map_x, k, y, full, keep);
+                if (kChunks == 2 && k + kChunk < p.width)
+                    load(at + kChunks * kWeightBytes + x_bytes, &map_x, k + kChunk, y, full, keep);
+            };
+            auto place = [&](int i, int& wy, int& xy) {
                 int tn, tt;
                 tile_at(w, i, tn, tt);
-                for (int kb = k_first; kb < k_last; ++kb, ++n) {
-                    const int s = n % w.stages, round = n / w.stages;
-                    if (round > 0 &&
-                        !mbar_wait_bounded(bar(kBarEmpty + s), (round - 1) & 1, limit)) {
+                wy = (kPair ? 2 * tn + rank : tn) * kFeatures;
+                xy = tt * w.tile_tokens + (kPair ? rank * x_rows : 0);
+            };
+            int ahead = 0, wy, xy;  // stages whose weights are fetched before the wait
+            if (w.overlap) {
+                int i = unit, d = d_first;
+                for (; ahead < w.stages; ++ahead, ++d) {
+                    if (d == d_last) {
+                        d = d_first;
+                        i += units;
+                    }
+                    if (i >= tiles) break;
+                    place(i, wy, xy);
+                    load_weights(base + ahead * stage_bytes, full0 + 8 * ahead, d * kDepth, wy);
+                }
+            }
+            grid_dependency_wait();
+            // One thread issues everything, so its instructions are what a stage costs:
+            // counters instead of divisions.
+            int s = 0, issued = 0;
+            uint32_t parity = 1;  // of the wait for a free stage: the first round's holds
+            uint32_t at = base;
+            for (int i = unit; i < tiles && ok; i += units) {
+                place(i, wy, xy);
+                for (int d = d_first; d < d_last; ++d) {
+                    const uint32_t full = full0 + 8 * s;
+                    if (!mbar_wait_bounded(bar(kBarEmpty + s), parity, limit)) {
                         ok = false;
                         break;
                     }
-                    if (!waited) {
-                        grid_dependency_wait();
-                        waited = true;
+                    if (issued >= ahead) load_weights(at, full, d * kDepth, wy);
+                    load_tokens(at, full, d * kDepth, xy);
+                    ++issued;
+                    at += stage_bytes;
+                    if (++s == w.stages) {
+                        s = 0;
+                        parity ^= 1;
+                        at = base;
                     }
-                    const uint32_t at = base + s * stage_bytes;
-                    if (n >= ahead) {
-                        mbar_arrive_expect_tx(bar(kBarFull + s), stage_bytes);
-                        tma_load_2d(at, &map_w, kb * kDepth, tn * kFeatures, bar(kBarFull + s),
-                                    w_policy);
-                    }
-                    tma_load_2d(at + kWeightBytes, &map_x, kb * kDepth, tt * w.tile_tokens,
-                                bar(kBarFull + s), keep);
                 }
             }
-            if (!waited) grid_dependency_wait();
-            // After a wait that gave up, the copies in flight land before the CTA ends.
-            if (!ok)
-                for (int k = n > w.stages ? n - w.stages : 0; k < n; ++k)
-                    mbar_wait_bounded(bar(kBarFull + k % w.stages), (k / w.stages) & 1);
+            // A wait gave up before all stages had their tokens: none of them is
+            // used, but what the barriers expect has to come.
+            for (; issued < ahead; ++issued)
+                load_tokens(base + issued * stage_bytes, full0 + 8 * issued, 0, 0);
+            *reinterpret_cast<volatile int*>(tail_ptr + kIssued) = issued;
         }
     } else if (warp == 9) {
         // ------------------------------------------------ tensor instructions
-        if (elect_one()) {
-            int n = 0, group = 0, it = 0;
-            bool issued = false;
+        if ((!kPair || rank == 0) && elect_one()) {
+            auto commit = [](uint32_t b) {
+                if constexpr (kPair) tc5::commit_pair(b);
+                else tc5::commit(b);
+            };
+            const uint64_t first = tc5::desc_sw128(base, 16, 1024);
+            const uint32_t idesc = tc5::idesc_mxf8(kPair ? 256 : 128, w.tile_tokens, 0);
+            uint64_t desc = first;
+            int s = 0, set = 0, it = 0;
+            uint32_t parity = 0, set_parity = 0;
             for (int i = unit; i < tiles && ok; i += units, ++it) {
                 const int b = it & 1;
-                if (it >= 2 && !mbar_wait_bounded(bar(kBarSumsFree + b), ((it >> 1) - 1) & 1, limit)) {
+                if (it >= 2 && !wait(bar(kBarSumsFree + b), ((it >> 1) - 1) & 1)) {
                     ok = false;
                     break;
                 }
                 tc5::fence_after_sync();
                 const uint32_t sums = tmem + b * kMaxTokens;
-                for (int kb = k_first; kb < k_last; ++kb, ++n) {
-                    const int set = group % kScaleSets;
-                    if ((kb == k_first || (kb & 3) == 0) &&
-                        !mbar_wait_bounded(bar(kBarScales + set), (group / kScaleSets) & 1, limit)) {
+                bool accumulate = false;
+                for (int word = word_first; word < word_end && ok; ++word) {
+                    if (!wait(bar(kBarScales + set), set_parity)) {
                         ok = false;
                         break;
                     }
-                    const int s = n % w.stages;
-                    if (!mbar_wait_bounded(bar(kBarFull + s), (n / w.stages) & 1, limit)) {
-                        ok = false;
-                        break;
-                    }
-                    tc5::fence_after_sync();
-                    const uint32_t at = base + s * stage_bytes;
                     const uint32_t scales = tmem + kScaleColumn + set * kSetColumns;
-                    const uint32_t idesc = tc5::idesc_mxf8(kFeatures, w.tile_tokens, kb & 3);
-                    const int steps = min(4, (p.width - kb * kDepth + 31) / 32);
-                    for (int k = 0; k < steps; ++k)
-                        tc5::mma_mxf8(sums, tc5::desc_sw128(at + 32 * k, 16, 1024),
-                                      tc5::desc_sw128(at + kWeightBytes + 32 * k, 16, 1024), idesc,
-                                      scales, scales + 4, kb > k_first || k > 0);
-                    issued = true;
-                    tc5::commit(bar(kBarEmpty + s));
-                    if ((kb & 3) == 3 || kb + 1 == k_last) {
-                        tc5::commit(bar(kBarScalesFree + set));
-                        ++group;
+#pragma unroll
+                    for (int h = 0; h < kPerWord; ++h) {
+                        const int d = kPerWord * word + h;
+                        if (d < d_first || d >= d_last) continue;
+                        if (!mbar_wait_bounded(bar(kBarFull + s), parity, limit)) {
+                            ok = false;
+                            break;
+                        }
+                        tc5::fence_after_sync();
+                        const int left = p.width - d * kDepth;
+#pragma unroll
+                        for (int k = 0; k < 4 * kChunks; ++k) {
+                            if (32 * k >= left) break;
+                            const uint32_t sf = kChunks * h + k / 4;
+                            tc5::mma_mxf8<kPair>(
+                                sums, desc + (k / 4) * (kWeightBytes >> 4) + 2 * (k % 4),
+                                desc + (kChunks * kWeightBytes >> 4) + (k / 4) * (x_bytes >> 4) + 2 * (k % 4),
+                                idesc | sf << 4 | sf << 29, scales, scales + 4, accumulate);
+                            accumulate = true;
+                        }
+                        commit(bar(kBarEmpty + s));
+                        desc += stage_bytes >> 4;
+                        if (++s == w.stages) {
+                            s = 0;
+                            parity ^= 1;
+                            desc = first;
+                        }
+                    }
+                    commit(bar(kBarScalesFree + set));
+                    if (++set == kScaleSets) {
+                        set = 0;
+                        set_parity ^= 1;
                     }
                 }
-                if (ok) tc5::commit(bar(kBarSums + b));
+                if (ok) commit(bar(kBarSums + b));
             }
-            if (!ok && issued) {  // nothing runs on when the CTA ends
-                tc5::commit(bar(kBarDrain));
+            if (!ok) {  // nothing runs on when the CTA ends
+                commit(bar(kBarDrain));
                 mbar_wait_bounded(bar(kBarDrain), 0);
             }
         }
@@ -280,132 +628,112 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ------------------------------------------------------------ scales
         grid_dependency_wait();
         grid_launch_dependents();
-        int group = 0;
-        const uint32_t lanes = (uint32_t)warp << 21;  // 32 warp, in the address's upper half
-        const int groups = w.blocks;
-        for (int i = unit; i < tiles && ok; i += units) {
-            int tn, tt;
-            tile_at(w, i, tn, tt);
-            const uint8_t* w_row = p.weight_scales + tn * p.weight_scales_stride;
-            const long long t0 = (long long)tt * w.tile_tokens + lane;
-            for (int word = k_first >> 2; word <= (k_last - 1) >> 2; ++word, ++group) {
-                uint32_t x[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const long long t = t0 + 32 * j;
-                    x[j] = 0x7f7f7f7fu;
-                    if (32 * j < w.tile_tokens && t < p.num_tokens)
-                        x[j] = scale_word(p.x_scales + t * p.x_scales_stride, word, groups, w.x_words);
-                }
-                const uint32_t wt = scale_word(w_row, word, groups, w.w_words);
-                const int set = group % kScaleSets;
-                if (group >= kScaleSets &&
-                    !__all_sync(0xffffffffu, mbar_wait_bounded(bar(kBarScalesFree + set),
-                                                               (group / kScaleSets - 1) & 1, limit))) {
-                    ok = false;
-                    break;
-                }
-                tc5::fence_after_sync();
-                const uint32_t to = tmem + lanes + kScaleColumn + set * kSetColumns;
-                tc5::st4(to, wt);
-                tc5::st8(to + 4, x);
-                tc5::st_wait();
-                tc5::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(kBarScales + set));
-            }
-        }
+        uint8_t* buffers = tail_ptr + kTail + w.parts_bytes;
+        ok = w.words ? feed_scales<kPair, true>(w, buffers, tmem, tail, tid, unit, units, tiles,
+                                                word_first, word_end, rank)
+                     : feed_scales<kPair, false>(w, buffers, tmem, tail, tid, unit, units, tiles,
+                                                 word_first, word_end, rank);
     } else {
         // ----------------------------------------------------------- results
         grid_dependency_wait();
-        const int quarter = warp & 3, feature = quarter * 32 + lane;
+        const int quarter = warp & 3;
+        uint8_t* stage = tail_ptr + kTail;
         int it = 0;
-        for (int i = unit; i < tiles && ok; i += units, ++it) {
+        for (int i = unit; i < tiles; i += units, ++it) {
             int tn, tt;
             tile_at(w, i, tn, tt);
-            const long long n = (long long)tn * kFeatures + feature;
+            const long long n0 = (kPair ? 2ll * tn + rank : tn) * kFeatures;
             const long long t0 = (long long)tt * w.tile_tokens;
             const int here = (int)min((long long)w.tile_tokens, p.num_tokens - t0);
-            const bool on = n < p.features;
-            float bias = 0.f;
-            if (p.bias && on) bias = Elem<T>::to_f(reinterpret_cast<const T*>(p.bias)[n]);
-            T* out = reinterpret_cast<T*>(p.out) + t0 * p.out_stride + n;
             const int b = it & 1;
-            if (!__all_sync(0xffffffffu,
-                            mbar_wait_bounded(bar(kBarSums + b), (it >> 1) & 1, limit))) {
+            const uint32_t sums = tmem + ((uint32_t)quarter << 21) + b * kMaxTokens;
+            ok = mbar_wait_bounded(bar(kBarSums + b), (it >> 1) & 1, limit);
+            if (split > 1 && it > 0)
+                ok = wait_cluster(bar(kBarPartsFree), (it - 1) & 1, limit) && ok;
+            if (!all_agree<1>(ok)) {
                 ok = false;
                 break;
             }
             tc5::fence_after_sync();
-            const uint32_t sums = tmem + ((uint32_t)quarter << 21) + b * kMaxTokens;
-            const int share = (here + split - 1) / split;  // tokens that a CTA of the cluster joins
-            if (split > 1 && it > 0 &&
-                !__all_sync(0xffffffffu, wait_cluster(bar(kBarPartsFree), (it - 1) & 1, limit))) {
-                ok = false;
-                break;
-            }
-            for (int j0 = 0; j0 < here; j0 += 32) {
-                float v[32];
-                tc5::ld32(sums + j0, v);
-                if (split == 1) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (on && j0 + j < here)
-                            out[(j0 + j) * p.out_stride] = Elem<T>::from_f(v[j] + bias);
-                } else {
-                    // token j of the tile goes to CTA j / share, at [from][j % share][feature]
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (j0 + j >= here) break;
-                        const int to = (j0 + j) / share, row = (j0 + j) - to * share;
-                        store_cluster(map_rank(parts, to) +
-                                          4u * (((int)rank * share + row) * kFeatures + feature),
-                                      v[j]);
-                    }
-                }
-            }
+            if (w.pieces)
+                store_pieces<T>(w, &map_out, sums, parts, n0, t0, here, quarter, lane);
+            else
+                ok = store_joined<T>(w, sums, stage, parts, bar(kBarParts), it & 1, n0, t0, here,
+                                     quarter, lane, rank);
             tc5::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kBarSumsFree + b));
-            if (split > 1) {
-                if (lane < split) arrive_cluster(map_rank(bar(kBarParts), lane));
-                if (!__all_sync(0xffffffffu, wait_cluster(bar(kBarParts), it & 1, limit))) {
-                    ok = false;
-                    break;
-                }
-                const int first = (int)rank * share, mine = max(0, min(share, here - first));
-                const float* in = reinterpret_cast<const float*>(tail_ptr + kTail) + feature;
-                for (int row = 0; row < mine; ++row) {
-                    float v = 0.f;
-                    for (int from = 0; from < split; ++from)
-                        v += in[(from * share + row) * kFeatures];
-                    if (on) out[(first + row) * p.out_stride] = Elem<T>::from_f(v + bias);
-                }
-                __syncwarp();
-                if (lane < split) arrive_cluster(map_rank(bar(kBarPartsFree), lane));
+            if (lane == 0) {
+                if constexpr (kPair) arrive_cluster(map_rank(bar(kBarSumsFree + b), 0));
+                else mbar_arrive(bar(kBarSumsFree + b));
             }
+            if (!ok) break;
+            if (split > 1 && lane < split) arrive_cluster(map_rank(bar(kBarPartsFree), lane));
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     if (!ok) flag_status(TLB_STATUS_WAIT_TIMEOUT);
     __syncwarp();
     tc5::fence_before_sync();
     __syncthreads();
-    if (split > 1) cluster_sync();  // no CTA ends while another one may write to it
+    // No CTA ends while another one may read its sums or arrive at its barriers, nor
+    // before the copies that were issued have landed (after a wait that gave up; they
+    // have otherwise).
+    if (cluster > 1) cluster_sync();
+    if (tid == 0 && (!kPair || rank == 0)) {
+        const int mine = *reinterpret_cast<volatile int*>(tail_ptr + kIssued);
+        int most = mine;
+        if constexpr (kPair) {
+            // both CTAs' copies complete here: expect those of the other CTA alone, and
+            // make up for those that it did not issue
+            int other;
+            asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                         : "=r"(other)
+                         : "r"(map_rank(tail + kIssued, 1))
+                         : "memory");
+            most = max(mine, other);
+            for (int k = min(mine, other); k < most; ++k) {
+                const int s = k % w.stages, x = k % w.depths * kDepth;
+                const uint32_t at = base + s * stage_bytes;
+                const bool both = kChunks == 2 && x + kChunk < p.width;
+                if (k >= mine) {
+                    mbar_arrive_expect_tx(bar(kBarFull + s), both ? stage_bytes : stage_bytes / kChunks);
+                    continue;
+                }
+                for (int c = 0; c < (both ? 2 : 1); ++c) {
+                    tma_load_2d(at + c * kWeightBytes, &map_w, x, 0, bar(kBarFull + s),
+                                l2_policy_evict_first());
+                    tma_load_2d(at + kChunks * kWeightBytes + c * x_bytes, &map_x, x, 0,
+                                bar(kBarFull + s), l2_policy_evict_first());
+                }
+            }
+        }
+        for (int k = max(0, most - w.stages); k < most; ++k)
+            mbar_wait_bounded(bar(kBarFull + k % w.stages), (k / w.stages) & 1);
+    }
+    __syncthreads();
+    if constexpr (kPair) cluster_sync();
     if (warp == 9) {
         tc5::fence_after_sync();
-        tc5::dealloc(tmem, kColumns);
+        if constexpr (kPair) tc5::dealloc_pair(tmem, kColumns);
+        else tc5::dealloc(tmem, kColumns);
     }
 }
 
-size_t smem_of(int tokens, int split, int stages) {
-    const size_t parts = split > 1 ? (size_t)(tokens + split) * kFeatures * 4 : 0;
-    return 1024 + (size_t)stages * (kWeightBytes + tokens * kDepth) + kTail + parts;
+// Results in shared memory: sums of the whole tile, or two buffers of 32 tokens (16-bit
+// results or sums).
+int parts_bytes_of(int tokens, int split, bool pieces) {
+    return (split > 1 ? tokens : 64) * kFeatures * (pieces ? 2 : 4);
+}
+size_t smem_of(int tokens, int split, bool pair, int chunks, bool pieces, int stages) {
+    const int rows = pair ? tokens / 2 : tokens;
+    return 1024 + (size_t)stages * chunks * (kWeightBytes + rows * kChunk) + kTail +
+           parts_bytes_of(tokens, split, pieces) + kScaleBytes;
 }
 
-template <typename T>
+template <typename T, bool kPair, int kChunks>
 cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& map_w,
-                   const CUtensorMap& map_x, cudaStream_t st) {
-    auto kernel = product_kernel<T>;
+                   const CUtensorMap& map_x, const CUtensorMap& map_out, cudaStream_t st) {
+    auto kernel = product_kernel<T, kPair, kChunks>;
     // the attribute is the kernel's on one device: set once for each
     static std::atomic<unsigned long long> set{0};
     int dev = 0;
@@ -421,7 +749,7 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = plan.split;
+    attr[1].val.clusterDim.x = kPair ? 2 : plan.split;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(plan.ctas);
@@ -429,56 +757,86 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
     cfg.dynamicSmemBytes = plan.smem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = plan.split > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, w);
+    cfg.numAttrs = kPair || plan.split > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, map_out, w);
 }
 
 }  // namespace
 
-ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, int sms) {
-    const int64_t blocks = (width + kDepth - 1) / kDepth;
-    const int64_t tiles_n = (features + kFeatures - 1) / kFeatures;
+// Which tile, and how many CTAs share it: the plan whose time, in microseconds by the
+// measurements below, is the shortest.
+//   * A chunk of a tile of n tokens takes 0.14 + n / 1000 (the issuing thread, then the
+//     tensor cores: 16 tokens 0.18, 160 0.30), of a pair's 0.155 + n / 1000; at least
+//     its bytes at 115 GB/s an SM (from the L2), and where every weight is read once, all
+//     CTAs' weights at 6.3 TB/s.
+//   * A tile's end takes 0.5, a pair's 1 (4853 x 896 -> 9728: 51 us with single CTAs, 60
+//     with pairs; 16384 x 4096 -> 8192: 457 and 415).
+//   * Sharing a tile costs 0.9 + n / 40 (64 x 8192 -> 2048: 16.3 us alone, 13.3 by two,
+//     10.4 by four CTAs; 64 x 2048 -> 2560: 7.1, 7.8 and 7.4).
+ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool wide_stores,
+                         int sms) {
+    const int64_t chunks = (width + kChunk - 1) / kChunk;
     ProductPlan best{};
-    double best_cost = 0;
-    for (int split = 1; split <= kMaxSplit && split <= blocks; split *= 2) {
-        const int units = sms / split;
-        if (units == 0) break;
-        for (int tokens = 16; tokens <= (split > 1 ? 128 : kMaxTokens); tokens += 16) {
-            if (tokens != 16 && tokens - 16 >= num_tokens) break;
-            const int64_t tiles = tiles_n * ((num_tokens + tokens - 1) / tokens);
-            const int64_t rounds = (tiles + units - 1) / units;
-            // cycles of a stage: the tensor cores' or the copies', whichever is longer
-            const double mma = 2.0 * tokens, copy = (kWeightBytes + tokens * kDepth) / 32.0;
-            const double per = (double)((blocks + split - 1) / split) * (mma > copy ? mma : copy);
-            const double cost = rounds * (per + 300) + (split > 1 ? 1500 + 4.0 * tokens : 0);
-            if (best_cost == 0 || cost < best_cost) {
-                best_cost = cost;
-                best.tile_tokens = tokens;
-                best.split = split;
-                best.ctas = (int)(tiles < units ? tiles : units) * split;
-            }
+    double best_time = 0;
+    auto consider = [&](int split, bool pair, int tokens) {
+        const int per_cta = pair ? 2 * kFeatures : kFeatures, cluster = pair ? 2 : split;
+        const int units = sms / cluster;
+        if (units == 0) return;
+        const int64_t tiles_t = (num_tokens + tokens - 1) / tokens;
+        const int64_t tiles = (features + per_cta - 1) / per_cta * tiles_t;
+        const int64_t rounds = (tiles + units - 1) / units;
+        const int ctas = (int)(tiles < units ? tiles : units) * cluster;
+        double chunk = (pair ? 0.155 : 0.14) + tokens * 1e-3;
+        const double copy = (kWeightBytes + (pair ? tokens / 2 : tokens) * kChunk) / 115e3;
+        if (copy > chunk) chunk = copy;
+        const double stream = tiles_t > 1 ? 0 : ctas * (double)kWeightBytes / 6.3e6;
+        if (stream > chunk) chunk = stream;
+        double time = rounds * ((double)((chunks + split - 1) / split) * chunk + (pair ? 1.0 : 0.5));
+        if (pair) time += 1.7;
+        if (split > 1) time += rounds * (0.9 + tokens / 40.0);
+        if (best_time == 0 || time < best_time) {
+            best_time = time;
+            best.tile_tokens = tokens;
+            best.split = split;
+            best.pair = pair;
+            best.ctas = ctas;
         }
+    };
+    for (int tokens = 16; tokens <= kMaxTokens; tokens += 16) {
+        if (tokens != 16 && tokens - 16 >= num_tokens) break;
+        for (int split = 1; split <= (tokens <= 128 ? kMaxSplit : 1) && 2 * split <= chunks + 1;
+             split *= 2)
+            consider(split, false, tokens);
+        if (tokens % 32 == 0 && tokens >= 64) consider(1, true, tokens);
     }
+    best.chunks = best.pair || best.tile_tokens < 128 || best.split > 1 ? 2 : 1;
+    best.pieces = best.split == 1 && wide_stores;
     int stages = kMaxStages;
-    while (smem_of(best.tile_tokens, best.split, stages) > 232448) --stages;
+    auto smem = [&] {
+        return smem_of(best.tile_tokens, best.split, best.pair, best.chunks, best.pieces, stages);
+    };
+    while (smem() > 232448) --stages;
     best.stages = stages;
     // One CTA an SM, also where two would fit: each takes all tensor memory, and two
     // clusters could otherwise wait for one another's.
-    best.smem = smem_of(best.tile_tokens, best.split, stages);
-    if (best.smem < 120 * 1024) best.smem = 120 * 1024;
+    best.smem = smem() < 120 * 1024 ? 120 * 1024 : smem();
     return best;
 }
 
 cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
-                           const CUtensorMap& map_w, const CUtensorMap& map_x, bool overlap,
-                           unsigned wait_limit, cudaStream_t st) {
+                           const CUtensorMap& map_w, const CUtensorMap& map_x,
+                           const CUtensorMap& map_out, bool overlap, unsigned wait_limit,
+                           cudaStream_t st) {
     Work w{};
     w.p = p;
     w.tile_tokens = plan.tile_tokens;
-    w.blocks = (p.width + kDepth - 1) / kDepth;
+    const int depth = plan.chunks * kChunk;
+    w.depths = (p.width + depth - 1) / depth;
+    w.groups = (p.width + kChunk - 1) / kChunk;
     w.stages = plan.stages;
     w.split = plan.split;
-    w.tiles_n = (int)((p.features + kFeatures - 1) / kFeatures);
+    const int per_cta = plan.pair ? 2 * kFeatures : kFeatures;
+    w.tiles_n = (int)((p.features + per_cta - 1) / per_cta);
     w.tiles_t = (int)((p.num_tokens + plan.tile_tokens - 1) / plan.tile_tokens);
     w.band = w.tiles_t < 8 ? w.tiles_t : 8;
     w.wait_limit = wait_limit;
@@ -486,13 +844,26 @@ cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductP
     auto words = [](const uint8_t* s, long long stride) {
         return reinterpret_cast<uintptr_t>(s) % 4 == 0 && stride % 4 == 0;
     };
-    w.x_words = words(p.x_scales, p.x_scales_stride);
-    w.w_words = words(p.weight_scales, p.weight_scales_stride);
-    switch (out_dtype) {
-        case TLB_FLOAT16: return launch<__half>(w, plan, map_w, map_x, st);
-        case TLB_BFLOAT16: return launch<__nv_bfloat16>(w, plan, map_w, map_x, st);
-        default: return launch<float>(w, plan, map_w, map_x, st);
-    }
+    w.words = w.groups % 4 == 0 && words(p.x_scales, p.x_scales_stride) &&
+              words(p.weight_scales, p.weight_scales_stride);
+    w.parts_bytes = parts_bytes_of(plan.tile_tokens, plan.split, plan.pieces);
+    const int e = out_dtype == TLB_FLOAT32 ? 4 : 2;
+    w.aligned = reinterpret_cast<uintptr_t>(p.out) % (4 * e) == 0 && p.out_stride % 4 == 0;
+    w.pieces = plan.pieces;
+    auto start = [&](auto pair, auto chunks) {
+        constexpr bool kPair = decltype(pair)::value;
+        constexpr int kChunks = decltype(chunks)::value;
+        switch (out_dtype) {
+            case TLB_FLOAT16: return launch<__half, kPair, kChunks>(w, plan, map_w, map_x, map_out, st);
+            case TLB_BFLOAT16:
+                return launch<__nv_bfloat16, kPair, kChunks>(w, plan, map_w, map_x, map_out, st);
+            default: return launch<float, kPair, kChunks>(w, plan, map_w, map_x, map_out, st);
+        }
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (plan.pair) return start(std::true_type{}, Two{});
+    return plan.chunks == 1 ? start(std::false_type{}, One{}) : start(std::false_type{}, Two{});
 }
 
 }  // namespace tlb

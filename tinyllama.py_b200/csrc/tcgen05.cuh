@@ -72,16 +72,30 @@ __host__ __device__ constexpr uint32_t idesc_mxf8(int m, int n, int sf) {
 // values of K an instruction, one scale for each row and instruction; issued by
 // one thread. The scale of row r is a byte of tensor-memory column r / 32 of the
 // scales' address, lane r % 32, the same in each of the four groups of 32 lanes.
+//
+// kPair: the two CTAs of a pair as one (cta_group::2), issued by the even one. Each
+// holds 128 rows of A, their scales and sums, half the rows of B, and the scales of
+// all rows of B, at the same addresses.
+template <bool kPair>
 __device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                          uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
                                          bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, "
-        "[%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales),
-        "r"(accumulate ? 1u : 0u)
-        : "memory");
+    if constexpr (kPair)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, "
+            "[%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales),
+            "r"(accumulate ? 1u : 0u)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, "
+            "[%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales),
+            "r"(accumulate ? 1u : 0u)
+            : "memory");
 }
 
 // The mbarrier at `bar` gets one arrival once every tcgen05 operation this
@@ -89,6 +103,15 @@ __device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint6
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile(
         "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+}
+
+// The same for a pair: the mbarriers at `bar` in both CTAs get an arrival.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
         : "memory");
 }
 
@@ -110,6 +133,16 @@ __device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols));
 }
 
+// The same by a warp of each CTA of a pair.
+__device__ __forceinline__ void alloc_pair(uint32_t slot, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot),
+                 "r"(cols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+}
+__device__ __forceinline__ void dealloc_pair(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols));
+}
+
 // 32 consecutive 32-bit columns of this thread's lane (warp w reads lanes
 // 32 w .. 32 w + 31), then waits for the load.
 __device__ __forceinline__ void ld32(uint32_t taddr, float (&v)[32]) {
@@ -126,6 +159,23 @@ __device__ __forceinline__ void ld32(uint32_t taddr, float (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 32 consecutive columns of 16 lanes (lanes 0 .. 15 or 16 .. 31 of the warp's, by the
+// address), in the layout of the mma fragments: thread l gets of columns 8 g .. 8 g + 7
+// v[4 g], v[4 g + 1] = lane l / 4, columns 2 (l % 4), + 1 and v[4 g + 2], v[4 g + 3] =
+// lane l / 4 + 8. Does not wait (ld_wait).
+__device__ __forceinline__ void ld_rows16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+        "%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void ld_wait() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // Stores 4 / 8 consecutive 32-bit columns of this thread's lane (st_wait completes
