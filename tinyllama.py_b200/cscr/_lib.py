@@ -111,7 +111,7 @@ def load():
             if fast is not None:
                 fast.bind(*(ctypes.cast(getattr(lib, entry[0]), ctypes.c_void_p).value
                             for entry in (SCORED_ATTENTION, QUANTIZED_WRITE, DEQUANTIZE,
-                                          QK_NORM_ROPE)))
+                                          QK_NORM_ROPE, QUANTIZE_ROWS, MATMUL_QUANTIZED)))
     return _lib
 
 

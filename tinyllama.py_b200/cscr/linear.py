@@ -56,6 +56,10 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float,
     [T, ceil(K / 128)] float8_e8m0fnu, h or None): h goes to ``residual_out``, which
     may be ``residual`` or ``x`` itself, or a new tensor.
     """
+    if _lib.fast is not None:
+        out = _lib.fast.rows(x, _RMS_NORM, weight, eps, residual, residual_out)
+        if out is not None:
+            return out
     index = _check_rows(x, "x")
     rows, width = x.shape
     dtype = x.dtype
@@ -89,6 +93,10 @@ def silu_and_mul_quantized(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.T
     gate values, then its up values (float16, bfloat16 or float32, rows possibly
     strided). Returns (values [T, K], scales [T, ceil(K / 128)]); fp32 math, one
     rounding. Results below 2^-126 in magnitude may count as 0."""
+    if _lib.fast is not None:
+        out = _lib.fast.rows(gate_up, _SILU_AND_MUL, None, 0.0, None, None)
+        if out is not None:
+            return out
     index = _check_rows(gate_up, "gate_up")
     rows, both = gate_up.shape
     torch_check(both % 2 == 0, "gate_up must hold as many gate as up values")
@@ -103,6 +111,10 @@ def silu_and_mul_quantized(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.T
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The rows of x [T, K] (float16, bfloat16 or float32, rows possibly strided) in 8
     bits: (values [T, K], scales [T, ceil(K / 128)])."""
+    if _lib.fast is not None:
+        out = _lib.fast.rows(x, _PLAIN, None, 0.0, None, None)
+        if out is not None:
+            return out
     index = _check_rows(x, "x")
     rows, width = x.shape
     q, scales = _rows_out(x, rows, width)
@@ -180,6 +192,11 @@ def matmul_quantized(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tens
     stream writes neither weight nor weight_scales: they are then read while that
     kernel ends (x, x_scales and bias are not).
     """
+    if _lib.fast is not None:
+        out = _lib.fast.product(x, x_scales, weight, weight_scales, out_dtype, bias,
+                                overlap_prologue)
+        if out is not None:
+            return out
     index, shape, wshape = x.get_device(), x.shape, weight.shape
     sshape, wsshape = x_scales.shape, weight_scales.shape
     if not (index >= 0 and len(shape) == 2 and len(wshape) == 2 and len(sshape) == 2

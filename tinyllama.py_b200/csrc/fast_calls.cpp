@@ -1,5 +1,5 @@
-// cscr._fast: the ordinary calls of the 8-bit cache, norm and scored-attention
-// ops without their Python argument handling.
+// cscr._fast: the ordinary calls of the 8-bit cache, norm, scored-attention and 8-bit
+// projection ops without their Python argument handling.
 //
 // Each function takes the op's tensors, looks them over, allocates the results
 // and calls the C ABI's entry point: about 5 us of host time less than the same
@@ -33,6 +33,8 @@ int (*g_attention)(const tlb_scored_attention_args*, void*) = nullptr;
 int (*g_write)(const tlb_quantized_write_args*, void*) = nullptr;
 int (*g_read)(const tlb_dequantize_args*, void*) = nullptr;
 int (*g_norm)(const tlb_qk_norm_rope_args*, void*) = nullptr;
+int (*g_rows)(const tlb_quantize_rows_args*, void*) = nullptr;
+int (*g_product)(const tlb_matmul_quantized_args*, void*) = nullptr;
 
 // Scratch of the attention op: owned by the Python side, one for each stream.
 struct Scratch {
@@ -383,15 +385,143 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(attention, write, read, norm): addresses of the library's entry points
+// [T, K] on this device, each row contiguous.
+bool rows_of(const Place& at, const Tensor* x) {
+    return x != nullptr && x->is_cuda() && x->get_device() == at.device && x->dim() == 2 &&
+           x->size(1) > 0 && (x->stride(1) == 1 || x->size(1) == 1);
+}
+int64_t groups_of(int64_t width) { return (width + 127) / 128; }
+
+// rows(x, op, weight, eps, residual, residual_out): (values, scales), and what the norm
+// returns as its third: residual_out, a new one, or None
+PyObject* rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6 || g_rows == nullptr) return later();
+    const Tensor *x = tensor(a[0]), *w = tensor(a[2]), *res = tensor(a[4]), *out = tensor(a[5]);
+    int64_t op;
+    double eps;
+    if (x == nullptr || !whole(a[1], &op) || !number(a[3], &eps)) return later();
+    const Place at(*x);
+    const ScalarType type = x->scalar_type();
+    if (!at.ok() || !rows_of(at, x) || !is_float(type) || x->size(0) == 0) return later();
+    const int64_t T = x->size(0), K = op == TLB_ROWS_SILU_AND_MUL ? x->size(1) / 2 : x->size(1);
+    tlb_quantize_rows_args p{};
+    Tensor h;
+    if (op == TLB_ROWS_RMS_NORM) {
+        if (!at.has(w) || w->dim() != 1 || w->size(0) != K || w->scalar_type() != type ||
+            !(eps >= 0))
+            return later();
+        p.weight = w->data_ptr();
+        if (res != nullptr) {
+            if (!rows_of(at, res) || res->sizes() != x->sizes() || res->scalar_type() != type)
+                return later();
+            if (out != nullptr) {
+                if (!rows_of(at, out) || out->sizes() != x->sizes() ||
+                    out->scalar_type() != type || (T > 1 && out->stride(0) < K))
+                    return later();
+                h = *out;
+            } else {
+                if (a[5] != Py_None) return later();
+                h = dense(*x, x->sizes(), type);
+            }
+            p.residual = res->data_ptr();
+            p.residual_stride = res->stride(0);
+            p.residual_out = h.data_ptr();
+            p.residual_out_stride = h.stride(0);
+        } else if (a[4] != Py_None || a[5] != Py_None) {
+            return later();
+        }
+    } else if (op == TLB_ROWS_SILU_AND_MUL && x->size(1) != 2 * K) {
+        return later();
+    }
+    Tensor q = dense(*x, {T, K}, ScalarType::Float8_e4m3fn),
+           s = dense(*x, {T, groups_of(K)}, ScalarType::Float8_e8m0fnu);
+    p.out = q.data_ptr();
+    p.scales = s.data_ptr();
+    p.x = x->data_ptr();
+    p.op = op;
+    p.num_rows = T;
+    p.width = K;
+    p.x_stride = x->stride(0);
+    p.dtype = code_of(type);
+    p.eps = eps;
+    if (g_rows(&p, at.stream) != TLB_OK) return later();
+    PyObject *pq = THPVariable_Wrap(std::move(q)), *ps = THPVariable_Wrap(std::move(s));
+    PyObject* all = nullptr;
+    if (op != TLB_ROWS_RMS_NORM) {
+        if (pq && ps) all = PyTuple_Pack(2, pq, ps);
+    } else if (res == nullptr || out != nullptr) {
+        if (pq && ps) all = PyTuple_Pack(3, pq, ps, res == nullptr ? Py_None : a[5]);
+    } else {
+        PyObject* ph = THPVariable_Wrap(std::move(h));
+        if (pq && ps && ph) all = PyTuple_Pack(3, pq, ps, ph);
+        Py_XDECREF(ph);
+    }
+    Py_XDECREF(pq);
+    Py_XDECREF(ps);
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// product(x, x_scales, weight, weight_scales, out_dtype, bias, overlap)
+PyObject* product(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7 || g_product == nullptr) return later();
+    const Tensor *x = tensor(a[0]), *xs = tensor(a[1]), *w = tensor(a[2]), *ws = tensor(a[3]),
+                 *bias = tensor(a[5]);
+    bool overlap;
+    if (x == nullptr || !THPDtype_Check(a[4]) || !truth(a[6], &overlap)) return later();
+    const ScalarType type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+    const Place at(*x);
+    if (!at.ok() || !is_float(type) || !rows_of(at, x) || !rows_of(at, w) || !rows_of(at, xs) ||
+        !rows_of(at, ws) || x->scalar_type() != ScalarType::Float8_e4m3fn ||
+        w->scalar_type() != ScalarType::Float8_e4m3fn ||
+        xs->scalar_type() != ScalarType::Float8_e8m0fnu ||
+        ws->scalar_type() != ScalarType::Float8_e8m0fnu)
+        return later();
+    const int64_t T = x->size(0), K = x->size(1), N = w->size(0), G = groups_of(K);
+    if (T == 0 || N == 0 || w->size(1) != K || xs->size(0) != T || xs->size(1) != G ||
+        ws->size(0) != groups_of(N) || ws->size(1) != G)
+        return later();
+    if (bias != nullptr ? !at.has(bias) || bias->dim() != 1 || bias->size(0) != N ||
+                              bias->scalar_type() != type
+                        : a[5] != Py_None)
+        return later();
+    Tensor out = dense(*x, {T, N}, type);
+    tlb_matmul_quantized_args p{};
+    p.out = out.data_ptr();
+    p.x = x->data_ptr();
+    p.x_scales = xs->data_ptr();
+    p.weight = w->data_ptr();
+    p.weight_scales = ws->data_ptr();
+    p.bias = bias ? bias->data_ptr() : nullptr;
+    p.num_tokens = T;
+    p.width = K;
+    p.features = N;
+    p.x_stride = x->stride(0);
+    p.x_scales_stride = xs->stride(0);
+    p.weight_stride = w->stride(0);
+    p.weight_scales_stride = ws->stride(0);
+    p.out_stride = N;
+    p.out_dtype = code_of(type);
+    p.flags = overlap ? TLB_PRODUCT_OVERLAP_PROLOGUE : 0;
+    if (g_product(&p, at.stream) != TLB_OK) return later();
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// bind(attention, write, read, norm, rows, product): addresses of the library's entry
+// points
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    void* p[4] = {};
-    for (Py_ssize_t i = 0; i < 4 && i < n; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+    void* p[6] = {};
+    for (Py_ssize_t i = 0; i < 6 && i < n; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
     g_attention = reinterpret_cast<decltype(g_attention)>(p[0]);
     g_write = reinterpret_cast<decltype(g_write)>(p[1]);
     g_read = reinterpret_cast<decltype(g_read)>(p[2]);
     g_norm = reinterpret_cast<decltype(g_norm)>(p[3]);
+    g_rows = reinterpret_cast<decltype(g_rows)>(p[4]);
+    g_product = reinterpret_cast<decltype(g_product)>(p[5]);
     Py_RETURN_NONE;
 }
 
@@ -417,7 +547,8 @@ PyObject* scratch(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define TLB_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), \
                        METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TLB_METHOD(attention), TLB_METHOD(write), TLB_METHOD(read),
-                         TLB_METHOD(norm),      TLB_METHOD(bind),  TLB_METHOD(scratch),
+                         TLB_METHOD(norm),      TLB_METHOD(rows),  TLB_METHOD(product),
+                         TLB_METHOD(bind),      TLB_METHOD(scratch),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
