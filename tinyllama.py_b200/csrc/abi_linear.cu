@@ -165,7 +165,8 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
                               plan.pair ? plan.tile_tokens / 2 : plan.tile_tokens, &map_x))
             return rc;
         if (plan.pieces)
-            if (int rc = rows_map(a.out, a.num_tokens, a.features, out_stride * 2, 2, 32, 16, &map_out))
+            if (int rc = rows_map(a.out, a.num_tokens, a.features, out_stride * 2, 2, 32,
+                                  plan.tile_tokens % 32 == 0 ? 32 : 16, &map_out))
                 return rc;
         return cuda_result(
             tlb::launch_product((int)a.out_dtype, p, plan, map_w, map_x, map_out,

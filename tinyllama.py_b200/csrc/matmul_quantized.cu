@@ -15,9 +15,9 @@
 // features as one, each fetching half of the tokens' rows.
 //
 // Warps of a CTA: 0-3 bring the scales to tensor memory (each the 32 lanes it can
-// reach), 4-7 read the sums and write the results, 8 issues the TMA copies (one or
-// two chunks of 128 of K a stage), 9 the tensor instructions. The accumulator is double buffered: a tile
-// is written out while the next one is summed.
+// reach), 4-11 read the sums and write the results, 12 issues the TMA copies (one or
+// two chunks of 128 of K a stage), 13 the tensor instructions. The accumulator is
+// double buffered: a tile is written out while the next one is summed.
 #include <atomic>
 #include <type_traits>
 
@@ -33,7 +33,9 @@ constexpr int kFeatures = 128;             // of a CTA's tile (M)
 constexpr int kChunk = 128;                // bytes of K of a shared-memory row
 constexpr int kMaxTokens = 224;            // of a tile (N): two accumulators and the scales
 constexpr int kWeightBytes = kFeatures * kChunk;  // of a chunk
-constexpr int kThreads = 320;
+constexpr int kThreads = 448;
+constexpr int kResultWarps = 8, kResultThreads = 32 * kResultWarps;
+constexpr int kCopyWarp = 12, kTensorWarp = 13;
 constexpr int kMaxStages = 12;
 constexpr int kScaleSets = 4;              // sets of scales in tensor memory, a word each
 constexpr int kSetColumns = 12;            // 4 of the weights, 8 of the tokens
@@ -130,16 +132,16 @@ __device__ __forceinline__ void tile_at(const Work& w, int i, int& tn, int& tt) 
     tt = b * w.band + rest % height;
 }
 
-// Whether `ok` holds in every thread of four warps. They meet at barriers, so they go
-// on or give up together.
-template <int kBarrier>
+// Whether `ok` holds in every thread of the kCount that meet at a barrier: they go on or
+// give up together.
+template <int kBarrier, int kCount>
 __device__ __forceinline__ bool all_agree(bool ok) {
     uint32_t all;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        "barrier.cta.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(all)
-        : "r"(ok ? 1u : 0u), "n"(kBarrier)
+        : "r"(ok ? 1u : 0u), "n"(kBarrier), "n"(kCount)
         : "memory");
     return all != 0;
 }
@@ -214,7 +216,7 @@ __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uin
             const int count = min(kWordsAtOnce, word_end - first);
             for (int k = 0; k < count; ++k) {
                 // a CTA's warps give up together: they meet at the barrier above
-                if (!all_agree<2>(mbar_wait_bounded(tail + 8u * (kBarScalesFree + set), parity,
+                if (!all_agree<2, 128>(mbar_wait_bounded(tail + 8u * (kBarScalesFree + set), parity,
                                                     w.wait_limit)))
                     return false;
                 tc5::fence_after_sync();
@@ -255,17 +257,20 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, 
 // tokens and turned round by stmatrix, so that a token's 32 features lie side by side
 // in shared memory (the 64-byte swizzle: unit u of 16 bytes at u ^ token / 2 % 4, free
 // of bank conflicts); a TMA store takes them from there, past the tensor's ends as
-// well. Each warp has two buffers of its own, so the warps do not wait for one another;
-// the next sums are read under the stores. (Written by the lanes, 32 tokens took 640
-// cycles, more than the instructions of a tile 896 wide.)
+// well. The warps of a feature quarter take every other 32 tokens; each has two buffers
+// of its own (`turn` is the next), so the warps do not wait for one another; the next
+// sums are read under the stores. 32 tokens take about 500 cycles of a warp (640 written
+// by the lanes): with four warps, more than the instructions of a tile 1024 wide.
 template <typename T>
 __device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* map, uint32_t sums,
                                              uint32_t stage, long long n0, long long t0, int here,
-                                             int quarter, int lane) {
+                                             int warp, int lane, uint32_t& turn) {
     if constexpr (sizeof(T) == 2) {
         const ProductParams& p = w.p;
-        n0 += quarter * 32;
-        if (n0 >= p.features) return;
+        const int first = (warp >> 2) * 32;  // of this warp's tokens
+        n0 += (warp & 3) * 32;
+        if (n0 >= p.features || first >= here) return;
+        const int box = w.tile_tokens % 32 == 0 ? 32 : 16;  // of the map
         float bias[4] = {};
         if (p.bias)
 #pragma unroll
@@ -273,15 +278,14 @@ __device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* m
                 const long long n = n0 + 8 * i + (lane >> 2);
                 if (n < p.features) bias[i] = Elem<T>::to_f(reinterpret_cast<const T*>(p.bias)[n]);
             }
-        const uint32_t buf = stage + quarter * 4096;  // two of 2 KB
+        const uint32_t buf = stage + warp * 4096;  // two of 2 KB
         // token 8 g + lane % 8, unit lane / 8
         const uint32_t put = buf + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
         uint32_t a[16], c[16];
-        tc5::ld_rows16(sums, a);
-        tc5::ld_rows16(sums + (16u << 16), c);
+        tc5::ld_rows16(sums + first, a);
+        tc5::ld_rows16(sums + first + (16u << 16), c);
 #pragma unroll 1
-        for (int j = 0; j < here; j += 32) {
-            const uint32_t half = (j & 32) << 6;
+        for (int j = first; j < here; j += 64, turn ^= 2048) {
             tc5::ld_wait();
             uint32_t m[16];
 #pragma unroll
@@ -292,9 +296,9 @@ __device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* m
                     m[4 * g + i] = pack2<T>(__uint_as_float(v[0]) + bias[i],
                                             __uint_as_float(v[1]) + bias[i]);
                 }
-            if (j + 32 < here) {
-                tc5::ld_rows16(sums + j + 32, a);
-                tc5::ld_rows16(sums + j + 32 + (16u << 16), c);
+            if (j + 64 < here) {
+                tc5::ld_rows16(sums + j + 64, a);
+                tc5::ld_rows16(sums + j + 64 + (16u << 16), c);
             }
             // the store before the last one has read this buffer
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -303,15 +307,16 @@ __device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* m
             for (int g = 0; g < 4; ++g)
                 asm volatile(
                     "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
-                        put + half + 512 * g),
+                        put + turn + 512 * g),
                     "r"(m[4 * g]), "r"(m[4 * g + 1]), "r"(m[4 * g + 2]), "r"(m[4 * g + 3])
                     : "memory");
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                store_box(map, (int)n0, (int)t0 + j, buf + half);
-                // of 16 tokens: a tile may end there
-                if (j + 16 < w.tile_tokens) store_box(map, (int)n0, (int)t0 + j + 16, buf + half + 1024);
+                store_box(map, (int)n0, (int)t0 + j, buf + turn);
+                // of 16 tokens where a tile may end after them
+                if (box == 16 && j + 16 < w.tile_tokens)
+                    store_box(map, (int)n0, (int)t0 + j + 16, buf + turn + 1024);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
         }
@@ -326,7 +331,7 @@ __device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* m
 template <typename T>
 __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8_t* stage,
                                              uint32_t parts, uint32_t bar, uint32_t parity,
-                                             long long n0, long long t0, int here, int quarter,
+                                             long long n0, long long t0, int here, int warp,
                                              int lane, int rank) {
     const ProductParams& p = w.p;
     const int split = w.split, f0 = lane * 4;
@@ -337,13 +342,12 @@ __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8
         for (int k = 0; k < 4; ++k)
             if (k < wide) bias[k] = Elem<T>::to_f(reinterpret_cast<const T*>(p.bias)[n0 + f0 + k]);
     T* out = reinterpret_cast<T*>(p.out) + t0 * p.out_stride + n0 + f0;
-    // tokens at a time: all of a cluster's tile, else 32 in either of two buffers
-    const int rows = split > 1 ? w.tile_tokens : 32;
+    // tokens at a time: all of a cluster's tile, else 64
+    const int rows = split > 1 ? w.tile_tokens : 64;
+    float* column = reinterpret_cast<float*>(stage) + (warp & 3) * 32 + lane;
     for (int j0 = 0; j0 < here; j0 += rows) {
         const int count = min(rows, here - j0);
-        const uint32_t offset = split > 1 ? 0u : (uint32_t)(j0 & 32) * (kFeatures * 4);
-        float* column = reinterpret_cast<float*>(stage + offset) + quarter * 32 + lane;
-        for (int j = 0; j < count; j += 32) {
+        for (int j = (warp >> 2) * 32; j < count; j += 64) {
             float v[32];
             tc5::ld32(sums + j0 + j, v);
 #pragma unroll
@@ -357,12 +361,12 @@ __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8
             mine = max(0, min(share, count - first));
             __syncwarp();
             if (lane < split) arrive_cluster(map_rank(bar, lane));
-            if (!all_agree<1>(wait_cluster(bar, parity, w.wait_limit))) return false;
+            if (!all_agree<1, kResultThreads>(wait_cluster(bar, parity, w.wait_limit))) return false;
         } else {
-            named_bar_sync(1, 128);
+            named_bar_sync(1, kResultThreads);
         }
-        const uint32_t from = parts + offset + f0 * 4;
-        for (int r0 = quarter; r0 < mine; r0 += 8) {  // two rows of all CTAs in flight
+        const uint32_t from = parts + f0 * 4;
+        for (int r0 = warp; r0 < mine; r0 += 2 * kResultWarps) {  // two rows of all CTAs in flight
             float4 v[2], x[kMaxSplit][2];
 #pragma unroll
             for (int c = 0; c < kMaxSplit; ++c) {
@@ -370,7 +374,8 @@ __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8
                 const uint32_t at = split > 1 ? map_rank(from, c) : from;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    x[c][k] = load_cluster(at + (first + min(r0 + 4 * k, mine - 1)) * (kFeatures * 4));
+                    x[c][k] = load_cluster(at + (first + min(r0 + kResultWarps * k, mine - 1)) *
+                                                    (kFeatures * 4));
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -386,7 +391,7 @@ __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int row = r0 + 4 * k;
+                const int row = r0 + kResultWarps * k;
                 if (row >= mine) break;
                 T* to = out + (j0 + first + row) * p.out_stride;
                 const float y[4] = {v[k].x + bias[0], v[k].y + bias[1], v[k].z + bias[2],
@@ -404,6 +409,7 @@ __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8
                 }
             }
         }
+        if (j0 + rows < here) named_bar_sync(1, kResultThreads);  // read before it is written again
     }
     return true;
 }
@@ -446,18 +452,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(kBarSums + i), 1);
-            mbar_init(bar(kBarSumsFree + i), kPair ? 8 : 4);
+            mbar_init(bar(kBarSumsFree + i), (kPair ? 2 : 1) * kResultWarps);
         }
-        mbar_init(bar(kBarParts), 4 * split);
-        mbar_init(bar(kBarPartsFree), 4 * split);
+        mbar_init(bar(kBarParts), kResultWarps * split);
+        mbar_init(bar(kBarPartsFree), kResultWarps * split);
         mbar_init(bar(kBarDrain), 1);
         fence_mbar_init();
     }
-    if (warp == 9) {
+    if (warp == kTensorWarp) {
         if constexpr (kPair) tc5::alloc_pair(tail + kSlot, kColumns);
         else tc5::alloc(tail + kSlot, kColumns);
     }
-    if (tid == 256) {
+    if (tid == 32 * kCopyWarp) {
         prefetch_tensormap(&map_w);
         prefetch_tensormap(&map_x);
     }
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     bool ok = true;
 
-    if (warp == 8) {
+    if (warp == kCopyWarp) {
         // ------------------------------------------------------------ copies
         if (elect_one()) {
             const uint64_t keep = l2_policy_evict_last();
@@ -556,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 load_tokens(base + issued * stage_bytes, full0 + 8 * issued, 0, 0);
             *reinterpret_cast<volatile int*>(tail_ptr + kIssued) = issued;
         }
-    } else if (warp == 9) {
+    } else if (warp == kTensorWarp) {
         // ------------------------------------------------ tensor instructions
         if ((!kPair || rank == 0) && elect_one()) {
             auto commit = [](uint32_t b) {
@@ -636,8 +642,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // ----------------------------------------------------------- results
         grid_dependency_wait();
-        const int quarter = warp & 3;
+        const int mine = warp - 4;
         uint8_t* stage = tail_ptr + kTail;
+        uint32_t turn = 0;
         int it = 0;
         for (int i = unit; i < tiles; i += units, ++it) {
             int tn, tt;
@@ -646,20 +653,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             const long long t0 = (long long)tt * w.tile_tokens;
             const int here = (int)min((long long)w.tile_tokens, p.num_tokens - t0);
             const int b = it & 1;
-            const uint32_t sums = tmem + ((uint32_t)quarter << 21) + b * kMaxTokens;
+            const uint32_t sums = tmem + ((uint32_t)(warp & 3) << 21) + b * kMaxTokens;
             ok = mbar_wait_bounded(bar(kBarSums + b), (it >> 1) & 1, limit);
             if (split > 1 && it > 0)
                 ok = wait_cluster(bar(kBarPartsFree), (it - 1) & 1, limit) && ok;
-            if (!all_agree<1>(ok)) {
-                ok = false;
-                break;
-            }
-            tc5::fence_after_sync();
-            if (w.pieces)
-                store_pieces<T>(w, &map_out, sums, parts, n0, t0, here, quarter, lane);
-            else
+            if (w.pieces) {
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc5::fence_after_sync();
+                store_pieces<T>(w, &map_out, sums, parts, n0, t0, here, mine, lane, turn);
+            } else {
+                ok = all_agree<1, kResultThreads>(ok);
+                if (!ok) break;
+                tc5::fence_after_sync();
                 ok = store_joined<T>(w, sums, stage, parts, bar(kBarParts), it & 1, n0, t0, here,
-                                     quarter, lane, rank);
+                                     mine, lane, rank);
+            }
             tc5::fence_before_sync();
             __syncwarp();
             if (lane == 0) {
@@ -712,17 +721,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     if constexpr (kPair) cluster_sync();
-    if (warp == 9) {
+    if (warp == kTensorWarp) {
         tc5::fence_after_sync();
         if constexpr (kPair) tc5::dealloc_pair(tmem, kColumns);
         else tc5::dealloc(tmem, kColumns);
     }
 }
 
-// Results in shared memory: sums of the whole tile, or two buffers of 32 tokens (16-bit
-// results or sums).
+// Results in shared memory: two buffers of 2 KB a warp, or sums of the whole tile or of
+// 64 tokens.
 int parts_bytes_of(int tokens, int split, bool pieces) {
-    return (split > 1 ? tokens : 64) * kFeatures * (pieces ? 2 : 4);
+    return pieces ? kResultWarps * 4096 : (split > 1 ? tokens : 64) * kFeatures * 4;
 }
 size_t smem_of(int tokens, int split, bool pair, int chunks, bool pieces, int stages) {
     const int rows = pair ? tokens / 2 : tokens;
