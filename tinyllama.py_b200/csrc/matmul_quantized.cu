@@ -99,6 +99,10 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The same where nothing written before has to be seen: a release waits for it.
+__device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, uint32_t limit) {
     for (uint32_t i = 0; i < limit; ++i) {
         uint32_t ok;
@@ -672,7 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc5::fence_before_sync();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (kPair) arrive_cluster(map_rank(bar(kBarSumsFree + b), 0));
+                // the sums have been read (wait::ld); nothing was written for the other CTA
+                if constexpr (kPair) arrive_cluster_relaxed(map_rank(bar(kBarSumsFree + b), 0));
                 else mbar_arrive(bar(kBarSumsFree + b));
             }
             if (!ok) break;
