@@ -27,10 +27,10 @@ __device__ __forceinline__ float add_keep(float a, float b) {
     asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-// silu(g) * u. exp(-|g|) never overflows; values below 2^-126 may come out as 0.
+// silu(g) * u as g / (1 + exp(-g)) * u: 0 where exp(-g) is infinite. The quotient counts
+// denominators from 2^126 on as infinite (g below -87).
 __device__ __forceinline__ float silu_mul(float g, float u) {
-    const float e = __expf(-fabsf(g));
-    return __fdividef(g < 0.f ? g * e : g, 1.f + e) * u;
+    return __fdividef(g, 1.f + __expf(-g)) * u;
 }
 
 // Eight fp32 values of a lane -> their 8 stored bytes, and the scale byte of the
@@ -49,46 +49,85 @@ __device__ __forceinline__ uint2 quantize_group(const float (&f)[8], uint32_t ma
     return quantized8<E4M3, false>(f, inverse_scale(byte));
 }
 
+// A plain group's lane: eight elements as read. The magnitudes are compared, and fp16
+// values converted, in pairs (as in the cache write).
+template <typename T>
+__device__ __forceinline__ uint2 quantize_raw(const Raw8<T>& x, uint32_t mask, uint32_t& byte) {
+    const uint32_t top = group_top<kLanes, T>(x.top(), mask);
+    if (top < 0x7f800000u) {
+        byte = scale_byte<E4M3>(top);
+        if constexpr (std::is_same<T, __half>::value) {
+            if (byte >= 112)  // 2^-E is an fp16 number (E >= -15)
+                return quantized8_half<E4M3>(x.u[0],
+                                             __half2half2(__float2half_rn(inverse_scale(byte))));
+        }
+        float f[8];
+        x.get(f);
+        return quantized8<E4M3, true>(f, inverse_scale(byte));
+    }
+    float f[8];
+    x.get(f);
+    byte = scale_byte<E4M3>(group_max<kLanes>(max_finite8(f), mask));
+    return quantized8<E4M3, false>(f, inverse_scale(byte));
+}
+
+// x / d for x < 2^31 and d < 2^31 by a product with the inverse (the round-up method for
+// invariant divisors): 32-bit division took a fifth of these kernels' instructions.
+struct FastDivisor {
+    uint32_t by, inverse;
+    int shift;
+    FastDivisor() = default;
+    explicit FastDivisor(uint32_t d) : by(d), shift(0) {
+        while ((1ull << shift) < d) ++shift;
+        inverse = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t divide(uint32_t x) const {
+        return (__umulhi(x, inverse) + x) >> shift;
+    }
+};
+
 // ------------------------------------------------- plain rows, gated activation
-// Flat over the eight-value pieces of all rows (K a multiple of 128, so a group
-// is half a warp wherever it lies), kSteps pieces of a lane in flight.
+// Flat over the eight-value pieces of all rows (K a multiple of 128, so a group is half
+// a warp wherever it lies), kSteps pieces of a lane in flight. Bounded by HBM and, the
+// gated form, nearly as much by its instructions.
 template <typename T, bool kSilu, int kSteps>
-__global__ void __launch_bounds__(256) quantize_pieces_kernel(const RowQuantParams p) {
+__global__ void __launch_bounds__(256) quantize_pieces_kernel(const RowQuantParams p,
+                                                              const FastDivisor row_pieces,
+                                                              const uint32_t pieces) {
     grid_dependency_wait();
     grid_launch_dependents();
-    const unsigned row_pieces = p.width / 8;
-    const long long pieces = p.num_rows * row_pieces;
     const uint32_t mask = group_mask<kLanes>();
-    const long long step = (long long)gridDim.x * 256 * kSteps;
-    for (long long base = (long long)blockIdx.x * 256 * kSteps + threadIdx.x;
-         base - threadIdx.x < pieces; base += step) {
+    const uint32_t step = gridDim.x * 256 * kSteps;
+    for (uint32_t base = blockIdx.x * 256 * kSteps; base < pieces; base += step) {
         Raw8<T> x[kSteps], u[kSilu ? kSteps : 1];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const long long i = base + s * 256;
+            const uint32_t i = base + s * 256 + threadIdx.x;
             x[s].zero();
             if constexpr (kSilu) u[s].zero();
             if (i < pieces) {
-                int rest;
-                const long long r = divide(i, (int)row_pieces, rest);
-                const T* src = reinterpret_cast<const T*>(p.x) + r * p.x_stride + (long long)rest * 8;
+                const uint32_t r = row_pieces.divide(i);
+                const T* src = reinterpret_cast<const T*>(p.x) + r * p.x_stride +
+                               (i - r * row_pieces.by) * 8;
                 x[s].load_stream(src);
                 if constexpr (kSilu) u[s].load_stream(src + p.width);
             }
         }
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const long long i = base + s * 256;
-            float f[8];
-            x[s].get(f);
+            const uint32_t i = base + s * 256 + threadIdx.x;
+            uint32_t byte;
+            uint2 q;
             if constexpr (kSilu) {
-                float v[8];
+                float f[8], v[8];
+                x[s].get(f);
                 u[s].get(v);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) f[j] = silu_mul(f[j], v[j]);
+                q = quantize_group(f, mask, byte);
+            } else {
+                q = quantize_raw<T>(x[s], mask, byte);
             }
-            uint32_t byte;
-            const uint2 q = quantize_group(f, mask, byte);
             if (i < pieces) {
                 reinterpret_cast<uint2*>(p.out)[i] = q;
                 if ((threadIdx.x & (kLanes - 1)) == 0) p.scales[i / kLanes] = (uint8_t)byte;
@@ -98,8 +137,10 @@ __global__ void __launch_bounds__(256) quantize_pieces_kernel(const RowQuantPara
 }
 
 // ------------------------------------------------------------------- RMS norm
-// A row is held by `warps` warps of a CTA, kPieces pieces a lane, between its one
-// read and its writes; the warps' sums of squares meet in shared memory.
+// A row is held by the warps of a CTA, kPieces pieces a lane, between its one read and
+// its writes; the warps' sums of squares meet in shared memory. (A warp for each short
+// row, eight a CTA, gained nothing: 4853 rows of 896 fp16 5.7 us instead of 6.0, fp32 7.3
+// instead of 6.7.)
 template <typename T, bool kResidual, int kPieces>
 __global__ void rms_norm_kernel(const RowQuantParams p) {
     grid_dependency_wait();
@@ -253,23 +294,36 @@ cudaError_t launch_norm(const RowQuantParams& p, cudaStream_t st) {
     return launch_early(rms_norm_kernel<T, kResidual, 4>, grid, threads(4), 0, st, p);
 }
 
+template <typename T, bool kSilu, int kSteps>
+cudaError_t launch_pieces(const RowQuantParams& p, int sms, cudaStream_t st) {
+    const long long pieces = p.num_rows * (p.width / 8);
+    const long long want = (pieces + 256 * kSteps - 1) / (256 * kSteps), cap = 8ll * sms;
+    return launch_early(quantize_pieces_kernel<T, kSilu, kSteps>,
+                        dim3((unsigned)(want < cap ? want : cap)), 256, 0, st, p,
+                        FastDivisor((uint32_t)(p.width / 8)), (uint32_t)pieces);
+}
+
 template <typename T>
 cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) {
-    // rows of the norm that a CTA holds in registers: 4 pieces of up to 512 threads
-    const bool held = p.op != TLB_ROWS_RMS_NORM || (p.width <= 16384 && p.num_rows < (1ll << 31));
+    // rows of the norm that a CTA holds in registers: 4 pieces of up to 512 threads;
+    // pieces of the others that 32-bit indexes count
+    const bool held = p.op == TLB_ROWS_RMS_NORM
+                          ? p.width <= 16384 && p.num_rows < (1ll << 31)
+                          : p.num_rows * (p.width / 8) < (1ll << 31) - (1 << 24);
     if (!vec || !held) {
         const long long rows = p.num_rows < 8ll * sms ? p.num_rows : 8ll * sms;
         return launch_early(quantize_rows_any_kernel<T>, dim3((unsigned)rows), 256, 0, st, p);
     }
     if (p.op == TLB_ROWS_RMS_NORM)
         return p.residual ? launch_norm<T, true>(p, st) : launch_norm<T, false>(p, st);
-    constexpr int kSteps = sizeof(T) == 2 ? 2 : 1;
-    const long long pieces = p.num_rows * (p.width / 8);
-    const long long want = (pieces + 256 * kSteps - 1) / (256 * kSteps), cap = 8ll * sms;
-    const dim3 grid((unsigned)(want < cap ? want : cap));
+    // 64 bytes of a lane in flight where there are enough pieces (16381 x 4096 fp16 rows
+    // 33.1 us, 38.3 with 32 bytes), one piece where more CTAs are worth more (64 x 2048:
+    // 1.3 us, 2.0 with four).
+    constexpr int kSteps = sizeof(T) == 2 ? 4 : 1, kSiluSteps = (kSteps + 1) / 2;
+    const bool few = p.num_rows * (p.width / 8) <= 256ll * 4 * sms;
     if (p.op == TLB_ROWS_SILU_AND_MUL)
-        return launch_early(quantize_pieces_kernel<T, true, kSteps>, grid, 256, 0, st, p);
-    return launch_early(quantize_pieces_kernel<T, false, kSteps>, grid, 256, 0, st, p);
+        return few ? launch_pieces<T, true, 1>(p, sms, st) : launch_pieces<T, true, kSiluSteps>(p, sms, st);
+    return few ? launch_pieces<T, false, 1>(p, sms, st) : launch_pieces<T, false, kSteps>(p, sms, st);
 }
 
 }  // namespace
