@@ -624,11 +624,7 @@ TLB_API int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream);
  * two scales may add up to -120 .. 110; results past fp32 are infinite or 0.
  * The tensor-core kernel wants x and weight on 16-byte boundaries with strides that
  * are multiples of 16; others go to a kernel for any alignment.
- * flags: TLB_PRODUCT_OVERLAP_PROLOGUE: the kernel before this one on the stream
- * writes neither weight nor weight_scales, which may then be read while it ends.
  * ---------------------------------------------------------------------- */
-#define TLB_PRODUCT_OVERLAP_PROLOGUE 0x1u
-
 typedef struct tlb_matmul_quantized_args {
     void* out;
     const void* x;
@@ -637,7 +633,7 @@ typedef struct tlb_matmul_quantized_args {
     const void* weight_scales;
     const void* bias;
     int64_t num_tokens, width, features, x_stride, x_scales_stride, weight_stride;
-    int64_t weight_scales_stride, out_stride, out_dtype, flags;
+    int64_t weight_scales_stride, out_stride, out_dtype;
 } tlb_matmul_quantized_args;
 
 TLB_API int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream);

@@ -59,16 +59,15 @@ def test_rows_refuse_before_any_cuda_call(built_lib):
     assert rows(lib, n=0) == OK  # nothing to do, nothing launched
 
 
-def product(lib, out=P, x=P, xs=P, w=P, ws=P, bias=0, t=4, k=256, n=64, dtype=BF16, flags=0):
-    return call(lib, _lib.MATMUL_QUANTIZED, out, x, xs, w, ws, bias, t, k, n, k, 2, k, 2, n, dtype,
-                flags)
+def product(lib, out=P, x=P, xs=P, w=P, ws=P, bias=0, t=4, k=256, n=64, dtype=BF16):
+    return call(lib, _lib.MATMUL_QUANTIZED, out, x, xs, w, ws, bias, t, k, n, k, 2, k, 2, n, dtype)
 
 
 def test_product_refuses_before_any_cuda_call(built_lib):
     lib = _lib.load()
     for kw, msg in ((dict(dtype=I32), "out dtype"), (dict(t=-1), "negative"),
                     (dict(n=-1), "negative"), (dict(k=0), "width"), (dict(t=1 << 31), "range"),
-                    (dict(flags=2), "unknown flags"), (dict(out=0), "null"), (dict(x=0), "null"),
+                    (dict(out=0), "null"), (dict(x=0), "null"),
                     (dict(xs=0), "null"), (dict(w=0), "null"), (dict(ws=0), "null"),
                     (dict(out=P + 1), "aligned"), (dict(bias=P + 1), "aligned")):
         assert product(lib, **kw) == BAD and msg in _lib.last_error(), kw

@@ -152,7 +152,7 @@ DEQUANTIZE = ("tlb_dequantize_blocks", struct.Struct("=15q").pack)
 QK_NORM_ROPE = ("tlb_qk_norm_rotary_embedding_neox", struct.Struct("=32qd").pack)
 SCORED_ATTENTION = ("tlb_paged_attention_scored", struct.Struct("=23q2d").pack)
 QUANTIZE_ROWS = ("tlb_quantize_rows", struct.Struct("=13qd").pack)
-MATMUL_QUANTIZED = ("tlb_matmul_quantized", struct.Struct("=16q").pack)
+MATMUL_QUANTIZED = ("tlb_matmul_quantized", struct.Struct("=15q").pack)
 
 
 def _load_fast():

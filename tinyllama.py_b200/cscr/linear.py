@@ -178,8 +178,7 @@ def _check_product(x, x_scales, weight, weight_scales, out_dtype, bias):
 
 def matmul_quantized(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor,
                      weight_scales: torch.Tensor, out_dtype: torch.dtype,
-                     bias: torch.Tensor | None = None, *, overlap_prologue: bool = False
-                     ) -> torch.Tensor:
+                     bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T + bias`` of 8-bit rows and weights -> [T, N] of ``out_dtype``.
 
     x [T, K] float8_e4m3fn with x_scales [T, ceil(K / 128)], weight [N, K] with
@@ -187,14 +186,9 @@ def matmul_quantized(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tens
     ``out_dtype`` (float16, bfloat16 or float32). Sums in fp32, one rounding. Rows of
     any operand may be strided; x and weight rows on 16-byte boundaries take the
     tensor cores, others a slower kernel.
-
-    ``overlap_prologue``: set it only when the kernel launched just before on this
-    stream writes neither weight nor weight_scales: they are then read while that
-    kernel ends (x, x_scales and bias are not).
     """
     if _lib.fast is not None:
-        out = _lib.fast.product(x, x_scales, weight, weight_scales, out_dtype, bias,
-                                overlap_prologue)
+        out = _lib.fast.product(x, x_scales, weight, weight_scales, out_dtype, bias)
         if out is not None:
             return out
     index, shape, wshape = x.get_device(), x.shape, weight.shape
@@ -219,5 +213,5 @@ def matmul_quantized(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tens
                     x_scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(),
                     0 if bias is None else bias.data_ptr(), shape[0], shape[1], wshape[0],
                     x.stride(0), x_scales.stride(0), weight.stride(0), weight_scales.stride(0),
-                    wshape[0], DTYPE_CODE[out_dtype], 1 if overlap_prologue else 0)
+                    wshape[0], DTYPE_CODE[out_dtype])
     return out

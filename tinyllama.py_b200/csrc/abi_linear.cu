@@ -78,7 +78,8 @@ int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream) {
     TLB_REQUIRE(is_float(a.dtype), "dtype must be float16, bfloat16 or float32");
     TLB_REQUIRE(a.num_rows >= 0, "num_rows must not be negative");
     TLB_REQUIRE(a.width > 0, "width must be positive");
-    TLB_REQUIRE(a.num_rows < (1ll << 40) && a.width < (1ll << 30), "sizes exceed the supported range");
+    TLB_REQUIRE(a.width < (1ll << 30) && a.num_rows <= (1ll << 46) / a.width,
+                "sizes exceed the supported range");
     const bool norm = a.op == TLB_ROWS_RMS_NORM;
     TLB_REQUIRE(norm || (!a.residual && !a.weight), "residual and weight belong to the norm");
     TLB_REQUIRE(!norm || a.eps >= 0, "eps must not be negative");
@@ -123,7 +124,6 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
     TLB_REQUIRE(a.num_tokens < (1ll << 31) - 1024 && a.features < (1ll << 31) - 1024 &&
                     a.width < (1ll << 30),
                 "sizes exceed the supported range");
-    TLB_REQUIRE((a.flags & ~(int64_t)TLB_PRODUCT_OVERLAP_PROLOGUE) == 0, "unknown flags");
     if (a.num_tokens == 0 || a.features == 0) return TLB_OK;
     TLB_REQUIRE(a.out && a.x && a.x_scales && a.weight && a.weight_scales,
                 "tensor pointers must not be null");
@@ -170,7 +170,6 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
                 return rc;
         return cuda_result(
             tlb::launch_product((int)a.out_dtype, p, plan, map_w, map_x, map_out,
-                                (a.flags & TLB_PRODUCT_OVERLAP_PROLOGUE) != 0,
                                 tlb::attention_wait_limit(), st),
             "matmul_quantized");
     }

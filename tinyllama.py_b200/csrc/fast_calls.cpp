@@ -463,14 +463,13 @@ PyObject* rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// product(x, x_scales, weight, weight_scales, out_dtype, bias, overlap)
+// product(x, x_scales, weight, weight_scales, out_dtype, bias)
 PyObject* product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 7 || g_product == nullptr) return later();
+    if (n != 6 || g_product == nullptr) return later();
     const Tensor *x = tensor(a[0]), *xs = tensor(a[1]), *w = tensor(a[2]), *ws = tensor(a[3]),
                  *bias = tensor(a[5]);
-    bool overlap;
-    if (x == nullptr || !THPDtype_Check(a[4]) || !truth(a[6], &overlap)) return later();
+    if (x == nullptr || !THPDtype_Check(a[4])) return later();
     const ScalarType type = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
     const Place at(*x);
     if (!at.ok() || !is_float(type) || !rows_of(at, x) || !rows_of(at, w) || !rows_of(at, xs) ||
@@ -504,7 +503,6 @@ PyObject* product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.weight_scales_stride = ws->stride(0);
     p.out_stride = N;
     p.out_dtype = code_of(type);
-    p.flags = overlap ? TLB_PRODUCT_OVERLAP_PROLOGUE : 0;
     if (g_product(&p, at.stream) != TLB_OK) return later();
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS

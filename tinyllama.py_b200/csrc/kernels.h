@@ -373,11 +373,11 @@ struct ProductPlan {
 ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool wide_stores,
                          int sms);
 // `map_w`, `map_x`: boxes of {128 bytes, 128 rows} and {128 bytes, tile_tokens rows (half
-// of them for a pair)}, 128-byte swizzle. overlap: see TLB_PRODUCT_OVERLAP_PROLOGUE.
+// of them for a pair)}, 128-byte swizzle; `map_out` (used with pieces): boxes of
+// {32 features, 32 tokens, or 16 if tile_tokens is no multiple of 32}, 64-byte swizzle.
 cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
                            const CUtensorMap& map_w, const CUtensorMap& map_x,
-                           const CUtensorMap& map_out, bool overlap, unsigned wait_limit,
-                           cudaStream_t stream);
+                           const CUtensorMap& map_out, unsigned wait_limit, cudaStream_t stream);
 // Any shape and alignment, on the CUDA cores.
 cudaError_t launch_product_any(int out_dtype, const ProductParams& p, cudaStream_t stream);
 

@@ -66,7 +66,6 @@ struct Work {
     int tiles_n, tiles_t;
     int band;                // token tiles whose weights' tiles follow one another
     unsigned wait_limit;
-    bool overlap;
     bool words;              // rows of scales allow 4-byte loads, and are whole words
     int parts_bytes;         // of shared memory for the results
     bool aligned;            // results allow stores of four features
@@ -502,39 +501,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (kPair) tma_load_pair(dst, map, x, y, b, policy);
                 else tma_load_2d(dst, map, x, y, b, policy);
             };
-            // the stage's bytes are expected (a pair's by its even CTA; a copy may complete
-            // before that), and its weights fetched
-            auto load_weights = [&](uint32_t at, uint32_t full, int k, int y) {
-                const bool both = kChunks == 2 && k + kChunk < p.width;
-                if (!kPair || rank == 0)
-                    mbar_arrive_expect_tx(full, (kPair ? 2 : 1) * (both ? stage_bytes : stage_bytes / kChunks));
-                load(at, &map_w, k, y, full, w_policy);
-                if (both) load(at + kWeightBytes, &map_w, k + kChunk, y, full, w_policy);
-            };
-            auto load_tokens = [&](uint32_t at, uint32_t full, int k, int y) {
-                load(at + kChunks * kWeightBytes, &map_x, k, y, full, keep);
-                if (kChunks == 2 && k + kChunk < p.width)
-                    load(at + kChunks * kWeightBytes + x_bytes, &map_x, k + kChunk, y, full, keep);
-            };
-            auto place = [&](int i, int& wy, int& xy) {
-                int tn, tt;
-                tile_at(w, i, tn, tt);
-                wy = (kPair ? 2 * tn + rank : tn) * kFeatures;
-                xy = tt * w.tile_tokens + (kPair ? rank * x_rows : 0);
-            };
-            int ahead = 0, wy, xy;  // stages whose weights are fetched before the wait
-            if (w.overlap) {
-                int i = unit, d = d_first;
-                for (; ahead < w.stages; ++ahead, ++d) {
-                    if (d == d_last) {
-                        d = d_first;
-                        i += units;
-                    }
-                    if (i >= tiles) break;
-                    place(i, wy, xy);
-                    load_weights(base + ahead * stage_bytes, full0 + 8 * ahead, d * kDepth, wy);
-                }
-            }
+            // The weights too: fetched under the kernel before (which mostly does not write
+            // them), a norm and a product of 64 x 2048 -> 2560 took 9.1 us, so 8.5.
             grid_dependency_wait();
             // One thread issues everything, so its instructions are what a stage costs:
             // counters instead of divisions.
@@ -542,15 +510,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t parity = 1;  // of the wait for a free stage: the first round's holds
             uint32_t at = base;
             for (int i = unit; i < tiles && ok; i += units) {
-                place(i, wy, xy);
+                int tn, tt;
+                tile_at(w, i, tn, tt);
+                const int wy = (kPair ? 2 * tn + rank : tn) * kFeatures;
+                const int xy = tt * w.tile_tokens + (kPair ? rank * x_rows : 0);
                 for (int d = d_first; d < d_last; ++d) {
                     const uint32_t full = full0 + 8 * s;
                     if (!mbar_wait_bounded(bar(kBarEmpty + s), parity, limit)) {
                         ok = false;
                         break;
                     }
-                    if (issued >= ahead) load_weights(at, full, d * kDepth, wy);
-                    load_tokens(at, full, d * kDepth, xy);
+                    const int k = d * kDepth;
+                    const bool both = kChunks == 2 && k + kChunk < p.width;
+                    // a pair's bytes are expected by its even CTA; copies may complete first
+                    if (!kPair || rank == 0)
+                        mbar_arrive_expect_tx(
+                            full, (kPair ? 2 : 1) * (both ? stage_bytes : stage_bytes / kChunks));
+                    load(at, &map_w, k, wy, full, w_policy);
+                    load(at + kChunks * kWeightBytes, &map_x, k, xy, full, keep);
+                    if (both) {
+                        load(at + kWeightBytes, &map_w, k + kChunk, wy, full, w_policy);
+                        load(at + kChunks * kWeightBytes + x_bytes, &map_x, k + kChunk, xy, full, keep);
+                    }
                     ++issued;
                     at += stage_bytes;
                     if (++s == w.stages) {
@@ -560,10 +541,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            // A wait gave up before all stages had their tokens: none of them is
-            // used, but what the barriers expect has to come.
-            for (; issued < ahead; ++issued)
-                load_tokens(base + issued * stage_bytes, full0 + 8 * issued, 0, 0);
             *reinterpret_cast<volatile int*>(tail_ptr + kIssued) = issued;
         }
     } else if (warp == kTensorWarp) {
@@ -780,11 +757,12 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
 // Which tile, and how many CTAs share it: the plan whose time, in microseconds by the
 // measurements below, is the shortest.
 //   * A chunk of a tile of n tokens takes 0.14 + n / 1000 (the issuing thread, then the
-//     tensor cores: 16 tokens 0.18, 160 0.30), of a pair's 0.155 + n / 1000; at least
+//     tensor cores: 16 tokens 0.18, 160 0.30), of a pair's 0.145 + n / 1000; at least
 //     its bytes at 115 GB/s an SM (from the L2), and where every weight is read once, all
 //     CTAs' weights at 6.3 TB/s.
-//   * A tile's end takes 0.5, a pair's 1 (4853 x 896 -> 9728: 51 us with single CTAs, 60
-//     with pairs; 16384 x 4096 -> 8192: 457 and 415).
+//   * A tile's end takes 0.5, a pair's 0.9 (4853 x 896 -> 9728: 57.0 us with single CTAs,
+//     63.6 with pairs; 16384 x 4096 -> 8192: 503 and 479; both sustained, at 1.3 to 1.6 GHz
+//     under the power cap).
 //   * Sharing a tile costs 0.9 + n / 40 (64 x 8192 -> 2048: 16.3 us alone, 13.3 by two,
 //     10.4 by four CTAs; 64 x 2048 -> 2560: 7.1, 7.8 and 7.4).
 ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool wide_stores,
@@ -800,12 +778,12 @@ ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bo
         const int64_t tiles = (features + per_cta - 1) / per_cta * tiles_t;
         const int64_t rounds = (tiles + units - 1) / units;
         const int ctas = (int)(tiles < units ? tiles : units) * cluster;
-        double chunk = (pair ? 0.155 : 0.14) + tokens * 1e-3;
+        double chunk = (pair ? 0.145 : 0.14) + tokens * 1e-3;
         const double copy = (kWeightBytes + (pair ? tokens / 2 : tokens) * kChunk) / 115e3;
         if (copy > chunk) chunk = copy;
         const double stream = tiles_t > 1 ? 0 : ctas * (double)kWeightBytes / 6.3e6;
         if (stream > chunk) chunk = stream;
-        double time = rounds * ((double)((chunks + split - 1) / split) * chunk + (pair ? 1.0 : 0.5));
+        double time = rounds * ((double)((chunks + split - 1) / split) * chunk + (pair ? 0.9 : 0.5));
         if (pair) time += 1.7;
         if (split > 1) time += rounds * (0.9 + tokens / 40.0);
         if (best_time == 0 || time < best_time) {
@@ -839,8 +817,7 @@ ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bo
 
 cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
                            const CUtensorMap& map_w, const CUtensorMap& map_x,
-                           const CUtensorMap& map_out, bool overlap, unsigned wait_limit,
-                           cudaStream_t st) {
+                           const CUtensorMap& map_out, unsigned wait_limit, cudaStream_t st) {
     Work w{};
     w.p = p;
     w.tile_tokens = plan.tile_tokens;
@@ -854,7 +831,6 @@ cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductP
     w.tiles_t = (int)((p.num_tokens + plan.tile_tokens - 1) / plan.tile_tokens);
     w.band = w.tiles_t < 8 ? w.tiles_t : 8;
     w.wait_limit = wait_limit;
-    w.overlap = overlap;
     auto words = [](const uint8_t* s, long long stride) {
         return reinterpret_cast<uintptr_t>(s) % 4 == 0 && stride % 4 == 0;
     };

@@ -21,6 +21,10 @@ position of every token is ``seq_lens - 1``; with full-width rotary
 ``PagedAttentionWithQKNorm`` (not in the reference) is the same layer for models
 that normalise each query and key head, cap their scores or limit them to a
 window, over caches of the model dtype or of 8 bits.
+
+``QuantizedLinear`` and ``QuantizedDecoderLayer`` (not in the reference) put
+projections with 8-bit weights and activations (``cscr.linear``) around either
+attention layer: a whole decoder layer.
 """
 
 from __future__ import annotations
@@ -30,6 +34,7 @@ from torch import nn
 
 from cscr import attention as _C
 from cscr import cache as _Cache
+from cscr import linear as _Linear
 from cscr import pos_encoding as _PE
 
 from . import metadata
@@ -214,3 +219,108 @@ class PagedAttentionWithQKNorm(PagedAttentionWithRoPE):
                 key_cache, value_cache, key_scales, value_scales, ids.view(-1), query.dtype)
         return _C.paged_prefill_attention(query, key_cache, value_cache, tables, query_start,
                                           context_lens, self.scale, max_query_len)
+
+
+class QuantizedLinear(nn.Module):
+    """A projection with 8-bit weights and activations (``cscr.linear.
+    matmul_quantized``): [T, in_features] -> [T, out_features] of ``dtype``.
+
+    The weight is kept as bytes, so that ``.to(dtype)`` and ``state_dict`` leave it
+    alone: ``weight_bytes`` [out_features, in_features] of float8_e4m3fn and
+    ``scale_bytes`` [ceil(out / 128), ceil(in / 128)] of float8_e8m0fnu.
+    """
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False,
+                 dtype: torch.dtype = torch.bfloat16, device: torch.device | str | None = None):
+        super().__init__()
+        groups = -(-in_features // _Linear.GROUP)
+        self.dtype = dtype
+        self.register_buffer("weight_bytes", torch.zeros(
+            (out_features, in_features), dtype=torch.uint8, device=device))
+        self.register_buffer("scale_bytes", torch.full(
+            (-(-out_features // _Linear.GROUP), groups), 127, dtype=torch.uint8, device=device))
+        self.bias = nn.Parameter(torch.zeros(out_features, dtype=dtype, device=device),
+                                 requires_grad=False) if bias else None
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, bias: torch.Tensor | None = None
+                    ) -> QuantizedLinear:
+        """The projection whose weight is ``weight`` [out, in] (float16, bfloat16 or
+        float32, of finite values) in 8 bits; results and bias have its dtype."""
+        m = cls(weight.size(1), weight.size(0), bias is not None, weight.dtype, weight.device)
+        values, scales = _Linear.quantize_weight(weight.detach())
+        m.weight_bytes, m.scale_bytes = values.view(torch.uint8), scales.view(torch.uint8)
+        if bias is not None:
+            m.bias = nn.Parameter(bias.detach().to(weight.dtype), requires_grad=False)
+        return m
+
+    def forward(self, x: torch.Tensor | tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
+        """x: rows in float16, bfloat16 or float32 (quantised first), or 8-bit rows as
+        (values, scales)."""
+        values, scales = _Linear.quantize_rows(x) if isinstance(x, torch.Tensor) else x
+        return _Linear.matmul_quantized(values, scales, self.weight_bytes.view(torch.float8_e4m3fn),
+                                        self.scale_bytes.view(torch.float8_e8m0fnu), self.dtype,
+                                        self.bias)
+
+
+class QuantizedDecoderLayer(nn.Module):
+    """A decoder layer with 8-bit projections around a paged attention layer.
+
+    ``attention``: ``PagedAttentionWithRoPE`` or ``PagedAttentionWithQKNorm``.
+    ``qkv`` gives each token's queries, keys and values side by side, ``gate_up`` its
+    gate and up values. Each half of the layer is a norm with the residual's addition
+    and an 8-bit output, the projections, and attention or the gated activation, whose
+    result is quantised for the projection behind it.
+    """
+
+    def __init__(self, attention: PagedAttention, num_kv_heads: int, qkv: QuantizedLinear,
+                 out: QuantizedLinear, gate_up: QuantizedLinear, down: QuantizedLinear,
+                 input_norm: torch.Tensor, post_norm: torch.Tensor, eps: float = 1e-6):
+        super().__init__()
+        self.attention, self.num_kv_heads, self.eps = attention, num_kv_heads, eps
+        self.qkv, self.out, self.gate_up, self.down = qkv, out, gate_up, down
+        self.input_norm = nn.Parameter(input_norm.detach(), requires_grad=False)
+        self.post_norm = nn.Parameter(post_norm.detach(), requires_grad=False)
+
+    def _project(self, hidden, residual):
+        values, scales, summed = _Linear.rms_norm_quantized(hidden, self.input_norm, self.eps,
+                                                            residual)
+        qkv = self.qkv((values, scales))
+        d = self.attention.head_size
+        q, k = self.attention.num_heads * d, self.num_kv_heads * d
+        parts = [p.unflatten(1, (-1, d)) for p in qkv.split([q, k, k], 1)]
+        return parts, hidden if summed is None else summed
+
+    def _rest(self, attended, residual):
+        hidden = self.out(attended.flatten(1))
+        values, scales, residual = _Linear.rms_norm_quantized(hidden, self.post_norm, self.eps,
+                                                              residual)
+        gated = _Linear.silu_and_mul_quantized(self.gate_up((values, scales)))
+        return self.down(gated), residual
+
+    def forward(self, positions: torch.Tensor | None, hidden: torch.Tensor,
+                residual: torch.Tensor | None, key_cache: torch.Tensor,
+                value_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                *scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """A decode step: hidden [S, width], what the layer before added to the residual
+        stream ``residual`` (None in front of the first layer: hidden is the stream).
+        ``scales``: key_scales and value_scales of 8-bit caches. Returns this layer's
+        addition and the stream before it, the next layer's (hidden, residual); neither
+        argument is modified."""
+        (q, k, v), residual = self._project(hidden, residual)
+        attended = self.attention(positions, q, k, v, key_cache, value_cache, block_tables,
+                                  seq_lens, *scales)
+        return self._rest(attended, residual)
+
+    def prompt(self, positions: torch.Tensor, hidden: torch.Tensor,
+               residual: torch.Tensor | None, key_cache: torch.Tensor,
+               value_cache: torch.Tensor, slot_mapping: torch.Tensor,
+               block_tables: torch.Tensor, query_start: torch.Tensor,
+               context_lens: torch.Tensor, max_query_len: int | None = None,
+               *scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Prompt chunks, as ``PagedAttentionWithQKNorm.prompt`` takes them."""
+        (q, k, v), residual = self._project(hidden, residual)
+        attended = self.attention.prompt(positions, q, k, v, key_cache, value_cache, slot_mapping,
+                                         block_tables, query_start, context_lens, max_query_len,
+                                         *scales)
+        return self._rest(attended, residual)
