@@ -48,10 +48,11 @@ constexpr int kBarFull = 0, kBarEmpty = kMaxStages, kBarScales = 2 * kMaxStages,
               kBarSumsFree = kBarSums + 2, kBarParts = kBarSumsFree + 2,
               kBarPartsFree = kBarParts + 1, kBarDrain = kBarPartsFree + 1,
               kNumBars = kBarDrain + 1;
-// behind the barriers: the tensor-memory address, the number of stages issued
-constexpr int kSlot = kNumBars * 8, kIssued = kSlot + 4;
+// behind the barriers: the tensor-memory address, the number of stages issued, and
+// whether a wait gave up
+constexpr int kSlot = kNumBars * 8, kIssued = kSlot + 4, kGaveUp = kSlot + 8;
 constexpr int kTail = 512;                 // bytes of all of it, after the stages
-static_assert(kIssued + 4 <= kTail, "barriers");
+static_assert(kGaveUp + 4 <= kTail, "barriers");
 // CTAs that share a tile. Eight were slower everywhere (64 x 8192 -> 2048: 17.7 us, 10.4
 // with four): fewer than 16 clusters of that many large CTAs run at once.
 constexpr int kMaxSplit = 4;
@@ -93,6 +94,11 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                  : "r"(addr)
                  : "memory");
+    return v;
+}
+__device__ __forceinline__ int load_cluster_int(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
@@ -215,7 +221,6 @@ __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uin
                     buf[(tid / kWordsAtOnce + kRowsAtOnce * m) * kScalePitch + (tid & (kWordsAtOnce - 1))] = x[m];
             if (tid < kWordsAtOnce) buf[kMaxTokens * kScalePitch + tid] = ws;
             named_bar_sync(2, 128);  // the other half's readers are past it too
-            read();
             const int count = min(kWordsAtOnce, word_end - first);
             for (int k = 0; k < count; ++k) {
                 // a CTA's warps give up together: they meet at the barrier above
@@ -242,6 +247,7 @@ __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uin
                     set = 0;
                     parity ^= 1;
                 }
+                if (k == 0) read();
             }
         }
     return true;
@@ -445,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
 
     if (tid == 0) {
+        *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) = 0;
         for (int i = 0; i < w.stages; ++i) {
             mbar_init(bar(kBarFull + i), 1);
             mbar_init(bar(kBarEmpty + i), 1);
@@ -550,9 +557,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (kPair) tc5::commit_pair(b);
                 else tc5::commit(b);
             };
-            const uint64_t first = tc5::desc_sw128(base, 16, 1024);
+            const uint64_t whole = tc5::desc_sw128(base, 16, 1024);
+            const uint32_t first = (uint32_t)whole, high = (uint32_t)(whole >> 32);
             const uint32_t idesc = tc5::idesc_mxf8(kPair ? 256 : 128, w.tile_tokens, 0);
-            uint64_t desc = first;
+            uint32_t desc = first;
             int s = 0, set = 0, it = 0;
             uint32_t parity = 0, set_parity = 0;
             for (int i = unit; i < tiles && ok; i += units, ++it) {
@@ -587,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tc5::mma_mxf8<kPair>(
                                 sums, desc + (k / 4) * (kWeightBytes >> 4) + 2 * (k % 4),
                                 desc + (kChunks * kWeightBytes >> 4) + (k / 4) * (x_bytes >> 4) + 2 * (k % 4),
-                                idesc | sf << 4 | sf << 29, scales, scales + 4, accumulate);
+                                high, idesc | sf << 4 | sf << 29, scales, scales + 4, accumulate);
                             accumulate = true;
                         }
                         commit(bar(kBarEmpty + s));
@@ -662,25 +670,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
-    if (!ok) flag_status(TLB_STATUS_WAIT_TIMEOUT);
+    if (!ok) {
+        flag_status(TLB_STATUS_WAIT_TIMEOUT);
+        *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) = 1;
+    }
     __syncwarp();
     tc5::fence_before_sync();
     __syncthreads();
-    // No CTA ends while another one may read its sums or arrive at its barriers, nor
-    // before the copies that were issued have landed (after a wait that gave up; they
-    // have otherwise).
+    // no CTA ends while another one may read its sums or arrive at its barriers
     if (cluster > 1) cluster_sync();
-    if (tid == 0 && (!kPair || rank == 0)) {
+    bool gave_up = *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) != 0;
+    if constexpr (kPair) gave_up = gave_up || load_cluster_int(map_rank(tail + kGaveUp, rank ^ 1)) != 0;
+    // After a wait that gave up, the copies that were issued land before the CTA ends
+    // (they have otherwise: their stages were used).
+    if (gave_up && tid == 0 && (!kPair || rank == 0)) {
         const int mine = *reinterpret_cast<volatile int*>(tail_ptr + kIssued);
         int most = mine;
         if constexpr (kPair) {
             // both CTAs' copies complete here: expect those of the other CTA alone, and
             // make up for those that it did not issue
-            int other;
-            asm volatile("ld.shared::cluster.u32 %0, [%1];"
-                         : "=r"(other)
-                         : "r"(map_rank(tail + kIssued, 1))
-                         : "memory");
+            const int other = load_cluster_int(map_rank(tail + kIssued, 1));
             most = max(mine, other);
             for (int k = min(mine, other); k < most; ++k) {
                 const int s = k % w.stages, x = k % w.depths * kDepth;
@@ -701,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = max(0, most - w.stages); k < most; ++k)
             mbar_wait_bounded(bar(kBarFull + k % w.stages), (k / w.stages) & 1);
     }
-    __syncthreads();
+    if (gave_up) __syncthreads();
     if constexpr (kPair) cluster_sync();
     if (warp == kTensorWarp) {
         tc5::fence_after_sync();

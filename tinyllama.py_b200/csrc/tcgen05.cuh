@@ -76,24 +76,28 @@ __host__ __device__ constexpr uint32_t idesc_mxf8(int m, int n, int sf) {
 // kPair: the two CTAs of a pair as one (cta_group::2), issued by the even one. Each
 // holds 128 rows of A, their scales and sums, half the rows of B, and the scales of
 // all rows of B, at the same addresses.
+// The descriptors come as their low words and the high word that both share: 64-bit
+// sums of them cost the issuing thread twice the moves to uniform registers.
 template <bool kPair>
-__device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                         uint32_t idesc, uint32_t a_scales, uint32_t b_scales,
-                                         bool accumulate) {
+__device__ __forceinline__ void mma_mxf8(uint32_t d_tmem, uint32_t a_desc, uint32_t b_desc,
+                                         uint32_t high, uint32_t idesc, uint32_t a_scales,
+                                         uint32_t b_scales, bool accumulate) {
     if constexpr (kPair)
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, "
-            "[%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales),
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+            "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %4, "
+            "[%5], [%6], p;\n\t}\n" ::"r"(d_tmem),
+            "r"(a_desc), "r"(b_desc), "r"(high), "r"(idesc), "r"(a_scales), "r"(b_scales),
             "r"(accumulate ? 1u : 0u)
             : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, "
-            "[%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales),
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+            "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %4, "
+            "[%5], [%6], p;\n\t}\n" ::"r"(d_tmem),
+            "r"(a_desc), "r"(b_desc), "r"(high), "r"(idesc), "r"(a_scales), "r"(b_scales),
             "r"(accumulate ? 1u : 0u)
             : "memory");
 }
