@@ -82,6 +82,10 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                      : "memory");
 }
+// The same where nothing written before has to be seen.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // Address in the cluster's CTA `rank` of what is at `addr` here.
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
     uint32_t r;
@@ -666,7 +670,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else mbar_arrive(bar(kBarSumsFree + b));
             }
             if (!ok) break;
-            if (split > 1 && lane < split) arrive_cluster(map_rank(bar(kBarPartsFree), lane));
+            // a release waits for the results' stores: only where another tile follows
+            if (split > 1 && i + units < tiles && lane < split)
+                arrive_cluster(map_rank(bar(kBarPartsFree), lane));
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
@@ -677,8 +683,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     tc5::fence_before_sync();
     __syncthreads();
-    // no CTA ends while another one may read its sums or arrive at its barriers
-    if (cluster > 1) cluster_sync();
+    // No CTA ends while another one may read its sums or arrive at its barriers (a pair's
+    // also tell one another whether a wait gave up).
+    if constexpr (kPair) cluster_sync();
+    else if (split > 1) cluster_sync_relaxed();
     bool gave_up = *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) != 0;
     if constexpr (kPair) gave_up = gave_up || load_cluster_int(map_rank(tail + kGaveUp, rank ^ 1)) != 0;
     // After a wait that gave up, the copies that were issued land before the CTA ends
