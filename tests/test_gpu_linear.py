@@ -196,6 +196,24 @@ def test_no_rows():
         assert L.matmul_quantized(q, s, wq, ws, torch.float16).shape == (0, 5)
 
 
+def test_rows_past_32_bit_offsets():
+    """2^31 values and more: the last rows are those of the rows alone."""
+    t, k = 68000, 32768
+    x = torch.empty(t, k, dtype=torch.float16, device="cuda")
+    g = torch.Generator().manual_seed(11)
+    last = rows(g, 40, k, torch.float16).cuda()
+    x[:-40] = 1.0
+    x[-40:] = last
+    want_q, want_s = O.quantize_rows(last)
+    q, s = L.quantize_rows(x)
+    assert same_bytes(q[-40:], want_q) and same_bytes(s[-40:], want_s)
+    assert bool((q[:5].float() == 256).all())  # 1 = 256 * 2^-8, the smallest scale
+    del q, s
+    w = torch.ones(k, dtype=torch.float16, device="cuda")
+    q, s, _ = L.rms_norm_quantized(x, w, 1e-6)
+    O.assert_rows_of(q[-40:], s[-40:], O.norm(last, w, 1e-6)[0], NORM_DELTA)
+
+
 # -------------------------------------------------------------------- product
 
 def operands(g, t, k, n, spread=1.0):
@@ -243,6 +261,19 @@ def test_product_of_whole_numbers_is_exact(t, k, n):
     want, mag = O.product(x, xs, w, ws)
     assert float(mag.max()) * 2 < 2 ** 24  # the smallest step is 1/2
     assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=short)
+def test_product_past_32_bit_offsets(dtype):
+    """2^31 results and more; the last tokens' are those of the tokens alone."""
+    g = torch.Generator().manual_seed(12)
+    t, k, n = 68000, 128, 32000
+    x, xs, w, ws = operands(g, 300, k, n)
+    where = torch.arange(t, device="cuda") % 300
+    x, xs = (v.view(torch.uint8)[where].view(v.dtype) for v in (x, xs))
+    got = L.matmul_quantized(x, xs, w, ws, dtype)[-300:]
+    y, mag = O.product(x[-300:], xs[-300:], w, ws)
+    assert bool(((got.double() - y).abs() <= O.product_bound(y, mag, k, dtype)).all())
 
 
 def test_product_of_strided_operands():

@@ -150,6 +150,22 @@ def test_rotated_attention_and_module_conversions():
     assert again.qkv.weight_bytes.dtype == torch.uint8
     got = again(None, h, None, *(c.clone() for c in kv), tables, ctx)
     assert torch.equal(got[0], want[0])
+    half = again.to(torch.float16)
+    assert half.qkv.dtype == torch.float16 and half.qkv.weight_bytes.dtype == torch.uint8
+    got = half(None, h.half(), None, *(c.half() for c in kv), tables, ctx)
+    assert got[0].dtype == torch.float16
+    with pytest.raises(NotImplementedError, match="PagedAttentionWithQKNorm"):
+        m.prompt(None, h, None, *kv, None, tables, None, ctx)
+
+
+def test_steps_without_tokens():
+    m = layer(torch.bfloat16)
+    kv = caches(torch.float8_e4m3fn, torch.bfloat16, 2)
+    none = torch.empty(0, WIDTH, dtype=torch.bfloat16, device="cuda")
+    i32 = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out, residual = m.prompt(i32.long(), none, none, kv[0], kv[1], i32.long(), i32.view(0, 1),
+                             torch.zeros(1, dtype=torch.int32, device="cuda"), i32, 0, *kv[2:])
+    assert out.shape == none.shape and residual.shape == none.shape
 
 
 def test_captured_steps_replayed_together():

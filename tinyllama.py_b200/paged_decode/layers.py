@@ -225,8 +225,8 @@ class QuantizedLinear(nn.Module):
     """A projection with 8-bit weights and activations (``cscr.linear.
     matmul_quantized``): [T, in_features] -> [T, out_features] of ``dtype``.
 
-    The weight is kept as bytes, so that ``.to(dtype)`` and ``state_dict`` leave it
-    alone: ``weight_bytes`` [out_features, in_features] of float8_e4m3fn and
+    The weight is kept as bytes, so that ``.to(dtype)`` (which sets the results' type)
+    and ``state_dict`` leave it alone: ``weight_bytes`` [out_features, in_features] of float8_e4m3fn and
     ``scale_bytes`` [ceil(out / 128), ceil(in / 128)] of float8_e8m0fnu.
     """
 
@@ -253,6 +253,11 @@ class QuantizedLinear(nn.Module):
         if bias is not None:
             m.bias = nn.Parameter(bias.detach().to(weight.dtype), requires_grad=False)
         return m
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self.dtype = fn(torch.empty(0, dtype=self.dtype)).dtype  # as the bias's
+        return self
 
     def forward(self, x: torch.Tensor | tuple[torch.Tensor, torch.Tensor]) -> torch.Tensor:
         """x: rows in float16, bfloat16 or float32 (quantised first), or 8-bit rows as
@@ -319,6 +324,8 @@ class QuantizedDecoderLayer(nn.Module):
                context_lens: torch.Tensor, max_query_len: int | None = None,
                *scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Prompt chunks, as ``PagedAttentionWithQKNorm.prompt`` takes them."""
+        if not isinstance(self.attention, PagedAttentionWithQKNorm):
+            raise NotImplementedError("prompt chunks need a PagedAttentionWithQKNorm layer")
         (q, k, v), residual = self._project(hidden, residual)
         attended = self.attention.prompt(positions, q, k, v, key_cache, value_cache, slot_mapping,
                                          block_tables, query_start, context_lens, max_query_len,
