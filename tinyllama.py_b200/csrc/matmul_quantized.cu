@@ -244,14 +244,17 @@ __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uin
                 __syncwarp();
                 if (lane == 0) {
                     const uint32_t full = tail + 8u * (kBarScales + set);
-                    if constexpr (kPair) arrive_cluster(map_rank(full, 0));
+                    // wait::st has completed the stores to tensor memory; a release would
+                    // wait for all others as well (a quarter of a pair's time)
+                    if constexpr (kPair) arrive_cluster_relaxed(map_rank(full, 0));
                     else mbar_arrive(full);
                 }
                 if (++set == kScaleSets) {
                     set = 0;
                     parity ^= 1;
                 }
-                if (k == 0) read();
+                // early; bytes are waited for at once, so after the last word
+                if (k == (kWords ? 0 : count - 1)) read();
             }
         }
     return true;
@@ -493,10 +496,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int d_last = (int)((long long)w.depths * (split > 1 ? rank + 1 : 1) / split);
     const int word_first = d_first / kPerWord, word_end = (d_last - 1) / kPerWord + 1;
     const uint32_t limit = w.wait_limit;
-    auto wait = [limit](uint32_t b, uint32_t parity) {
-        if constexpr (kPair) return wait_cluster(b, parity, limit);
-        else return mbar_wait_bounded(b, parity, limit);
-    };
     bool ok = true;
 
     if (warp == kCopyWarp) {
@@ -569,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t parity = 0, set_parity = 0;
             for (int i = unit; i < tiles && ok; i += units, ++it) {
                 const int b = it & 1;
-                if (it >= 2 && !wait(bar(kBarSumsFree + b), ((it >> 1) - 1) & 1)) {
+                if (it >= 2 && !mbar_wait_bounded(bar(kBarSumsFree + b), ((it >> 1) - 1) & 1, limit)) {
                     ok = false;
                     break;
                 }
@@ -577,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t sums = tmem + b * kMaxTokens;
                 bool accumulate = false;
                 for (int word = word_first; word < word_end && ok; ++word) {
-                    if (!wait(bar(kBarScales + set), set_parity)) {
+                    if (!mbar_wait_bounded(bar(kBarScales + set), set_parity, limit)) {
                         ok = false;
                         break;
                     }
@@ -772,16 +771,17 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
 }  // namespace
 
 // Which tile, and how many CTAs share it: the plan whose time, in microseconds by the
-// measurements below, is the shortest.
-//   * A chunk of a tile of n tokens takes 0.14 + n / 1000 (the issuing thread, then the
-//     tensor cores: 16 tokens 0.18, 160 0.30), of a pair's 0.145 + n / 1000; at least
-//     its bytes at 115 GB/s an SM (from the L2), and where every weight is read once, all
-//     CTAs' weights at 6.3 TB/s.
-//   * A tile's end takes 0.5, a pair's 0.9 (4853 x 896 -> 9728: 57.0 us with single CTAs,
-//     63.6 with pairs; 16384 x 4096 -> 8192: 503 and 479; both sustained, at 1.3 to 1.6 GHz
-//     under the power cap).
-//   * Sharing a tile costs 0.9 + n / 40 (64 x 8192 -> 2048: 16.3 us alone, 13.3 by two,
-//     10.4 by four CTAs; 64 x 2048 -> 2560: 7.1, 7.8 and 7.4).
+// measurements below (short runs, at 1.9 GHz), is the shortest.
+//   * A chunk of a tile of n tokens takes 0.13 + n / 1000 (the issuing thread, then the
+//     tensor cores; 16 tokens 0.17, 160 0.29), of a pair's 0.13 + n / 1250 (160 tokens
+//     0.26, 224 0.31); at least its bytes at 115 GB/s an SM (from the L2), and where every
+//     weight is read once, all CTAs' weights at 6.3 TB/s.
+//   * A tile's end takes 0.5, and a tile no less than its results' way to memory, 0.0118 a
+//     token (13863 x 208 -> 9928: 106 us with single CTAs, 91 with pairs, 275 MB).
+//   * Pairs start 1.2 later (1024 x 2048 -> 2560: 9.0 us with single CTAs, 9.7 with pairs;
+//     4096 x 4096 -> 4096: 59.4 and 53.1; 16384 x 4096 -> 8192: 426 and 399).
+//   * Sharing a tile costs 0.9 + n / 40 (64 x 8192 -> 2048: 15.2 us alone, 10.7 by two,
+//     9.4 by four CTAs; 64 x 2048 -> 2560: 6.2, 6.2 and 6.4).
 ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool wide_stores,
                          int sms) {
     const int64_t chunks = (width + kChunk - 1) / kChunk;
@@ -795,13 +795,14 @@ ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bo
         const int64_t tiles = (features + per_cta - 1) / per_cta * tiles_t;
         const int64_t rounds = (tiles + units - 1) / units;
         const int ctas = (int)(tiles < units ? tiles : units) * cluster;
-        double chunk = (pair ? 0.145 : 0.14) + tokens * 1e-3;
+        double chunk = 0.13 + tokens * (pair ? 0.8e-3 : 1e-3);
         const double copy = (kWeightBytes + (pair ? tokens / 2 : tokens) * kChunk) / 115e3;
         if (copy > chunk) chunk = copy;
         const double stream = tiles_t > 1 ? 0 : ctas * (double)kWeightBytes / 6.3e6;
         if (stream > chunk) chunk = stream;
-        double time = rounds * ((double)((chunks + split - 1) / split) * chunk + (pair ? 0.9 : 0.5));
-        if (pair) time += 1.7;
+        double tile = (double)((chunks + split - 1) / split) * chunk + 0.5;
+        if (tile < 0.0118 * tokens) tile = 0.0118 * tokens;
+        double time = rounds * tile + (pair ? 1.2 : 0);
         if (split > 1) time += rounds * (0.9 + tokens / 40.0);
         if (best_time == 0 || time < best_time) {
             best_time = time;
