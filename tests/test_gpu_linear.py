@@ -234,7 +234,7 @@ def check_product(ops, dtype, bias=None, **kw):
 PRODUCTS = [(1, 16, 1), (1, 128, 128), (1, 896, 1152), (7, 640, 100), (16, 48, 17), (64, 2048, 640),
             (65, 512, 129), (100, 144, 333), (128, 1024, 256), (200, 400, 513), (257, 2064, 384),
             (600, 896, 1152), (1000, 128, 64), (33, 8192, 128), (5, 33, 7), (70, 130, 200),
-            (1, 1, 1)]
+            (1, 1, 1), (228, 992, 19036), (424, 992, 13112)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=short)
@@ -246,7 +246,8 @@ def test_product(t, k, n, dtype):
 
 
 @pytest.mark.parametrize("t,k,n", [(1, 2048, 256), (40, 896, 300), (300, 1152, 260), (130, 200, 129),
-                                   (9, 250, 70), (520, 640, 1000)])
+                                   (9, 250, 70), (520, 640, 1000), (228, 992, 19036),
+                                   (424, 992, 13112)])
 def test_product_of_whole_numbers_is_exact(t, k, n):
     """Small whole values and scales that keep every partial sum below 2^24: no
     rounding anywhere, so each group's scale and each element shows."""

@@ -775,7 +775,9 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
 //   * A chunk of a tile of n tokens takes 0.13 + n / 1000 (the issuing thread, then the
 //     tensor cores; 16 tokens 0.17, 160 0.29), of a pair's 0.13 + n / 1250 (160 tokens
 //     0.26, 224 0.31); at least its bytes at 115 GB/s an SM (from the L2), and where every
-//     weight is read once, all CTAs' weights at 6.3 TB/s.
+//     weight is read once, all CTAs' weights at 6.3 TB/s. Weights too many for the L2 cost
+//     0.7 of that where several tiles read them (33 x 4096 -> 28672: 23.6 us in a tile of
+//     48 tokens, 33.5 in two of 32).
 //   * A tile's end takes 0.5, and a tile no less than its results' way to memory, 0.0118 a
 //     token (13863 x 208 -> 9928: 106 us with single CTAs, 91 with pairs, 275 MB).
 //   * Pairs start 1.2 later (1024 x 2048 -> 2560: 9.0 us with single CTAs, 9.7 with pairs;
@@ -798,7 +800,8 @@ ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bo
         double chunk = 0.13 + tokens * (pair ? 0.8e-3 : 1e-3);
         const double copy = (kWeightBytes + (pair ? tokens / 2 : tokens) * kChunk) / 115e3;
         if (copy > chunk) chunk = copy;
-        const double stream = tiles_t > 1 ? 0 : ctas * (double)kWeightBytes / 6.3e6;
+        double stream = ctas * (double)kWeightBytes / 6.3e6;
+        if (tiles_t > 1) stream *= features * width > (64 << 20) ? 0.7 : 0;
         if (stream > chunk) chunk = stream;
         double tile = (double)((chunks + split - 1) / split) * chunk + 0.5;
         if (tile < 0.0118 * tokens) tile = 0.0118 * tokens;
