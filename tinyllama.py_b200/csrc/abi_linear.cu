@@ -88,7 +88,8 @@ int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream) {
                 "tensor pointers must not be null");
     const int e = elem_bytes(a.dtype);
     bool vec = a.width % kGroup == 0 && aligned(a.out, 8);
-    for (const void* p : {a.x, a.residual, a.weight, (const void*)(a.residual ? a.residual_out : nullptr)}) {
+    const void* h = a.residual ? a.residual_out : nullptr;
+    for (const void* p : {a.x, a.residual, a.weight, h}) {
         TLB_REQUIRE(!p || aligned(p, e), "tensor pointers must be aligned to the element size");
         vec = vec && (!p || aligned(p, 16));
     }

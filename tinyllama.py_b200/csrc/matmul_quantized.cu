@@ -84,7 +84,8 @@ __device__ __forceinline__ void cluster_sync() {
 }
 // The same where nothing written before has to be seen.
 __device__ __forceinline__ void cluster_sync_relaxed() {
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    asm volatile(
+        "barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 // Address in the cluster's CTA `rank` of what is at `addr` here.
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
@@ -106,11 +107,13 @@ __device__ __forceinline__ int load_cluster_int(uint32_t addr) {
     return v;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
 }
 // The same where nothing written before has to be seen: a release waits for it.
 __device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, uint32_t limit) {
     for (uint32_t i = 0; i < limit; ++i) {
@@ -182,9 +185,9 @@ constexpr int kScaleRows = kMaxTokens + 1;     // the weights' behind the tokens
 constexpr int kScaleBytes = 2 * kScaleRows * kScalePitch * 4;
 
 template <bool kPair, bool kWords>
-__device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uint32_t tmem, uint32_t tail, int tid,
-                            int unit, int units, int tiles, int word_first, int word_end,
-                            int rank) {
+__device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uint32_t tmem,
+                                            uint32_t tail, int tid, int unit, int units, int tiles,
+                                            int word_first, int word_end, int rank) {
     const ProductParams& p = w.p;
     const int warp = tid >> 5, lane = tid & 31;
     const long long last_block = (p.features - 1) / kFeatures;
@@ -222,7 +225,8 @@ __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uin
 #pragma unroll
             for (int m = 0; m < kItems; ++m)
                 if (kRowsAtOnce * m < w.tile_tokens)
-                    buf[(tid / kWordsAtOnce + kRowsAtOnce * m) * kScalePitch + (tid & (kWordsAtOnce - 1))] = x[m];
+                    buf[(tid / kWordsAtOnce + kRowsAtOnce * m) * kScalePitch +
+                        (tid & (kWordsAtOnce - 1))] = x[m];
             if (tid < kWordsAtOnce) buf[kMaxTokens * kScalePitch + tid] = ws;
             named_bar_sync(2, 128);  // the other half's readers are past it too
             const int count = min(kWordsAtOnce, word_end - first);
@@ -432,8 +436,8 @@ __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8
 
 // kChunks: of 128 values of K a stage. Two halve the waits and commits of the one thread
 // that issues the tensor instructions, which a tile of few tokens is bounded by; one
-// gives a wide tile's stages finer steps (2048 x 4096 -> 4096: 32.5 us with one, 36.3
-// with two; 64 x 2048 -> 16384: 10.4 and 9.1).
+// gives a wide tile's stages finer steps (64 x 2048 -> 2560 in tiles of 16 tokens: 7.4 us
+// with one, 6.6 with two; 1024 x 2048 -> 2560 in tiles of 160: 9.0 and 9.9).
 template <typename T, bool kPair, int kChunks>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -491,7 +495,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tail_ptr + kSlot);
 
     // this CTA's tiles, and its part of their width
-    const int tiles = w.tiles_n * w.tiles_t, units = gridDim.x / cluster, unit = blockIdx.x / cluster;
+    const int tiles = w.tiles_n * w.tiles_t;
+    const int units = gridDim.x / cluster, unit = blockIdx.x / cluster;
     const int d_first = (int)((long long)w.depths * (split > 1 ? rank : 0) / split);
     const int d_last = (int)((long long)w.depths * (split > 1 ? rank + 1 : 1) / split);
     const int word_first = d_first / kPerWord, word_end = (d_last - 1) / kPerWord + 1;
@@ -597,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint32_t sf = kChunks * h + k / 4;
                             tc5::mma_mxf8<kPair>(
                                 sums, desc + (k / 4) * (kWeightBytes >> 4) + 2 * (k % 4),
-                                desc + (kChunks * kWeightBytes >> 4) + (k / 4) * (x_bytes >> 4) + 2 * (k % 4),
+                                desc + (kChunks * kWeightBytes >> 4) + (k / 4) * (x_bytes >> 4) +
+                                    2 * (k % 4),
                                 high, idesc | sf << 4 | sf << 29, scales, scales + 4, accumulate);
                             accumulate = true;
                         }
@@ -687,7 +693,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (kPair) cluster_sync();
     else if (split > 1) cluster_sync_relaxed();
     bool gave_up = *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) != 0;
-    if constexpr (kPair) gave_up = gave_up || load_cluster_int(map_rank(tail + kGaveUp, rank ^ 1)) != 0;
+    if constexpr (kPair)
+        gave_up = gave_up || load_cluster_int(map_rank(tail + kGaveUp, rank ^ 1)) != 0;
     // After a wait that gave up, the copies that were issued land before the CTA ends
     // (they have otherwise: their stages were used).
     if (gave_up && tid == 0 && (!kPair || rank == 0)) {
@@ -703,7 +710,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t at = base + s * stage_bytes;
                 const bool both = kChunks == 2 && x + kChunk < p.width;
                 if (k >= mine) {
-                    mbar_arrive_expect_tx(bar(kBarFull + s), both ? stage_bytes : stage_bytes / kChunks);
+                    mbar_arrive_expect_tx(bar(kBarFull + s),
+                                          both ? stage_bytes : stage_bytes / kChunks);
                     continue;
                 }
                 for (int c = 0; c < (both ? 2 : 1); ++c) {

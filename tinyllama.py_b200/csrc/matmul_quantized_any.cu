@@ -66,7 +66,8 @@ __global__ void __launch_bounds__(256) product_any_kernel(const ProductParams p)
                 for (int j = 0; j < 4; ++j) {
                     const long long n = n0 + tx + 16 * j;
                     const uint32_t b =
-                        n < p.features ? p.weight_scales[n / kGroup * p.weight_scales_stride + g] : 127u;
+                        n < p.features ? p.weight_scales[n / kGroup * p.weight_scales_stride + g]
+                                       : 127u;
                     total[i][j] += scaled(acc[i][j], a, b);
                     acc[i][j] = 0.f;
                 }

@@ -322,8 +322,10 @@ cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) 
     constexpr int kSteps = sizeof(T) == 2 ? 4 : 1, kSiluSteps = (kSteps + 1) / 2;
     const bool few = p.num_rows * (p.width / 8) <= 256ll * 4 * sms;
     if (p.op == TLB_ROWS_SILU_AND_MUL)
-        return few ? launch_pieces<T, true, 1>(p, sms, st) : launch_pieces<T, true, kSiluSteps>(p, sms, st);
-    return few ? launch_pieces<T, false, 1>(p, sms, st) : launch_pieces<T, false, kSteps>(p, sms, st);
+        return few ? launch_pieces<T, true, 1>(p, sms, st)
+                   : launch_pieces<T, true, kSiluSteps>(p, sms, st);
+    return few ? launch_pieces<T, false, 1>(p, sms, st)
+               : launch_pieces<T, false, kSteps>(p, sms, st);
 }
 
 }  // namespace
