@@ -303,11 +303,18 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantPa
 }
 
 template <typename T, bool kResidual>
-cudaError_t launch_norm(const RowQuantParams& p, cudaStream_t st) {
+cudaError_t launch_norm(const RowQuantParams& p, int sms, cudaStream_t st) {
     const int pieces = p.width / 8;
     const dim3 grid((unsigned)p.num_rows);
     auto threads = [&](int each) { return ((pieces + each - 1) / each + 31) / 32 * 32; };
-    if (pieces <= 256)
+    // Many rows of 16 bits: more pieces a lane and fewer lanes a row (16383 x 4096 with
+    // residual 83.1 us, 85.2 with two pieces; 16384 x 2048 26.1 and 31.9 with one); fewer
+    // rows are better spread (2000 x 4096: 12.0 with two, 12.7 with four), fp32 gains
+    // nothing. CTAs that go through several rows took 92 us for the first of these.
+    const bool many = sizeof(T) == 2 && p.num_rows >= 24ll * sms;
+    if (many && pieces >= 256 && pieces <= 2048)
+        return launch_early(rms_norm_kernel<T, kResidual, 4>, grid, threads(4), 0, st, p);
+    if (pieces <= 64 || (pieces <= 256 && !many))
         return launch_early(rms_norm_kernel<T, kResidual, 1>, grid, threads(1), 0, st, p);
     if (pieces <= 1024)
         return launch_early(rms_norm_kernel<T, kResidual, 2>, grid, threads(2), 0, st, p);
@@ -335,7 +342,7 @@ cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) 
         return launch_early(quantize_rows_any_kernel<T>, dim3((unsigned)rows), 256, 0, st, p);
     }
     if (p.op == TLB_ROWS_RMS_NORM)
-        return p.residual ? launch_norm<T, true>(p, st) : launch_norm<T, false>(p, st);
+        return p.residual ? launch_norm<T, true>(p, sms, st) : launch_norm<T, false>(p, sms, st);
     // 64 bytes of a lane in flight where there are enough pieces (16381 x 4096 fp16 rows
     // 33.1 us, 38.3 with 32 bytes), one piece where more CTAs are worth more (64 x 2048:
     // 1.3 us, 2.0 with four).
