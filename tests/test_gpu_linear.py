@@ -178,6 +178,7 @@ def test_weight_blocks():
     g = torch.Generator().manual_seed(6)
     for n, k in ((1, 1), (128, 128), (300, 200), (129, 640), (64, 1000)):
         w = (0.05 * torch.randn(n, k, generator=g)).to(torch.bfloat16)
+        w[:128, :128] *= n % 2  # a block of zeros
         for dev in ("cpu", "cuda"):
             q, s = L.quantize_weight(w.to(dev))
             want_q, want_s = O.quantize_weight(w)
@@ -275,6 +276,20 @@ def test_product_past_32_bit_offsets(dtype):
     got = L.matmul_quantized(x, xs, w, ws, dtype)[-300:]
     y, mag = O.product(x[-300:], xs[-300:], w, ws)
     assert bool(((got.double() - y).abs() <= O.product_bound(y, mag, k, dtype)).all())
+
+
+def test_product_of_rows_that_end_off_16_bytes():
+    """Rows of 250 values 256 apart: what lies between them does not count."""
+    g = torch.Generator().manual_seed(13)
+    t, k, n = 150, 250, 300
+    x, w = (torch.randint(-2, 3, (r, 256), generator=g).float() for r in (t, n))
+    x[:, k:], w[:, k:] = 448, float("nan")
+    x, w = (v.to(E4M3).cuda()[:, :k] for v in (x, w))
+    xs = torch.randint(127, 131, (t, 2), generator=g).to(torch.uint8).cuda().view(E8M0)
+    ws = torch.randint(126, 130, (3, 2), generator=g).to(torch.uint8).cuda().view(E8M0)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = L.matmul_quantized(x, xs, w, ws, dtype)
+        assert torch.equal(got, O.product(x, xs, w, ws)[0].to(torch.float32).to(dtype))
 
 
 def test_product_of_strided_operands():

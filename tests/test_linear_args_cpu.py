@@ -164,5 +164,6 @@ def test_oracle_rounds_as_torch_converts():
     top = O.groups(x).abs().amax(-1).double()
     assert bool((top <= 448 * O.scale_of(s)).all() and (top > 224 * O.scale_of(s)).all())
     w = 0.05 * torch.randn(200, 300, generator=g)
+    w[128:, :128] = 0
     for a, b in zip(L.quantize_weight(w), O.quantize_weight(w)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

@@ -133,18 +133,19 @@ def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     n, k = weight.shape
     cols = -(-k // GROUP)
     values = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=weight.device)
-    scales = torch.empty((-(-n // GROUP), cols), dtype=torch.uint8, device=weight.device)
+    scale_bytes = torch.empty((-(-n // GROUP), cols), dtype=torch.uint8, device=weight.device)
+    scales = scale_bytes.view(torch.float8_e8m0fnu)
     for i in range(scales.size(0)):  # a row of blocks at a time: little memory beside the weight
         rows = weight[i * GROUP:(i + 1) * GROUP].float()
         blocks = torch.nn.functional.pad(rows, (0, cols * GROUP - k)).view(-1, cols, GROUP)
-        mantissa, exponent = torch.frexp(blocks.abs().amax((0, 2)))  # top = mantissa * 2^exponent
-        # 448 = 0.875 * 2^9
-        exponent = torch.where(mantissa > 0.875, exponent - 8, exponent - 9).clamp(-126, 127)
-        scale = torch.ldexp(torch.ones_like(mantissa), exponent)
-        blocks = (blocks / scale.view(1, cols, 1)).view(-1, cols * GROUP)[:, :k]
+        top = blocks.abs().amax((0, 2))
+        mantissa, exponent = torch.frexp(top)  # top = mantissa * 2^exponent; 448 = 0.875 * 2^9
+        exponent = torch.where(mantissa > 0.875, exponent - 8, exponent - 9)
+        exponent = torch.where(top == 0, -126, exponent).clamp(-126, 127)
+        scale_bytes[i] = (exponent + 127).to(torch.uint8)
+        blocks = (blocks / scales[i].float().view(1, cols, 1)).view(-1, cols * GROUP)[:, :k]
         values[i * GROUP:(i + 1) * GROUP] = blocks.to(torch.float8_e4m3fn)
-        scales[i] = (exponent + 127).to(torch.uint8)
-    return values, scales.view(torch.float8_e8m0fnu)
+    return values, scales
 
 
 def _check_product(x, x_scales, weight, weight_scales, out_dtype, bias):
