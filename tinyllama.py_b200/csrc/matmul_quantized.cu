@@ -142,6 +142,11 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
 
 // Tile `i` of the order in which a band of token tiles goes through all features.
 __device__ __forceinline__ void tile_at(const Work& w, int i, int& tn, int& tt) {
+    if (w.tiles_t == 1) {  // few tokens: the divisions would be in front of the first load
+        tn = i;
+        tt = 0;
+        return;
+    }
     const int per_band = w.band * w.tiles_n, b = i / per_band, rest = i % per_band;
     const int height = min(w.band, w.tiles_t - b * w.band);
     tn = rest / height;
@@ -461,24 +466,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int split = kPair ? 1 : w.split, cluster = kPair ? 2 : split;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
 
-    if (tid == 0) {
-        *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) = 0;
-        for (int i = 0; i < w.stages; ++i) {
-            mbar_init(bar(kBarFull + i), 1);
-            mbar_init(bar(kBarEmpty + i), 1);
-        }
-        for (int i = 0; i < kScaleSets; ++i) {
-            mbar_init(bar(kBarScales + i), kPair ? 8 : 4);
-            mbar_init(bar(kBarScalesFree + i), 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(kBarSums + i), 1);
-            mbar_init(bar(kBarSumsFree + i), (kPair ? 2 : 1) * kResultWarps);
-        }
-        mbar_init(bar(kBarParts), kResultWarps * split);
-        mbar_init(bar(kBarPartsFree), kResultWarps * split);
-        mbar_init(bar(kBarDrain), 1);
+    if (tid < kNumBars) {  // a barrier a thread
+        int arrivals = 1;
+        if (tid >= kBarScales && tid < kBarScalesFree) arrivals = kPair ? 8 : 4;
+        if (tid >= kBarSumsFree && tid < kBarParts) arrivals = (kPair ? 2 : 1) * kResultWarps;
+        if (tid >= kBarParts && tid < kBarDrain) arrivals = kResultWarps * split;
+        mbar_init(bar(tid), arrivals);
         fence_mbar_init();
+        if (tid == 0) *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) = 0;
     }
     if (warp == kTensorWarp) {
         if constexpr (kPair) tc5::alloc_pair(tail + kSlot, kColumns);
