@@ -198,11 +198,12 @@ __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uin
     const long long last_block = (p.features - 1) / kFeatures;
     constexpr int kItems = kMaxTokens * kWordsAtOnce / 128;
     uint32_t x[kItems], ws = 0;
-    int tile = unit, word = word_first;  // of the next read
+    int tile = unit, word = word_first, tn = 0, tt = 0;  // of the next read
+    tile_at(w, tile, tn, tt);  // its divisions before the wait
+    grid_dependency_wait();
+    grid_launch_dependents();
     auto read = [&]() {
         if (tile >= tiles) return;
-        int tn, tt;
-        tile_at(w, tile, tn, tt);
         const int at = min(word + (tid & (kWordsAtOnce - 1)), word_end - 1);
         const long long last = p.num_tokens - 1;
         long long t = (long long)tt * w.tile_tokens + tid / kWordsAtOnce;
@@ -218,6 +219,7 @@ __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uin
         if (word >= word_end) {
             word = word_first;
             tile += units;
+            if (tile < tiles) tile_at(w, tile, tn, tt);
         }
     };
     read();
@@ -513,6 +515,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             // The weights too: fetched under the kernel before (which mostly does not write
             // them), a norm and a product of 64 x 2048 -> 2560 took 9.1 us, so 8.5.
+            int tn, tt;
+            tile_at(w, unit, tn, tt);
             grid_dependency_wait();
             // One thread issues everything, so its instructions are what a stage costs:
             // counters instead of divisions.
@@ -520,8 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t parity = 1;  // of the wait for a free stage: the first round's holds
             uint32_t at = base;
             for (int i = unit; i < tiles && ok; i += units) {
-                int tn, tt;
-                tile_at(w, i, tn, tt);
+                if (i != unit) tile_at(w, i, tn, tt);
                 const int wy = (kPair ? 2 * tn + rank : tn) * kFeatures;
                 const int xy = tt * w.tile_tokens + (kPair ? rank * x_rows : 0);
                 for (int d = d_first; d < d_last; ++d) {
@@ -625,8 +628,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp < 4) {
         // ------------------------------------------------------------ scales
-        grid_dependency_wait();
-        grid_launch_dependents();
         uint8_t* buffers = tail_ptr + kTail + w.parts_bytes;
         ok = w.words ? feed_scales<kPair, true>(w, buffers, tmem, tail, tid, unit, units, tiles,
                                                 word_first, word_end, rank)
