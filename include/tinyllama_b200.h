@@ -623,7 +623,7 @@ TLB_API int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream);
  * A scale byte b stands for 2^(b - 127), 255 for NaN. The exponents of a product's
  * two scales may add up to -120 .. 110; results past fp32 are infinite or 0.
  * The tensor-core kernel wants x and weight on 16-byte boundaries with strides that
- * are multiples of 16; others go to a kernel for any alignment.
+ * are multiples of 16, and a width of 2^22 at most; others go to a kernel for any shape.
  * ---------------------------------------------------------------------- */
 typedef struct tlb_matmul_quantized_args {
     void* out;

@@ -292,6 +292,17 @@ def test_product_of_rows_that_end_off_16_bytes():
         assert torch.equal(got, O.product(x, xs, w, ws)[0].to(torch.float32).to(dtype))
 
 
+@pytest.mark.parametrize("k", [1 << 22, (1 << 22) + 256])
+def test_product_of_the_widest_rows(k):
+    """The tensor cores' widest rows, and wider ones; sums of ones stay below 2^24."""
+    g = torch.Generator().manual_seed(14)
+    x, w = (torch.randint(-1, 2, (r, k), generator=g).to(torch.int8).cuda().float().to(E4M3)
+            for r in (2, 3))
+    one = torch.full((3, k // 128), 127, dtype=torch.uint8, device="cuda").view(E8M0)
+    got = L.matmul_quantized(x, one[:2], w, one[:1], torch.float32)
+    assert torch.equal(got.double(), x.double() @ w.double().t())
+
+
 def test_product_of_strided_operands():
     """Rows of wider tensors, scales among others, one scale row for all tokens."""
     g = torch.Generator().manual_seed(8)

@@ -150,7 +150,8 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
     // A row's stride only counts where there is a second row.
     const int64_t x_stride = a.num_tokens > 1 ? a.x_stride : (a.width + 15) / 16 * 16;
     const int64_t w_stride = a.features > 1 ? a.weight_stride : (a.width + 15) / 16 * 16;
-    const bool tiled = aligned(a.x, 16) && aligned(a.weight, 16) && x_stride % 16 == 0 &&
+    // wider rows would take a tile longer than the bound of its waits (10 ms at 2^22)
+    const bool tiled = a.width <= (1 << 22) && aligned(a.x, 16) && aligned(a.weight, 16) && x_stride % 16 == 0 &&
                        w_stride % 16 == 0 && x_stride >= a.width && w_stride >= a.width;
     if (tiled) {
         int sms = 0;
