@@ -77,7 +77,8 @@ TLB_API const char* tlb_version(void);
  * prefix itself (a kernel that gave up a wait may leave counters set). */
 TLB_API int tlb_get_device_status(uint32_t* status_out, int clear, void* stream);
 
-/* Bounded waits of the tensor-core attention kernels. Every wait of the
+/* Bounded waits of the tensor-core attention kernels and of the kernel of
+ * tlb_matmul_quantized (which keeps no workspace). Every wait of the
  * kernel's pipeline (a stage's data, a free stage, a hand-off between warps,
  * a phase of the merge) gives up after `tries` mbarrier probes, sets
  * TLB_STATUS_WAIT_TIMEOUT, lets the copies it already issued land and

@@ -220,7 +220,7 @@ STATUS_BITS = {
 }
 
 def set_wait_limit(tries: int) -> None:
-    """Probes before a pipeline wait of the attention kernels gives up
+    """Probes before a pipeline wait of the attention kernels or the product's gives up
     (failure injection for tests; TLB_WAIT_LIMIT_DEFAULT restores)."""
     check(load().tlb_attention_set_wait_limit(int(tries)))
 
