@@ -157,21 +157,21 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
         int sms = 0;
         if (int rc = sm_count(&sms)) return rc;
         const int64_t out_stride = a.num_tokens > 1 ? a.out_stride : (a.features + 7) / 8 * 8;
-        const bool wide_stores = e == 2 && aligned(a.out, 16) && out_stride % 8 == 0 &&
-                                 out_stride >= a.features;
         const tlb::ProductPlan plan =
-            tlb::plan_product(a.num_tokens, a.features, a.width, wide_stores, sms);
+            tlb::plan_product(a.num_tokens, a.features, a.width, e == 2, sms);
+        const bool tma_out = plan.pieces && aligned(a.out, 16) && out_stride % 8 == 0 &&
+                             out_stride >= a.features;
         CUtensorMap map_w, map_x, map_out{};
         if (int rc = rows_map(a.weight, a.features, a.width, w_stride, 1, 128, 128, &map_w)) return rc;
         if (int rc = rows_map(a.x, a.num_tokens, a.width, x_stride, 1, 128,
                               plan.pair ? plan.tile_tokens / 2 : plan.tile_tokens, &map_x))
             return rc;
-        if (plan.pieces)
+        if (tma_out)
             if (int rc = rows_map(a.out, a.num_tokens, a.features, out_stride * 2, 2, 32,
                                   plan.tile_tokens % 32 == 0 ? 32 : 16, &map_out))
                 return rc;
         return cuda_result(
-            tlb::launch_product((int)a.out_dtype, p, plan, map_w, map_x, map_out,
+            tlb::launch_product((int)a.out_dtype, p, plan, map_w, map_x, map_out, tma_out,
                                 tlb::attention_wait_limit(), st),
             "matmul_quantized");
     }

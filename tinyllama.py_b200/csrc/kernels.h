@@ -364,20 +364,21 @@ struct ProductPlan {
     int split;                 // CTAs (a cluster) that share a tile's width
     bool pair;                 // two CTAs take 256 features as one
     int chunks;                // of 128 values of the width a stage
-    bool pieces;               // 16-bit results leave by TMA stores
+    bool pieces;               // 16-bit results by way of a warp's 32 features
     int stages;
     int ctas;
     size_t smem;
 };
-// wide_stores: results in 16 bits whose rows allow stores of 16 bytes.
-ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool wide_stores,
-                         int sms);
+// half: results in 16 bits.
+ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool half, int sms);
 // `map_w`, `map_x`: boxes of {128 bytes, 128 rows} and {128 bytes, tile_tokens rows (half
-// of them for a pair)}, 128-byte swizzle; `map_out` (used with pieces): boxes of
-// {32 features, 32 tokens, or 16 if tile_tokens is no multiple of 32}, 64-byte swizzle.
+// of them for a pair)}, 128-byte swizzle; `map_out` (with tma_out, which goes with
+// pieces): boxes of {32 features, 32 tokens, or 16 if tile_tokens is no multiple of 32},
+// 64-byte swizzle.
 cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
                            const CUtensorMap& map_w, const CUtensorMap& map_x,
-                           const CUtensorMap& map_out, unsigned wait_limit, cudaStream_t stream);
+                           const CUtensorMap& map_out, bool tma_out, unsigned wait_limit,
+                           cudaStream_t stream);
 // Any shape and alignment, on the CUDA cores.
 cudaError_t launch_product_any(int out_dtype, const ProductParams& p, cudaStream_t stream);
 

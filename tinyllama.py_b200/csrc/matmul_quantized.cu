@@ -70,7 +70,9 @@ struct Work {
     bool words;              // rows of scales allow 4-byte loads, and are whole words
     int parts_bytes;         // of shared memory for the results
     bool aligned;            // results allow stores of four features
-    bool pieces;             // 16-bit results of one CTA a tile, eight features a store
+    bool pieces;             // 16-bit results of one CTA a tile
+    bool tma_out;            // whose rows allow TMA stores
+    bool pairs_out;          // whose rows allow stores of two features
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -279,12 +281,48 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, 
         : "memory");
 }
 
+// A warp's 32 features of up to 32 tokens where the rows of results are off 16 bytes
+// (features no multiple of 8): two features a lane and two tokens at a time, or, off 4
+// bytes, one and one.
+template <typename T>
+__device__ __forceinline__ void store_rows(const Work& w, uint32_t from, long long n0, long long t0,
+                                           int rows, int lane) {
+    const ProductParams& p = w.p;
+    const int left = (int)min(32ll, p.features - n0);
+    // feature f of token t: byte 2 (f % 8) of unit f / 8 ^ t / 2 % 4 of the token's 64
+    auto at = [from](int t, int f) {
+        return from + t * 64 + (((f >> 3) ^ ((t >> 1) & 3)) << 4) + (f & 7) * 2;
+    };
+    if (w.pairs_out) {
+        const int f = (lane & 15) * 2;
+        T* out = reinterpret_cast<T*>(p.out) + (t0 + (lane >> 4)) * p.out_stride + n0 + f;
+#pragma unroll 4
+        for (int t = lane >> 4; t < rows; t += 2, out += 2 * p.out_stride) {
+            uint32_t v;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at(t, f)) : "memory");
+            const uint16_t low = (uint16_t)v;
+            if (f + 1 < left)
+                *reinterpret_cast<uint32_t*>(out) = v;
+            else if (f < left)
+                memcpy(out, &low, 2);
+        }
+    } else {
+        T* out = reinterpret_cast<T*>(p.out) + t0 * p.out_stride + n0 + lane;
+#pragma unroll 4
+        for (int t = 0; t < rows; ++t, out += p.out_stride) {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at(t, lane)) : "memory");
+            if (lane < left) memcpy(out, &v, 2);
+        }
+    }
+}
+
 // A tile's results in 16 bits, a warp's 32 features and 32 tokens at a time: the sums
 // leave tensor memory in the layout of matrix fragments, are rounded in pairs of
 // tokens and turned round by stmatrix, so that a token's 32 features lie side by side
 // in shared memory (the 64-byte swizzle: unit u of 16 bytes at u ^ token / 2 % 4, free
 // of bank conflicts); a TMA store takes them from there, past the tensor's ends as
-// well. The warps of a feature quarter take every other 32 tokens; each has two buffers
+// well (or the lanes do, store_rows). The warps of a feature quarter take every other 32 tokens; each has two buffers
 // of its own (`turn` is the next), so the warps do not wait for one another; the next
 // sums are read under the stores. 32 tokens take about 500 cycles of a warp (640 written
 // by the lanes): with four warps, more than the instructions of a tile 1024 wide.
@@ -337,6 +375,11 @@ __device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* m
                         put + turn + 512 * g),
                     "r"(m[4 * g]), "r"(m[4 * g + 1]), "r"(m[4 * g + 2]), "r"(m[4 * g + 3])
                     : "memory");
+            if (!w.tma_out) {
+                __syncwarp();
+                store_rows<T>(w, buf + turn, n0, t0 + j, min(32, here - j), lane);
+                continue;
+            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -353,8 +396,7 @@ __device__ __forceinline__ void store_pieces(const Work& w, const CUtensorMap* m
 // A tile's results by way of fp32 sums in shared memory: of a cluster's CTAs, each
 // joins its share of the tile's tokens, reading its part of the sums from every CTA
 // (in the order of their ranks, so results do not depend on which is first). Also
-// for one CTA where the results are fp32 or not aligned for store_pieces. False: a
-// wait gave up.
+// for one CTA's fp32 results. False: a wait gave up.
 template <typename T>
 __device__ __forceinline__ bool store_joined(const Work& w, uint32_t sums, uint8_t* stage,
                                              uint32_t parts, uint32_t bar, uint32_t parity,
@@ -789,7 +831,7 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
 //     4096 x 4096 -> 4096: 59.4 and 53.1; 16384 x 4096 -> 8192: 426 and 399).
 //   * Sharing a tile costs 0.9 + n / 40 (64 x 8192 -> 2048: 15.2 us alone, 10.7 by two,
 //     9.4 by four CTAs; 64 x 2048 -> 2560: 6.2, 6.2 and 6.4).
-ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool wide_stores,
+ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool half,
                          int sms) {
     const int64_t chunks = (width + kChunk - 1) / kChunk;
     ProductPlan best{};
@@ -828,7 +870,7 @@ ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bo
         if (tokens % 32 == 0 && tokens >= 64) consider(1, true, tokens);
     }
     best.chunks = best.pair || best.tile_tokens < 128 || best.split > 1 ? 2 : 1;
-    best.pieces = best.split == 1 && wide_stores;
+    best.pieces = best.split == 1 && half;
     int stages = kMaxStages;
     auto smem = [&] {
         return smem_of(best.tile_tokens, best.split, best.pair, best.chunks, best.pieces, stages);
@@ -843,7 +885,8 @@ ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bo
 
 cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
                            const CUtensorMap& map_w, const CUtensorMap& map_x,
-                           const CUtensorMap& map_out, unsigned wait_limit, cudaStream_t st) {
+                           const CUtensorMap& map_out, bool tma_out, unsigned wait_limit,
+                           cudaStream_t st) {
     Work w{};
     w.p = p;
     w.tile_tokens = plan.tile_tokens;
@@ -867,6 +910,8 @@ cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductP
     const int e = out_dtype == TLB_FLOAT32 ? 4 : 2;
     w.aligned = reinterpret_cast<uintptr_t>(p.out) % (4 * e) == 0 && p.out_stride % 4 == 0;
     w.pieces = plan.pieces;
+    w.tma_out = tma_out;
+    w.pairs_out = reinterpret_cast<uintptr_t>(p.out) % 4 == 0 && p.out_stride % 2 == 0;
     auto start = [&](auto pair, auto chunks) {
         constexpr bool kPair = decltype(pair)::value;
         constexpr int kChunks = decltype(chunks)::value;
