@@ -825,8 +825,8 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
 //     weight is read once, all CTAs' weights at 6.3 TB/s. Weights too many for the L2 cost
 //     0.7 of that where several tiles read them (33 x 4096 -> 28672: 23.6 us in a tile of
 //     48 tokens, 33.5 in two of 32).
-//   * A tile's end takes 0.5, and a tile no less than its results' way to memory, 0.0118 a
-//     token (13863 x 208 -> 9928: 106 us with single CTAs, 91 with pairs, 275 MB).
+//   * A tile's end takes 0.5, and a tile no less than its results' way to memory, 0.3 and
+//     0.0118 a token (13863 x 208 -> 9928: 106 us with single CTAs, 91 with pairs, 275 MB).
 //   * Pairs start 1.2 later (1024 x 2048 -> 2560: 9.0 us with single CTAs, 9.7 with pairs;
 //     4096 x 4096 -> 4096: 59.4 and 53.1; 16384 x 4096 -> 8192: 426 and 399).
 //   * Sharing a tile costs 0.9 + n / 40 (64 x 8192 -> 2048: 15.2 us alone, 10.7 by two,
@@ -851,7 +851,7 @@ ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bo
         if (tiles_t > 1) stream *= features * width > (64 << 20) ? 0.7 : 0;
         if (stream > chunk) chunk = stream;
         double tile = (double)((chunks + split - 1) / split) * chunk + 0.5;
-        if (tile < 0.0118 * tokens) tile = 0.0118 * tokens;
+        if (tile < 0.3 + 0.0118 * tokens) tile = 0.3 + 0.0118 * tokens;
         double time = rounds * tile + (pair ? 1.2 : 0);
         if (split > 1) time += rounds * (0.9 + tokens / 40.0);
         if (best_time == 0 || time < best_time) {
