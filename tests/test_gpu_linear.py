@@ -74,7 +74,7 @@ def test_rows_with_infinities_nan_and_extremes(dtype):
         assert torch.equal(q.float().cpu()[keep], want_q.float().cpu()[keep])
 
 
-# |y' - y| <= delta |y|. The sum of squares: a lane's chain of at most 32 (64 for any
+# |y' - y| <= delta |y|. The sum of squares: a lane's chain of at most 32 (80 for any
 # width) additions and 10 (13) across lanes and warps, halved by the root; rsqrtf 2 ulp
 # (2^-22); the quotient, eps and two products 2^-24 each: under 2^-18.
 NORM_DELTA = 2.0 ** -18
@@ -172,6 +172,35 @@ def test_strided_and_unaligned_rows():
         O.assert_rows_of(q, s, O.silu_mul(x), delta)
     x = wide[:1, :256].expand(7, -1)  # one row seven times
     assert same_bytes(L.quantize_rows(x)[0], O.quantize_rows(x)[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=short)
+@pytest.mark.parametrize("t,k", [(3, 8), (700, 136), (700, 2008), (2, 16376), (40, 4092),
+                                 (40, 4097)])
+def test_rows_that_end_in_a_short_group(t, k, dtype):
+    """Rows of whole 16-byte pieces and others, parts of wider ones that hold infinities
+    behind them: neither a scale nor a norm takes in what is not the row's."""
+    g = torch.Generator().manual_seed(t + k)
+    pad = 16 + -k % 8
+    wide = torch.full((t, 2 * k + pad), float("inf"), dtype=dtype)
+    wide[:, :k] = rows(g, t, k, dtype, 0.5)
+    wide = wide.cuda()
+    x = wide[:, :k]
+    q, s = L.quantize_rows(x)
+    want = O.quantize_rows(x)
+    assert same_bytes(q, want[0]) and same_bytes(s, want[1])
+    w = (1 + 0.2 * torch.randn(k, generator=g)).to(dtype).cuda()
+    q, s, _ = L.rms_norm_quantized(x, w, 1e-6)
+    O.assert_rows_of(q, s, O.norm(x, w, 1e-6, None)[0], NORM_DELTA)
+    q, s, h = L.rms_norm_quantized(x, w, 1e-6, x.clone())
+    want, want_h = O.norm(x, w, 1e-6, x)
+    assert torch.equal(h, want_h)
+    O.assert_rows_of(q, s, want, NORM_DELTA)
+    wide[:, k:2 * k] = 2 * torch.randn(t, k, generator=g).to(dtype).cuda()
+    x = wide[:, :2 * k]
+    q, s = L.silu_and_mul_quantized(x)
+    delta = (6 + 1.2 * x[:, :k].double().abs()) * 2.0 ** -23
+    O.assert_rows_of(q, s, O.silu_mul(x), delta)
 
 
 def test_weight_blocks():

@@ -44,8 +44,6 @@ int sm_count(int* sms) {
     return cuda_result(e, "a device query");
 }
 
-constexpr int64_t kGroup = 128;
-
 // Rows of bytes or 16-bit elements as a 2-D tensor {width, rows}, read or written in
 // boxes of {box_width, box_rows}, swizzled by rows of a box, zeros past the ends.
 // Encoded for each call (under a microsecond): nothing is kept by address.
@@ -87,7 +85,7 @@ int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream) {
     TLB_REQUIRE(a.out && a.scales && a.x && (!norm || a.weight) && (!a.residual || a.residual_out),
                 "tensor pointers must not be null");
     const int e = elem_bytes(a.dtype);
-    bool vec = a.width % kGroup == 0 && aligned(a.out, 8);
+    bool vec = a.width % 8 == 0 && aligned(a.out, 8);
     const void* h = a.residual ? a.residual_out : nullptr;
     for (const void* p : {a.x, a.residual, a.weight, h}) {
         TLB_REQUIRE(!p || aligned(p, e), "tensor pointers must be aligned to the element size");

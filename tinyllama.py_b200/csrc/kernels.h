@@ -343,7 +343,8 @@ struct RowQuantParams {
     int op;                    // TLB_ROWS_*
     float eps;
 };
-// `vec`: pointers, strides and the width allow 16-byte accesses and whole groups.
+// `vec`: pointers, strides and the width allow pieces of eight values, 16 bytes of a
+// 16-bit type.
 cudaError_t launch_quantize_rows(int dtype, const RowQuantParams& p, int sms, bool vec,
                                  cudaStream_t stream);
 

@@ -107,28 +107,30 @@ struct FastDivisor {
 };
 
 // ------------------------------------------------- plain rows, gated activation
-// Flat over the eight-value pieces of all rows (K a multiple of 128, so a group is half
-// a warp wherever it lies), kSteps pieces of a lane in flight. Bounded by HBM and, the
-// gated form, nearly as much by its instructions.
+// Flat over the eight-value pieces of all rows, each row's filled up to whole groups
+// (so that a group is half a warp wherever it lies), kSteps pieces of a lane in flight.
+// Bounded by HBM and, the gated form, nearly as much by its instructions.
 template <typename T, bool kSilu, int kSteps>
 __global__ void __launch_bounds__(256) quantize_pieces_kernel(const RowQuantParams p,
-                                                              const FastDivisor row_pieces,
+                                                              const FastDivisor padded,
                                                               const uint32_t pieces) {
     grid_dependency_wait();
     grid_launch_dependents();
     const uint32_t mask = group_mask<kLanes>();
-    const uint32_t step = gridDim.x * 256 * kSteps;
+    const uint32_t step = gridDim.x * 256 * kSteps, row_pieces = p.width / 8;
     for (uint32_t base = blockIdx.x * 256 * kSteps; base < pieces; base += step) {
         Raw8<T> x[kSteps], u[kSilu ? kSteps : 1];
+        long long to[kSteps];  // the piece's place in the result, -1: none
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const uint32_t i = base + s * 256 + threadIdx.x;
             x[s].zero();
             if constexpr (kSilu) u[s].zero();
-            if (i < pieces) {
-                const uint32_t r = row_pieces.divide(i);
-                const T* src = reinterpret_cast<const T*>(p.x) + r * p.x_stride +
-                               (i - r * row_pieces.by) * 8;
+            const uint32_t r = padded.divide(i), piece = i - r * padded.by;
+            to[s] = -1;
+            if (i < pieces && piece < row_pieces) {
+                to[s] = (long long)r * row_pieces + piece;
+                const T* src = reinterpret_cast<const T*>(p.x) + r * p.x_stride + piece * 8;
                 x[s].load_stream(src);
                 if constexpr (kSilu) u[s].load_stream(src + p.width);
             }
@@ -148,8 +150,8 @@ __global__ void __launch_bounds__(256) quantize_pieces_kernel(const RowQuantPara
             } else {
                 q = quantize_raw<T>(x[s], mask, byte);
             }
-            if (i < pieces) {
-                reinterpret_cast<uint2*>(p.out)[i] = q;
+            if (to[s] >= 0) {
+                reinterpret_cast<uint2*>(p.out)[to[s]] = q;
                 if ((threadIdx.x & (kLanes - 1)) == 0) p.scales[i / kLanes] = (uint8_t)byte;
             }
         }
@@ -230,26 +232,35 @@ __global__ void rms_norm_kernel(const RowQuantParams p) {
         if (i < row_pieces) {
             reinterpret_cast<uint2*>(p.out)[r * row_pieces + i] = q;
             if ((tid & (kLanes - 1)) == 0)
-                p.scales[r * (row_pieces / kLanes) + i / kLanes] = (uint8_t)byte;
+                p.scales[r * ((row_pieces + kLanes - 1) / kLanes) + i / kLanes] = (uint8_t)byte;
         }
     }
 }
 
 // ------------------------------------------------------- any width, any alignment
-// A CTA a row, a warp a group, element by element; rows are read twice (three
-// times by the norm).
-template <typename T>
+// A CTA a row, a warp a group, element by element; the norm reads its rows twice. Bounded
+// by the instructions that an element takes (16000 x 3001 bf16: plain 50 us, gated 66, norm
+// with residual 159; by pieces, at 3000 values a row, 28, 43 and 59). Four groups of a warp
+// at once were slower (124, 183, 232: too many registers).
+template <typename T, int kOp>
 __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
+    constexpr bool kNorm = kOp == TLB_ROWS_RMS_NORM, kSilu = kOp == TLB_ROWS_SILU_AND_MUL;
     __shared__ float sums[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.width;
     const int groups = (K + kGroup - 1) / kGroup;
+    // a lane's values of a group are 32 apart; element i is the same thread's every time,
+    // so that it reads back what it stored
+    auto load = [&](const T* from, int first, float (&to)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            to[j] = first + 32 * j < K ? Elem<T>::to_f(from[first + 32 * j]) : 0.f;
+    };
     for (long long r = blockIdx.x; r < p.num_rows; r += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(p.x) + r * p.x_stride;
-        const T* w = reinterpret_cast<const T*>(p.weight);
         InverseRoot inv(1.f);
-        if (p.op == TLB_ROWS_RMS_NORM) {
+        if constexpr (kNorm) {
             const T* res = reinterpret_cast<const T*>(p.residual);
             T* h = nullptr;
             if (res) {
@@ -257,17 +268,23 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantPa
                 h = reinterpret_cast<T*>(p.residual_out) + r * p.residual_out_stride;
             }
             float sum = 0.f;
-            // element i is the same thread's here and below, so that it reads back
-            // what it stored
-            for (int g = warp; g < groups; g += 8)
-                for (int i = g * kGroup + lane; i < min(K, (g + 1) * kGroup); i += 32) {
-                    float v = Elem<T>::to_f(x[i]);
-                    if (h) {
-                        h[i] = Elem<T>::from_f(add_keep(v, Elem<T>::to_f(res[i])));
-                        v = Elem<T>::to_f(h[i]);
+            for (int g = warp; g < groups; g += 8) {
+                const int first = g * kGroup + lane;
+                float f[4];
+                load(x, first, f);
+                if (h) {
+                    float y[4];
+                    load(res, first, y);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const T e = Elem<T>::from_f(add_keep(f[j], y[j]));
+                        if (first + 32 * j < K) h[first + 32 * j] = e;
+                        f[j] = Elem<T>::to_f(e);
                     }
-                    sum = fmaf(v, v, sum);
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum = fmaf(f[j], f[j], sum);
+            }
             sum = group_sum<32>(sum, 0xffffffffu);
             if (lane == 0) sums[warp] = sum;
             __syncthreads();
@@ -277,26 +294,28 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantPa
             if (h) x = h;
         }
         for (int g = warp; g < groups; g += 8) {
+            const int first = g * kGroup + lane;
             float f[4];
+            load(x, first, f);
+            if constexpr (kNorm || kSilu) {
+                float y[4];
+                load(kNorm ? reinterpret_cast<const T*>(p.weight) : x + K, first, y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (first + 32 * j < K)  // 0 * an infinite root would be NaN
+                        f[j] = kNorm ? inv.scaled(f[j], y[j]) : silu_mul(f[j], y[j]);
+                }
+            }
             uint32_t m = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = g * kGroup + lane + 32 * j;
-                f[j] = 0.f;
-                if (i < K) {
-                    f[j] = Elem<T>::to_f(x[i]);
-                    if (p.op == TLB_ROWS_RMS_NORM) f[j] = inv.scaled(f[j], Elem<T>::to_f(w[i]));
-                    if (p.op == TLB_ROWS_SILU_AND_MUL) f[j] = silu_mul(f[j], Elem<T>::to_f(x[K + i]));
-                }
-                m = max(m, finite_abs_bits(f[j]));
-            }
+            for (int j = 0; j < 4; ++j) m = max(m, finite_abs_bits(f[j]));
             const uint32_t byte = scale_byte<E4M3>(group_max<32>(m, 0xffffffffu));
-            const float scale = inverse_scale(byte);
+            const uint32_t q =
+                quantize4<E4M3, false>(f[0], f[1], f[2], f[3], inverse_scale(byte));
+            uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + r * K;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = g * kGroup + lane + 32 * j;
-                if (i < K) store_quantized1(reinterpret_cast<E4M3*>(p.out) + r * K + i, f[j], scale);
-            }
+            for (int j = 0; j < 4; ++j)
+                if (first + 32 * j < K) out[first + 32 * j] = (uint8_t)(q >> (8 * j));
             if (lane == 0) p.scales[r * groups + g] = (uint8_t)byte;
         }
     }
@@ -321,13 +340,16 @@ cudaError_t launch_norm(const RowQuantParams& p, int sms, cudaStream_t st) {
     return launch_early(rms_norm_kernel<T, kResidual, 4>, grid, threads(4), 0, st, p);
 }
 
+// Eight-value pieces of a row's groups, the last of them filled up.
+long long padded_pieces(int width) { return (width + kGroup - 1ll) / kGroup * kLanes; }
+
 template <typename T, bool kSilu, int kSteps>
 cudaError_t launch_pieces(const RowQuantParams& p, int sms, cudaStream_t st) {
-    const long long pieces = p.num_rows * (p.width / 8);
+    const long long padded = padded_pieces(p.width), pieces = p.num_rows * padded;
     const long long want = (pieces + 256 * kSteps - 1) / (256 * kSteps), cap = 8ll * sms;
     return launch_early(quantize_pieces_kernel<T, kSilu, kSteps>,
                         dim3((unsigned)(want < cap ? want : cap)), 256, 0, st, p,
-                        FastDivisor((uint32_t)(p.width / 8)), (uint32_t)pieces);
+                        FastDivisor((uint32_t)padded), (uint32_t)pieces);
 }
 
 template <typename T>
@@ -336,10 +358,14 @@ cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) 
     // pieces of the others that 32-bit indexes count
     const bool held = p.op == TLB_ROWS_RMS_NORM
                           ? p.width <= 16384 && p.num_rows < (1ll << 31)
-                          : p.num_rows * (p.width / 8) < (1ll << 31) - (1 << 24);
+                          : p.num_rows * padded_pieces(p.width) < (1ll << 31) - (1 << 24);
     if (!vec || !held) {
-        const long long rows = p.num_rows < 8ll * sms ? p.num_rows : 8ll * sms;
-        return launch_early(quantize_rows_any_kernel<T>, dim3((unsigned)rows), 256, 0, st, p);
+        const long long rows = p.num_rows < 32ll * sms ? p.num_rows : 32ll * sms;
+        return launch_early(p.op == TLB_ROWS_RMS_NORM ? quantize_rows_any_kernel<T, TLB_ROWS_RMS_NORM>
+                            : p.op == TLB_ROWS_SILU_AND_MUL
+                                ? quantize_rows_any_kernel<T, TLB_ROWS_SILU_AND_MUL>
+                                : quantize_rows_any_kernel<T, TLB_ROWS_PLAIN>,
+                            dim3((unsigned)rows), 256, 0, st, p);
     }
     if (p.op == TLB_ROWS_RMS_NORM)
         return p.residual ? launch_norm<T, true>(p, sms, st) : launch_norm<T, false>(p, sms, st);
@@ -347,7 +373,7 @@ cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) 
     // 33.1 us, 38.3 with 32 bytes), one piece where more CTAs are worth more (64 x 2048:
     // 1.3 us, 2.0 with four).
     constexpr int kSteps = sizeof(T) == 2 ? 4 : 1, kSiluSteps = (kSteps + 1) / 2;
-    const bool few = p.num_rows * (p.width / 8) <= 256ll * 4 * sms;
+    const bool few = p.num_rows * padded_pieces(p.width) <= 256ll * 4 * sms;
     if (p.op == TLB_ROWS_SILU_AND_MUL)
         return few ? launch_pieces<T, true, 1>(p, sms, st)
                    : launch_pieces<T, true, kSiluSteps>(p, sms, st);
