@@ -612,6 +612,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t desc = first;
             int s = 0, set = 0, it = 0;
             uint32_t parity = 0, set_parity = 0;
+            // Nothing is read here, but the scales and stages come no earlier: a bounded wait
+            // begun before this would count the rest of the kernel before as well, which
+            // may be longer than the bound.
+            grid_dependency_wait();
             for (int i = unit; i < tiles && ok; i += units, ++it) {
                 const int b = it & 1;
                 if (it >= 2 && !mbar_wait_bounded(bar(kBarSumsFree + b), ((it >> 1) - 1) & 1, limit)) {
