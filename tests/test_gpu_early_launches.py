@@ -5,7 +5,9 @@ import pytest
 import torch
 
 from cscr import _lib
+from cscr import attention as A
 from cscr import linear as L
+from cscr import pos_encoding as PE
 
 pytestmark = pytest.mark.gpu
 
@@ -55,6 +57,42 @@ def test_product_behind_a_long_kernel(t, k, n):
     _lib.set_wait_limit(FEW_PROBES)
     L.matmul_quantized(*long, torch.float32)
     got = L.matmul_quantized(*ops, torch.bfloat16)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("h,kvh,d", [(16, 2, 128), (32, 2, 64)])
+def test_attention_behind_a_long_kernel(h, kvh, d):
+    """A rotation that overlaps the kernel before it lets the attention behind it begin
+    while that kernel still runs."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    seqs, bs, blocks = 8, 16, 64
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(torch.bfloat16)
+
+    query, key, value = randn(seqs, h * d), randn(seqs, kvh * d), randn(seqs, kvh, d)
+    caches = [randn(blocks, kvh, bs, d) for _ in range(2)]
+    tables = torch.arange(blocks, dtype=torch.int32, device="cuda").view(seqs, -1)
+    lens = torch.arange(1, 8 * bs, 8 * bs // seqs, dtype=torch.int32, device="cuda")[:seqs]
+    positions, table = lens.long() - 1, randn(8 * bs, d)
+
+    def step(overlap):
+        kc, vc = (c.clone() for c in caches)
+        k = key.clone()
+        if overlap:
+            L.matmul_quantized(*long, torch.float32)
+        q = PE.rotary_embedding_neox_with_cache(positions, query, k, value, kc, vc, None, d, table,
+                                                tables, overlap_previous=overlap)
+        return A.paged_attention(q.view(seqs, h, d), kc, vc, tables, lens, d ** -0.5,
+                                 overlap_prologue=overlap)
+
+    long = long_kernel()
+    want = step(False)
+    torch.cuda.synchronize()
+    _lib.set_wait_limit(FEW_PROBES)
+    got = step(True)
     torch.cuda.synchronize()
     assert _lib.device_status() == 0
     assert torch.equal(got, want)

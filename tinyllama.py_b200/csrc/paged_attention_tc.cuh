@@ -863,6 +863,8 @@ __global__ void __launch_bounds__((CW + 2) * 32, (NT == 1 && CW == 4) ? 2 : 1)
         // all of them. None of this stalls the KV stream.
         constexpr int kPer4 = GP * D / 128;  // float4 groups of the piece per lane
         uint32_t ephase = 0;
+        // no bounded wait begins while the kernel before may still run (see the consumers)
+        grid_dependency_wait();
         while (true) {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(bar_epi_full, ephase, wlim))) {
                 if (lane == 0) flag_status(TLB_STATUS_WAIT_TIMEOUT);
@@ -1334,6 +1336,10 @@ __global__ void __launch_bounds__((CW + 2) * 32, (NT == 1 && CW == 4) ? 2 : 1)
         }
     };
 
+    // The producer's copies start behind this wait, so nothing arrives earlier; a bounded
+    // wait begun before it would count the rest of the kernel before as well, which may be
+    // longer than the bound.
+    grid_dependency_wait();
     while (true) {
         bool got = true;
         // warp-uniform outcome: the warp's mma and shuffles below need all lanes
