@@ -583,7 +583,8 @@ TLB_API int tlb_paged_attention_scored(const tlb_scored_attention_args* args, vo
  * op:
  *   TLB_ROWS_PLAIN        : the rows of x [num_rows, width]
  *   TLB_ROWS_SILU_AND_MUL : x [num_rows, 2 * width] holds gate and up:
- *                           gate / (1 + exp(-gate)) * up
+ *                           gate / (1 + exp(-gate)) * up; 0 where exp(-gate) is
+ *                           infinite in fp32 (gates below -88.7)
  *   TLB_ROWS_RMS_NORM     : h = x, or x + residual rounded to dtype and written to
  *                           residual_out (which may be residual or x itself) when
  *                           residual is not NULL; h * rsqrt(mean(h^2) + eps) * weight

@@ -1,0 +1,57 @@
+"""Calls of the 8-bit projection operators at the edges of what their documentation
+allows, against the 64-bit oracle."""
+
+import pytest
+import torch
+
+from cscr import _lib
+from cscr import linear as L
+from oracle import linear_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def short(p):
+    return str(p).replace("torch.", "") if isinstance(p, torch.dtype) else None
+
+
+@pytest.fixture(autouse=True)
+def _clean(built_lib):
+    torch.cuda.set_device(0)
+    _lib.set_wait_limit(_lib.WAIT_LIMIT_DEFAULT)
+    _lib.device_status()
+    yield
+    _lib.set_wait_limit(_lib.WAIT_LIMIT_DEFAULT)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("k", [8, 5, 264])
+@pytest.mark.parametrize("dtype", TYPES, ids=short)
+def test_silu_of_far_gates_and_large_values(dtype, k):
+    """Where exp(-gate) is a number of fp32, the gate's factor is none below 2^-126."""
+    top = torch.finfo(dtype).max
+    gate = torch.tensor([-79.5, -80.0, -84.0, -87.0, -87.5, -88.0, -88.5])  # exact in every type
+    up = torch.tensor([1.0, 1e3, 1e4, -5e4, 1e20, -1e30, top, -top]).clamp(-top, top)
+    x = torch.stack([v.flatten() for v in torch.meshgrid(gate, up, indexing="ij")], 1).to(dtype)
+    assert torch.equal(x[::8, 0].float(), gate)
+    x = x.cuda().repeat_interleave(k, 1)  # each row a value of its own
+    q, s = L.silu_and_mul_quantized(x)
+    delta = (6 + 1.2 * x[:, :k].double().abs()) * 2.0 ** -23
+    O.assert_rows_of(q, s, O.silu_mul(x), delta)
+
+
+@pytest.mark.parametrize("k", [8, 5])
+def test_silu_of_gates_past_fp32(k):
+    """exp(-gate) infinite: 0, and NaN times an infinite value or from an infinite gate."""
+    inf = float("inf")
+    gate = torch.tensor([-89.0, -120.0, -300.0, -3e38, -1e4, -inf, -inf, -90.0, inf, 3e38])
+    up = torch.tensor([3e38, 3e38, 3e38, -3e38, 1.0, 0.0, 1.0, inf, 2.0, 1e-38])
+    x = torch.stack((gate, up), 1).cuda().repeat_interleave(k, 1)
+    q, s = L.silu_and_mul_quantized(x)
+    assert not q[:5].float().any()
+    assert bool(torch.isnan(q[5:8].float()).all()) and bool((q[8].float() == 448).all())
+    O.assert_rows_of(q[9:], s[9:], O.silu_mul(x[9:]), 2.0 ** -20)  # a gate is not scaled up

@@ -92,7 +92,8 @@ def silu_and_mul_quantized(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.T
     """``gate / (1 + exp(-gate)) * up`` in 8 bits: gate_up [T, 2 K] holds each token's
     gate values, then its up values (float16, bfloat16 or float32, rows possibly
     strided). Returns (values [T, K], scales [T, ceil(K / 128)]); fp32 math, one
-    rounding. Results below 2^-126 in magnitude may count as 0."""
+    rounding: gates below -88.7, whose ``exp(-gate)`` is infinite in fp32, give 0
+    (NaN where up is infinite), and results below 2^-126 in magnitude may count as 0."""
     if _lib.fast is not None:
         out = _lib.fast.rows(gate_up, _SILU_AND_MUL, None, 0.0, None, None)
         if out is not None:
