@@ -55,3 +55,20 @@ def test_silu_of_gates_past_fp32(k):
     assert not q[:5].float().any()
     assert bool(torch.isnan(q[5:8].float()).all()) and bool((q[8].float() == 448).all())
     O.assert_rows_of(q[9:], s[9:], O.silu_mul(x[9:]), 2.0 ** -20)  # a gate is not scaled up
+
+
+@pytest.mark.parametrize("k", [40, 896, 1000, 1111, 1536, 2336, 3001, 3584, 5632, 13000, 20000])
+@pytest.mark.parametrize("dtype", TYPES, ids=short)
+def test_norm_of_values_on_a_border(dtype, k):
+    """Rows of +-c have a mean square of c^2, whatever their width (sums of few bits, exact
+    in any order): the normed values are the weights with x's signs, exactly, and lie on
+    borders of 8 bits, which go to even."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    c = torch.tensor([2.0, 2.5, 3.0, 1.25, 5.0, 7.0, 0.75, 11.0, 2.75, 13.0, 3.25], device="cuda")
+    x = torch.randint(0, 2, (len(c), k), generator=g, device="cuda") * 2 - 1
+    w = (1 + 0.2 * torch.randn(k, generator=g, device="cuda")).to(torch.bfloat16).to(dtype)
+    want_q, want_s = O.quantize_rows(x * w.double())
+    x = (x * c[:, None]).to(dtype)
+    q, s, _ = L.rms_norm_quantized(x, w, 0.0)
+    assert torch.equal(s.view(torch.uint8), want_s.view(torch.uint8))
+    assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))

@@ -342,6 +342,7 @@ struct RowQuantParams {
     int width;
     int op;                    // TLB_ROWS_*
     float eps;
+    float inverse_width, inverse_width_rest;  // their sum is 1 / width
 };
 // `vec`: pointers, strides and the width allow pieces of eight values, 16 bytes of a
 // 16-bit type.
