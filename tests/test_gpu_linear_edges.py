@@ -72,3 +72,44 @@ def test_norm_of_values_on_a_border(dtype, k):
     q, s, _ = L.rms_norm_quantized(x, w, 0.0)
     assert torch.equal(s.view(torch.uint8), want_s.view(torch.uint8))
     assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
+
+
+# as the other norms of random values: under 2^-18 (a chain of at most 80 additions and 13
+# across lanes and warps, halved by the root, and some roundings)
+NORM_DELTA = 2.0 ** -18
+
+
+def norm_delta(h, w, y):
+    """The same with values and results among fp32's subnormal numbers: a product of value
+    and weight below 2^-126 is a multiple of 2^-149, so off by 2^-150 before the root scales
+    it, and so is a result; both by as much again in the root's second part."""
+    product = (h.double() * w.double()).abs()
+    steps = (2.0 ** -149 / product) * (product < 2.0 ** -126) + (2.0 ** -149 / y.abs()) * (
+        y.abs() < 2.0 ** -126)
+    return NORM_DELTA + torch.where(y == 0, 0, steps)
+
+
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("k", [264, 1000, 1111, 4096, 20000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=short)
+def test_norm_of_far_rows(dtype, k, with_residual):
+    """Rows whose squares leave fp32's range, upwards or downwards: small enough ones count
+    against eps, or, without one, are normed as any other."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    e = torch.tensor([-132, -126, -110, -80, -70, -64, -58, -51, -49, -40, 0, 50, 58, 62, 64, 70,
+                      90, 110, 124], device="cuda")
+    x = torch.randn(len(e), k, generator=g, device="cuda", dtype=torch.float64).clamp(-7, 7)
+    x = (x * 2.0 ** e[:, None]).to(dtype)
+    w = (1 + 0.2 * torch.randn(k, generator=g, device="cuda")).to(dtype)
+    res = x / 2 if with_residual else None
+    for eps in (0.0, 1e-38, 1e-30, 1e-6, 1.0):
+        q, s, h = L.rms_norm_quantized(x, w, eps, res)
+        want, want_h = O.norm(x, w, eps, res)
+        assert h is None or torch.equal(h, want_h)
+        O.assert_rows_of(q, s, want, norm_delta(want_h, w, want))
+    # a weight that takes a product of small values below 2^-126, which the root makes up for
+    x = torch.full((2, k), 2.0 ** -120, device="cuda").to(dtype)
+    w = torch.full((k,), 1.25 * 2.0 ** -10, device="cuda").to(dtype)
+    q, s, _ = L.rms_norm_quantized(x, w, 1e-6)
+    want = O.norm(x, w, 1e-6)[0]
+    O.assert_rows_of(q, s, want, norm_delta(x, w, want))

@@ -98,11 +98,35 @@ struct InverseRoot {
     // values are rounded to 8 bits next, and each rounding before that moves some of
     // them over a border (16383 x 4096: 31 to 44 of 67 M, 50 to 190 with one rounding for
     // each step).
-    __device__ __forceinline__ float scaled(float x, float w) const {
-        const float v = x * w;
-        return fmaf(v, high, v * low);
+    template <int N>
+    __device__ __forceinline__ void scale(float (&x)[N], const float (&w)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const Pair v = Pair(x[i], x[i + 1]) * Pair(w[i], w[i + 1]);
+            fma2(v, Pair(high, high), v * Pair(low, low)).get(x[i], x[i + 1]);
+        }
     }
 };
+
+// A row's values are taken this much larger (smaller) where their squares would leave fp32's
+// range: a mean below 2^-100 has lost squares below 2^-126, and an infinite one may come from
+// finite values. Squares of the former are then below 2^92 a value, of the latter below 2^96;
+// widths are below 2^30. Results do not depend on it. fp16 has no such values.
+template <typename T> __device__ __forceinline__ float range_shift(float mean) {
+    if (std::is_same<T, __half>::value || (mean >= 0x1p-100f && mean < INFINITY)) return 1.f;
+    return mean < 0x1p-100f ? 0x1p96f : 0x1p-80f;
+}
+template <int N>
+__device__ __forceinline__ void shift(float (&x)[N], float by) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = mul_keep(x[i], by);
+}
+template <int N>
+__device__ __forceinline__ float squares(const float (&x)[N], float sum) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum = fmaf(x[i], x[i], sum);
+    return sum;
+}
 
 // Eight fp32 values of a lane -> their 8 stored bytes, and the scale byte of the
 // 16 lanes' group.
@@ -252,20 +276,37 @@ __global__ void rms_norm_kernel(const RowQuantParams p) {
                 x[s].store(reinterpret_cast<T*>(p.residual_out) + r * p.residual_out_stride + i * 8);
         }
     }
+    // of the CTA's threads, the same bits in all of them
+    auto total = [&](float v) {
+        v = group_sum<32>(v, 0xffffffffu);
+        if (threads > 32) {
+            if ((tid & 31) == 0) sums[tid >> 5] = v;
+            __syncthreads();
+            v = group_sum<32>((tid & 31) < threads / 32 ? sums[tid & 31] : 0.f, 0xffffffffu);
+        }
+        return v;
+    };
 #pragma unroll
     for (int s = 0; s < kPieces; ++s) {
         float a[8];
         x[s].get(a);
+        sum = squares(a, sum);
+    }
+    float mean = mean_of(total(sum), p) + p.eps;
+    const float by = range_shift<T>(mean);
+    if (by != 1.f) {
+        sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(a[j], a[j], sum);
+        for (int s = 0; s < kPieces; ++s) {
+            float a[8];
+            x[s].get(a);
+            shift(a, by);
+            sum = squares(a, sum);
+        }
+        __syncthreads();  // before the sums are written again
+        mean = mean_of(total(sum), p) + mul_keep(mul_keep(p.eps, by), by);
     }
-    sum = group_sum<32>(sum, 0xffffffffu);
-    if (threads > 32) {
-        if ((tid & 31) == 0) sums[tid >> 5] = sum;
-        __syncthreads();
-        sum = group_sum<32>((tid & 31) < threads / 32 ? sums[tid & 31] : 0.f, 0xffffffffu);
-    }
-    const InverseRoot inv(mean_of(sum, p) + p.eps);
+    const InverseRoot inv(mean);
 #pragma unroll
     for (int s = 0; s < kPieces; ++s) {
         const int i = tid + s * threads;
@@ -275,8 +316,8 @@ __global__ void rms_norm_kernel(const RowQuantParams p) {
         if (i < row_pieces) wt.load(reinterpret_cast<const T*>(p.weight) + i * 8);
         x[s].get(a);
         wt.get(w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] = inv.scaled(a[j], w[j]);
+        if (by != 1.f) shift(a, by);
+        inv.scale(a, w);
         uint32_t byte;
         const uint2 q = quantize_group(a, mask, byte);
         if (i < row_pieces) {
@@ -289,11 +330,16 @@ __global__ void rms_norm_kernel(const RowQuantParams p) {
 
 // ------------------------------------------------------- any width, any alignment
 // A CTA a row, a warp a group, element by element; the norm reads its rows twice. Bounded
-// by the instructions that an element takes (16000 x 3001 bf16: plain 50 us, gated 68, norm
-// with residual 159; by pieces, at 3000 values a row, 28, 43 and 59). Four groups of a warp
-// at once were slower (124, 183, 232: too many registers).
+// by the instructions that an element takes (16000 x 3001 bf16: plain 50 us, gated 65, norm
+// with residual 127; by pieces, at 3000 values a row, 28, 43 and 58). Four groups of a warp
+// at once were slower (124, 183, 232: too many registers). Left to itself the compiler gives
+// the norm 56 registers and the gated form 38: 173 and 68 us.
+constexpr int any_ctas(int op) {
+    return op == TLB_ROWS_RMS_NORM ? 5 : op == TLB_ROWS_SILU_AND_MUL ? 8 : 1;
+}
 template <typename T, int kOp>
-__global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantParams p) {
+__global__ void __launch_bounds__(256, any_ctas(kOp))
+    quantize_rows_any_kernel(const RowQuantParams p) {
     grid_dependency_wait();
     grid_launch_dependents();
     constexpr bool kNorm = kOp == TLB_ROWS_RMS_NORM, kSilu = kOp == TLB_ROWS_SILU_AND_MUL;
@@ -310,6 +356,7 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantPa
     for (long long r = blockIdx.x; r < p.num_rows; r += gridDim.x) {
         const T* x = reinterpret_cast<const T*>(p.x) + r * p.x_stride;
         InverseRoot inv(1.f);
+        float by = 1.f;
         if constexpr (kNorm) {
             const T* res = reinterpret_cast<const T*>(p.residual);
             T* h = nullptr;
@@ -332,16 +379,30 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantPa
                         f[j] = Elem<T>::to_f(e);
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum = fmaf(f[j], f[j], sum);
+                sum = squares(f, sum);
             }
-            sum = group_sum<32>(sum, 0xffffffffu);
-            if (lane == 0) sums[warp] = sum;
-            __syncthreads();
-            sum = group_sum<32>(lane < 8 ? sums[lane] : 0.f, 0xffffffffu);
-            __syncthreads();  // before the next row's sums
-            inv = InverseRoot(mean_of(sum, p) + p.eps);
+            auto total = [&](float v) {
+                v = group_sum<32>(v, 0xffffffffu);
+                if (lane == 0) sums[warp] = v;
+                __syncthreads();
+                v = group_sum<32>(lane < 8 ? sums[lane] : 0.f, 0xffffffffu);
+                __syncthreads();  // before the next sums
+                return v;
+            };
             if (h) x = h;
+            float mean = mean_of(total(sum), p) + p.eps;
+            by = range_shift<T>(mean);
+            if (by != 1.f) {
+                sum = 0.f;
+                for (int g = warp; g < groups; g += 8) {
+                    float f[4];
+                    load(x, g * kGroup + lane, f);
+                    shift(f, by);
+                    sum = squares(f, sum);
+                }
+                mean = mean_of(total(sum), p) + mul_keep(mul_keep(p.eps, by), by);
+            }
+            inv = InverseRoot(mean);
         }
         for (int g = warp; g < groups; g += 8) {
             const int first = g * kGroup + lane;
@@ -350,13 +411,13 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const RowQuantPa
             if constexpr (kNorm || kSilu) {
                 float y[4];
                 load(kNorm ? reinterpret_cast<const T*>(p.weight) : x + K, first, y);
+                // values past the row's end count neither for a scale (0, or NaN where the
+                // root is infinite) nor are they written
                 if constexpr (kSilu) {
                     silu_mul(f, y);
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (first + 32 * j < K)  // 0 * an infinite root would be NaN
-                            f[j] = inv.scaled(f[j], y[j]);
+                    if (by != 1.f) shift(f, by);
+                    inv.scale(f, y);
                 }
             }
             uint32_t m = 0;
