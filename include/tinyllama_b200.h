@@ -586,9 +586,10 @@ TLB_API int tlb_paged_attention_scored(const tlb_scored_attention_args* args, vo
  *                           gate / (1 + exp(-gate)) * up; 0 where exp(-gate) is
  *                           infinite in fp32 (gates below -88.7)
  *   TLB_ROWS_RMS_NORM     : h = x, or x + residual rounded to dtype and written to
- *                           residual_out (which may be residual or x itself) when
- *                           residual is not NULL; h * rsqrt(mean(h^2) + eps) * weight
- * in fp32 with no rounding before the one to 8 bits.
+ *                           residual_out when residual is not NULL;
+ *                           h * rsqrt(mean(h^2) + eps) * weight
+ * residual_out may be residual or x itself, but no other part of the inputs' memory.
+ * Computed in fp32 with no rounding before the one to 8 bits.
  *   out : [num_rows, width] dense;  scales : [num_rows, ceil(width / 128)] dense
  *   x, residual, residual_out : rows their strides (in elements) apart
  *   weight : [width] of dtype

@@ -113,3 +113,21 @@ def test_norm_of_far_rows(dtype, k, with_residual):
     q, s, _ = L.rms_norm_quantized(x, w, 1e-6)
     want = O.norm(x, w, 1e-6)[0]
     O.assert_rows_of(q, s, want, norm_delta(x, w, want))
+
+
+def test_residual_out_over_other_rows_is_refused():
+    """Written while other rows are read: an error, not a race. Rows beside them are fine."""
+    k = 256
+    flat = torch.randn(9 * k, device="cuda").to(torch.bfloat16)
+    x, res = flat[:8 * k].view(8, k), torch.randn(8, k, device="cuda").to(torch.bfloat16)
+    w = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    for out in (flat[k:].view(8, k), flat[16:16 + 8 * k].view(8, k)):
+        for a, b in ((x, res), (res, x)):
+            with pytest.raises(RuntimeError, match="share no memory"):
+                L.rms_norm_quantized(a, w, 1e-6, b, residual_out=out)
+    wide = torch.randn(8, 2 * k, device="cuda").to(torch.bfloat16)
+    x, out = wide[:, :k], wide[:, k:]
+    want, want_h = O.norm(x, w, 1e-6, res)
+    q, s, h = L.rms_norm_quantized(x, w, 1e-6, res, residual_out=out)
+    assert torch.equal(out, want_h) and h.data_ptr() == out.data_ptr()
+    O.assert_rows_of(q, s, want, NORM_DELTA)

@@ -54,7 +54,7 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, eps: float,
     x and residual [T, K] in float16, bfloat16 or float32 (one type), rows possibly
     strided; weight [K] of that type. Returns (values [T, K] float8_e4m3fn, scales
     [T, ceil(K / 128)] float8_e8m0fnu, h or None): h goes to ``residual_out``, which
-    may be ``residual`` or ``x`` itself, or a new tensor.
+    may be ``residual`` or ``x`` itself, or a tensor that shares no memory with the inputs.
     """
     if _lib.fast is not None:
         out = _lib.fast.rows(x, _RMS_NORM, weight, eps, residual, residual_out)

@@ -44,6 +44,42 @@ int sm_count(int* sms) {
     return cuda_result(e, "a device query");
 }
 
+// Whether a call that writes rows `out` (of one CTA each) while it reads rows `in` reads what
+// it may have written: rows are the same ones, or have no byte in common. In bytes.
+struct Rows {
+    int64_t at, count, stride, width;
+};
+bool rows_clash(const Rows& in, const Rows& out) {
+    using wide = __int128;
+    if (in.at == out.at && in.count == out.count && in.width == out.width &&
+        (in.count == 1 || in.stride == out.stride))
+        return false;
+    const wide in_last = in.at + (wide)(in.count - 1) * in.stride;
+    const wide out_last = out.at + (wide)(out.count - 1) * out.stride;
+    auto low = [](wide a, wide b) { return a < b ? a : b; };
+    auto high = [](wide a, wide b) { return a < b ? b : a; };
+    if (high(in.at, in_last) + in.width <= low(out.at, out_last) ||
+        high(out.at, out_last) + out.width <= low(in.at, in_last))
+        return false;
+    const wide step = in.stride < 0 ? -(wide)in.stride : in.stride;
+    if (in.count > 1 && out.count > 1 && in.stride == out.stride && step > 0) {
+        // parts of the same wider rows: one place of the row decides
+        const wide away = (((wide)out.at - in.at) % step + step) % step;
+        return away < in.width || away > step - out.width;
+    }
+    // row by row of `out`: the first row of `in` (from its lowest) that ends behind its begin
+    const wide first = low(in.at, in_last);
+    for (int64_t r = 0; r < out.count; ++r) {
+        const wide begin = out.at + (wide)r * out.stride;
+        wide j = 0;
+        if (step > 0 && begin - first >= in.width) j = (begin - first - in.width) / step + 1;
+        if (j < in.count && first + j * step < begin + out.width &&
+            first + j * step + in.width > begin)
+            return true;
+    }
+    return false;
+}
+
 // Rows of bytes or 16-bit elements as a 2-D tensor {width, rows}, read or written in
 // boxes of {box_width, box_rows}, swizzled by rows of a box, zeros past the ends.
 // Encoded for each call (under a microsecond): nothing is kept by address.
@@ -93,6 +129,18 @@ int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream) {
     }
     vec = vec && a.x_stride * e % 16 == 0 &&
           (!a.residual || (a.residual_stride * e % 16 == 0 && a.residual_out_stride * e % 16 == 0));
+    if (a.residual) {
+        TLB_REQUIRE(a.num_rows < 2 || a.residual_out_stride >= a.width ||
+                        a.residual_out_stride <= -a.width,
+                    "residual_out's rows overlap");
+        const int64_t w = a.width * e;
+        auto at = [](const void* ptr) { return (int64_t)reinterpret_cast<uintptr_t>(ptr); };
+        const Rows written{at(a.residual_out), a.num_rows, a.residual_out_stride * e, w};
+        TLB_REQUIRE(!rows_clash({at(a.x), a.num_rows, a.x_stride * e, w}, written) &&
+                        !rows_clash({at(a.residual), a.num_rows, a.residual_stride * e, w}, written) &&
+                        !rows_clash({at(a.weight), 1, 0, w}, written),
+                    "residual_out must be x or residual itself, or share no memory with the inputs");
+    }
     tlb::RowQuantParams p{};
     p.out = a.out;
     p.scales = static_cast<uint8_t*>(a.scales);
