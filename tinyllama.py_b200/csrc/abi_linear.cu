@@ -153,14 +153,13 @@ int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream) {
     p.residual_stride = a.residual_stride;
     p.residual_out_stride = a.residual_out_stride;
     p.width = (int)a.width;
-    p.op = (int)a.op;
     p.eps = (float)a.eps;
     const double inverse = 1.0 / (double)a.width;
     p.inverse_width = (float)inverse;
     p.inverse_width_rest = (float)(inverse - p.inverse_width);
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
-    return cuda_result(tlb::launch_quantize_rows((int)a.dtype, p, sms, vec,
+    return cuda_result(tlb::launch_quantize_rows((int)a.dtype, (int)a.op, p, sms, vec,
                                                  reinterpret_cast<cudaStream_t>(stream)),
                        "quantize_rows");
 }

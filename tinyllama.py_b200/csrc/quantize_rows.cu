@@ -467,28 +467,28 @@ cudaError_t launch_pieces(const RowQuantParams& p, int sms, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) {
+cudaError_t launch(int op, const RowQuantParams& p, int sms, bool vec, cudaStream_t st) {
     // rows of the norm that a CTA holds in registers: 4 pieces of up to 512 threads;
     // pieces of the others that 32-bit indexes count
-    const bool held = p.op == TLB_ROWS_RMS_NORM
+    const bool held = op == TLB_ROWS_RMS_NORM
                           ? p.width <= 16384 && p.num_rows < (1ll << 31)
                           : p.num_rows * padded_pieces(p.width) < (1ll << 31) - (1 << 24);
     if (!vec || !held) {
         const long long rows = p.num_rows < 32ll * sms ? p.num_rows : 32ll * sms;
-        return launch_early(p.op == TLB_ROWS_RMS_NORM ? quantize_rows_any_kernel<T, TLB_ROWS_RMS_NORM>
-                            : p.op == TLB_ROWS_SILU_AND_MUL
+        return launch_early(op == TLB_ROWS_RMS_NORM ? quantize_rows_any_kernel<T, TLB_ROWS_RMS_NORM>
+                            : op == TLB_ROWS_SILU_AND_MUL
                                 ? quantize_rows_any_kernel<T, TLB_ROWS_SILU_AND_MUL>
                                 : quantize_rows_any_kernel<T, TLB_ROWS_PLAIN>,
                             dim3((unsigned)rows), 256, 0, st, p);
     }
-    if (p.op == TLB_ROWS_RMS_NORM)
+    if (op == TLB_ROWS_RMS_NORM)
         return p.residual ? launch_norm<T, true>(p, sms, st) : launch_norm<T, false>(p, sms, st);
     // 64 bytes of a lane in flight where there are enough pieces (16381 x 4096 fp16 rows
     // 33.1 us, 38.3 with 32 bytes), one piece where more CTAs are worth more (64 x 2048:
     // 1.3 us, 2.0 with four).
     constexpr int kSteps = sizeof(T) == 2 ? 4 : 1, kSiluSteps = (kSteps + 1) / 2;
     const bool few = p.num_rows * padded_pieces(p.width) <= 256ll * 4 * sms;
-    if (p.op == TLB_ROWS_SILU_AND_MUL)
+    if (op == TLB_ROWS_SILU_AND_MUL)
         return few ? launch_pieces<T, true, 1>(p, sms, st)
                    : launch_pieces<T, true, kSiluSteps>(p, sms, st);
     return few ? launch_pieces<T, false, 1>(p, sms, st)
@@ -497,12 +497,12 @@ cudaError_t launch(const RowQuantParams& p, int sms, bool vec, cudaStream_t st) 
 
 }  // namespace
 
-cudaError_t launch_quantize_rows(int dtype, const RowQuantParams& p, int sms, bool vec,
+cudaError_t launch_quantize_rows(int dtype, int op, const RowQuantParams& p, int sms, bool vec,
                                  cudaStream_t st) {
     switch (dtype) {
-        case TLB_FLOAT16: return launch<__half>(p, sms, vec, st);
-        case TLB_BFLOAT16: return launch<__nv_bfloat16>(p, sms, vec, st);
-        default: return launch<float>(p, sms, vec, st);
+        case TLB_FLOAT16: return launch<__half>(op, p, sms, vec, st);
+        case TLB_BFLOAT16: return launch<__nv_bfloat16>(op, p, sms, vec, st);
+        default: return launch<float>(op, p, sms, vec, st);
     }
 }
 
