@@ -14,6 +14,8 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <ATen/record_function.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -130,8 +132,19 @@ bool truth(PyObject* o, bool* x) {
 
 PyObject* later() { Py_RETURN_NONE; }
 
-// Straight from the allocator: through the dispatcher a tensor takes 0.3 us longer.
+// Whether nothing but the allocator takes part in an allocation: no dispatch mode or other
+// key of this thread, no fill of new memory under deterministic algorithms, no profiler.
+bool only_allocates() {
+    const auto keys = c10::impl::tls_local_dispatch_key_set().included_;
+    const at::Context& context = at::globalContext();
+    return (keys - c10::default_included_set).empty() && !at::hasCallbacks() &&
+           !(context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory());
+}
+
+// A new dense tensor; through the dispatcher it takes 0.3 us longer.
 Tensor dense(const Tensor& like, at::IntArrayRef sizes, ScalarType type) {
+    if (!only_allocates())
+        return at::empty(sizes, like.options().dtype(type), at::MemoryFormat::Contiguous);
     return Tensor(at::detail::empty_cuda(sizes, type, like.device(), at::MemoryFormat::Contiguous));
 }
 
