@@ -1,4 +1,5 @@
-"""Refusals of the 8-bit projection operators that need no GPU: outputs over inputs."""
+"""The 8-bit projection operators where no GPU is needed: outputs over inputs are refused,
+weights are converted without a graph."""
 
 import itertools
 
@@ -6,11 +7,11 @@ import pytest
 import torch
 
 from cscr import _lib
+from cscr import linear as L
 
 P = 1 << 20  # stands in for an aligned device pointer; nothing is dereferenced
 BAD, BF16, NORM = 1, 2, 2
 WEIGHT = 1 << 30  # far from the rows
-
 
 no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="calls that are taken would be "
                             "launched, on addresses that stand for none")
@@ -63,3 +64,13 @@ def test_refusals_are_those_of_rows_with_a_byte_in_common(built_lib, rows):
         clash = not same and any(abs(i - o) < 2 * width for i in ins for o in out)
         got = norm(lib, (base, a), (P << 10, 8), (base + 2 * away, b), rows, width)
         assert (got == BAD) == clash, (a, b, away, _lib.last_error())
+
+
+def test_weights_are_converted_without_gradients():
+    """A parameter's values and scales hold no graph (with copies of its blocks in fp32)."""
+    weight = torch.nn.Parameter(torch.randn(200, 300))
+    values, scales = L.quantize_weight(weight)
+    assert not values.requires_grad and values.grad_fn is None and not scales.requires_grad
+    want = L.quantize_weight(weight.detach())
+    for a, b in zip((values, scales), want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

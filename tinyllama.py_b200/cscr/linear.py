@@ -125,10 +125,11 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q, scales
 
 
+@torch.no_grad()
 def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """A weight [N, K] of finite values in 8 bits, with a scale for each block of
     128 x 128: (values [N, K], scales [ceil(N / 128), ceil(K / 128)]). Plain torch, on
-    the weight's device: a model's weights are converted once."""
+    the weight's device, without gradients: a model's weights are converted once."""
     torch_check(weight.dim() == 2 and weight.dtype in _FLOAT_TYPES,
                 "weight must be [features, width] in float16, bfloat16 or float32")
     n, k = weight.shape
