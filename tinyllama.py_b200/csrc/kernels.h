@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "product_plan.h"
+
 namespace tlb {
 
 // Message returned by tlb_last_error() on this thread (defined in abi.cu).
@@ -361,19 +363,6 @@ struct ProductParams {
     long long x_stride, x_scales_stride, weight_stride, weight_scales_stride, out_stride;
     int width;
 };
-// How the tensor-core kernel takes a product (plan_product).
-struct ProductPlan {
-    int tile_tokens;           // tokens of a tile, a multiple of 16, 224 at most
-    int split;                 // CTAs (a cluster) that share a tile's width
-    bool pair;                 // two CTAs take 256 features as one
-    int chunks;                // of 128 values of the width a stage
-    bool pieces;               // 16-bit results by way of a warp's 32 features
-    int stages;
-    int ctas;
-    size_t smem;
-};
-// half: results in 16 bits.
-ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool half, int sms);
 // `map_w`, `map_x`: boxes of {128 bytes, 128 rows} and {128 bytes, tile_tokens rows (half
 // of them for a pair)}, 128-byte swizzle; `map_out` (with tma_out, which goes with
 // pieces): boxes of {32 features, 32 tokens, or 16 if tile_tokens is no multiple of 32},

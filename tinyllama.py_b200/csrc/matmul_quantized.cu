@@ -27,16 +27,13 @@
 
 namespace tlb {
 
+using namespace product;
+
 namespace {
 
-constexpr int kFeatures = 128;             // of a CTA's tile (M)
-constexpr int kChunk = 128;                // bytes of K of a shared-memory row
-constexpr int kMaxTokens = 224;            // of a tile (N): two accumulators and the scales
-constexpr int kWeightBytes = kFeatures * kChunk;  // of a chunk
 constexpr int kThreads = 448;
-constexpr int kResultWarps = 8, kResultThreads = 32 * kResultWarps;
+constexpr int kResultThreads = 32 * kResultWarps;
 constexpr int kCopyWarp = 12, kTensorWarp = 13;
-constexpr int kMaxStages = 12;
 constexpr int kScaleSets = 4;              // sets of scales in tensor memory, a word each
 constexpr int kSetColumns = 12;            // 4 of the weights, 8 of the tokens
 constexpr int kScaleColumn = 512 - kScaleSets * kSetColumns;
@@ -48,15 +45,10 @@ constexpr int kBarFull = 0, kBarEmpty = kMaxStages, kBarScales = 2 * kMaxStages,
               kBarSumsFree = kBarSums + 2, kBarParts = kBarSumsFree + 2,
               kBarPartsFree = kBarParts + 1, kBarDrain = kBarPartsFree + 1,
               kNumBars = kBarDrain + 1;
-// behind the barriers: the tensor-memory address, the number of stages issued, and
-// whether a wait gave up
+// behind the barriers, in kTail bytes with them: the tensor-memory address, the number of
+// stages issued, and whether a wait gave up
 constexpr int kSlot = kNumBars * 8, kIssued = kSlot + 4, kGaveUp = kSlot + 8;
-constexpr int kTail = 512;                 // bytes of all of it, after the stages
 static_assert(kGaveUp + 4 <= kTail, "barriers");
-// CTAs that share a tile. Eight were slower everywhere (64 x 8192 -> 2048: 17.7 us, 10.4
-// with four): fewer than 16 clusters of that many large CTAs run at once.
-constexpr int kMaxSplit = 4;
-
 struct Work {
     ProductParams p;
     int tile_tokens;
@@ -185,11 +177,7 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int word, int
 // memory, while the words before them go to tensor memory: four columns of the tile's
 // weight scale, the same in all lanes, and a column for each 32 tokens. Each warp
 // writes the 32 lanes it can reach. False: a wait gave up.
-constexpr int kWordsAtOnce = 4;
 constexpr int kRowsAtOnce = 128 / kWordsAtOnce;
-constexpr int kScalePitch = kWordsAtOnce + 1;  // words: rows in different banks
-constexpr int kScaleRows = kMaxTokens + 1;     // the weights' behind the tokens'
-constexpr int kScaleBytes = 2 * kScaleRows * kScalePitch * 4;
 
 template <bool kPair, bool kWords>
 __device__ __forceinline__ bool feed_scales(const Work& w, uint8_t* buffers, uint32_t tmem,
@@ -777,17 +765,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Results in shared memory: two buffers of 2 KB a warp, or sums of the whole tile or of
-// 64 tokens.
-int parts_bytes_of(int tokens, int split, bool pieces) {
-    return pieces ? kResultWarps * 4096 : (split > 1 ? tokens : 64) * kFeatures * 4;
-}
-size_t smem_of(int tokens, int split, bool pair, int chunks, bool pieces, int stages) {
-    const int rows = pair ? tokens / 2 : tokens;
-    return 1024 + (size_t)stages * chunks * (kWeightBytes + rows * kChunk) + kTail +
-           parts_bytes_of(tokens, split, pieces) + kScaleBytes;
-}
-
 template <typename T, bool kPair, int kChunks>
 cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& map_w,
                    const CUtensorMap& map_x, const CUtensorMap& map_out, cudaStream_t st) {
@@ -799,7 +776,8 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
     if (e != cudaSuccess) return e;
     const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
     if (!(set.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)kMaxSmem);
         if (e != cudaSuccess) return e;
         set.fetch_or(bit, std::memory_order_relaxed);
     }
@@ -820,72 +798,6 @@ cudaError_t launch(const Work& w, const ProductPlan& plan, const CUtensorMap& ma
 }
 
 }  // namespace
-
-// Which tile, and how many CTAs share it: the plan whose time, in microseconds by the
-// measurements below (short runs, at 1.9 GHz), is the shortest.
-//   * A chunk of a tile of n tokens takes 0.13 + n / 1000 (the issuing thread, then the
-//     tensor cores; 16 tokens 0.17, 160 0.29), of a pair's 0.13 + n / 1250 (160 tokens
-//     0.26, 224 0.31); at least its bytes at 115 GB/s an SM (from the L2), and where every
-//     weight is read once, all CTAs' weights at 6.3 TB/s. Weights too many for the L2 cost
-//     0.7 of that where several tiles read them (33 x 4096 -> 28672: 23.6 us in a tile of
-//     48 tokens, 33.5 in two of 32).
-//   * A tile's end takes 0.5, and a tile no less than its results' way to memory, 0.3 and
-//     0.0118 a token (13863 x 208 -> 9928: 106 us with single CTAs, 91 with pairs, 275 MB).
-//   * Pairs start 1.2 later (1024 x 2048 -> 2560: 9.0 us with single CTAs, 9.7 with pairs;
-//     4096 x 4096 -> 4096: 59.4 and 53.1; 16384 x 4096 -> 8192: 426 and 399).
-//   * Sharing a tile costs 0.9 + n / 40 (64 x 8192 -> 2048: 15.2 us alone, 10.7 by two,
-//     9.4 by four CTAs; 64 x 2048 -> 2560: 6.2, 6.2 and 6.4).
-ProductPlan plan_product(int64_t num_tokens, int64_t features, int64_t width, bool half,
-                         int sms) {
-    const int64_t chunks = (width + kChunk - 1) / kChunk;
-    ProductPlan best{};
-    double best_time = 0;
-    auto consider = [&](int split, bool pair, int tokens) {
-        const int per_cta = pair ? 2 * kFeatures : kFeatures, cluster = pair ? 2 : split;
-        const int units = sms / cluster;
-        if (units == 0) return;
-        const int64_t tiles_t = (num_tokens + tokens - 1) / tokens;
-        const int64_t tiles = (features + per_cta - 1) / per_cta * tiles_t;
-        const int64_t rounds = (tiles + units - 1) / units;
-        const int ctas = (int)(tiles < units ? tiles : units) * cluster;
-        double chunk = 0.13 + tokens * (pair ? 0.8e-3 : 1e-3);
-        const double copy = (kWeightBytes + (pair ? tokens / 2 : tokens) * kChunk) / 115e3;
-        if (copy > chunk) chunk = copy;
-        double stream = ctas * (double)kWeightBytes / 6.3e6;
-        if (tiles_t > 1) stream *= features * width > (64 << 20) ? 0.7 : 0;
-        if (stream > chunk) chunk = stream;
-        double tile = (double)((chunks + split - 1) / split) * chunk + 0.5;
-        if (tile < 0.3 + 0.0118 * tokens) tile = 0.3 + 0.0118 * tokens;
-        double time = rounds * tile + (pair ? 1.2 : 0);
-        if (split > 1) time += rounds * (0.9 + tokens / 40.0);
-        if (best_time == 0 || time < best_time) {
-            best_time = time;
-            best.tile_tokens = tokens;
-            best.split = split;
-            best.pair = pair;
-            best.ctas = ctas;
-        }
-    };
-    for (int tokens = 16; tokens <= kMaxTokens; tokens += 16) {
-        if (tokens != 16 && tokens - 16 >= num_tokens) break;
-        for (int split = 1; split <= (tokens <= 128 ? kMaxSplit : 1) && 2 * split <= chunks + 1;
-             split *= 2)
-            consider(split, false, tokens);
-        if (tokens % 32 == 0 && tokens >= 64) consider(1, true, tokens);
-    }
-    best.chunks = best.pair || best.tile_tokens < 128 || best.split > 1 ? 2 : 1;
-    best.pieces = best.split == 1 && half;
-    int stages = kMaxStages;
-    auto smem = [&] {
-        return smem_of(best.tile_tokens, best.split, best.pair, best.chunks, best.pieces, stages);
-    };
-    while (smem() > 232448) --stages;
-    best.stages = stages;
-    // One CTA an SM, also where two would fit: each takes all tensor memory, and two
-    // clusters could otherwise wait for one another's.
-    best.smem = smem() < 120 * 1024 ? 120 * 1024 : smem();
-    return best;
-}
 
 cudaError_t launch_product(int out_dtype, const ProductParams& p, const ProductPlan& plan,
                            const CUtensorMap& map_w, const CUtensorMap& map_x,
