@@ -1,5 +1,5 @@
 """Each plan of the 8-bit product, over tiles of several stages and words of scales: exact on
-whole numbers."""
+whole numbers, and a token alone as among others."""
 
 import pytest
 import torch
@@ -29,6 +29,12 @@ def _clean(built_lib):
     torch.cuda.synchronize()
 
 
+def operands(g, t, k, n):
+    x = L.quantize_rows(torch.randn(t, k, generator=g, device="cuda"))
+    w = L.quantize_weight(torch.randn(n, k, generator=g, device="cuda") * k ** -0.5)
+    return (*x, *w)
+
+
 @pytest.mark.parametrize("t,k,n", P.CASES)
 def test_whole_numbers_are_exact(t, k, n):
     """Small whole values and scales that keep every partial sum a multiple of 1/2 below 2^23:
@@ -48,4 +54,22 @@ def test_whole_numbers_are_exact(t, k, n):
     for dtype in TYPES:
         got = L.matmul_quantized(x, xs, w, ws, dtype, bias.to(dtype))
         assert torch.equal(got, want.float().to(dtype)), dtype
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("t,k,n", P.CASES)
+def test_a_token_alone_and_among_others(t, k, n):
+    """Within the bound of their sums, whose order goes with the sizes; the same bits from
+    calls of the same sizes, wherever the token stands."""
+    g = torch.Generator(device="cuda").manual_seed(t * 3 + k + n)
+    x, xs, w, ws = operands(g, t, k, n)
+    got = L.matmul_quantized(x, xs, w, ws, torch.float32)
+    for i in (0, t // 2, t - 1):
+        alone = L.matmul_quantized(x[i:i + 1], xs[i:i + 1], w, ws, torch.float32)
+        y, mag = O.product(x[i:i + 1], xs[i:i + 1], w, ws)
+        bound = O.product_bound(y, mag, k, torch.float32)
+        assert bool(((alone.double() - y).abs() <= bound).all())
+        assert bool(((got[i:i + 1].double() - y).abs() <= bound).all())
+    turned = [v.view(torch.uint8).roll(1, 0).view(v.dtype) for v in (x, xs)]
+    assert torch.equal(L.matmul_quantized(*turned, w, ws, torch.float32).roll(-1, 0), got)
     assert _lib.device_status() == 0

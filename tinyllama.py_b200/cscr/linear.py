@@ -186,9 +186,11 @@ def matmul_quantized(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tens
 
     x [T, K] float8_e4m3fn with x_scales [T, ceil(K / 128)], weight [N, K] with
     weight_scales [ceil(N / 128), ceil(K / 128)] (float8_e8m0fnu), bias [N] of
-    ``out_dtype`` (float16, bfloat16 or float32). Sums in fp32, one rounding. Rows of
-    any operand may be strided; x and weight rows on 16-byte boundaries take the
-    tensor cores, others a slower kernel.
+    ``out_dtype`` (float16, bfloat16 or float32). Sums in fp32, one rounding; their order
+    goes with sizes and alignment, so a token's bits may differ between calls with other
+    numbers of tokens, not between calls that are alike. Rows of any operand may be
+    strided; x and weight rows on 16-byte boundaries take the tensor cores, others a
+    slower kernel.
     """
     if _lib.fast is not None:
         out = _lib.fast.product(x, x_scales, weight, weight_scales, out_dtype, bias)
