@@ -1,5 +1,5 @@
 """Each plan of the 8-bit product, over tiles of several stages and words of scales: exact on
-whole numbers, and a token alone as among others."""
+whole numbers, the same for a token alone, and with waits that give up."""
 
 import pytest
 import torch
@@ -73,3 +73,26 @@ def test_a_token_alone_and_among_others(t, k, n):
     turned = [v.view(torch.uint8).roll(1, 0).view(v.dtype) for v in (x, xs)]
     assert torch.equal(L.matmul_quantized(*turned, w, ws, torch.float32).roll(-1, 0), got)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("limit", [0, 1, 8, 64, 512])
+@pytest.mark.parametrize("t,k,n", P.CASES)
+def test_waits_that_give_up(t, k, n, limit):
+    """Every input is valid and every wait ends, some before their time: the call returns,
+    says so in the status word, and the next one is exact again."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    ops = operands(g, t, k, n)
+    for dtype in (torch.bfloat16, torch.float32):
+        want = L.matmul_quantized(*ops, dtype)
+        torch.cuda.synchronize()
+        _lib.set_wait_limit(limit)
+        L.matmul_quantized(*ops, dtype)
+        L.matmul_quantized(*ops, dtype)
+        torch.cuda.synchronize()
+        _lib.set_wait_limit(_lib.WAIT_LIMIT_DEFAULT)
+        status = _lib.device_status()
+        assert status & ~_lib.STATUS_WAIT_TIMEOUT == 0
+        if limit == 0:
+            assert status & _lib.STATUS_WAIT_TIMEOUT
+        assert torch.equal(L.matmul_quantized(*ops, dtype), want)
+        assert _lib.device_status() == 0

@@ -521,6 +521,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc5::fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tail_ptr + kSlot);
 
+    auto commit = [](uint32_t b) {
+        if constexpr (kPair) tc5::commit_pair(b);
+        else tc5::commit(b);
+    };
     // this CTA's tiles, and its part of their width
     const int tiles = w.tiles_n * w.tiles_t;
     const int units = gridDim.x / cluster, unit = blockIdx.x / cluster;
@@ -528,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int d_last = (int)((long long)w.depths * (split > 1 ? rank + 1 : 1) / split);
     const int word_first = d_first / kPerWord, word_end = (d_last - 1) / kPerWord + 1;
     const uint32_t limit = w.wait_limit;
-    bool ok = true;
+    bool ok = true, issues = false;  // issues: this thread, the tensor instructions
 
     if (warp == kCopyWarp) {
         // ------------------------------------------------------------ copies
@@ -590,10 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kTensorWarp) {
         // ------------------------------------------------ tensor instructions
         if ((!kPair || rank == 0) && elect_one()) {
-            auto commit = [](uint32_t b) {
-                if constexpr (kPair) tc5::commit_pair(b);
-                else tc5::commit(b);
-            };
+            issues = true;
             const uint64_t whole = tc5::desc_sw128(base, 16, 1024);
             const uint32_t first = (uint32_t)whole, high = (uint32_t)(whole >> 32);
             const uint32_t idesc = tc5::idesc_mxf8(kPair ? 256 : 128, w.tile_tokens, 0);
@@ -655,10 +656,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (ok) commit(bar(kBarSums + b));
-            }
-            if (!ok) {  // nothing runs on when the CTA ends
-                commit(bar(kBarDrain));
-                mbar_wait_bounded(bar(kBarDrain), 0);
             }
         }
     } else if (warp < 4) {
@@ -726,8 +723,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool gave_up = *reinterpret_cast<volatile int*>(tail_ptr + kGaveUp) != 0;
     if constexpr (kPair)
         gave_up = gave_up || load_cluster_int(map_rank(tail + kGaveUp, rank ^ 1)) != 0;
-    // After a wait that gave up, the copies that were issued land before the CTA ends
-    // (they have otherwise: their stages were used).
+    // After a wait that gave up, the tensor instructions that were issued complete before the
+    // tensor memory is freed, whichever thread gave up (results that were read were complete,
+    // but a thread that waits for them may have given up where the one that issues them went
+    // on to its end), of a pair in both CTAs, whose operands they read.
+    if (gave_up && issues) commit(bar(kBarDrain));
+    if (gave_up && tid == 32 * kTensorWarp) mbar_wait_bounded(bar(kBarDrain), 0);
+    // And the copies that were issued land before the CTA ends (they have otherwise: their
+    // stages were used).
     if (gave_up && tid == 0 && (!kPair || rank == 0)) {
         const int mine = *reinterpret_cast<volatile int*>(tail_ptr + kIssued);
         int most = mine;
