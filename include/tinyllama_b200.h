@@ -623,8 +623,9 @@ TLB_API int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream);
  *                   weight_scales_stride apart
  *   bias          : [features] of out_dtype, or NULL
  *   out           : rows out_stride apart
- * A scale byte b stands for 2^(b - 127), 255 for NaN. The exponents of a product's
- * two scales may add up to -120 .. 110; results past fp32 are infinite or 0.
+ * A scale byte b stands for 2^(b - 127), 255 for NaN; any two may meet. Sums past fp32
+ * are infinite (NaN where both signs meet), those below 2^-126, of a group of 128 values
+ * or of all, may count as 0.
  * The tensor-core kernel wants x and weight on 16-byte boundaries with strides that
  * are multiples of 16, and a width of 2^22 at most; others go to a kernel for any shape.
  * ---------------------------------------------------------------------- */

@@ -131,3 +131,38 @@ def test_residual_out_over_other_rows_is_refused():
     q, s, h = L.rms_norm_quantized(x, w, 1e-6, res, residual_out=out)
     assert torch.equal(out, want_h) and h.data_ptr() == out.data_ptr()
     O.assert_rows_of(q, s, want, NORM_DELTA)
+
+
+@pytest.mark.parametrize("k", [256, 250])
+def test_product_of_any_two_scales(k):
+    """Every scale byte with every other, on the tensor cores and off: exact (sums of a few
+    bits), infinite past fp32, but for sums below 2^-126, which may count as 0: each of the
+    two groups', so that a result is off by less than 2^-125. Zeros are zeros at any scale."""
+    for value in (1.0, -448.0, 2.0 ** -9, 0.0):
+        x = torch.full((255, k), value, device="cuda").to(E4M3)
+        w = torch.ones(255 * 128, k, device="cuda").to(E4M3)
+        byte = torch.arange(255, dtype=torch.uint8, device="cuda")[:, None].repeat(1, 2)
+        got = L.matmul_quantized(x, byte.view(E8M0), w, byte.view(E8M0), torch.float32)
+        assert torch.equal(got, got[:, ::128].repeat_interleave(128, 1))
+        got = got[:, ::128].double()
+        e = byte[:, :1].double() + byte[:, 0].double() - 254
+        want = (k * value * torch.exp2(e)).float().double()
+        group = ((k - 128) * abs(value) * torch.exp2(e)).double()  # the smaller one's sum
+        exact = (group >= 2.0 ** -126) | (value == 0)
+        assert torch.equal(got[exact], want[exact])
+        assert bool(((got - want).abs() < 2.0 ** -125)[~exact].all())
+
+
+@pytest.mark.parametrize("k", [512, 500])
+def test_product_of_scales_far_apart(k):
+    """Groups whose scales multiply to 2^-250 and to 2^110 side by side."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    t, n, groups = 40, 300, 4
+    x, w = (torch.randn(r, k, generator=g, device="cuda").to(E4M3) for r in (t, n))
+    xs = torch.randint(2, 180, (t, groups), generator=g, device="cuda").to(torch.uint8)
+    ws = torch.randint(2, 180, (3, groups), generator=g, device="cuda").to(torch.uint8)
+    got = L.matmul_quantized(x, xs.view(E8M0), w, ws.view(E8M0), torch.float32)
+    y, mag = O.product(x, xs.view(E8M0), w, ws.view(E8M0))
+    # and each group's sum and each sum of them may be taken for 0 below 2^-126
+    bound = O.product_bound(y, mag, k, torch.float32) + (2 * groups) * 2.0 ** -126
+    assert bool(((got.double() - y).abs() <= bound).all())

@@ -191,6 +191,9 @@ def matmul_quantized(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tens
     numbers of tokens, not between calls that are alike. Rows of any operand may be
     strided; x and weight rows on 16-byte boundaries take the tensor cores, others a
     slower kernel.
+
+    Any scales may meet: sums past fp32 are infinite (NaN where both signs meet), those
+    below 2^-126 (of a group of 128, or of all) may count as 0.
     """
     if _lib.fast is not None:
         out = _lib.fast.product(x, x_scales, weight, weight_scales, out_dtype, bias)
