@@ -166,8 +166,9 @@ __device__ __forceinline__ uint2 quantize_raw(const Raw8<T>& x, uint32_t mask, u
     return quantized8<E4M3, false>(f, inverse_scale(byte));
 }
 
-// x / d for x < 2^31 and d < 2^31 by a product with the inverse (the round-up method for
-// invariant divisors): 32-bit division took a fifth of these kernels' instructions.
+// x / d for x < 2^31 and d < 2^31 by a product with the inverse, rounded up (Granlund and
+// Montgomery, Division by invariant integers using multiplication, 1994): 32-bit division
+// took a fifth of these kernels' instructions.
 struct FastDivisor {
     uint32_t by, inverse;
     int shift;
