@@ -110,8 +110,8 @@ struct InverseRoot {
 
 // A row's values are taken this much larger (smaller) where their squares would leave fp32's
 // range: a mean below 2^-100 has lost squares below 2^-126, and an infinite one may come from
-// finite values. Squares of the former are then below 2^92 a value, of the latter below 2^96;
-// widths are below 2^30. Results do not depend on it. fp16 has no such values.
+// finite values. Rows are at most 2^30 wide, so the former's squares then sum to less than
+// 2^122, the latter's to less than 2^126. Results do not depend on it. fp16 has no such rows.
 template <typename T> __device__ __forceinline__ float range_shift(float mean) {
     if (std::is_same<T, __half>::value || (mean >= 0x1p-100f && mean < INFINITY)) return 1.f;
     return mean < 0x1p-100f ? 0x1p96f : 0x1p-80f;
