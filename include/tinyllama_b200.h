@@ -622,7 +622,7 @@ TLB_API int tlb_quantize_rows(const tlb_quantize_rows_args* args, void* stream);
  *   weight_scales : [ceil(features / 128), ceil(width / 128)] scale bytes, rows
  *                   weight_scales_stride apart
  *   bias          : [features] of out_dtype, or NULL
- *   out           : rows out_stride apart
+ *   out           : rows out_stride apart, which do not overlap
  * A scale byte b stands for 2^(b - 127), 255 for NaN; any two may meet. Sums past fp32
  * are infinite (NaN where both signs meet), those below 2^-126, of a group of 128 values
  * or of all, may count as 0.

@@ -66,6 +66,14 @@ def test_refusals_are_those_of_rows_with_a_byte_in_common(built_lib, rows):
         assert (got == BAD) == clash, (a, b, away, _lib.last_error())
 
 
+def test_product_rows_that_overlap_are_refused(built_lib):
+    name, pack = _lib.MATMUL_QUANTIZED
+    for stride in (0, 63, -63):
+        call = pack(P, P << 1, P << 2, P << 3, P << 4, 0, 4, 256, 64, 256, 2, 256, 2, stride, BF16)
+        assert getattr(_lib.load(), name)(call, None) == BAD
+        assert "overlap" in _lib.last_error()
+
+
 def test_weights_are_converted_without_gradients():
     """A parameter's values and scales hold no graph (with copies of its blocks in fp32)."""
     weight = torch.nn.Parameter(torch.randn(200, 300))

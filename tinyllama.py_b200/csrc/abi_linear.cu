@@ -176,6 +176,8 @@ int tlb_matmul_quantized(const tlb_matmul_quantized_args* args, void* stream) {
     if (a.num_tokens == 0 || a.features == 0) return TLB_OK;
     TLB_REQUIRE(a.out && a.x && a.x_scales && a.weight && a.weight_scales,
                 "tensor pointers must not be null");
+    TLB_REQUIRE(a.num_tokens < 2 || a.out_stride >= a.features || a.out_stride <= -a.features,
+                "out's rows overlap");
     const int e = elem_bytes(a.out_dtype);
     TLB_REQUIRE(aligned(a.out, e) && (!a.bias || aligned(a.bias, e)),
                 "tensor pointers must be aligned to the element size");
