@@ -86,6 +86,18 @@ def test_dispatch_modes_see_the_allocations():
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), name
 
 
+def test_the_python_code_answers_the_same(monkeypatch):
+    """Each of the calls with its Python argument handling alone."""
+    calls = ordinary_calls()
+    calls["heads and cache"][0]()  # what it writes is there for every read
+    want = {name: call() for name, (call, _) in calls.items()}
+    monkeypatch.setattr(_lib, "fast", None)
+    for name, (call, _) in calls.items():
+        for a, b in zip(call(), want[name], strict=True):
+            assert a.dtype == b.dtype and a.stride() == b.stride(), name
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), name
+
+
 def test_profilers_see_the_allocations():
     for name, (call, count) in ordinary_calls().items():
         with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as profile:
